@@ -18,12 +18,18 @@ STATUS_TEXT = {0: "ok", 1: "invalid argument", 2: "unsupported configuration", 3
 DEVICE_ERRORS = {101: "timed out waiting for a plane block", 102: "timed out waiting for a basis tile",
                  103: "timed out waiting for an operand tile", 104: "timed out waiting for a free stage",
                  105: "timed out waiting for the accumulator", 106: "timed out waiting for TMEM to drain",
-                 107: "timed out draining async work", 110: "descriptor out of bounds"}
+                 107: "timed out draining async work", 110: "descriptor out of bounds",
+                 111: "no free page for the planned tokens", 112: "token count or length out of range",
+                 113: "key or value that a 4-bit cell cannot hold (not finite, or beyond 2^15)",
+                 114: "no room for a token in the history",
+                 115: "the attention mask hides other tokens than the causal order of the 4-bit cache"}
 
 EXPORTS = ("dkv_attend_layer", "dkv_key_scores", "dkv_softmax_stats", "dkv_value_weights", "dkv_finalize",
            "dkv_attend_tail",
            "dkv_unpack", "dkv_importance", "dkv_topk", "dkv_refine_merge", "dkv_attend_layer_static",
            "dkv_vpart_floats", "dkv_encode_groups", "dkv_storage_unpack", "dkv_demote", "dkv_alloc_workspace_bytes", "dkv_allocate_rungs",
+           "dkv_q4_page_bytes", "dkv_page_plan", "dkv_page_trim", "dkv_page_slots", "dkv_q4_append", "dkv_q4_read",
+           "dkv_q4_attend", "dkv_logit_rules",
            "dkv_version", "dkv_status_string")
 
 
@@ -144,6 +150,49 @@ class RefineArgs(ctypes.Structure):
     ]
 
 
+class PageArgs(ctypes.Structure):
+    """Mirror of ``dkv_page_args``."""
+
+    _fields_ = [
+        ("blocks", c_void_p), ("max_blocks", c_int32), ("lengths", c_void_p), ("starts", c_void_p),
+        ("free_pages", c_void_p), ("n_free", c_void_p), ("n_pages", c_int32), ("n_seq", c_int32),
+        ("counts", c_void_p), ("q_len", c_int32), ("slots", c_void_p), ("status", c_void_p),
+    ]
+
+
+class Q4RowsArgs(ctypes.Structure):
+    """Mirror of ``dkv_q4_rows_args``."""
+
+    _fields_ = [
+        ("cells", c_void_p), ("n_pages", c_int32), ("n_kv_heads", c_int32), ("head_dim", c_int32), ("fp16", c_int32),
+        ("slots", c_void_p), ("n_seq", c_int32), ("q_len", c_int32), ("key", c_void_p), ("value", c_void_p),
+        ("k_stride", c_int64 * 3), ("v_stride", c_int64 * 3), ("status", c_void_p),
+    ]
+
+
+class Q4AttendArgs(ctypes.Structure):
+    """Mirror of ``dkv_q4_attend_args``."""
+
+    _fields_ = [
+        ("cells", c_void_p), ("n_pages", c_int32), ("n_kv_heads", c_int32), ("n_q_heads", c_int32),
+        ("head_dim", c_int32), ("fp16", c_int32), ("blocks", c_void_p), ("max_blocks", c_int32), ("lengths", c_void_p),
+        ("starts", c_void_p), ("n_seq", c_int32), ("q_len", c_int32), ("len_bound", c_int32), ("query", c_void_p),
+        ("q_stride", c_int64 * 3), ("scaling", c_float), ("out", c_void_p), ("out_f32", c_int32), ("status", c_void_p),
+    ]
+
+
+class LogitsArgs(ctypes.Structure):
+    """Mirror of ``dkv_logits_args``."""
+
+    _fields_ = [
+        ("logits", c_void_p), ("dtype", c_int32), ("row_stride", c_int64), ("n_rows", c_int32), ("vocab", c_int32),
+        ("history", c_void_p), ("capacity", c_int32), ("lengths", c_void_p), ("prompts", c_void_p),
+        ("repetition", c_void_p), ("frequency", c_void_p), ("presence", c_void_p), ("bias_ids", c_void_p),
+        ("bias_values", c_void_p), ("n_bias", c_int32), ("allowed", c_void_p), ("adjusted", c_void_p),
+        ("tokens", c_void_p), ("append", c_int32), ("status", c_void_p),
+    ]
+
+
 _LIB = None
 
 
@@ -170,12 +219,17 @@ def lib():
         handle.dkv_unpack.restype = c_int32
         for name, st in (("dkv_importance", ImportanceArgs), ("dkv_topk", TopkArgs), ("dkv_refine_merge", RefineArgs),
                          ("dkv_encode_groups", EncodeArgs), ("dkv_storage_unpack", StorageArgs),
-                         ("dkv_allocate_rungs", AllocArgs), ("dkv_demote", DemoteArgs)):
+                         ("dkv_allocate_rungs", AllocArgs), ("dkv_demote", DemoteArgs),
+                         ("dkv_page_plan", PageArgs), ("dkv_page_trim", PageArgs), ("dkv_page_slots", PageArgs),
+                         ("dkv_q4_append", Q4RowsArgs), ("dkv_q4_read", Q4RowsArgs), ("dkv_q4_attend", Q4AttendArgs),
+                         ("dkv_logit_rules", LogitsArgs)):
             fn = getattr(handle, name)
             fn.argtypes = [ctypes.POINTER(st), c_void_p]
             fn.restype = c_int32
         handle.dkv_alloc_workspace_bytes.argtypes = [c_int64, c_int32]
         handle.dkv_alloc_workspace_bytes.restype = c_int64
+        handle.dkv_q4_page_bytes.argtypes = [c_int32]
+        handle.dkv_q4_page_bytes.restype = c_int64
         handle.dkv_vpart_floats.argtypes = [c_int32, c_int32, c_int32, c_int32]
         handle.dkv_vpart_floats.restype = c_int64
         handle.dkv_version.argtypes = []
@@ -192,7 +246,31 @@ def check(rc: int, what: str) -> None:
 
 
 DEVICE_SITES = {1: "key_scores_pair", 2: "key_scores", 3: "value_weights", 4: "value_dense", 5: "unpack",
-                6: "key_scores_dense"}
+                6: "key_scores_dense", 7: "q4_attend", 8: "q4_append / q4_read", 9: "page tables"}
+
+
+def launch(name: str, args, device) -> None:
+    """Enqueue entry point ``name`` on the current stream of ``device``, whichever device is current."""
+    import torch
+
+    fn = getattr(lib(), name)
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        rc = fn(args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(args, stream)
+    check(rc, name)
+
+
+def cuda_device(device):
+    """``device`` with its index, for the modules whose kernels have no CPU form."""
+    import torch
+
+    device = torch.device(device)
+    if device.type != "cuda":
+        raise ValueError(f"{device} is not a CUDA device (there is no CPU fallback)")
+    return torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
 
 
 def describe_device_error(code: int) -> str:

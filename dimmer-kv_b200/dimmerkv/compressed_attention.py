@@ -14,7 +14,7 @@ from __future__ import annotations
 
 import torch
 
-from . import dimmer
+from . import _lib, dimmer
 from .codes import from_coefficients, retype_raw
 from .common import build_cache
 from .context import CompressedBatch, ConversationCodes, TokenCodes, rope_tables
@@ -110,12 +110,18 @@ def _to(t: TokenCodes, device) -> TokenCodes:
 
 
 def greedy_answer(model, tokenizer, context, cache, input_ids: torch.Tensor, start_position: int,
-                  max_new_tokens: int = 12, evicted=None, stop_at_eos: bool = True):
+                  max_new_tokens: int = 12, evicted=None, stop_at_eos: bool = True, rules=None, grammar=None):
     """Greedy decoding on top of a prefilled cache (compressed_attention.py:140-169).
 
     With ``context`` set, attention runs over the compressed tokens directly and ``cache`` must be
     ``context.exact_cache``; otherwise ``cache`` is a full cache. Returns (text, first-step logits).
+
+    ``rules`` (a one-row ``LogitRules``) adjusts the logits of every step before the choice and takes the chosen
+    token into its history; ``grammar(last)`` gives that step's mask (``allow_mask``; None: everything) from the
+    token before it (None at the first step). A step whose mask leaves nothing ends the answer.
     """
+    if grammar is not None and rules is None:
+        raise ValueError("a grammar needs rules (LogitRules)")
     device = input_ids.device
     dimmer.STATE.compressed = context
     dimmer.set_eviction(evicted)
@@ -129,7 +135,14 @@ def greedy_answer(model, tokenizer, context, cache, input_ids: torch.Tensor, sta
             if first_logits is None:
                 first_logits = logits[0, -1].float()
             position += ids.shape[1]
-            token = int(logits[0, -1].argmax())
+            if rules is None:
+                token = int(logits[0, -1].argmax())
+            else:
+                mask = grammar(generated[-1] if generated else None) if grammar is not None else None
+                token = int(rules.pick(logits[:, -1], mask)[0])
+                rules.check_status()
+                if token < 0:
+                    break
             if stop_at_eos and (token == tokenizer.eos_token_id or token in tokenizer.all_special_ids):
                 break
             generated.append(token)
@@ -141,14 +154,20 @@ def greedy_answer(model, tokenizer, context, cache, input_ids: torch.Tensor, sta
 
 
 def greedy_decode_batch(model, batch: CompressedBatch, cache, host_ids: torch.Tensor, host_positions: torch.Tensor,
-                        steps: int):
+                        steps: int, rules=None, grammar=None):
     """Greedy decode of every conversation of ``batch`` for ``steps`` tokens.
+
+    ``batch``: a ``CompressedBatch`` or a ``Q4Batch`` (with its ``cache``). ``rules`` (a ``LogitRules`` of one row per
+    conversation) adjusts every step's logits and keeps the histories; ``grammar(last)`` gives a step's mask from the
+    host tensor of the tokens before it ([B], None at the first step). A mask that leaves a row nothing raises.
 
     ``host_ids`` / ``host_positions``: [B, 1] int64 in (pinned) host memory. Every step copies the
     ids to the device, runs the model with attention over the codes and reads the next ids back, with
     the batch's status word behind them; the host waits for them at most ``batch.poll_wait_s`` seconds
     and raises ``DimmerKVError`` on a device error (``CompressedBatch.poll_status``).
     Returns (tokens [B, steps] int64 on the host, byte counts of the per-step copies)."""
+    if grammar is not None and rules is None:
+        raise ValueError("a grammar needs rules (LogitRules)")
     device = batch.device
     ids_host = host_ids.clone().pin_memory() if not host_ids.is_pinned() else host_ids.clone()
     pos = host_positions.to(device)
@@ -158,10 +177,18 @@ def greedy_decode_batch(model, batch: CompressedBatch, cache, host_ids: torch.Te
         for i in range(steps):
             ids = ids_host.to(device, non_blocking=True)
             logits = model(input_ids=ids, past_key_values=cache, position_ids=pos, use_cache=True).logits
-            nxt = logits[:, -1].argmax(-1, keepdim=True)
+            if rules is None:
+                nxt = logits[:, -1].argmax(-1, keepdim=True)
+            else:
+                mask = grammar(out[:, i - 1] if i else None) if grammar is not None else None
+                nxt = rules.pick(logits[:, -1], mask)[:, None]
             ids_host.copy_(nxt, non_blocking=True)  # device -> pinned host
             batch.poll_status(depth=0)  # bounded wait for the ids and the status word behind them
             out[:, i] = ids_host[:, 0]
+            if rules is not None and bool((out[:, i] < 0).any()):
+                rules.check_status()
+                rows = (out[:, i] < 0).nonzero().flatten().tolist()
+                raise _lib.DimmerKVError(f"step {i}: no token is allowed in conversations {rows}")
             pos = pos + 1
     finally:
         dimmer.STATE.compressed = None

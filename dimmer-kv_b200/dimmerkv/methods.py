@@ -1,6 +1,7 @@
 """Drop-in for the accelerated entry points of scripts/methods.py: ``dkvtc@…`` / ``kvtc@…`` /
 ``kvtcf@…`` (kvtc transform coding, DimmerKV per-token rungs) and ``prog@…`` (progressive bit-planes with
-question-time refinement), plus ``full``.
+question-time refinement), plus ``full``, and ``q4``: every token in 4 bits without a fitted basis (a method of this
+package; ``Q4Context`` attends over its cells directly).
 
 ``Methods.apply`` returns the reference's ``Compressed`` record (rebuilt caches, bytes, timings, the
 ``refine`` callable, per-token bytes) computed the same way (methods.py:167-254). The B200 path starts
@@ -22,6 +23,7 @@ import torch
 
 from .kvtc import KVTCCodec
 from .progressive import ProgressiveCodec, question_importance
+from .q4 import cell_bytes, restore
 
 
 @dataclass
@@ -83,6 +85,12 @@ class Methods:
             used = 2 * len(keys) * keys[0].numel() * 2
             per_token = torch.full((keys[0].shape[2],), used / keys[0].shape[2], device=self.device)
             return Compressed(keys, values, None, used, 0.0, token_bytes=per_token)
+        if name == "q4":
+            (new_keys, new_values), seconds = self._timed(lambda: restore(keys, values))
+            _, heads, tokens, dim = keys[0].shape
+            per_token = 2 * len(keys) * heads * cell_bytes(dim)
+            return Compressed(new_keys, new_values, None, per_token * tokens, seconds,
+                              token_bytes=torch.full((tokens,), float(per_token), device=self.device))
         if name.startswith("prog@"):
             return self._progressive(name, keys, values, scores)
         if name.startswith(("kvtc@", "kvtcf@", "dkvtc@")):
@@ -106,7 +114,7 @@ class Methods:
                 weights=weights, evict=evict, floor_share=floor_share, key_weight=key_weight))
             return Compressed(new_keys, new_values, codec.last_evicted, used, seconds, histogram,
                               token_bytes=self._kvtc_token_bytes(codec, keys[0].shape[2]))
-        raise NotImplementedError(f"method {name!r} is outside the accelerated path (full, kvtc@, kvtcf@, dkvtc@, prog@)")
+        raise NotImplementedError(f"method {name!r} is outside the accelerated path (full, q4, kvtc@, kvtcf@, dkvtc@, prog@)")
 
     def _progressive(self, name: str, keys, values, scores) -> Compressed:
         """prog@<budget>[:snap][:r<frac>] (methods.py:228-254)."""

@@ -375,6 +375,129 @@ typedef struct dkv_alloc_args {
 int64_t dkv_alloc_workspace_bytes(int64_t slots, int32_t levels);
 int dkv_allocate_rungs(const dkv_alloc_args* args, void* stream);
 
+/* ---- Paged 4-bit cache --------------------------------------------------------------------------
+ * A cache that needs no fitted basis: the keys and values of a batch of conversations in 4 bits, in pages of
+ * 64 tokens taken from one pool. No counterpart in the reference (its uncompressed method, `full`, keeps 16
+ * bits; scripts/methods.py:167-172).
+ *
+ * A cell is one token's keys or values of one KV head, in groups of 64 dimensions:
+ *   low   = float16(min)      scale = float16((max - low) / 15)   (float32 arithmetic)
+ *   code  = (x - low) / scale to the nearest whole number of 0..15, ties to even, decided without rounding
+ *   value = low + code * scale (code 0 where scale is 0)
+ * One layer's cells: [n_pages][n_kv_heads][dkv_q4_page_bytes(head_dim)] bytes, 16-byte aligned. A slot is
+ * page * 64 + the token's place in its page. */
+#define DKV_PAGE_TOKENS 64
+
+/* Bytes of one page of one KV head (keys and values of 64 tokens); -1: no kernel for this head_dim. */
+int64_t dkv_q4_page_bytes(int32_t head_dim);
+
+/* Block tables. `blocks` [n_seq][max_blocks] holds each conversation's pages in token order (-1: none),
+ * `lengths` its tokens, `starts` its tokens before the newest plan, `free_pages` [n_pages] a stack whose top
+ * is free_pages[n_free[0] - 1].
+ * dkv_page_plan makes room for counts[s] more tokens of every conversation: the pages that they need come off
+ * the stack (conversations ascending, blocks ascending), starts = lengths, lengths += counts, and
+ * slots[s][i] is the slot of new token i < counts[s], -1 behind them. Without a free page for every need,
+ * or with a count outside 0..q_len or a length beyond max_blocks * 64, nothing changes, every slot is -1 and
+ * the status word tells.
+ * dkv_page_trim keeps the first min(lengths[s], counts[s]) tokens of every conversation; pages that hold none
+ * of them go back on the stack (the lowest conversation's lowest block on top, so that a trim to `starts`
+ * undoes a plan), and starts = lengths. q_len and slots are not used.
+ * dkv_page_slots writes slots[s][i] = the slot of token starts[s] + i for i < counts[s] (those must be held),
+ * -1 behind them, and changes nothing else. n_seq at most 8192. */
+typedef struct dkv_page_args {
+  int32_t* blocks;
+  int32_t max_blocks;
+  int32_t* lengths;
+  int32_t* starts;
+  int32_t* free_pages;
+  int32_t* n_free;               /* [1] */
+  int32_t n_pages;
+  int32_t n_seq;
+  const int32_t* counts;         /* [n_seq]: new tokens (plan), kept tokens (trim), tokens to place (slots) */
+  int32_t q_len;
+  int32_t* slots;                /* [n_seq][q_len] */
+  int* status;
+} dkv_page_args;
+int dkv_page_plan(const dkv_page_args* args, void* stream);
+int dkv_page_trim(const dkv_page_args* args, void* stream);
+int dkv_page_slots(const dkv_page_args* args, void* stream);
+
+/* dkv_q4_append quantises keys and values into their cells; dkv_q4_read writes the values that the cells of
+ * the given slots stand for, rounded once to the 16-bit type (zeros for slot -1). key / value hold
+ * [n_seq][n_kv_heads][q_len][head_dim] at the given strides (elements; multiples of 8, 16-byte aligned, the
+ * last dimension dense). A key or value that is not finite or is beyond 2^15 in magnitude has no cell: the
+ * append reports it in the status word. Rows with slot -1 are neither read nor written. */
+typedef struct dkv_q4_rows_args {
+  uint8_t* cells;                /* the layer's cells */
+  int32_t n_pages, n_kv_heads, head_dim;
+  int32_t fp16;                  /* the 16-bit type of key and value: 0 bf16, 1 fp16 */
+  const int32_t* slots;          /* [n_seq][q_len] */
+  int32_t n_seq, q_len;
+  void* key;
+  void* value;
+  int64_t k_stride[3];           /* conversation, head, token */
+  int64_t v_stride[3];
+  int* status;
+} dkv_q4_rows_args;
+int dkv_q4_append(const dkv_q4_rows_args* args, void* stream);
+int dkv_q4_read(const dkv_q4_rows_args* args, void* stream);
+
+/* Causal attention of the newest tokens' queries over the 4-bit cells: query row i of conversation s sees the
+ * tokens 0 .. starts[s] + i. Rows behind the last new token (i >= lengths[s] - starts[s]) come back as
+ * zeros. Scores, softmax statistics and sums are float32; probabilities enter the value product as float16
+ * against the values rounded to float16. */
+typedef struct dkv_q4_attend_args {
+  const uint8_t* cells;          /* the layer's cells */
+  int32_t n_pages, n_kv_heads, n_q_heads, head_dim;
+  int32_t fp16;                  /* the 16-bit type of the query and of a 16-bit output: 0 bf16, 1 fp16 */
+  const int32_t* blocks;         /* [n_seq][max_blocks] */
+  int32_t max_blocks;
+  const int32_t* lengths;
+  const int32_t* starts;
+  int32_t n_seq, q_len;
+  int32_t len_bound;             /* no length is above this (it only chooses how the work is split) */
+  const void* query;             /* [n_seq][n_q_heads][q_len][head_dim] at q_stride */
+  int64_t q_stride[3];           /* conversation, head, token (elements; multiples of 8, 16-byte aligned) */
+  float scaling;
+  void* out;                     /* [n_seq][q_len][n_q_heads][head_dim] */
+  int32_t out_f32;
+  int* status;
+} dkv_q4_attend_args;
+int dkv_q4_attend(const dkv_q4_attend_args* args, void* stream);
+
+/* The choice of the next token. For every row, with the tokens of its history (the first prompts[r] of
+ * lengths[r] are the prompt, the rest were generated) and in this order, in float32:
+ *   seen anywhere in the history:      x = x > 0 ? x / repetition : x * repetition
+ *   generated c > 0 times:             x = x - frequency * c;  x = x - presence
+ *   listed in the biases:              x = x + value   (a token listed twice gets the values' sum first)
+ *   not allowed by the bit mask:       x = -infinity
+ * `adjusted` gets x, `tokens` the row's largest x (the lowest token of equal ones, a NaN above all), -1 where
+ * every x is -infinity. Tokens outside 0..vocab-1 in the history and the biases are skipped. With `append` the
+ * chosen token, unless it is -1, goes to the end of the row's history; a full history is told in the status
+ * word. */
+typedef struct dkv_logits_args {
+  const void* logits;            /* [n_rows][vocab] at row_stride elements */
+  int32_t dtype;                 /* 0 bf16, 1 fp16, 2 fp32 */
+  int64_t row_stride;
+  int32_t n_rows, vocab;
+  int32_t* history;              /* [n_rows][capacity] */
+  int32_t capacity;
+  int32_t* lengths;              /* [n_rows] */
+  const int32_t* prompts;        /* [n_rows] */
+  const float* repetition;       /* [n_rows], above 0 */
+  const float* frequency;        /* [n_rows] */
+  const float* presence;         /* [n_rows] */
+  const int32_t* bias_ids;       /* [n_rows][n_bias] or NULL */
+  const float* bias_values;
+  int32_t n_bias;                /* at most 1024 */
+  const uint32_t* allowed;       /* [n_rows][ceil(vocab / 32)], bit t % 32 of word t / 32; NULL: all */
+  float* adjusted;               /* [n_rows][vocab] or NULL */
+  int64_t* tokens;               /* [n_rows] */
+  int32_t append;
+  int* status;
+} dkv_logits_args;
+int dkv_logit_rules(const dkv_logits_args* args, void* stream);
+
 /* Library version (major * 10000 + minor * 100 + patch). */
 int dkv_version(void);
 

@@ -1,0 +1,112 @@
+"""The paged 4-bit cache's operators in plain operations of 64 bits, for the tests."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import torch
+
+GROUP = 64
+PAGE = 64
+
+
+def half(x: torch.Tensor) -> torch.Tensor:
+    return x.float().half().double()
+
+
+def cells64(x: torch.Tensor):
+    """(values, scales, lows) in float64 that 4 bits hold for x [..., dim]; scales / lows [..., dim / 64]."""
+    g = x.double().unflatten(-1, (-1, GROUP))
+    low = half(g.amin(-1))
+    scale = half(((g.amax(-1) - low).float() / 15.0))
+    step = scale[..., None]
+    code = torch.where(step > 0, ((g - low[..., None]) / step.clamp_min(1e-30)).round().clamp(0, 15), 0.0)
+    return (low[..., None] + code * step).flatten(-2), scale, low
+
+
+def attend64(query, key, value, held, scaling):
+    """One conversation: query [hq, n, d] of the tokens held .. held + n - 1 over key / value [hkv, held + n, d]
+    (16-bit tensors). Returns the output [n, hq, d] in float64 and, for tolerances, sum p |v| per output and the
+    largest sum of a score's absolute terms per row."""
+    hq, n, d = query.shape
+    share = hq // key.shape[0]
+    k, ks, kl = (t.repeat_interleave(share, 0) for t in cells64(key))
+    v = cells64(value)[0].repeat_interleave(share, 0)
+    q = query.double()
+    scores = q @ k.transpose(1, 2) * scaling
+    hidden = torch.arange(k.shape[1], device=q.device) > held + torch.arange(n, device=q.device)[:, None]
+    p = torch.softmax(scores.masked_fill(hidden, -math.inf), -1)
+    width = (15 * ks + kl.abs()).repeat_interleave(GROUP, -1)
+    terms = (q.abs() @ width.transpose(1, 2) * scaling).masked_fill(hidden, 0.0).amax(-1)
+    return (p @ v).transpose(0, 1), (p @ v.abs()).transpose(0, 1), terms.transpose(0, 1)
+
+
+def attend_tolerance(out, weight, terms, eps):
+    """Largest error of dkv_q4_attend against attend64. Probabilities and values are each rounded to float16 (2^-12
+    relative, half a step each) inside sums whose absolute terms add up to ``weight``; a score, a float32 sum of
+    absolute terms ``terms`` in at most 2 * 128 additions whose operands the tensor core may cut at 2^-22, is off by
+    at most 2^-17 of them in all, which moves numerator and denominator by that much each; the output is rounded
+    once, to half a step of eps."""
+    return weight * (2 * 2**-12 + 2 * 2**-17 * terms[..., None] + 2**-16) + out.abs() * eps / 2 + 1e-12
+
+
+class PlainTable:
+    """PageTable in plain Python."""
+
+    def __init__(self, n_seq, n_pages, max_tokens):
+        self.free = list(range(n_pages - 1, -1, -1))
+        self.blocks = [[] for _ in range(n_seq)]
+        self.lengths = [0] * n_seq
+        self.starts = [0] * n_seq
+        self.cols = -(-max_tokens // PAGE)
+
+    def plan(self, counts, q_len):
+        slots = np.full((len(counts), q_len), -1, dtype=np.int32)
+        for s, c in enumerate(counts):
+            self.starts[s] = self.lengths[s]
+            for i in range(c):
+                at = self.lengths[s] + i
+                if at // PAGE == len(self.blocks[s]):
+                    self.blocks[s].append(self.free.pop())
+                slots[s, i] = self.blocks[s][at // PAGE] * PAGE + at % PAGE
+            self.lengths[s] += c
+        return slots
+
+    def trim(self, keep):
+        back = []
+        for s, k in enumerate(keep):
+            self.lengths[s] = self.starts[s] = min(self.lengths[s], k)
+            held = -(-self.lengths[s] // PAGE)
+            back += self.blocks[s][held:]
+            del self.blocks[s][held:]
+        self.free += back[::-1]
+
+    def array(self):
+        out = np.full((len(self.blocks), self.cols), -1, dtype=np.int32)
+        for s, row in enumerate(self.blocks):
+            out[s, :len(row)] = row
+        return out
+
+
+def rules64(logits, history, lengths, prompts, repetition, frequency, presence, bias=None, allowed=None):
+    """Adjusted logits in float64 [rows, vocab] from lists / arrays on the host."""
+    x = logits.double().cpu().clone()
+    for r in range(x.shape[0]):
+        ids = [int(t) for t in history[r][:lengths[r]]]
+        for t in sorted({t for t in ids if 0 <= t < x.shape[1]}):
+            made = sum(1 for u in ids[prompts[r]:] if u == t)
+            v = float(x[r, t])
+            v = v / repetition[r] if v > 0 else v * repetition[r]
+            if made:
+                v = v - frequency[r] * made - presence[r]
+            x[r, t] = v
+        if bias is not None:
+            for t, b in zip(bias[0][r], bias[1][r]):
+                if 0 <= int(t) < x.shape[1]:
+                    x[r, int(t)] += float(b)
+        if allowed is not None:
+            for t in range(x.shape[1]):
+                if not (int(allowed[r, t // 32]) >> (t % 32)) & 1:
+                    x[r, t] = -math.inf
+    return x

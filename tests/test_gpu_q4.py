@@ -1,0 +1,556 @@
+"""The paged 4-bit cache on the GPU against plain implementations: tables, cells, attention, and a decode of a model
+over them."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import tinymodel as tm
+from dimmerkv import _lib, dimmer
+from dimmerkv.compressed_attention import greedy_answer, greedy_decode_batch
+from dimmerkv.logits import LogitRules, allow_mask
+from dimmerkv.methods import Methods
+from dimmerkv.paging import PageTable
+from dimmerkv.q4 import Q4Batch, Q4Context, dequantise4, quantise4
+from q4_reference import PlainTable, attend64, attend_tolerance, cells64
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda")
+
+
+# ------------------------------------------------------------------------------------------------ tables
+def _same(table, plain):
+    n = int(table.n_free)
+    assert table.free[:n].tolist() == plain.free
+    assert np.array_equal(table.blocks.cpu().numpy(), plain.array())
+    assert table.lengths.tolist() == plain.lengths and table.starts.tolist() == plain.starts
+
+
+@pytest.mark.parametrize("n_seq,q_len", [(1, 1), (3, 65), (40, 7), (1500, 3), (5, 4000)])
+def test_tables_follow_the_plain_ones(n_seq, q_len):
+    rng = np.random.default_rng(n_seq)
+    cap = 2 * q_len + 130
+    table, plain = PageTable(n_seq, n_seq * 70 + 200, cap), PlainTable(n_seq, n_seq * 70 + 200, cap)
+    for step in range(6):
+        if step in (2, 4):
+            keep = [int(k) for k in rng.integers(0, q_len + 70, n_seq)]
+            keep[0] = 0
+            table.trim(torch.tensor(keep, dtype=torch.int32, device=DEV))
+            plain.trim(keep)
+            _same(table, plain)
+        counts = [int(c) for c in rng.integers(0, q_len + 1, n_seq)]
+        counts = [min(c, cap - l) for c, l in zip(counts, plain.lengths)]
+        slots = table.plan(counts, q_len)
+        want = plain.plan(counts, q_len)
+        assert np.array_equal(slots.cpu().numpy(), want)
+        _same(table, plain)
+    full = table.slots(cap).cpu().numpy()
+    for s in range(n_seq):
+        n = plain.lengths[s]
+        assert (full[s, n:] == -1).all()
+        assert full[s, :n].tolist() == [plain.blocks[s][i // 64] * 64 + i % 64 for i in range(n)]
+    table.trim(table.starts)  # a count vector that the kernel changes
+    plain.trim(list(plain.starts))
+    _same(table, plain)
+    table.check_status()
+
+
+def test_a_plan_that_fails_changes_nothing():
+    def state(t):
+        return [x.clone() for x in (t.blocks, t.lengths, t.starts, t.free, t.n_free)]
+
+    table = PageTable(3, 4, 192)
+    table.plan([64, 1, 0], 64)
+    before = state(table)
+    for counts, q_len, code in (([1, 64, 65], 65, 111), ([129, 0, 0], 129, 112), ([2, 0, 0], 1, 112), ([-1, 0, 0], 1, 112)):
+        slots = table.plan(counts, q_len)
+        assert bool((slots == -1).all())
+        for a, b in zip(state(table), before):
+            assert torch.equal(a, b)
+        with pytest.raises(_lib.DimmerKVError) as e:
+            table.check_status()
+        assert str(9000 + code) in str(e.value)
+        # inert until it is reset
+        assert bool((table.plan([1, 1, 1], 1) == -1).all()) and torch.equal(table.lengths, before[1])
+        assert bool((table.slots(8) == -1).all())
+        table.reset_status()
+    table.trim([0, -1, 0])
+    with pytest.raises(_lib.DimmerKVError):
+        table.check_status()
+    table.reset_status()
+    for a, b in zip(state(table), before):
+        assert torch.equal(a, b)
+    table.plan([0, 63, 128], 128)  # exactly the pages that are left
+    table.check_status()
+    assert int(table.n_free) == 0
+
+
+def test_tables_refuse_wrong_counts():
+    table = PageTable(2, 4, 64)
+    for counts in ([1], torch.ones(2, dtype=torch.int64, device=DEV), torch.ones(2, dtype=torch.int32),
+                   torch.ones(3, dtype=torch.int32, device=DEV)):
+        with pytest.raises(ValueError):
+            table.plan(counts, 1)
+    with pytest.raises(ValueError):
+        table.plan(None, -1)
+    with pytest.raises(ValueError):
+        table.slots(65)
+
+
+# ------------------------------------------------------------------------------------------------ cells
+def _rows(n, heads, tokens, dim, dtype, seed, kind="value"):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(n, tokens, heads, dim, generator=g, device=DEV)
+    if kind == "key":
+        c = torch.arange(dim, device=DEV)
+        x = x * (0.6 + 2.0 * (c % 29 == 3)) + torch.sin(c * 1.7) * 1.5
+    return x.to(dtype).transpose(1, 2)  # the strides that a projection leaves
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,heads,n,q_len", [(64, 2, 1, 1), (128, 8, 3, 67), (64, 3, 5, 130), (128, 1, 2, 64)])
+def test_cells_hold_what_the_definition_says(dim, heads, n, q_len, dtype):
+    batch = Q4Batch(n, layers=2, kv_heads=heads, q_heads=heads, head_dim=dim, max_tokens=q_len + 9, dtype=dtype)
+    batch.plan([7] + [5] * (n - 1), 9)  # the rows below start inside a page
+    k0, v0 = (_rows(n, heads, 9, dim, dtype, s) for s in (8, 9))
+    for layer in range(2):
+        batch.append(layer, k0, v0)
+    counts = [max(0, q_len - 3 * s) for s in range(n)]
+    first = batch._slots
+    batch.plan(counts, q_len)
+    k, v = _rows(n, heads, q_len, dim, dtype, 1, "key"), _rows(n, heads, q_len, dim, dtype, 2)
+    k[:, 0, 0, :4] = 0.0
+    v[0, 0, 0] = -3.0                                # constant groups
+    k[0, 0, 0, 0], k[0, 0, 0, 1] = 32768.0, -32768.0  # the largest that a cell holds
+    pad = torch.arange(q_len, device=DEV) >= torch.tensor(counts, device=DEV)[:, None]
+    k.masked_fill_(pad[:, None, :, None], float("nan"))  # behind the counts: never read
+    v.masked_fill_(pad[:, None, :, None], float("inf"))
+    batch.append(1, k, v)
+    got = batch.read(1)
+    for x, y in zip((k, v), got):
+        # The float32 value is the exact one to 2^-24, and rounds to the 16-bit neighbour of it: equal, or one
+        # 16-bit step apart where the exact value lies within that of a border.
+        want = torch.where(pad[:, None, :, None], 0.0, torch.nan_to_num(cells64(x)[0], nan=0.0))
+        assert bool(((y.double() - want).abs() <= want.abs() * (torch.finfo(dtype).eps / 2 + 2**-23) + 1e-7).all())
+        codes = quantise4(torch.where(pad[:, None, :, None], 0.0, x.float()))
+        assert torch.equal(y, torch.where(pad[:, None, :, None], 0.0, dequantise4(*codes)).to(dtype))
+    # what was there stays, in this layer and in the other
+    for layer in range(2):
+        a, b = batch.read(layer, first)
+        for x, y in zip((k0, v0), (a, b)):
+            for s, c in enumerate([7] + [5] * (n - 1)):
+                assert torch.equal(y[s, :, :c], dequantise4(*quantise4(x[s, :, :c])).to(dtype))
+                assert not y[s, :, c:].any()
+    batch.check_status()
+
+
+def test_codes_at_the_borders_between_two():
+    """x exactly half way between two codes goes to the even one, one 16-bit step beside it to its own side."""
+    dim = 64
+    x = torch.zeros(1, 1, 3, dim, dtype=torch.float16, device=DEV)
+    half = (torch.arange(15, device=DEV) + 0.5).half()
+    x[..., 15] = 15.0                                   # scale 1, low 0
+    x[0, 0, 0, 16:31] = half
+    x[0, 0, 1, 16:31] = torch.nextafter(half, torch.full_like(half, 100))
+    x[0, 0, 2, 16:31] = torch.nextafter(half, torch.zeros_like(half))
+    batch = Q4Batch(1, layers=1, kv_heads=1, q_heads=1, head_dim=dim, max_tokens=3, dtype=torch.float16)
+    batch.plan(None, 3)
+    batch.append(0, x, x)
+    k, v = batch.read(0)
+    assert torch.equal(k, v) and torch.equal(k.double(), cells64(x)[0])
+    assert k[0, 0, 0, 16:31].tolist() == [0, 2, 2, 4, 4, 6, 6, 8, 8, 10, 10, 12, 12, 14, 14]
+    assert k[0, 0, 1, 16:31].tolist() == list(range(1, 16)) and k[0, 0, 2, 16:31].tolist() == list(range(15))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf"), 40000.0])
+def test_values_without_a_cell_are_told(bad):
+    batch = Q4Batch(1, layers=1, kv_heads=2, q_heads=2, head_dim=64, max_tokens=64)
+    batch.plan(None, 2)
+    k = torch.ones(1, 2, 2, 64, dtype=torch.bfloat16, device=DEV)
+    v = k.clone()
+    v[0, 1, 1, 63] = bad
+    batch.append(0, k, v)
+    with pytest.raises(_lib.DimmerKVError, match="8113"):
+        batch.check_status()
+    assert not any(x.any() for x in batch.read(0))  # inert
+    batch.reset_status()
+    batch.append(0, k, k)
+    batch.check_status()
+
+
+def test_batch_refuses_wrong_tensors():
+    batch = Q4Batch(2, layers=1, kv_heads=2, q_heads=4, head_dim=64, max_tokens=64)
+    k = torch.zeros(2, 2, 1, 64, dtype=torch.bfloat16, device=DEV)
+    q = torch.zeros(2, 4, 1, 64, dtype=torch.bfloat16, device=DEV)
+    for call in (lambda: batch.append(0, k, k), lambda: batch.read(0), lambda: batch.attend_layer(0, q, k, k, 1.0)):
+        with pytest.raises(RuntimeError):
+            call()
+    batch.plan()
+    for call in (lambda: batch.append(1, k, k), lambda: batch.append(0, k[:, :1], k), lambda: batch.append(0, k.cpu(), k),
+                 lambda: batch.attend_layer(0, q[:, :3], k, k, 1.0), lambda: batch.attend_layer(0, q, k, None, 1.0),
+                 lambda: batch.attend_layer(0, q, k, k, 1.0, out_dtype=torch.float16),
+                 lambda: batch.read(0, torch.zeros(2, 3, device=DEV)),
+                 lambda: batch.read(0, torch.zeros(3, 3, dtype=torch.int32, device=DEV))):
+        with pytest.raises(ValueError):
+            call()
+
+
+# ------------------------------------------------------------------------------------------------ attention
+def _filled(n, q_heads, kv_heads, dim, dtype, held, counts, q_len, seed=0, chunk=1000):
+    """A batch that holds ``held`` tokens and has ``counts`` more planned, with every key and value of it."""
+    total = max(h + c for h, c in zip(held, counts))
+    batch = Q4Batch(n, layers=1, kv_heads=kv_heads, q_heads=q_heads, head_dim=dim, max_tokens=max(1, total) + 70, dtype=dtype)
+    batch.cells.fill_(0xff)  # NaN headers wherever nothing was stored
+    keys, values = _rows(n, kv_heads, total, dim, dtype, seed, "key"), _rows(n, kv_heads, total, dim, dtype, seed + 1)
+    for first in range(0, max(held), chunk):
+        part = [min(chunk, max(0, h - first)) for h in held]
+        size = max(part)
+        batch.plan(part, size)
+        batch.append(0, keys[:, :, first:first + size], values[:, :, first:first + size])
+    batch.plan(counts, q_len)
+    query = _rows(n, q_heads, q_len, dim, dtype, seed + 2)
+    new = [torch.zeros(n, kv_heads, q_len, dim, dtype=dtype, device=DEV) for _ in range(2)]
+    for s in range(n):
+        for x, y in zip(new, (keys, values)):
+            x[s, :, :counts[s]] = y[s, :, held[s]:held[s] + counts[s]]
+    return batch, query, new[0], new[1], keys, values
+
+
+def _check(out, query, keys, values, held, counts, scaling, eps):
+    for s, (h, c) in enumerate(zip(held, counts)):
+        assert not out[s, c:].any()
+        if c:
+            want, weight, terms = attend64(query[s, :, :c], keys[s, :, :h + c], values[s, :, :h + c], h, scaling)
+            err = (out[s, :c].double() - want).abs() - attend_tolerance(want, weight, terms, eps)
+            assert float(err.max()) <= 0, (s, float(err.max()))
+
+
+CASES = [
+    # q_heads, kv_heads, dim, held, counts, q_len
+    (4, 1, 64, [0], [1], 1),
+    (24, 8, 128, [1], [1], 1),
+    (24, 8, 128, [63, 64, 65, 0, 200], [1, 1, 1, 0, 1], 1),
+    (32, 8, 64, [127, 16, 1000], [1, 1, 1], 1),
+    (32, 8, 64, [700, 0, 5, 63], [3, 5, 0, 2], 5),
+    (24, 8, 128, [129, 300], [4, 1], 4),
+    (8, 8, 128, [500], [1], 1),
+    (7, 1, 64, [333], [2], 2),
+    (40, 2, 128, [80, 64], [1, 1], 1),
+    (24, 8, 128, [1000, 0, 77], [37, 40, 0], 40),
+    (32, 8, 64, [130, 513], [100, 33], 100),
+    (6, 2, 128, [4000], [200], 200),
+    (32, 8, 64, [20000], [1], 1),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", CASES, ids=[f"{c[0]}x{c[1]}x{c[2]}-{max(c[3])}+{c[5]}" for c in CASES])
+def test_attention_over_cells(case, dtype):
+    q_heads, kv_heads, dim, held, counts, q_len = case
+    batch, query, k, v, keys, values = _filled(len(held), q_heads, kv_heads, dim, dtype, held, counts, q_len)
+    scaling = dim ** -0.5
+    out = batch.attend_layer(0, query, k, v, scaling)
+    _check(out, query, keys, values, held, counts, scaling, torch.finfo(dtype).eps)
+    out32 = batch.attend_layer(0, query, None, None, scaling, out_dtype=torch.float32)
+    _check(out32, query, keys, values, held, counts, scaling, torch.finfo(torch.float32).eps)
+    assert torch.equal(out32.to(dtype), out)
+    batch.check_status()
+
+
+def test_attention_of_peaked_and_flat_rows():
+    """Scores far apart (one token takes all), equal ones, ones that grow along the context (the running maximum moves
+    page after page), and queries of very small and very large size."""
+    held, n, dim = [3000, 3000, 3000, 3000], 4, 128
+    batch, query, k, v, keys, values = _filled(n, 24, 8, dim, torch.bfloat16, held, [1] * n, 1, seed=5)
+    query[0] *= 30
+    query[1] *= 0
+    query[2] *= 2.0**-100
+    query[3] *= 8
+    out = batch.attend_layer(0, query, k, v, dim ** -0.5, out_dtype=torch.float32)
+    _check(out, query, keys, values, held, [1] * n, dim ** -0.5, torch.finfo(torch.float32).eps)
+    ramp = torch.linspace(-4, 4, 3001, device=DEV)[:, None] * torch.ones(dim, device=DEV)
+    batch, query, k, v, keys, values = _filled(n, 24, 8, dim, torch.bfloat16, held, [1] * n, 1, seed=6)
+    batch.trim([0] * n)
+    keys = (ramp + 0.1 * keys.float()).to(torch.bfloat16)
+    query = query.abs()
+    batch.plan(None, 3001)
+    batch.append(0, keys, values)
+    batch.trim([3000] * n)
+    batch.plan()
+    out = batch.attend_layer(0, query, keys[:, :, -1:], values[:, :, -1:], dim ** -0.5, out_dtype=torch.float32)
+    _check(out, query, keys, values, held, [1] * n, dim ** -0.5, torch.finfo(torch.float32).eps)
+    batch.check_status()
+
+
+def test_a_query_that_is_not_finite_stays_in_its_row():
+    held, counts = [300, 90], [3, 3]
+    batch, query, k, v, keys, values = _filled(2, 8, 2, 64, torch.float16, held, counts, 3, seed=9)
+    query[0, 5, 1, 7] = float("nan")
+    out = batch.attend_layer(0, query, k, v, 0.125)
+    assert bool(out[0, 1, 5].isnan().all())
+    out[0, 1, 5] = 0
+    assert bool(torch.isfinite(out).all())
+    query[0, 5, 1] = 0
+    want = batch.attend_layer(0, query, None, None, 0.125)
+    want[0, 1, 5] = 0
+    assert torch.equal(out, want)
+
+
+def test_strides_offsets_streams_and_graphs():
+    """Tensors at other strides and odd offsets, a step captured and replayed (the tables advance on the device),
+    and two conversations' pages shared out again."""
+    n, q_heads, kv_heads, dim = 3, 24, 8, 128
+    held = [70, 1, 130]
+    batch, query, k, v, keys, values = _filled(n, q_heads, kv_heads, dim, torch.bfloat16, held, [1] * n, 1, seed=11)
+    want = batch.attend_layer(0, query, k, v, 0.1)
+    flat = torch.zeros(query.numel() + 3, dtype=query.dtype, device=DEV)
+    odd = flat[3:].view(n, q_heads, 1, dim)
+    odd.copy_(query)
+    assert torch.equal(batch.attend_layer(0, odd, k.contiguous(), v.expand(n, kv_heads, 1, dim), 0.1), want)
+    wide = torch.zeros(n, kv_heads, 1, dim + 4, dtype=k.dtype, device=DEV)
+    wide[..., :dim] = k
+    assert torch.equal(batch.attend_layer(0, query, wide[..., :dim], v, 0.1), want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = batch.attend_layer(0, query, k, v, 0.1)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, want)
+
+    # three steps one by one, and the same three as replays of one captured step
+    steps = [(_rows(n, q_heads, 1, dim, torch.bfloat16, 50 + i), _rows(n, kv_heads, 1, dim, torch.bfloat16, 60 + i),
+              _rows(n, kv_heads, 1, dim, torch.bfloat16, 70 + i)) for i in range(3)]
+    mark = batch.lengths.clone()
+    eager = []
+    for q, a, b in steps:
+        batch.plan()
+        eager.append(batch.attend_layer(0, q, a, b, 0.1))
+    batch.trim(mark)
+    static = [x.clone() for x in steps[0]]
+    batch.plan()
+    batch.attend_layer(0, *static, 0.1)
+    batch.trim(mark)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        batch.plan()
+        held_out = batch.attend_layer(0, *static, 0.1)
+    for (q, a, b), e in zip(steps, eager):
+        for x, y in zip(static, (q, a, b)):
+            x.copy_(y)
+        graph.replay()
+        assert torch.equal(held_out, e)
+    assert torch.equal(batch.lengths, mark + 3)
+    # a finished conversation's pages serve another
+    batch.trim([0, 4, 133])
+    batch.plan([0, 130, 0], 130)
+    fresh = [_rows(n, kv_heads, 130, dim, torch.bfloat16, 80 + i) for i in range(2)]
+    batch.append(0, *fresh)
+    got = batch.read(0)
+    for x, y in zip(fresh, got):
+        assert torch.equal(y[1], dequantise4(*quantise4(x[1])).to(x.dtype))
+    batch.check_status()
+
+
+def test_far_pages_of_a_large_pool():
+    """Cells beyond 2^32 bytes: the pages of one conversation lie at the end of a pool of 5 GB."""
+    dim, kv = 128, 8
+    pages = 70000
+    batch = Q4Batch(1, layers=1, kv_heads=kv, q_heads=24, head_dim=dim, max_tokens=200, n_pages=pages)
+    assert batch.cells.numel() > 2**32
+    batch.table.free.copy_(torch.arange(pages, dtype=torch.int32, device=DEV))  # the last page first
+    k, v, q = _rows(1, kv, 130, dim, torch.bfloat16, 1, "key"), _rows(1, kv, 130, dim, torch.bfloat16, 2), _rows(1, 24, 130, dim, torch.bfloat16, 3)
+    batch.plan(None, 130)
+    out = batch.attend_layer(0, q, k, v, 0.09)
+    assert batch.table.blocks[0, :3].tolist() == [pages - 1, pages - 2, pages - 3]
+    _check(out, q, k, v, [0], [130], 0.09, torch.finfo(torch.bfloat16).eps)
+    a, b = batch.read(0)
+    assert torch.equal(a, dequantise4(*quantise4(k)).to(k.dtype)) and torch.equal(b, dequantise4(*quantise4(v)).to(v.dtype))
+    batch.check_status()
+
+
+# ------------------------------------------------------------------------------------------------ a model over it
+class _Plain:
+    """Q4Batch.attend in plain operations of float32 over the dequantised tokens, row by row."""
+
+    def __init__(self, n, batch):
+        self.n, self.device, self.status, self.poll_wait_s = n, DEV, torch.zeros(1, dtype=torch.int32, device=DEV), 60.0
+        self.keys, self.values = [{} for _ in range(n)], [{} for _ in range(n)]
+
+    def poll_status(self, depth=None):
+        torch.cuda.synchronize()
+
+    def attend(self, module, query, key, value, attention_mask, scaling):
+        outs = []
+        for s in range(self.n):
+            for store, x in ((self.keys[s], key[s]), (self.values[s], value[s])):
+                x = dequantise4(*quantise4(x))
+                store[module.layer_idx] = x if module.layer_idx not in store else torch.cat([store[module.layer_idx], x], 1)
+            k, v = self.keys[s][module.layer_idx], self.values[s][module.layer_idx]
+            share = query.shape[1] // k.shape[0]
+            q_len, held = query.shape[2], k.shape[1] - query.shape[2]
+            scores = query[s].float() @ k.repeat_interleave(share, 0).transpose(1, 2) * scaling
+            hidden = torch.arange(k.shape[1], device=DEV) > held + torch.arange(q_len, device=DEV)[:, None]
+            p = torch.softmax(scores.masked_fill(hidden, float("-inf")), -1)
+            outs.append((p @ v.repeat_interleave(share, 0)).transpose(0, 1))
+        return torch.stack(outs).to(query.dtype), None
+
+
+class _Tokens:
+    eos_token_id, all_special_ids = -1, []
+
+    def decode(self, ids, skip_special_tokens=True):
+        return " ".join(map(str, ids))
+
+
+def test_a_model_decodes_over_cells():
+    """Prefill, question and greedy decode of the tiny model through the hook: kernels against plain operations. The
+    model runs in float32 with a bf16 cache, so both round queries, keys and values alike; attention outputs differ
+    by 2^-11 of their weights at most (attend_tolerance with float32 outputs), and the model is two layers deep."""
+    model = tm.build_model(torch.float32, DEV)
+    dimmer.install(model)
+    ids = tm.context_ids().to(DEV)[:, :300]
+
+    def run(context):
+        dimmer.STATE.compressed = context
+        try:
+            with torch.inference_mode():
+                outs, cache = [], Q4Batch(1, layers=2, kv_heads=8, q_heads=32, head_dim=64, max_tokens=8).cache
+                for first, end in ((0, 129), (129, 300), (300, 301)):
+                    x = ids[:, first:end] if first < 300 else ids[:, :1]
+                    pos = torch.arange(first, end, device=DEV)[None]
+                    outs.append(model(input_ids=x, past_key_values=cache, position_ids=pos, use_cache=True).logits)
+        finally:
+            dimmer.STATE.compressed = None
+        return outs
+
+    batch = Q4Batch(1, layers=2, kv_heads=8, q_heads=32, head_dim=64, max_tokens=400)
+
+    class Rounded(_Plain):
+        def attend(self, module, query, key, value, attention_mask, scaling):
+            b = torch.bfloat16
+            out, _ = super().attend(module, query.to(b).float(), key.to(b), value.to(b), attention_mask, scaling)
+            return out, None
+
+    got, want = run(batch), run(Rounded(1, None))
+    batch.check_status()
+    assert batch.lengths.tolist() == [301]
+    for a, b in zip(got, want):
+        # 2^-11 of the attention's weights twice, times the model's gain: logits are of order 1 here
+        assert float((a - b).abs().max()) < 2e-3
+
+
+def test_answers_with_rules_over_a_context():
+    """Q4Context and greedy_answer with penalties and a grammar: the answer holds no token twice, and only allowed
+    ones; the first logits are the plain cache's within 4 bits of noise."""
+    model = tm.build_model(torch.bfloat16, DEV)
+    dimmer.install(model)
+    ids = tm.context_ids().to(DEV)[:, :200]
+    with torch.inference_mode():
+        cache, _ = dimmer.prefill_with_scores(model, ids)
+        keys, values = [l.keys for l in cache.layers], [l.values for l in cache.layers]
+        context = Q4Context(keys, values, model, dtype=torch.bfloat16)
+        assert context.code_bytes() == 200 * 2 * 8 * 2 * 36
+        question = tm.question_ids().to(DEV)[None]
+        text, first = greedy_answer(model, _Tokens(), context, context.exact_cache, question, 200)
+        again = Q4Context(keys, values, model, dtype=torch.bfloat16)
+        rules = LogitRules(1, 1024, capacity=32, presence=1000.0)
+        allowed = allow_mask([list(range(0, 1024, 3))], 1024)
+        even = lambda last: allowed
+        text2, first2 = greedy_answer(model, _Tokens(), again, again.exact_cache, question, 200, rules=rules, grammar=even)
+    assert torch.equal(first, first2)
+    tokens = [int(t) for t in text2.split()]
+    assert len(tokens) == 12 == len(set(tokens)) and all(t % 3 == 0 for t in tokens)
+    assert rules.lengths.tolist() == [12] and rules.history[0, :12].tolist() == tokens
+    assert tokens[0] == int(torch.where(torch.arange(1024, device=DEV) % 3 == 0, first, float("-inf")).argmax())
+    context.batch.check_status()
+    again.batch.check_status()
+
+
+def test_batch_decodes_with_rules():
+    """greedy_decode_batch over a Q4Batch: ragged conversations, each as if it were alone."""
+    model = tm.build_model(torch.bfloat16, DEV)
+    dimmer.install(model)
+    ids = tm.context_ids().to(DEV)
+    lengths = [150, 64, 33]
+    with torch.inference_mode():
+        def context(rows):
+            n = len(rows)
+            batch = Q4Batch(n, layers=2, kv_heads=8, q_heads=32, head_dim=64, max_tokens=300)
+            longest = max(lengths[r] for r in rows)
+            x = torch.zeros(n, longest, dtype=torch.int64, device=DEV)
+            for i, r in enumerate(rows):
+                x[i, :lengths[r]] = ids[0, r * 150:r * 150 + lengths[r]]
+            batch.begin([lengths[r] for r in rows])
+            dimmer.STATE.compressed = batch
+            try:
+                model(input_ids=x, past_key_values=batch.cache, position_ids=torch.arange(longest, device=DEV)[None].expand(n, -1),
+                      use_cache=True)
+            finally:
+                dimmer.STATE.compressed = None
+            rules = LogitRules(n, 1024, capacity=64, repetition=1.3, frequency=0.2)
+            rules.load(x.to(torch.int32)[:, :33], [33] * n)
+            start = torch.tensor([[r + 1] for r in rows])
+            out, _ = greedy_decode_batch(model, batch, batch.cache, start, torch.tensor([[lengths[r]] for r in rows]), 6,
+                                         rules=rules)
+            batch.check_status()
+            rules.check_status()
+            assert rules.lengths.tolist() == [39] * n
+            return out, [x.float() for x in batch.read(1, batch.table.slots(lengths[rows[0]]))]
+
+        together, kv = context([0, 1, 2])
+        for r in range(3):
+            alone, kv1 = context([r])
+            # the same tokens unless the model's own batched products (cuBLAS) decide a near tie otherwise: the first
+            # token's cells are equal up to one code of a value that a rounding of the projection moved
+            assert float((kv[0][r, :, :1] - kv1[0][0, :, :1]).abs().max()) < 0.5
+            assert together.shape == (3, 6) and int(together.min()) >= 0
+        rules = LogitRules(1, 1024)
+        batch = Q4Batch(1, layers=2, kv_heads=8, q_heads=32, head_dim=64, max_tokens=300)
+        with pytest.raises(_lib.DimmerKVError, match="no token is allowed"):
+            greedy_decode_batch(model, batch, batch.cache, torch.tensor([[1]]), torch.tensor([[0]]), 2, rules=rules,
+                                grammar=lambda last: allow_mask([[]], 1024))
+
+
+def test_the_hook_refuses_another_cache_and_another_mask():
+    model = tm.build_model(torch.bfloat16, DEV)
+    dimmer.install(model)
+    ids = tm.context_ids().to(DEV)[:, :6].repeat(2, 1)
+    pos = torch.arange(6, device=DEV)[None].expand(2, -1)
+    batch = Q4Batch(2, layers=2, kv_heads=8, q_heads=32, head_dim=64, max_tokens=64)
+    full = torch.ones(2, 6, dtype=torch.int64, device=DEV)
+    left = full.clone()
+    left[1, :2] = 0
+    right = full.clone()
+    right[1, 4:] = 0
+    dimmer.STATE.compressed = batch
+    try:
+        with torch.inference_mode():
+            call = lambda mask: model(input_ids=ids, past_key_values=batch.cache, position_ids=pos, attention_mask=mask)
+            call(full)
+            batch.check_status()
+            batch.begin([6, 4])
+            call(right)  # padded behind the counts: what the batch is told
+            batch.check_status()
+            call(left)
+            with pytest.raises(_lib.DimmerKVError, match="115"):
+                batch.check_status()
+            batch.reset_status()
+            dyn = model(input_ids=ids[:, :2], position_ids=pos[:, :2], use_cache=True).past_key_values
+            with pytest.raises(ValueError, match="own cache"):
+                model(input_ids=ids[:, :1], past_key_values=dyn, position_ids=pos[:, 2:3])
+    finally:
+        dimmer.STATE.compressed = None
+
+
+def test_methods_q4_rebuilds_the_cells():
+    g = torch.Generator().manual_seed(5)
+    keys = [torch.randn(1, 8, 130, 64, generator=g).half() for _ in range(2)]
+    values = [torch.randn(1, 8, 130, 64, generator=g).half() for _ in range(2)]
+    host = Methods("m", "none", "none", "cpu").apply("q4", keys, values, {})
+    gpu = Methods("m", "none", "none", DEV).apply("q4", [k.to(DEV) for k in keys], [v.to(DEV) for v in values], {})
+    assert gpu.used_bytes == host.used_bytes
+    for a, b in zip(gpu.keys + gpu.values, host.keys + host.values):
+        assert torch.equal(a.cpu(), b)
