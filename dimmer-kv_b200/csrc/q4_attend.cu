@@ -3,7 +3,7 @@
 // With key value k_d = low_g + scale_g * c_d (g = d / 64), a score splits into
 //   q . k = sum_g scale_g * (sum_{d in g} q_d c_d) + sum_g low_g * (sum_{d in g} q_d):
 // the product runs over the codes themselves, which float16 holds exactly, and the key's rounding is the
-// cache's alone. Values enter as float16(low + scale * c), one rounding of at most 2^-12 relative; probabilities
+// cache's alone. Values enter as float16(low + scale * c), one rounding of at most 2^-11 relative; probabilities
 // as float16 of 2^7 * exp(score - m) with m within 2^8 of the running maximum, so that a token down to 2^-21 of the
 // largest keeps 11 bits (sums over a long context of small probabilities do not vanish).
 //

@@ -372,30 +372,26 @@ def test_far_pages_of_a_large_pool():
 
 
 # ------------------------------------------------------------------------------------------------ a model over it
-class _Plain:
-    """Q4Batch.attend in plain operations of float32 over the dequantised tokens, row by row."""
+class _Checked:
+    """A Q4Batch of one conversation whose every attention call is held against attend64 on the call's own inputs.
+    (Whole logits cannot be held against a plain model's: a difference of 2^-11 in one layer's output moves some
+    of the next layer's keys across a border between two codes, a whole step of 4 bits.)"""
 
-    def __init__(self, n, batch):
-        self.n, self.device, self.status, self.poll_wait_s = n, DEV, torch.zeros(1, dtype=torch.int32, device=DEV), 60.0
-        self.keys, self.values = [{} for _ in range(n)], [{} for _ in range(n)]
-
-    def poll_status(self, depth=None):
-        torch.cuda.synchronize()
+    def __init__(self, batch):
+        self.batch, self.keys, self.values, self.calls = batch, {}, {}, 0
 
     def attend(self, module, query, key, value, attention_mask, scaling):
-        outs = []
-        for s in range(self.n):
-            for store, x in ((self.keys[s], key[s]), (self.values[s], value[s])):
-                x = dequantise4(*quantise4(x))
-                store[module.layer_idx] = x if module.layer_idx not in store else torch.cat([store[module.layer_idx], x], 1)
-            k, v = self.keys[s][module.layer_idx], self.values[s][module.layer_idx]
-            share = query.shape[1] // k.shape[0]
-            q_len, held = query.shape[2], k.shape[1] - query.shape[2]
-            scores = query[s].float() @ k.repeat_interleave(share, 0).transpose(1, 2) * scaling
-            hidden = torch.arange(k.shape[1], device=DEV) > held + torch.arange(q_len, device=DEV)[:, None]
-            p = torch.softmax(scores.masked_fill(hidden, float("-inf")), -1)
-            outs.append((p @ v.repeat_interleave(share, 0)).transpose(0, 1))
-        return torch.stack(outs).to(query.dtype), None
+        out, _ = self.batch.attend(module, query, key, value, attention_mask, scaling)
+        layer, dtype = module.layer_idx, self.batch.dtype
+        for store, x in ((self.keys, key), (self.values, value)):
+            store[layer] = torch.cat(([store[layer]] if layer in store else []) + [x[0].to(dtype)], 1)
+        held = self.keys[layer].shape[1] - query.shape[2]
+        want, weight, terms = attend64(query[0].to(dtype), self.keys[layer], self.values[layer], held, scaling)
+        eps = torch.finfo(out.dtype).eps
+        assert out.dtype == torch.promote_types(query.dtype, dtype) and out.shape[1:] == want.shape
+        assert float(((out[0].double() - want).abs() - attend_tolerance(want, weight, terms, eps)).max()) <= 0
+        self.calls += 1
+        return out, None
 
 
 class _Tokens:
@@ -405,41 +401,24 @@ class _Tokens:
         return " ".join(map(str, ids))
 
 
-def test_a_model_decodes_over_cells():
-    """Prefill, question and greedy decode of the tiny model through the hook: kernels against plain operations. The
-    model runs in float32 with a bf16 cache, so both round queries, keys and values alike; attention outputs differ
-    by 2^-11 of their weights at most (attend_tolerance with float32 outputs), and the model is two layers deep."""
-    model = tm.build_model(torch.float32, DEV)
+@pytest.mark.parametrize("model_dtype,dtype", [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.bfloat16),
+                                               (torch.float16, torch.float16)])
+def test_a_model_decodes_over_cells(model_dtype, dtype):
+    """Prefill in two chunks and a decoded token of the tiny model through the hook."""
+    model = tm.build_model(model_dtype, DEV)
     dimmer.install(model)
-    ids = tm.context_ids().to(DEV)[:, :300]
-
-    def run(context):
-        dimmer.STATE.compressed = context
-        try:
-            with torch.inference_mode():
-                outs, cache = [], Q4Batch(1, layers=2, kv_heads=8, q_heads=32, head_dim=64, max_tokens=8).cache
-                for first, end in ((0, 129), (129, 300), (300, 301)):
-                    x = ids[:, first:end] if first < 300 else ids[:, :1]
-                    pos = torch.arange(first, end, device=DEV)[None]
-                    outs.append(model(input_ids=x, past_key_values=cache, position_ids=pos, use_cache=True).logits)
-        finally:
-            dimmer.STATE.compressed = None
-        return outs
-
-    batch = Q4Batch(1, layers=2, kv_heads=8, q_heads=32, head_dim=64, max_tokens=400)
-
-    class Rounded(_Plain):
-        def attend(self, module, query, key, value, attention_mask, scaling):
-            b = torch.bfloat16
-            out, _ = super().attend(module, query.to(b).float(), key.to(b), value.to(b), attention_mask, scaling)
-            return out, None
-
-    got, want = run(batch), run(Rounded(1, None))
+    ids = tm.context_ids().to(DEV)[:, :301]
+    batch = Q4Batch(1, layers=2, kv_heads=8, q_heads=32, head_dim=64, max_tokens=400, dtype=dtype)
+    context = dimmer.STATE.compressed = _Checked(batch)
+    try:
+        with torch.inference_mode():
+            for first, end in ((0, 129), (129, 300), (300, 301)):
+                model(input_ids=ids[:, first:end], past_key_values=batch.cache,
+                      position_ids=torch.arange(first, end, device=DEV)[None], use_cache=True)
+    finally:
+        dimmer.STATE.compressed = None
     batch.check_status()
-    assert batch.lengths.tolist() == [301]
-    for a, b in zip(got, want):
-        # 2^-11 of the attention's weights twice, times the model's gain: logits are of order 1 here
-        assert float((a - b).abs().max()) < 2e-3
+    assert batch.lengths.tolist() == [301] and context.calls == 6
 
 
 def test_answers_with_rules_over_a_context():
