@@ -1,13 +1,7 @@
 // q4_rows.cu — keys and values into the cells of the paged 4-bit cache, and back (dkv_q4_append, dkv_q4_read).
 //
-// Eight lanes hold a group of 64 dimensions, eight dimensions each (one 16-byte load): the group's minimum and
-// maximum are three shuffles, and a lane's eight key codes are exactly one word of the key cell, its value codes
-// the halves of two words of the pair's. Memory bound: 2 bytes read and 0.56 written per element.
-//
-// The code is the nearest whole number to the true quotient (x - low) / scale, not to its float32 rounding: the
-// float32 quotient, off by less than 2^-18, decides unless it lies within 2^-16 of a half; then the border
-// low + (c + 1/2) * scale, which float64 holds exactly (two float16 numbers, exponents -25 .. 15, and 5 bits),
-// is compared with x. So the codes do not depend on how a device rounds a division.
+// A lane takes eight dimensions of a token (one 16-byte load or store; q4_cells.cuh quantises). Memory bound: 2
+// bytes read and 0.56 written per element, and the reverse.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -21,33 +15,10 @@ namespace {
 using q4::Cells;
 constexpr int kRowThreads = 256;
 
-template <bool F16>
-__device__ __forceinline__ float from16(uint16_t v) {
-  return F16 ? __half2float(__ushort_as_half(v)) : __bfloat162float(__ushort_as_bfloat16(v));
-}
-template <bool F16>
-__device__ __forceinline__ uint16_t to16(float v) {
-  return F16 ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
-}
-
-// Nearest whole number of 0..15 to (x - low) / scale, ties to even; inv = 1 / scale to float32 accuracy.
-__device__ __forceinline__ uint32_t code_of(float x, float low, float scale, float inv) {
-  const float q = __fmul_rn(__fsub_rn(x, low), inv);
-  float c = rintf(q);
-  const float below = floorf(q);
-  if (fabsf(q - below - 0.5f) < 0x1p-16f && q > -1.f && q < 16.f) {
-    const double border = static_cast<double>(low) + (static_cast<double>(below) + 0.5) * static_cast<double>(scale);
-    const double xd = static_cast<double>(x);
-    const bool up = xd > border || (xd == border && (static_cast<int>(below) & 1));
-    c = up ? below + 1.f : below;
-  }
-  return static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f));
-}
-
 // One lane: 8 dimensions (the j-th eight of its row) of one token's keys (z = 0) or values (z = 1).
 template <int D, bool F16>
 __global__ void __launch_bounds__(kRowThreads) q4_append_kernel(const dkv_q4_rows_args a) {
-  if (status_at_entry(a.status) != 0) return;
+  if (__any_sync(0xffffffffu, status_at_entry(a.status) != 0)) return;  // one answer for the warp's shuffles
   constexpr int kLanes = D / 8;  // lanes of a row
   using C = Cells<D>;
   const int64_t rows = static_cast<int64_t>(a.n_seq) * a.q_len * a.n_kv_heads;
@@ -71,51 +42,12 @@ __global__ void __launch_bounds__(kRowThreads) q4_append_kernel(const dkv_q4_row
   }
   uint4 raw = make_uint4(0u, 0u, 0u, 0u);
   if (slot >= 0) raw = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(is_value ? a.value : a.key) + src);
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  float x[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = from16<F16>(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1))));
-  float lo = x[0], hi = x[0];
-  bool fits = true;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    lo = fminf(lo, x[e]);
-    hi = fmaxf(hi, x[e]);
-    fits = fits && fabsf(x[e]) <= q4::kCellMax;  // false for a NaN
-  }
-#pragma unroll
-  for (int d = 1; d < 8; d <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
-  }
-  if (!fits) record_error(a.status, kSiteQ4Rows + kErrCellRange);
+  const q4::Cell8 c = q4::quantise8<F16>(raw);
+  if (!c.fits) record_error(a.status, kSiteQ4Rows + kErrCellRange);
   if (slot < 0) return;
-  const __half low_h = __float2half_rn(lo);
-  const float low = __half2float(low_h);
-  const __half scale_h = __float2half_rn(__fdiv_rn(__fsub_rn(hi, low), 15.f));
-  const float scale = __half2float(scale_h);
-  const float inv = scale > 0.f ? __fdiv_rn(1.f, scale) : 0.f;
-  uint32_t codes = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) codes |= code_of(x[e], low, scale, inv) << (4 * e);
-  if (!(scale > 0.f)) codes = 0;
   uint8_t* page = a.cells + (static_cast<int64_t>(slot / q4::kPage) * a.n_kv_heads + head) * C::kBytes;
-  const int r = slot % q4::kPage;
-  if (!is_value) {
-    *reinterpret_cast<uint32_t*>(page + C::key_word(r, j)) = codes;
-    if (j % 8 == 0)
-      *reinterpret_cast<uint32_t*>(page + C::key_head(r, j / 8)) =
-          static_cast<uint32_t>(__half_as_ushort(scale_h)) | static_cast<uint32_t>(__half_as_ushort(low_h)) << 16;
-  } else {
-    const int pair = r >> 1, odd = r & 1;
-    *reinterpret_cast<uint16_t*>(page + C::value_word(pair, 2 * j) + 2 * odd) = static_cast<uint16_t>(codes);
-    *reinterpret_cast<uint16_t*>(page + C::value_word(pair, 2 * j + 1) + 2 * odd) = static_cast<uint16_t>(codes >> 16);
-    if (j % 8 == 0) {
-      uint8_t* h = page + C::value_head(pair, j / 8) + 2 * odd;
-      *reinterpret_cast<uint16_t*>(h) = __half_as_ushort(scale_h);
-      *reinterpret_cast<uint16_t*>(h + 4) = __half_as_ushort(low_h);
-    }
-  }
+  if (is_value) q4::store_value8<D>(page, slot % q4::kPage, j, c);
+  else q4::store_key8<D>(page, slot % q4::kPage, j, c);
 }
 
 template <int D, bool F16>
@@ -163,7 +95,7 @@ __global__ void __launch_bounds__(kRowThreads) q4_read_kernel(const dkv_q4_rows_
     for (int e = 0; e < 8; ++e) {
       // code * scale is exact in float32 (4 and 11 bits): one rounding to float32, one to 16 bits
       const float v = __fmaf_rn(static_cast<float>((codes >> (4 * e)) & 15u), scale, low);
-      out[e >> 1] |= static_cast<uint32_t>(to16<F16>(v)) << (16 * (e & 1));
+      out[e >> 1] |= static_cast<uint32_t>(q4::to16<F16>(v)) << (16 * (e & 1));
     }
   }
   *reinterpret_cast<uint4*>(dst) = make_uint4(out[0], out[1], out[2], out[3]);

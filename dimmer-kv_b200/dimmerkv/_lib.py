@@ -29,7 +29,7 @@ EXPORTS = ("dkv_attend_layer", "dkv_key_scores", "dkv_softmax_stats", "dkv_value
            "dkv_unpack", "dkv_importance", "dkv_topk", "dkv_refine_merge", "dkv_attend_layer_static",
            "dkv_vpart_floats", "dkv_encode_groups", "dkv_storage_unpack", "dkv_demote", "dkv_alloc_workspace_bytes", "dkv_allocate_rungs",
            "dkv_q4_page_bytes", "dkv_page_plan", "dkv_page_trim", "dkv_page_slots", "dkv_q4_append", "dkv_q4_read",
-           "dkv_q4_attend", "dkv_logit_rules",
+           "dkv_q4_attend", "dkv_q4_attend_floats", "dkv_logit_rules",
            "dkv_version", "dkv_status_string")
 
 
@@ -177,7 +177,9 @@ class Q4AttendArgs(ctypes.Structure):
         ("cells", c_void_p), ("n_pages", c_int32), ("n_kv_heads", c_int32), ("n_q_heads", c_int32),
         ("head_dim", c_int32), ("fp16", c_int32), ("blocks", c_void_p), ("max_blocks", c_int32), ("lengths", c_void_p),
         ("starts", c_void_p), ("n_seq", c_int32), ("q_len", c_int32), ("len_bound", c_int32), ("query", c_void_p),
-        ("q_stride", c_int64 * 3), ("scaling", c_float), ("out", c_void_p), ("out_f32", c_int32), ("status", c_void_p),
+        ("q_stride", c_int64 * 3), ("key", c_void_p), ("value", c_void_p), ("k_stride", c_int64 * 3),
+        ("v_stride", c_int64 * 3), ("slots", c_void_p), ("scaling", c_float), ("out", c_void_p), ("out_f32", c_int32),
+        ("workspace", c_void_p), ("workspace_floats", c_int64), ("status", c_void_p),
     ]
 
 
@@ -228,6 +230,8 @@ def lib():
             fn.restype = c_int32
         handle.dkv_alloc_workspace_bytes.argtypes = [c_int64, c_int32]
         handle.dkv_alloc_workspace_bytes.restype = c_int64
+        handle.dkv_q4_attend_floats.argtypes = [ctypes.POINTER(Q4AttendArgs)]
+        handle.dkv_q4_attend_floats.restype = c_int64
         handle.dkv_q4_page_bytes.argtypes = [c_int32]
         handle.dkv_q4_page_bytes.restype = c_int64
         handle.dkv_vpart_floats.argtypes = [c_int32, c_int32, c_int32, c_int32]

@@ -91,6 +91,7 @@ class Q4Batch:
         a.fp16, a.blocks, a.max_blocks = r.fp16, self.table.blocks.data_ptr(), self.table.max_blocks
         a.lengths, a.starts, a.n_seq = self.table.lengths.data_ptr(), self.table.starts.data_ptr(), n_seq
         a.status = self.status.data_ptr()
+        self._floats: dict[int, int] = {}  # workspace of dkv_q4_attend by q_len
         self._layer_bytes = self.cells[0].numel()
         self._cells_ptr = self.cells.data_ptr()
 
@@ -185,13 +186,21 @@ class Q4Batch:
             raise RuntimeError("attend_layer needs a plan")
         q_len = self._slots.shape[1]
         query = self._tensor("query", query, self.q_heads, q_len)
-        if key is not None:
-            self.append(layer, key, value)
         out = torch.empty(self.n_seq, q_len, self.q_heads, self.head_dim, dtype=out_dtype, device=self.device)
         a = _lib.Q4AttendArgs.from_buffer_copy(self._attend)
         a.cells, a.q_len, a.len_bound = self._layer(layer), q_len, self.table.bound
         a.query, a.q_stride, a.scaling = query.data_ptr(), self._strides(query), float(scaling)
+        if key is not None:
+            key = self._tensor("key", key, self.kv_heads, q_len)
+            value = self._tensor("value", value, self.kv_heads, q_len)
+            a.key, a.value, a.slots = key.data_ptr(), value.data_ptr(), self._slots.data_ptr()
+            a.k_stride, a.v_stride = self._strides(key), self._strides(value)
         a.out, a.out_f32 = out.data_ptr(), int(out_dtype == torch.float32)
+        floats = self._floats.get(q_len)
+        if floats is None:
+            floats = self._floats[q_len] = int(self.lib.dkv_q4_attend_floats(a))
+        workspace = torch.empty(floats, dtype=torch.float32, device=self.device)
+        a.workspace, a.workspace_floats = workspace.data_ptr(), floats
         _lib.launch("dkv_q4_attend", a, self.device)
         return out
 

@@ -444,12 +444,13 @@ int dkv_q4_read(const dkv_q4_rows_args* args, void* stream);
 
 /* Causal attention of the newest tokens' queries over the 4-bit cells: query row i of conversation s sees the
  * tokens 0 .. starts[s] + i. Rows behind the last new token (i >= lengths[s] - starts[s]) come back as
- * zeros. Scores, softmax statistics and sums are float32; probabilities enter the value product as float16
- * against the values rounded to float16. */
+ * zeros. With `key` and `value` (as in dkv_q4_append, slots of the newest plan) the new tokens are stored as well,
+ * without a launch of its own where the query rows are few. Scores, softmax statistics and sums are float32;
+ * probabilities enter the value product as float16 against the values rounded to float16. */
 typedef struct dkv_q4_attend_args {
-  const uint8_t* cells;          /* the layer's cells */
+  uint8_t* cells;                /* the layer's cells */
   int32_t n_pages, n_kv_heads, n_q_heads, head_dim;
-  int32_t fp16;                  /* the 16-bit type of the query and of a 16-bit output: 0 bf16, 1 fp16 */
+  int32_t fp16;                  /* the 16-bit type of query, key, value and a 16-bit output: 0 bf16, 1 fp16 */
   const int32_t* blocks;         /* [n_seq][max_blocks] */
   int32_t max_blocks;
   const int32_t* lengths;
@@ -458,11 +459,20 @@ typedef struct dkv_q4_attend_args {
   int32_t len_bound;             /* no length is above this (it only chooses how the work is split) */
   const void* query;             /* [n_seq][n_q_heads][q_len][head_dim] at q_stride */
   int64_t q_stride[3];           /* conversation, head, token (elements; multiples of 8, 16-byte aligned) */
+  const void* key;               /* the new tokens, [n_seq][n_kv_heads][q_len][head_dim]; NULL: they are stored */
+  const void* value;
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  const int32_t* slots;          /* [n_seq][q_len], with key and value */
   float scaling;
   void* out;                     /* [n_seq][q_len][n_q_heads][head_dim] */
   int32_t out_f32;
+  float* workspace;              /* dkv_q4_attend_floats(args) floats, 16-byte aligned */
+  int64_t workspace_floats;
   int* status;
 } dkv_q4_attend_args;
+/* Floats of workspace that dkv_q4_attend needs for the sizes in args (pointers, strides and len_bound are not read). */
+int64_t dkv_q4_attend_floats(const dkv_q4_attend_args* args);
 int dkv_q4_attend(const dkv_q4_attend_args* args, void* stream);
 
 /* The choice of the next token. For every row, with the tokens of its history (the first prompts[r] of

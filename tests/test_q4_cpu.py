@@ -112,8 +112,10 @@ def test_entry_points_refuse_on_the_host():
             assert fn(_lib.Q4RowsArgs(**{**rows, **bad}), None) == rc, bad
     att = dict(cells=p, n_pages=4, n_kv_heads=2, n_q_heads=4, head_dim=64, fp16=0, blocks=p, max_blocks=1, lengths=p,
                starts=p, n_seq=1, q_len=1, len_bound=64, query=p, q_stride=i64(8, 8, 8), scaling=1.0, out=p, out_f32=0,
-               status=p)
-    for bad, rc in ((dict(n_q_heads=3), 1), (dict(query=p + 8), 1), (dict(q_stride=i64(8, 8, 12)), 1),
+               workspace=p, workspace_floats=1 << 40, status=p)
+    for bad, rc in ((dict(n_q_heads=3), 1), (dict(key=p), 1), (dict(key=p, value=p), 1), (dict(workspace=None), 5),
+                    (dict(workspace_floats=100), 5), (dict(out=p + 4), 1), (dict(n_seq=8193), 2),
+                    (dict(key=p, value=p, slots=p, v_stride=i64(8, 8, 1)), 1), (dict(query=p + 8), 1), (dict(q_stride=i64(8, 8, 12)), 1),
                     (dict(head_dim=32), 2), (dict(status=None), 1), (dict(q_len=-1), 1), (dict(n_seq=70000), 2),
                     (dict(n_seq=0), 0), (dict(q_len=0), 0)):
         assert lib.dkv_q4_attend(_lib.Q4AttendArgs(**{**att, **bad}), None) == rc, bad
