@@ -1,24 +1,28 @@
 // q4_attend.cu — causal attention of new tokens' queries over the paged 4-bit cache (dkv_q4_attend), and the new
 // tokens' cells with it.
 //
-// With key value k_d = low_g + scale_g * c_d (g = d / 64), a score splits into
-//   q . k = sum_g scale_g * (sum_{d in g} q_d c_d) + sum_g low_g * (sum_{d in g} q_d):
-// the product runs over the codes themselves, which float16 holds exactly, and the key's rounding is the
-// cache's alone. Values enter as float16(low + scale * c), one rounding of at most 2^-11 relative; probabilities
-// as float16 of 2^7 * exp(score - m) with m within 2^8 of the running maximum, so that a token down to 2^-21 of the
-// largest keeps 11 bits (sums over a long context of small probabilities do not vanish). For float16 outputs, whose
-// own step is as small, a probability enters as two float16 numbers (the rounded one and what it lacks).
+// With k_d = low_g + scale_g * c_d (g = d / 64, the token's own scales and lows), a score splits into
+//   q . k = sum_g scale_g * (sum_{d in g} q_d c_d) + sum_g low_g * (sum_{d in g} q_d),
+// and a weighted value likewise into
+//   sum_j p_j v_jd = sum_j (p_j scale_jg) c_jd + sum_j p_j low_jg:
+// both products run over the codes themselves, which float16 holds exactly, the low terms in float32. The query enters
+// as float16 times a power of two of its row (exact but for what is below 2^-38 of the row's largest), so a score is
+// good to float32. p * scale enters as float16 of 2^7 * exp(score - m) * scale / 2^k, with m within 2^8 of the running
+// maximum and 2^k above the scales so far: a token down to 2^-21 of the largest keeps 11 bits, so that sums over a
+// long context of small probabilities do not vanish. That is one rounding of 2^-11 at most of each term; for float16
+// outputs, whose own step is as small, the factor enters as two float16 numbers (the rounded one and what it lacks).
 //
-// q4_decode_kernel: few query rows per KV head (one token, or a short draft). Bound by the cells' bytes. The pages of
-// all (conversation, KV head, row chunk) units form one line, cut into equal pieces, one per WARP, so that any mix
-// of lengths, heads and conversations fills the GPU evenly; a unit that several warps share leaves partial
-// (m, l, O) in the workspace, which q4_combine_kernel joins. A page of one KV head is one contiguous block: each warp
-// keeps a ring of bulk copies of its own and meets no other warp. It contracts tokens as the 16 rows of m16n8k16
-// and query rows as its 8 columns (3 or 4 heads that share a KV head are the rule), S^T = C Q^T, then O^T = V^T P^T;
-// P^T in the layout of the second product is one 8 x 8 transpose per 8 tokens (movmatrix). A code pair of a word is a
-// float16 pair after ONE mask: the 4 bits are a subnormal c * 2^-24 (or 16 times that, from the odd nibbles,
-// against q / 16), and the power of two goes into the score's factor. The warp that owns a new token's page
-// quantises the token itself, into the page's copy and into the cache.
+// q4_decode_kernel: few query rows per KV head (one token, or a short draft). Bound by the cells' bytes, and close to it
+// by unpacking them (the integer pipe runs at half rate). The pages of all (conversation, KV head, row chunk) units
+// form one line, cut into equal pieces, one per WARP, so that any mix of lengths, heads and conversations fills the
+// GPU evenly; a unit that several warps share leaves partial (m, l, O) in the workspace, which q4_combine_kernel
+// joins. A page of one KV head is one contiguous block: each warp keeps a ring of bulk copies of its own and meets no
+// other warp. It contracts tokens as the 16 rows of m16n8k16 and query rows as its 8 columns (3 or 4 heads that share a
+// KV head are the rule), S^T = C Q^T, then O^T = C^T P^T; P^T in the layout of the second product is one 8 x 8
+// transpose per 8 tokens (movmatrix). A code pair of a word is a float16 pair after ONE mask: the 4 bits are a
+// subnormal c * 2^-24 (or 16 times that from the odd nibbles, against q / 16 in the first product, and divided out at
+// the end in the second). The warp that owns a new token's page quantises the token itself, into the page's copy and
+// into the cache.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -44,16 +48,29 @@ __device__ __forceinline__ float exp2_fast(float x) {
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// x += u, y += w, as one packed addition.
+__device__ __forceinline__ void add2(float& x, float& y, float u, float w) {
+  const uint64_t r = add_f32x2(f32x2_pack(__float_as_uint(x), __float_as_uint(y)),
+                               f32x2_pack(__float_as_uint(u), __float_as_uint(w)));
+  x = __uint_as_float(static_cast<uint32_t>(r));
+  y = __uint_as_float(static_cast<uint32_t>(r >> 32));
 }
 
 // Transpose of an 8 x 8 matrix of 16-bit elements held one pair per lane.
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 
@@ -66,8 +83,17 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) { return as_u
 struct Deal {
   int64_t total;
   int workers;
-  __device__ __forceinline__ int64_t begin(int w) const { return total * w / workers; }
-  __device__ __forceinline__ int owner(int64_t x) const { return static_cast<int>(((x + 1) * workers - 1) / total); }
+  __device__ __forceinline__ Deal(int64_t total_, int workers_)
+      : total(total_), workers(static_cast<int>(total_ < workers_ ? total_ : workers_)) {}
+  __device__ __forceinline__ int64_t begin(int w) const {
+    const int64_t x = total * w;
+    return x <= 0xffffffffll ? static_cast<uint32_t>(x) / static_cast<uint32_t>(workers) : x / workers;
+  }
+  // The worker that has place x; none is without a place.
+  __device__ __forceinline__ int owner(int64_t x) const {
+    const int64_t y = (x + 1) * workers - 1;
+    return static_cast<int>(y <= 0xffffffffll ? static_cast<uint32_t>(y) / static_cast<uint32_t>(total) : y / total);
+  }
 };
 
 // Tokens that conversation s attends over (0 if it has no new token).
@@ -97,6 +123,7 @@ struct Decode {
   using C = Cells<D>;
   static constexpr int kRows = 8 * NT;
   static constexpr int kStages = D == 128 ? 2 : 4;
+  static constexpr int kTiles = NT == 1 ? 2 : 1;  // of 16 tokens at a time, for the latencies to overlap
   static constexpr int kBlocksPerSm = D == 128 && NT == 2 ? 2 : 3;  // two accumulators of 128 need the registers
   static constexpr int kWarpBytes = kStages * C::kBytes;
   static constexpr int kBars = kWarps * kWarpBytes;
@@ -178,27 +205,40 @@ __device__ __forceinline__ void load_query(const dkv_q4_attend_args& a, int seq,
   }
 }
 
-// Running softmax of a unit: per column (query row) the reference -(m - kBias), the sum, and O^T.
+// Running softmax of a unit: per column (query row) the reference -(m - kBias), the sums of p and of p * low, and O^T
+// over the codes in units of 2^k * 2^-24 (even dimensions) or 2^-20 (odd ones).
 template <int D, int NT>
 struct State {
   float o[D / 16][NT][4];
-  float l[NT][2], neg[NT][2];
+  float l[NT][2], neg[NT][2], low[NT][2][Cells<D>::kGroups];
+  float unit;      // 2^-k: scales so far times it are at most 1
   uint32_t known;  // bit 2 nt + c: the column has a reference
   bool open;       // some column has none yet (warp-uniform)
 };
 
-// 16 tokens of a page in shared memory (rows tile * 16 ..), the first of them token `base` of the conversation. EDGE:
-// some row does not see some of the 16.
-template <int D, int NT, bool F16, bool EDGE>
-__device__ __forceinline__ void attend16(const uint8_t* page, int tile, int base, int seen, const Query<D, NT>& q,
-                                         State<D, NT>& st) {
+// 2^-k for the largest scale: scale * 2^-k in [1/4, 1/2).
+__device__ __forceinline__ float unit_for(float scale) {
+  const int ex = (__float_as_uint(scale) >> 23) & 255;
+  return scale > 0.f ? __uint_as_float(static_cast<uint32_t>(252 - ex) << 23) : 0x1p24f;
+}
+
+// 16 * TT tokens of a page in shared memory (rows 16 * tile ..), the first of them token `base` of the conversation.
+// EDGE: some row does not see some of them.
+template <int D, int NT, int TT, bool F16, bool EDGE>
+__device__ __forceinline__ void attend(const uint8_t* page, int tile, int base, int seen, const Query<D, NT>& q,
+                                       State<D, NT>& st) {
   using C = Cells<D>;
   constexpr int kGroups = C::kGroups;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  // ---- scores: rows g and g + 8
-  float acc[kGroups][NT][4];
-  {
-    const uint8_t* kr = page + C::kKeyCodes + (tile * 16 + g) * (D / 2) + t * (D / 8);
+  float p[TT][NT][4];
+  __half2 vhead[TT][2][kGroups];
+  bool rise = EDGE || st.open;
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt) {
+    // ---- scores of tokens g and g + 8
+    const int row = (tile + tt) * 16 + g;
+    float acc[kGroups][NT][4];
+    const uint8_t* kr = page + C::kKeyCodes + row * (D / 2) + t * (D / 8);
     uint32_t x[2 * kGroups], y[2 * kGroups];
     if constexpr (D == 128) {
       const uint4 u = *reinterpret_cast<const uint4*>(kr), v = *reinterpret_cast<const uint4*>(kr + 8 * (D / 2));
@@ -210,77 +250,108 @@ __device__ __forceinline__ void attend16(const uint8_t* page, int tile, int base
       y[0] = v.x, y[1] = v.y;
     }
 #pragma unroll
-    for (int gr = 0; gr < kGroups; ++gr) {
+    for (int w = 0; w < 2; ++w) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[gr][nt][e] = 0.f;
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
+      for (int gr = 0; gr < kGroups; ++gr) {
         const uint32_t u = x[gr * 2 + w], v = y[gr * 2 + w], u8 = u >> 8, v8 = v >> 8;
 #pragma unroll
         for (int odd = 0; odd < 2; ++odd) {
           const uint32_t mask = odd ? 0x00f000f0u : 0x000f000fu;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            mma16816(acc[gr][nt], u & mask, v & mask, u8 & mask, v8 & mask, q.frag[gr * 4 + w * 2 + odd][nt][0],
-                     q.frag[gr * 4 + w * 2 + odd][nt][1]);
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint32_t* b = q.frag[gr * 4 + w * 2 + odd][nt];
+            if (w == 0 && odd == 0) mma16816_first(acc[gr][nt], u & mask, v & mask, u8 & mask, v8 & mask, b[0], b[1]);
+            else mma16816(acc[gr][nt], u & mask, v & mask, u8 & mask, v8 & mask, b[0], b[1]);
+          }
         }
       }
     }
-  }
-  float ks[2][kGroups], kl[2][kGroups];
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int gr = 0; gr < kGroups; ++gr) {
-      const float2 f = __half22float2(
-          as_half2(*reinterpret_cast<const uint32_t*>(page + C::key_head(tile * 16 + g + 8 * h, gr))));
-      ks[h][gr] = f.x;
-      kl[h][gr] = f.y;
-    }
-  float p[NT][4];
-  bool rise = EDGE || st.open;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int h = e >> 1, c = e & 1;
-      float dot = ks[h][0] * acc[0][nt][e];
-      float s = fmaf(kl[h][0], q.sum[nt][c][0], st.neg[nt][c]);
+    for (int h = 0; h < 2; ++h) {
+      uint32_t hd[2 * kGroups];
+      const uint8_t* hp = page + C::kHeads + (row + 8 * h) * C::kHeadBytes;
       if constexpr (kGroups == 2) {
-        dot = fmaf(ks[h][1], acc[1][nt][e], dot);
-        s = fmaf(kl[h][1], q.sum[nt][c][1], s);
+        const uint4 u = *reinterpret_cast<const uint4*>(hp);
+        hd[0] = u.x, hd[1] = u.y, hd[2] = u.z, hd[3] = u.w;
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(hp);
+        hd[0] = u.x, hd[1] = u.y;
       }
-      s = fmaf(dot, q.factor[nt][c], s);
-      if constexpr (EDGE) {
-        if (base + g + 8 * h >= q.limit[nt][c]) s = -INFINITY;
+      const bool gone = EDGE && base + tt * 16 + g + 8 * h >= seen;
+      float ks[kGroups], kl[kGroups];
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr) {
+        const float2 f = __half22float2(as_half2(hd[gr]));
+        ks[gr] = f.x;
+        kl[gr] = f.y;
+        // tokens that no row sees may never have been written: no NaN of theirs into the sums
+        vhead[tt][h][gr] = as_half2(gone ? 0u : hd[kGroups + gr]);
+        rise = rise || __low2float(vhead[tt][h][gr]) * st.unit > 1.f;
       }
-      p[nt][e] = s;
-      rise = rise || s > kBias + kSlack;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float dot = ks[0] * acc[0][nt][2 * h + c];
+          float s = fmaf(kl[0], q.sum[nt][c][0], st.neg[nt][c]);
+          if constexpr (kGroups == 2) {
+            dot = fmaf(ks[1], acc[1][nt][2 * h + c], dot);
+            s = fmaf(kl[1], q.sum[nt][c][1], s);
+          }
+          s = fmaf(dot, q.factor[nt][c], s);
+          if constexpr (EDGE) {
+            if (base + tt * 16 + g + 8 * h >= q.limit[nt][c]) s = -INFINITY;
+          }
+          p[tt][nt][2 * h + c] = s;
+          rise = rise || s > kBias + kSlack;
+        }
     }
+  }
   if (__any_sync(0xffffffffu, rise)) {
-    // ---- a score above the reference's slack, or a column without a reference: references move up to the columns'
-    // maxima, and what is summed so far scales down
+    // ---- a score above the reference's slack, a scale above the unit, or a column without a reference: references
+    // move up to the columns' maxima, and what is summed so far scales down
+    float big = 0.f;
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int gr = 0; gr < kGroups; ++gr) big = fmaxf(big, __low2float(vhead[tt][h][gr]));
+    big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));  // not negative: ordered as its bits
+    float shrink = 1.f;
+    if (big * st.unit > 1.f) {
+      const float unit = unit_for(big);
+      shrink = unit / st.unit;
+      st.unit = unit;
+    }
     bool open = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float f[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float top = fmaxf(p[nt][c], p[nt][c + 2]);
+        float top = -INFINITY;
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) top = fmaxf(top, fmaxf(p[tt][nt][c], p[tt][nt][c + 2]));
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        // a column's first tokens set the reference wherever they are; later ones only raise it
+        // a column's first tokens set the reference wherever they are; later ones raise it, and only from beyond the
+        // slack, so that a row's result does not depend on the rows beside it
         const uint32_t bit = 1u << (2 * nt + c);
         const bool first = (st.known & bit) == 0, none = first && top == -INFINITY;
-        const float move = none ? 0.f : first ? top - kBias : fmaxf(top - kBias, 0.f);
+        const float move = none ? 0.f : first || top > kBias + kSlack ? top - kBias : 0.f;
         st.known |= none ? 0u : bit;
         f[c] = first ? 0.f : exp2_fast(-move);
         st.neg[nt][c] -= move;
         st.l[nt][c] *= f[c];
-        p[nt][c] -= move;
-        p[nt][c + 2] -= move;
+#pragma unroll
+        for (int gr = 0; gr < kGroups; ++gr) st.low[nt][c][gr] *= f[c];
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) {
+          p[tt][nt][c] -= move;
+          p[tt][nt][c + 2] -= move;
+        }
+        f[c] *= shrink;
         open = open || none;
       }
 #pragma unroll
@@ -290,71 +361,73 @@ __device__ __forceinline__ void attend16(const uint8_t* page, int tile, int base
     }
     st.open = __any_sync(0xffffffffu, open);
   }
-  uint32_t pf[NT][2], pr[NT][2];
+  uint32_t pf[TT][kGroups][NT][2], pr[F16 ? TT : 1][kGroups][NT][2], v[TT][2][D / 32];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      p[nt][e] = exp2_fast(p[nt][e]);
-      st.l[nt][e & 1] += p[nt][e];
-    }
+  for (int tt = 0; tt < TT; ++tt) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t hi = pack_half2(p[nt][2 * h], p[nt][2 * h + 1]);
-      pf[nt][h] = transpose8(hi);
-      if constexpr (F16) {
-        const float2 back = __half22float2(as_half2(hi));
-        pr[nt][h] = transpose8(pack_half2(p[nt][2 * h] - back.x, p[nt][2 * h + 1] - back.y));
-      }
-    }
-  }
-  // ---- values: token pairs t and t + 4 of the 16
-  uint32_t v[2][D / 32];
-  __half2 vs[2], vl[2];
+      float vs[kGroups], vl[kGroups];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int pair = tile * 8 + t + 4 * h;
-    const uint8_t* vr = page + C::value_piece(pair, g);
-    if constexpr (D == 128) {
-      const uint4 u = *reinterpret_cast<const uint4*>(vr);
-      v[h][0] = u.x, v[h][1] = u.y, v[h][2] = u.z, v[h][3] = u.w;
-    } else {
-      const uint2 u = *reinterpret_cast<const uint2*>(vr);
-      v[h][0] = u.x, v[h][1] = u.y;
-    }
-    uint2 hd = *reinterpret_cast<const uint2*>(page + C::value_head(pair, kGroups == 2 ? g >> 2 : 0));
-    if constexpr (EDGE) {
-      // tokens that no row sees may never have been written: no NaN of theirs into the sums
-      const int tok = base + 2 * (t + 4 * h);
-      const uint32_t keep = (tok < seen ? 0x0000ffffu : 0u) | (tok + 1 < seen ? 0xffff0000u : 0u);
-      hd.x &= keep;
-      hd.y &= keep;
-    }
-    vs[h] = as_half2(hd.x);
-    vl[h] = as_half2(hd.y);
-  }
-  const __half2 k1024 = as_half2(0x64006400u), k16th = as_half2(0x2c002c00u), k64 = as_half2(0xd400d400u);
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      uint32_t x[2][2];  // [tokens t / t + 4][dimension 2 b, 2 b + 1]
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t w = b ? v[h][i] >> 8 : v[h][i];
-        // 1024 + c and 1024 + 16 c, both exact; then c, then the value with its one rounding
-        const __half2 even = __hsub2(as_half2((w & 0x000f000fu) | 0x64006400u), k1024);
-        const __half2 odd = __hfma2(as_half2((w & 0x00f000f0u) | 0x64006400u), k16th, k64);
-        x[h][0] = as_u32(__hfma2(even, vs[h], vl[h]));
-        x[h][1] = as_u32(__hfma2(odd, vs[h], vl[h]));
+      for (int gr = 0; gr < kGroups; ++gr) {
+        const float2 f = __half22float2(vhead[tt][h][gr]);
+        vs[gr] = f.x * st.unit;
+        vl[gr] = f.y;
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        mma16816(st.o[i * 2 + b][nt], x[0][0], x[0][1], x[1][0], x[1][1], pf[nt][0], pf[nt][1]);
-        if constexpr (F16) mma16816(st.o[i * 2 + b][nt], x[0][0], x[0][1], x[1][0], x[1][1], pr[nt][0], pr[nt][1]);
+        const float e0 = exp2_fast(p[tt][nt][2 * h]), e1 = exp2_fast(p[tt][nt][2 * h + 1]);
+        st.l[nt][0] += e0;
+        st.l[nt][1] += e1;
+#pragma unroll
+        for (int gr = 0; gr < kGroups; ++gr) {
+          st.low[nt][0][gr] = fmaf(e0, vl[gr], st.low[nt][0][gr]);
+          st.low[nt][1][gr] = fmaf(e1, vl[gr], st.low[nt][1][gr]);
+          const float w0 = e0 * vs[gr], w1 = e1 * vs[gr];
+          const uint32_t hi = pack_half2(w0, w1);
+          pf[tt][gr][nt][h] = transpose8(hi);
+          if constexpr (F16) {
+            const float2 back = __half22float2(as_half2(hi));
+            pr[tt][gr][nt][h] = transpose8(pack_half2(w0 - back.x, w1 - back.y));
+          }
+        }
+      }
+    }
+    // ---- values: token pairs t and t + 4 of the 16
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint8_t* vr = page + C::value_piece((tile + tt) * 8 + t + 4 * h, g);
+      if constexpr (D == 128) {
+        const uint4 u = *reinterpret_cast<const uint4*>(vr);
+        v[tt][h][0] = u.x, v[tt][h][1] = u.y, v[tt][h][2] = u.z, v[tt][h][3] = u.w;
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(vr);
+        v[tt][h][0] = u.x, v[tt][h][1] = u.y;
       }
     }
   }
+  // The products of these tokens on their own, then added to O by the float32 units: the tensor core cuts a sum where
+  // it does not round it, and the codes are not negative, so a long chain of its sums would drift (by 4e-5 over 10000
+  // tokens, as much as 1e-3 of outputs that average to little).
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float sum[4];
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) {
+          const uint32_t u = b ? v[tt][0][i] >> 8 : v[tt][0][i], w = b ? v[tt][1][i] >> 8 : v[tt][1][i];
+          const uint32_t u0 = u & 0x000f000fu, u1 = u & 0x00f000f0u, w0 = w & 0x000f000fu, w1 = w & 0x00f000f0u;
+          const uint32_t* hi = pf[tt][i >> 1][nt];
+          if (tt == 0) mma16816_first(sum, u0, u1, w0, w1, hi[0], hi[1]);
+          else mma16816(sum, u0, u1, w0, w1, hi[0], hi[1]);
+          if constexpr (F16) mma16816(sum, u0, u1, w0, w1, pr[tt][i >> 1][nt][0], pr[tt][i >> 1][nt][1]);
+        }
+        float* o = st.o[i * 2 + b][nt];
+        add2(o[0], o[1], sum[0], sum[1]);
+        add2(o[2], o[3], sum[2], sum[3]);
+      }
 }
 
 // The new tokens of a page (tokens first .. last of the conversation), quantised by the warp into the page's copy in
@@ -422,10 +495,10 @@ q4_decode_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int w
   const int worker = warp * gridDim.x + blockIdx.x;  // neighbours in the line on different SMs
   int64_t unused;
   const int units = a.n_kv_heads * chunks;  // of a conversation
-  const Deal deal = {count_pages(a, 0, unused) * units, workers};
+  const Deal deal(count_pages(a, 0, unused) * units, workers);
   if (__any_sync(0xffffffffu, failed != 0)) return;
+  if (worker >= deal.workers) return;
   const int64_t begin = deal.begin(worker), end = deal.begin(worker + 1);
-  if (begin >= end) return;
 
   // the conversation of the first page
   int seq = 0;
@@ -501,9 +574,12 @@ q4_decode_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int w
     State<D, NT> st;
     st.open = true;
     st.known = 0;
+    st.unit = 0x1p24f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       st.l[nt][0] = st.l[nt][1] = st.neg[nt][0] = st.neg[nt][1] = 0.f;
+#pragma unroll
+      for (int gr = 0; gr < C::kGroups; ++gr) st.low[nt][0][gr] = st.low[nt][1][gr] = 0.f;
 #pragma unroll
       for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
@@ -524,12 +600,11 @@ q4_decode_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int w
                             cells + id * page_stride);
       }
       if (base + q4::kPage <= full_below) {
-#pragma unroll 2
-        for (int tile = 0; tile < q4::kPage / 16; ++tile)
-          attend16<D, NT, F16, false>(page, tile, base + tile * 16, seen, q, st);
+        for (int tile = 0; tile < q4::kPage / 16; tile += S::kTiles)
+          attend<D, NT, S::kTiles, F16, false>(page, tile, base + tile * 16, seen, q, st);
       } else {
         for (int tile = 0; tile < q4::kPage / 16 && base + tile * 16 < seen; ++tile)
-          attend16<D, NT, F16, true>(page, tile, base + tile * 16, seen, q, st);
+          attend<D, NT, 1, F16, true>(page, tile, base + tile * 16, seen, q, st);
       }
       __syncwarp();
       if (p + S::kStages < pe) fetch(p + S::kStages);
@@ -544,33 +619,35 @@ q4_decode_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int w
     // ---- the segment's result
     const bool whole = p0 == 0 && p1 == n_pages;
     float* slot = a.workspace + (worker * 2 + (at == begin ? 0 : 1)) * slot_floats(rows, D);
+    const float even = 0x1p24f / st.unit, odd = 0x1p20f / st.unit;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float sum = st.l[nt][c];
+        float sum = st.l[nt][c], low[C::kGroups];
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        for (int gr = 0; gr < C::kGroups; ++gr) low[gr] = st.low[nt][c][gr];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, d);
+#pragma unroll
+          for (int gr = 0; gr < C::kGroups; ++gr) low[gr] += __shfl_xor_sync(0xffffffffu, low[gr], d);
+        }
         const int col = nt * 8 + 2 * t + c, r = row0 + col, i = r / share;
         if (r >= a.q_len * share || i >= fresh) continue;  // q4_combine_kernel writes the zeros behind the new tokens
-        if (whole) {
-          const float inv = sum != 0.f ? 1.f / sum : 0.f;
-          const int64_t to =
-              ((static_cast<int64_t>(seq) * a.q_len + i) * a.n_q_heads + head * share + r - i * share) * D + g * (D / 8);
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;
+        const int64_t to =
+            ((static_cast<int64_t>(seq) * a.q_len + i) * a.n_q_heads + head * share + r - i * share) * D + g * 8;
 #pragma unroll
-          for (int k = 0; k < D / 32; ++k)
-            store_out4<F16>(a, to + k * 4, st.o[2 * k][nt][c] * inv, st.o[2 * k][nt][c + 2] * inv,
-                            st.o[2 * k + 1][nt][c] * inv, st.o[2 * k + 1][nt][c + 2] * inv);
-        } else {
-#pragma unroll
-          for (int k = 0; k < D / 32; ++k)
-            *reinterpret_cast<float4*>(slot + col * D + g * (D / 8) + k * 4) =
-                make_float4(st.o[2 * k][nt][c], st.o[2 * k][nt][c + 2], st.o[2 * k + 1][nt][c], st.o[2 * k + 1][nt][c + 2]);
-          if (g == 0) {
-            slot[rows * D + col * 4] = st.neg[nt][c];
-            slot[rows * D + col * 4 + 1] = sum;
-          }
+        for (int k = 0; k < D / 32; ++k) {
+          const float y0 = fmaf(st.o[2 * k][nt][c], even, low[k >> 1]), y1 = fmaf(st.o[2 * k][nt][c + 2], odd, low[k >> 1]);
+          const float y2 = fmaf(st.o[2 * k + 1][nt][c], even, low[k >> 1]),
+                      y3 = fmaf(st.o[2 * k + 1][nt][c + 2], odd, low[k >> 1]);
+          const int dim = (k >> 1) * 64 + (k & 1) * 4;
+          if (whole) store_out4<F16>(a, to + dim, y0 * inv, y1 * inv, y2 * inv, y3 * inv);
+          else *reinterpret_cast<float4*>(slot + col * D + g * 8 + dim) = make_float4(y0, y1, y2, y3);
         }
+        if (!whole && g == 0) *reinterpret_cast<float2*>(slot + rows * D + col * 4) = make_float2(st.neg[nt][c], sum);
       }
     at = unit_at + p1;
     if (at == seq_at + static_cast<int64_t>(units) * n_pages) {
@@ -581,77 +658,106 @@ q4_decode_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int w
 }
 
 // Joins the partial results of the units that several workers share, and writes the zeros of the rows behind the new
-// tokens. One CTA per (query row of a KV head, KV head, conversation): D / 4 lanes of 4 dimensions, in kSlices
-// slices over the unit's workers.
+// tokens. One CTA per (query row of a KV head, KV head, conversation): the workers' factors first, then D / 4 lanes of
+// 4 dimensions in kSlices slices over the workers, with nothing that one load has to wait for another.
 constexpr int kCombineThreads = 256;
+constexpr int kFactors = 512;  // workers of a unit whose factors are held at a time
 template <int D, int NT, bool F16>
 __global__ void __launch_bounds__(kCombineThreads)
 q4_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int workers) {
   constexpr int kLanes = D / 4, kSlices = kCombineThreads / kLanes;
   __shared__ int64_t line[2];
   __shared__ float4 part[kSlices][kLanes];
-  __shared__ float2 stat[kSlices];
+  __shared__ float factor[kFactors];
+  __shared__ float warp_ref[kCombineThreads / 32], warp_den[kCombineThreads / 32];
   const int share = a.n_q_heads / a.n_kv_heads;
   const int rows = min(8 * NT, a.q_len * share);
   const int r = blockIdx.x, head = blockIdx.y, seq = blockIdx.z;
   const int chunk = r / (8 * NT), col = r - chunk * 8 * NT, i = r / share;
-  const int x = threadIdx.x % kLanes, slice = threadIdx.x / kLanes;
+  const int tid = threadIdx.x, x = tid % kLanes, slice = tid / kLanes;
   const int tokens = tokens_of(a, seq), n_pages = pages_of(tokens);
   const int fresh = tokens == 0 ? 0 : min(tokens - a.starts[seq], a.q_len);
-  if (threadIdx.x < 32) {
+  if (tid < 32) {
     int64_t before;
     const int64_t all = count_pages(a, seq, before);
-    if (threadIdx.x == 0) line[0] = all, line[1] = before;
+    if (tid == 0) line[0] = all, line[1] = before;
   }
   __syncthreads();
   const int units = a.n_kv_heads * chunks;
-  const Deal deal = {line[0] * units, workers};
   const int64_t to = ((static_cast<int64_t>(seq) * a.q_len + i) * a.n_q_heads + head * share + r - i * share) * D + x * 4;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (i >= fresh || status_at_entry(a.status) != 0) {
+  // The main kernel of this call may have set the status word while others of its warps finished: the CTA's one answer.
+  if (i >= fresh || cta_failed_at_entry(a.status)) {
     if (slice == 0) store_out4<F16>(a, to, 0.f, 0.f, 0.f, 0.f);
     return;
   }
+  const Deal deal(line[0] * units, workers);
   const int64_t unit_at = line[1] * units + static_cast<int64_t>(head * chunks + chunk) * n_pages;
   const int w0 = deal.owner(unit_at), w1 = deal.owner(unit_at + n_pages - 1);
   if (w0 == w1) return;  // one worker had the whole unit
   const int64_t stride = slot_floats(rows, D);
-  const int second = deal.begin(w0) < unit_at ? 1 : 0;  // the unit is the last segment of w0, the first of the others
-  // x2^-neg is what a slot's sums are relative to: the smallest neg is the largest reference
+  // the unit is the last segment of w0 unless w0 begins with it, and the first segment of the others
+  const float* first = a.workspace + (2 * static_cast<int64_t>(w0) + (deal.begin(w0) < unit_at ? 1 : 0)) * stride;
+  const float* rest = a.workspace + 2 * static_cast<int64_t>(w0) * stride;
+  auto slot = [&](int k) { return k == 0 ? first : rest + 2 * k * stride; };
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  float den = 0.f, ref = INFINITY;
-  for (int w = w0 + slice; w <= w1; w += kSlices) {
-    if (deal.begin(w) == deal.begin(w + 1)) continue;  // fewer pages than workers
-    const float* slot = a.workspace + (2 * w + (w == w0 ? second : 0)) * stride;
-    const float2 s = *reinterpret_cast<const float2*>(slot + rows * D + col * 4);
-    const float4 o = *reinterpret_cast<const float4*>(slot + col * D + x * 4);
-    if (s.y == 0.f) continue;  // it saw no token of this row
-    const float now = fminf(ref, s.x);
-    const float keep = ref == INFINITY ? 0.f : exp2_fast(now - ref), add = exp2_fast(now - s.x);
-    sum.x = fmaf(o.x, add, sum.x * keep);
-    sum.y = fmaf(o.y, add, sum.y * keep);
-    sum.z = fmaf(o.z, add, sum.z * keep);
-    sum.w = fmaf(o.w, add, sum.w * keep);
-    den = fmaf(s.y, add, den * keep);
+  float den = 0.f, ref = INFINITY;  // sums are relative to 2^-ref; the smallest ref is the largest maximum
+  const int n = w1 - w0 + 1;
+  for (int base = 0; base < n; base += kFactors) {
+    const int m = min(kFactors, n - base);
+    float mine[kFactors / kCombineThreads], weight[kFactors / kCombineThreads];
+    float low = INFINITY;
+#pragma unroll
+    for (int k = 0; k < kFactors / kCombineThreads; ++k) {
+      const int w = k * kCombineThreads + tid;
+      const float2 s = w < m ? *reinterpret_cast<const float2*>(slot(base + w) + rows * D + col * 4) : make_float2(0.f, 0.f);
+      mine[k] = s.y == 0.f ? INFINITY : s.x;  // a worker that saw no token of this row
+      weight[k] = s.y;
+      low = fminf(low, mine[k]);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, d));
+    if ((tid & 31) == 0) warp_ref[tid >> 5] = low;
+    __syncthreads();
+    float now = ref;
+#pragma unroll
+    for (int k = 0; k < kCombineThreads / 32; ++k) now = fminf(now, warp_ref[k]);
+    float add = 0.f;
+#pragma unroll
+    for (int k = 0; k < kFactors / kCombineThreads; ++k) {
+      const int w = k * kCombineThreads + tid;
+      const float f = mine[k] == INFINITY ? 0.f : exp2_fast(now - mine[k]);
+      if (w < m) factor[w] = f;
+      add = fmaf(weight[k], f, add);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
+    if ((tid & 31) == 0) warp_den[tid >> 5] = add;
+    __syncthreads();
+    const float keep = ref == INFINITY ? 0.f : exp2_fast(now - ref);
+    den *= keep;
+#pragma unroll
+    for (int k = 0; k < kCombineThreads / 32; ++k) den += warp_den[k];
+    sum.x *= keep, sum.y *= keep, sum.z *= keep, sum.w *= keep;
     ref = now;
+#pragma unroll 8
+    for (int w = slice; w < m; w += kSlices) {
+      const float4 o = *reinterpret_cast<const float4*>(slot(base + w) + col * D + x * 4);
+      const float f = factor[w];
+      sum.x = fmaf(o.x, f, sum.x);
+      sum.y = fmaf(o.y, f, sum.y);
+      sum.z = fmaf(o.z, f, sum.z);
+      sum.w = fmaf(o.w, f, sum.w);
+    }
+    __syncthreads();
   }
   part[slice][x] = sum;
-  if (x == 0) stat[slice] = make_float2(ref, den);
   __syncthreads();
   if (slice != 0) return;
-  float top = INFINITY;
 #pragma unroll
-  for (int k = 0; k < kSlices; ++k) top = fminf(top, stat[k].x);
-  sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  den = 0.f;
-#pragma unroll
-  for (int k = 0; k < kSlices; ++k) {
-    const float f = stat[k].x == INFINITY ? 0.f : exp2_fast(top - stat[k].x);
-    sum.x = fmaf(part[k][x].x, f, sum.x);
-    sum.y = fmaf(part[k][x].y, f, sum.y);
-    sum.z = fmaf(part[k][x].z, f, sum.z);
-    sum.w = fmaf(part[k][x].w, f, sum.w);
-    den = fmaf(stat[k].y, f, den);
+  for (int k = 1; k < kSlices; ++k) {
+    const float4 o = part[k][x];
+    sum.x += o.x, sum.y += o.y, sum.z += o.z, sum.w += o.w;
   }
   const float inv = den != 0.f ? 1.f / den : 0.f;
   store_out4<F16>(a, to, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);

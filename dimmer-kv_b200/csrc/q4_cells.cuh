@@ -1,20 +1,19 @@
 // q4_cells.cuh — layout of the paged 4-bit cache.
 //
-// One page of one KV head holds 64 tokens: [key codes][key headers][value codes][value headers], one contiguous
-// block of page_bytes() that a single bulk copy fetches. The codes lie in the order in which the lanes of an
-// m16n8k16 product (lane = 4 * g + t) hold its first operand, so that a lane gets its share of the operand
-// with one 16-byte (head_dim 128) or 8-byte (64) shared-memory load and unpacks it with masks alone:
+// One page of one KV head holds 64 tokens: [key codes][value codes][headers], one contiguous block of kBytes that a
+// single bulk copy fetches. The codes lie in the order in which the lanes of an m16n8k16 product (lane = 4 * g + t)
+// hold its first operand, so that a lane gets its share of the operand with one 16-byte (head_dim 128) or 8-byte
+// (64) shared-memory load and unpacks it with masks alone:
 //
 //   keys: a token's D / 2 bytes are 4 pieces, one per t; piece t holds, per group of 64 dimensions, the 16
 //     dimensions gr * 64 + t * 16 .. + 15 in two words, nibble n of word w = dimension t * 16 + 8 w + n.
 //     Masks 0x000f000f and 0x00f000f0 (of the word and of the word >> 8) give the pairs (n, n + 4).
-//   values: two tokens (2p, 2p + 1) share D bytes in 8 pieces, one per g, of the D / 8 dimensions g * D / 8 ..;
-//     word i of a piece holds 4 dimensions, the even token in its low half, the odd one in its high half, so
-//     the same masks give (even token, odd token) pairs, which is how the second product contracts over tokens.
-//     The piece's place is rotated by the pair, (g + 2 p) % 8 for D = 128, and (g + 4 (p / 2 % 2)) % 8 for 64:
-//     lanes t = 0..3 read four pairs at once, a multiple of 64 bytes apart, and would share banks otherwise.
-//   headers: float16 (scale, low) per key token and group; (scale even, scale odd, low even, low odd) per value
-//     pair and group.
+//   values: two tokens (2p, 2p + 1) share D bytes in 8 pieces, one per g; piece g holds, per group, the 8 dimensions
+//     gr * 64 + g * 8 .. in two words of 4 dimensions, the even token in a word's low half, the odd one in its high
+//     half, so the same masks give (even token, odd token) pairs, which is how the second product contracts over
+//     tokens. The piece's place is rotated by the pair, (g + 2 p) % 8 for D = 128, and (g + 4 (p / 2 % 2)) % 8 for
+//     64: lanes t = 0..3 read four pairs at once, a multiple of 64 bytes apart, and would share banks otherwise.
+//   headers: float16 (scale, low) of a token's key groups, then of its value groups: one load per token.
 //
 // Quantising: eight lanes hold a group of 64 dimensions, eight each; minimum and maximum are three shuffles, a
 // lane's eight key codes are exactly one word of the key cell, its value codes the halves of two words of the pair's.
@@ -41,29 +40,26 @@ struct Cells {
   static_assert(D == 64 || D == 128, "head_dim");
   static constexpr int kGroups = D / kGroup;
   static constexpr int kKeyCodes = 0;
-  static constexpr int kKeyHeads = kPage * D / 2;
-  static constexpr int kValueCodes = kKeyHeads + kPage * kGroups * 4;
-  static constexpr int kValueHeads = kValueCodes + kPage * D / 2;
-  static constexpr int kBytes = kValueHeads + kPage * kGroups * 4;
+  static constexpr int kValueCodes = kPage * D / 2;
+  static constexpr int kHeads = 2 * kValueCodes;
+  static constexpr int kHeadBytes = kGroups * 8;  // of a token
+  static constexpr int kBytes = kHeads + kPage * kHeadBytes;
 
   // Byte of the 8 key codes of dimensions 8 * j .. + 7 (one word, nibble n = dimension 8 j + n) of token r.
   static __device__ __forceinline__ int key_word(int r, int j) {
     const int gr = j >> 3, t = (j & 7) >> 1, w = j & 1;
     return kKeyCodes + r * (D / 2) + t * (D / 8) + gr * 8 + w * 4;
   }
-  static __device__ __forceinline__ int key_head(int r, int gr) { return kKeyHeads + (r * kGroups + gr) * 4; }
-
   static __device__ __forceinline__ int value_piece(int pair, int g) {
     const int at = D == 128 ? (g + 2 * pair) & 7 : (g + 4 * ((pair >> 1) & 1)) & 7;
     return kValueCodes + pair * D + at * (D / 8);
   }
-  // Byte of the word that holds dimensions 4 * j .. + 3 of the two tokens of `pair`.
-  static __device__ __forceinline__ int value_word(int pair, int j) {
-    return value_piece(pair, j / (D / 32)) + (j % (D / 32)) * 4;
+  // Byte of the two words that hold dimensions 8 * j .. + 7 of the two tokens of `pair`.
+  static __device__ __forceinline__ int value_words(int pair, int j) {
+    return value_piece(pair, j & 7) + (j >> 3) * 8;
   }
-  static __device__ __forceinline__ int value_head(int pair, int gr) {
-    return kValueHeads + (pair * kGroups + gr) * 8;
-  }
+  static __device__ __forceinline__ int key_head(int r, int gr) { return kHeads + r * kHeadBytes + gr * 4; }
+  static __device__ __forceinline__ int value_head(int r, int gr) { return key_head(r, kGroups + gr); }
 };
 
 template <bool F16>
@@ -140,15 +136,12 @@ __device__ __forceinline__ void store_key8(uint8_t* page, int r, int j, const Ce
 }
 template <int D>
 __device__ __forceinline__ void store_value8(uint8_t* page, int r, int j, const Cell8& c) {
-  const int pair = r >> 1, odd = r & 1;
-  *reinterpret_cast<uint16_t*>(page + Cells<D>::value_word(pair, 2 * j) + 2 * odd) = static_cast<uint16_t>(c.codes);
-  *reinterpret_cast<uint16_t*>(page + Cells<D>::value_word(pair, 2 * j + 1) + 2 * odd) =
-      static_cast<uint16_t>(c.codes >> 16);
-  if (j % 8 == 0) {
-    uint8_t* h = page + Cells<D>::value_head(pair, j / 8) + 2 * odd;
-    *reinterpret_cast<uint16_t*>(h) = c.scale;
-    *reinterpret_cast<uint16_t*>(h + 4) = c.low;
-  }
+  uint8_t* w = page + Cells<D>::value_words(r >> 1, j) + 2 * (r & 1);
+  *reinterpret_cast<uint16_t*>(w) = static_cast<uint16_t>(c.codes);
+  *reinterpret_cast<uint16_t*>(w + 4) = static_cast<uint16_t>(c.codes >> 16);
+  if (j % 8 == 0)
+    *reinterpret_cast<uint32_t*>(page + Cells<D>::value_head(r, j / 8)) =
+        static_cast<uint32_t>(c.scale) | static_cast<uint32_t>(c.low) << 16;
 }
 
 }  // namespace q4

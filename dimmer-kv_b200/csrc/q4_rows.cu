@@ -81,13 +81,10 @@ __global__ void __launch_bounds__(kRowThreads) q4_read_kernel(const dkv_q4_rows_
       codes = *reinterpret_cast<const uint32_t*>(page + C::key_word(r, j));
       scale_low = *reinterpret_cast<const uint32_t*>(page + C::key_head(r, j / 8));
     } else {
-      const int pair = r >> 1, odd = r & 1;
-      codes = *reinterpret_cast<const uint16_t*>(page + C::value_word(pair, 2 * j) + 2 * odd) |
-              static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(page + C::value_word(pair, 2 * j + 1) + 2 * odd))
-                  << 16;
-      const uint8_t* h = page + C::value_head(pair, j / 8) + 2 * odd;
-      scale_low = *reinterpret_cast<const uint16_t*>(h) |
-                  static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(h + 4)) << 16;
+      const uint8_t* w = page + C::value_words(r >> 1, j) + 2 * (r & 1);
+      codes = *reinterpret_cast<const uint16_t*>(w) |
+              static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(w + 4)) << 16;
+      scale_low = *reinterpret_cast<const uint32_t*>(page + C::value_head(r, j / 8));
     }
     const float scale = __half2float(__ushort_as_half(static_cast<uint16_t>(scale_low)));
     const float low = __half2float(__ushort_as_half(static_cast<uint16_t>(scale_low >> 16)));

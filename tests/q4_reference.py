@@ -27,32 +27,40 @@ def cells64(x: torch.Tensor):
 
 def attend64(query, key, value, held, scaling):
     """One conversation: query [hq, n, d] of the tokens held .. held + n - 1 over key / value [hkv, held + n, d]
-    (16-bit tensors). Returns the output [n, hq, d] in float64 and, for tolerances, sum p |v| per output (with what
-    float16's subnormals may cut: see attend_tolerance) and the largest sum of a score's absolute terms per row."""
+    (16-bit tensors). Returns the output [n, hq, d] in float64 and what attend_tolerance goes by: the sums of
+    p * scale * code and of p * |low| per output, the largest sum of a score's absolute terms per row, the number of
+    tokens and the largest value scale."""
     hq, n, d = query.shape
     share = hq // key.shape[0]
     k, ks, kl = (t.repeat_interleave(share, 0) for t in cells64(key))
-    v = cells64(value)[0].repeat_interleave(share, 0)
+    v, vs, vl = (t.repeat_interleave(share, 0) for t in cells64(value))
+    vl = vl.repeat_interleave(GROUP, -1)
     q = query.double()
     scores = q @ k.transpose(1, 2) * scaling
     hidden = torch.arange(k.shape[1], device=q.device) > held + torch.arange(n, device=q.device)[:, None]
     p = torch.softmax(scores.masked_fill(hidden, -math.inf), -1)
     width = (15 * ks + kl.abs()).repeat_interleave(GROUP, -1)
     terms = (q.abs() @ width.transpose(1, 2) * scaling).masked_fill(hidden, 0.0).amax(-1)
-    cut = 2**-25 + k.shape[1] * 2**-32 * float(v.abs().max())
-    weight = p @ v.abs() + cut * 2**10
-    return (p @ v).transpose(0, 1), weight.transpose(0, 1), terms.transpose(0, 1)
+    parts = (p @ (v - vl)).transpose(0, 1), (p @ vl.abs()).transpose(0, 1), terms.transpose(0, 1), k.shape[1], float(vs.max())
+    return (p @ v).transpose(0, 1), parts
 
 
-def attend_tolerance(out, weight, terms, eps):
-    """Largest error of dkv_q4_attend against attend64. Probabilities and values are each rounded to float16 (half a
-    step: 2^-11 relative each) inside sums whose absolute terms add up to ``weight``. Below 2^-14 the half step is
-    2^-25: of a value, against probabilities that sum to 1; of a probability, which carries a factor of 2^7 or more
-    against its sum, 2^-32 of the largest value for every token; attend64 has both in ``weight`` (times 2^10, the
-    factor here being 2^-10). A score, a float32 sum of absolute terms ``terms`` in at most 2 * 128 additions whose
-    operands the tensor core may cut at 2^-22, is off by at most 2^-17 of them in all, which moves numerator and
-    denominator by that much each; the output is rounded once, to half a step of eps."""
-    return weight * (2 * 2**-11 + 2 * 2**-17 * terms[..., None] + 2**-16) + out.abs() * eps / 2 + 1e-12
+def attend_tolerance(out, parts, dtype, out_dtype):
+    """Largest error of dkv_q4_attend against attend64, for a cache of ``dtype``.
+
+    p * scale is rounded to float16 (half a step: 2^-11) in front of its code, or, for float16 caches, to two float16
+    numbers (2^-21 between them): that much of the sum of p * scale * code. Below 2^-14 the half step is 2^-25
+    instead, of p * 2^7 * scale / 2^k with 2^k at most 4 times the largest scale, times a code of at most 15: 2^-26
+    of the largest scale for every token. A score, a float32 sum of absolute terms ``terms`` in at most 2 * 128
+    additions whose operands the tensor core may cut at 2^-22, is off by at most 2^-17 of them in all, which moves
+    numerator and denominator by that much each. The float32 sums over tokens, chains of at most four products that
+    the tensor core may cut at 2^-22 each and float32 additions of their sums, a few hundred per warp, are good to
+    2^-16 of their absolute terms. The output is
+    rounded once, to half a step of its type."""
+    coded, low, terms, tokens, scale = parts
+    step = 2**-11 if dtype == torch.bfloat16 else 2**-21
+    return (coded * step + (coded + low) * (2 * 2**-17 * terms[..., None] + 2**-16) + tokens * 2**-26 * scale
+            + out.abs() * torch.finfo(out_dtype).eps / 2 + 1e-12)
 
 
 class PlainTable:

@@ -218,12 +218,12 @@ def _filled(n, q_heads, kv_heads, dim, dtype, held, counts, q_len, seed=0, chunk
     return batch, query, new[0], new[1], keys, values
 
 
-def _check(out, query, keys, values, held, counts, scaling, eps):
+def _check(out, query, keys, values, held, counts, scaling):
     for s, (h, c) in enumerate(zip(held, counts)):
         assert not out[s, c:].any()
         if c:
-            want, weight, terms = attend64(query[s, :, :c], keys[s, :, :h + c], values[s, :, :h + c], h, scaling)
-            err = (out[s, :c].double() - want).abs() - attend_tolerance(want, weight, terms, eps)
+            want, parts = attend64(query[s, :, :c], keys[s, :, :h + c], values[s, :, :h + c], h, scaling)
+            err = (out[s, :c].double() - want).abs() - attend_tolerance(want, parts, query.dtype, out.dtype)
             assert float(err.max()) <= 0, (s, float(err.max()))
 
 
@@ -252,9 +252,9 @@ def test_attention_over_cells(case, dtype):
     batch, query, k, v, keys, values = _filled(len(held), q_heads, kv_heads, dim, dtype, held, counts, q_len)
     scaling = dim ** -0.5
     out = batch.attend_layer(0, query, k, v, scaling)
-    _check(out, query, keys, values, held, counts, scaling, torch.finfo(dtype).eps)
+    _check(out, query, keys, values, held, counts, scaling)
     out32 = batch.attend_layer(0, query, None, None, scaling, out_dtype=torch.float32)
-    _check(out32, query, keys, values, held, counts, scaling, torch.finfo(torch.float32).eps)
+    _check(out32, query, keys, values, held, counts, scaling)
     assert torch.equal(out32.to(dtype), out)
     batch.check_status()
 
@@ -269,7 +269,7 @@ def test_attention_of_peaked_and_flat_rows():
     query[2] *= 2.0**-100
     query[3] *= 8
     out = batch.attend_layer(0, query, k, v, dim ** -0.5, out_dtype=torch.float32)
-    _check(out, query, keys, values, held, [1] * n, dim ** -0.5, torch.finfo(torch.float32).eps)
+    _check(out, query, keys, values, held, [1] * n, dim ** -0.5)
     ramp = torch.linspace(-4, 4, 3001, device=DEV)[:, None] * torch.ones(dim, device=DEV)
     batch, query, k, v, keys, values = _filled(n, 24, 8, dim, torch.bfloat16, held, [1] * n, 1, seed=6)
     batch.trim([0] * n)
@@ -280,7 +280,7 @@ def test_attention_of_peaked_and_flat_rows():
     batch.trim([3000] * n)
     batch.plan()
     out = batch.attend_layer(0, query, keys[:, :, -1:], values[:, :, -1:], dim ** -0.5, out_dtype=torch.float32)
-    _check(out, query, keys, values, held, [1] * n, dim ** -0.5, torch.finfo(torch.float32).eps)
+    _check(out, query, keys, values, held, [1] * n, dim ** -0.5)
     batch.check_status()
 
 
@@ -365,7 +365,7 @@ def test_far_pages_of_a_large_pool():
     batch.plan(None, 130)
     out = batch.attend_layer(0, q, k, v, 0.09)
     assert batch.table.blocks[0, :3].tolist() == [pages - 1, pages - 2, pages - 3]
-    _check(out, q, k, v, [0], [130], 0.09, torch.finfo(torch.bfloat16).eps)
+    _check(out, q, k, v, [0], [130], 0.09)
     a, b = batch.read(0)
     assert torch.equal(a, dequantise4(*quantise4(k)).to(k.dtype)) and torch.equal(b, dequantise4(*quantise4(v)).to(v.dtype))
     batch.check_status()
@@ -386,10 +386,9 @@ class _Checked:
         for store, x in ((self.keys, key), (self.values, value)):
             store[layer] = torch.cat(([store[layer]] if layer in store else []) + [x[0].to(dtype)], 1)
         held = self.keys[layer].shape[1] - query.shape[2]
-        want, weight, terms = attend64(query[0].to(dtype), self.keys[layer], self.values[layer], held, scaling)
-        eps = torch.finfo(out.dtype).eps
+        want, parts = attend64(query[0].to(dtype), self.keys[layer], self.values[layer], held, scaling)
         assert out.dtype == torch.promote_types(query.dtype, dtype) and out.shape[1:] == want.shape
-        assert float(((out[0].double() - want).abs() - attend_tolerance(want, weight, terms, eps)).max()) <= 0
+        assert float(((out[0].double() - want).abs() - attend_tolerance(want, parts, dtype, out.dtype)).max()) <= 0
         self.calls += 1
         return out, None
 
