@@ -1,18 +1,21 @@
 // logits.cu — the choice of the next token (dkv_logit_rules): penalties for repeated tokens, biases and a grammar
 // mask on a row of logits, and its largest entry.
 //
-// Eight CTAs of a cluster share a row, each a slice of the vocabulary. A CTA counts the history's tokens of its
-// slice in shared memory (one word per token: bit 31 = seen in the prompt, the low bits = times generated; integer
-// atomics, so the order does not matter), then passes over the slice's logits once: read, adjust, write, and keep
-// the largest as a 64-bit key (the float's order above, the inverted token below, so that equal values give the
-// lowest token). The slices' keys meet in distributed shared memory: one launch, no workspace in memory. Every
-// step is a single float32 operation with the rounding that the header's formulas state (no contraction), so that
-// the choice between near-equal tokens does not depend on the compiler. Bound by the logits' bytes.
+// Eight CTAs of a cluster share a row, each a slice of the vocabulary. The few tokens that a rule touches (those of
+// the history, and the biased ones) are separated from the many that none does: a CTA counts its slice's in
+// shared memory (a few flag bits and the times generated in one word per token; integer atomics, so their order
+// does not matter) and lists each at its first count. Then one pass over the slice, loaded ahead of the counting,
+// writes the untouched tokens with the mask alone, and a second, dense one goes over the list. The largest entry
+// is a 64-bit key (the float's order above, the inverted token below, so that equal values give the lowest
+// token); the slices' keys meet in distributed shared memory: one launch, no workspace in memory. Every step is a
+// single float32 operation with the rounding that the header's formulas state (no contraction), so that the choice
+// between near-equal tokens does not depend on the compiler. Bound by the logits' bytes.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "../../include/dimmer_kv.h"
+#include "dkv_launch.h"
 #include "dkv_ptx.cuh"
 
 namespace dkv {
@@ -20,8 +23,23 @@ namespace {
 
 constexpr int kRuleThreads = 512;
 constexpr int kRuleSplits = 8;       // CTAs of a row
-constexpr int kSlice = 16384;        // tokens that a CTA counts at a time
+constexpr int kVec = 8;              // tokens that a thread loads at a time
+constexpr int kHeld = 4;             // such loads that it holds
+constexpr int kSlice = kRuleThreads * kVec * kHeld - 32;  // tokens that a CTA takes at a time (a multiple of 32)
 constexpr int kMaxBias = 1024;
+
+// A token's word: seen in the prompt, biased, and the times generated. 16 bits where the history is short enough.
+template <typename W>
+struct Word {
+  static constexpr uint32_t kSeen = 1u << (8 * sizeof(W) - 1), kBiased = kSeen >> 1, kCount = kBiased - 1;
+  // Adds to the word of token `at`; true for the first to touch it.
+  static __device__ __forceinline__ bool add(W* words, uint32_t at, uint32_t flag, bool counted) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(words) + (sizeof(W) == 2 ? at >> 1 : at);
+    const int sh = sizeof(W) == 2 ? 16 * (at & 1) : 0;
+    const uint32_t old = counted ? atomicAdd(w, 1u << sh) : atomicOr(w, flag << sh);
+    return ((old >> sh) & (sizeof(W) == 2 ? 0xffffu : 0xffffffffu)) == 0;
+  }
+};
 
 __device__ __forceinline__ uint64_t order_key(float x, uint32_t token) {
   if (x == -INFINITY) return 0ull;
@@ -37,122 +55,143 @@ __device__ __forceinline__ float logit_at(const void* p, int64_t i) {
   return static_cast<const float*>(p)[i];
 }
 
-// Four logits from an address that is a multiple of four elements.
-template <int DT>
-__device__ __forceinline__ void logits4(const void* p, int64_t i, float (&x)[4]) {
-  if constexpr (DT == 2) {
-    const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-  } else {
-    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
-    const uint32_t w[2] = {v.x, v.y};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint16_t h = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
-      x[e] = DT == 0 ? __bfloat162float(__ushort_as_bfloat16(h)) : __half2float(__ushort_as_half(h));
-    }
-  }
-}
-
 struct RowRules {
   float repetition, frequency, presence;
 };
 
-__device__ __forceinline__ float adjust(float x, uint32_t word, float bias, bool biased, bool allowed, const RowRules& r) {
-  if (word != 0) {
-    x = x > 0.f ? __fdiv_rn(x, r.repetition) : __fmul_rn(x, r.repetition);
-    const uint32_t made = word & 0x7fffffffu;
-    if (made != 0) {
-      x = __fsub_rn(x, __fmul_rn(r.frequency, static_cast<float>(made)));
-      x = __fsub_rn(x, r.presence);
-    }
-  }
-  if (biased) x = __fadd_rn(x, bias);
-  return allowed ? x : -INFINITY;
-}
-
 template <int DT>
-__global__ void __cluster_dims__(kRuleSplits, 1, 1) __launch_bounds__(kRuleThreads)
-logit_rules_kernel(const dkv_logits_args a) {
+struct Raw {  // kVec logits as they lie in memory
+  uint4 v[DT == 2 ? 2 : 1];
+  __device__ __forceinline__ float get(int e) const {
+    const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[DT == 2].x, v[DT == 2].y, v[DT == 2].z, v[DT == 2].w};
+    if constexpr (DT == 2) return __uint_as_float(w[e]);
+    const uint16_t h = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+    return DT == 0 ? __bfloat162float(__ushort_as_bfloat16(h)) : __half2float(__ushort_as_half(h));
+  }
+};
+
+template <int DT, typename W>
+__global__ void __cluster_dims__(kRuleSplits, 1, 1) __launch_bounds__(kRuleThreads, 2)
+logit_rules_kernel(const __grid_constant__ dkv_logits_args a) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ uint64_t keys[kRuleThreads / 32];
   __shared__ uint64_t slice_key;
-  uint32_t* count = reinterpret_cast<uint32_t*>(smem);
-  float* bias = reinterpret_cast<float*>(smem + kSlice * 4);  // only with biases
+  __shared__ int listed;
+  constexpr int kWords = kSlice + 32;
+  W* words = reinterpret_cast<W*>(smem);
+  uint16_t* list = reinterpret_cast<uint16_t*>(smem + kWords * sizeof(W));
   const int row = blockIdx.x / kRuleSplits, rank = blockIdx.x % kRuleSplits;
   const int tid = threadIdx.x;
+  constexpr int kSize = DT == 2 ? 4 : 2;
+  const uint8_t* in = static_cast<const uint8_t*>(a.logits) + row * a.row_stride * kSize;
+  float* out = a.adjusted ? a.adjusted + static_cast<int64_t>(row) * a.vocab : nullptr;
+  const uint32_t* allowed = a.allowed ? a.allowed + static_cast<int64_t>(row) * ((a.vocab + 31) / 32) : nullptr;
+  const int per = ((a.vocab + kRuleSplits - 1) / kRuleSplits + 31) / 32 * 32;  // tokens of a CTA
+  const int end = min(a.vocab, (rank + 1) * per);
   const bool failed = cta_failed_at_entry(a.status);
-  const int length = failed ? 0 : max(0, min(a.lengths[row], a.capacity));
+  const int length = max(0, min(a.lengths[row], a.capacity));
   const int prompt = a.prompts[row];
   const int32_t* hist = a.history + static_cast<int64_t>(row) * a.capacity;
   const RowRules rules = {a.repetition[row], a.frequency[row], a.presence[row]};
-  const uint32_t* allowed = a.allowed ? a.allowed + static_cast<int64_t>(row) * ((a.vocab + 31) / 32) : nullptr;
-  const int esize = DT == 2 ? 4 : 2;
-  const uint8_t* in = static_cast<const uint8_t*>(a.logits) + row * a.row_stride * esize;
-  float* out = a.adjusted ? a.adjusted + static_cast<int64_t>(row) * a.vocab : nullptr;
-  // Four tokens at a time where the row starts on their boundary.
-  const bool wide = reinterpret_cast<uintptr_t>(in) % (4 * esize) == 0 &&
-                    (out == nullptr || reinterpret_cast<uintptr_t>(out) % 16 == 0);
-  const int per = ((a.vocab + kRuleSplits - 1) / kRuleSplits + 31) / 32 * 32;  // tokens of a CTA
-  const int end = min(a.vocab, (rank + 1) * per);
   uint64_t best = 0;
   for (int lo = rank * per; lo < end && !failed; lo += kSlice) {
     const int n = min(kSlice, end - lo);
+    // Place p of the slice is token lo - pad + p: vectors of kVec places start on 16-byte boundaries of the logits.
+    const int pad = static_cast<int>(reinterpret_cast<uintptr_t>(in + static_cast<int64_t>(lo) * kSize) / kSize % kVec);
+    const int first = lo - pad, last = pad + n;
+    const bool out_wide = out != nullptr && reinterpret_cast<uintptr_t>(out + first) % 16 == 0;
+    // ---- the slice's logits, on their way while the words are made
+    Raw<DT> raw[kHeld];
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int p = (k * kRuleThreads + tid) * kVec;
+      if (p >= pad && p + kVec <= last) {
+        const uint4* src = reinterpret_cast<const uint4*>(in + static_cast<int64_t>(first + p) * kSize);
+#pragma unroll
+        for (int h = 0; h < (DT == 2 ? 2 : 1); ++h) raw[k].v[h] = src[h];
+      }
+    }
     __syncthreads();
-    for (int i = tid; i < (n + 3) / 4; i += kRuleThreads) reinterpret_cast<uint4*>(count)[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (a.n_bias)
-      for (int i = tid; i < (n + 3) / 4; i += kRuleThreads)
-        reinterpret_cast<float4*>(bias)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int kFill = kWords * sizeof(W) / 16;
+    for (int i = tid; i < kFill; i += kRuleThreads) reinterpret_cast<uint4*>(words)[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (tid == 0) listed = 0;
     __syncthreads();
     for (int i = tid; i < length; i += kRuleThreads) {
       const uint32_t at = static_cast<uint32_t>(hist[i]) - static_cast<uint32_t>(lo);
       if (at < static_cast<uint32_t>(n)) {
-        if (i < prompt) atomicOr(&count[at], 0x80000000u);
-        else atomicAdd(&count[at], 1u);
+        const uint32_t p = at + pad;
+        if (Word<W>::add(words, p, Word<W>::kSeen, i >= prompt)) list[atomicAdd(&listed, 1)] = static_cast<uint16_t>(p);
       }
     }
-    if (a.n_bias) {
-      const int32_t* ids = a.bias_ids + static_cast<int64_t>(row) * a.n_bias;
-      const float* vals = a.bias_values + static_cast<int64_t>(row) * a.n_bias;
-      for (int i = tid; i < a.n_bias; i += kRuleThreads) {
-        const int id = ids[i];
-        const uint32_t at = static_cast<uint32_t>(id) - static_cast<uint32_t>(lo);
-        if (at >= static_cast<uint32_t>(n)) continue;
-        // the first entry of a token adds up all of them, in their order
-        bool first = true;
-        for (int k = 0; k < i && first; ++k) first = ids[k] != id;
-        if (!first) continue;
-        float sum = vals[i];
-        for (int k = i + 1; k < a.n_bias; ++k)
-          if (ids[k] == id) sum = __fadd_rn(sum, vals[k]);
-        bias[at] = sum;
+    const int32_t* ids = a.bias_ids + static_cast<int64_t>(row) * a.n_bias;
+    const float* values = a.bias_values + static_cast<int64_t>(row) * a.n_bias;
+    for (int i = tid; i < a.n_bias; i += kRuleThreads) {
+      const uint32_t at = static_cast<uint32_t>(ids[i]) - static_cast<uint32_t>(lo);
+      if (at < static_cast<uint32_t>(n)) {
+        const uint32_t p = at + pad;
+        if (Word<W>::add(words, p, Word<W>::kBiased, false)) list[atomicAdd(&listed, 1)] = static_cast<uint16_t>(p);
       }
     }
     __syncthreads();
-    const int n4 = wide ? n / 4 : 0;
-    for (int q = tid; q < n4; q += kRuleThreads) {
-      const int token = lo + q * 4;
-      float x[4];
-      logits4<DT>(in, token, x);
-      const uint4 w = reinterpret_cast<const uint4*>(count)[q];
-      const float4 b = a.n_bias ? reinterpret_cast<const float4*>(bias)[q] : make_float4(0.f, 0.f, 0.f, 0.f);
-      const uint32_t ok = allowed ? allowed[token >> 5] >> (token & 31) : 0xfu;
-      x[0] = adjust(x[0], w.x, b.x, b.x != 0.f, ok & 1u, rules);
-      x[1] = adjust(x[1], w.y, b.y, b.y != 0.f, ok & 2u, rules);
-      x[2] = adjust(x[2], w.z, b.z, b.z != 0.f, ok & 4u, rules);
-      x[3] = adjust(x[3], w.w, b.w, b.w != 0.f, ok & 8u, rules);
-      if (out) *reinterpret_cast<float4*>(out + token) = make_float4(x[0], x[1], x[2], x[3]);
+    // ---- the untouched tokens (what is written for the others is overwritten below)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint64_t key = order_key(x[e], token + e);
+    for (int k = 0; k < kHeld; ++k) {
+      const int p = (k * kRuleThreads + tid) * kVec;
+      if (p >= last) break;
+      const int token = first + p;
+      const bool whole = p >= pad && p + kVec <= last;
+      uint32_t ok = 0xffu;
+      if (allowed) {
+        const int at = max(token, 0), words_in = (a.vocab + 31) / 32;
+        const uint32_t w0 = allowed[at >> 5], w1 = (at >> 5) + 1 < words_in ? allowed[(at >> 5) + 1] : 0u;
+        ok = __funnelshift_r(w0, w1, at & 31) << (at - token);
+      }
+      float x[kVec];
+      uint32_t touched = 0;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        const bool here = whole || (p + e >= pad && p + e < last);
+        float v = 0.f;
+        if (whole) v = raw[k].get(e);
+        else if (here) v = logit_at<DT>(in, token + e);
+        x[e] = (ok >> e) & 1u ? v : -INFINITY;
+        touched |= (words[p + e] != 0 || !here ? 1u : 0u) << e;
+      }
+      if (whole && out_wide) {
+        reinterpret_cast<float4*>(out + token)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(out + token)[1] = make_float4(x[4], x[5], x[6], x[7]);
+      } else if (out != nullptr) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)
+          if (p + e >= pad && p + e < last) out[token + e] = x[e];
+      }
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        const uint64_t key = (touched >> e) & 1u ? 0ull : order_key(x[e], token + e);
         best = key > best ? key : best;
       }
     }
-    for (int i = n4 * 4 + tid; i < n; i += kRuleThreads) {
-      const int token = lo + i;
-      const float b = a.n_bias ? bias[i] : 0.f;
-      const bool ok = allowed == nullptr || (allowed[token >> 5] >> (token & 31)) & 1u;
-      const float x = adjust(logit_at<DT>(in, token), count[i], b, b != 0.f, ok, rules);
+    __syncthreads();
+    // ---- the touched ones
+    for (int i = tid; i < listed; i += kRuleThreads) {
+      const int p = list[i], token = first + p;
+      const uint32_t word = words[p];
+      float x = logit_at<DT>(in, token);
+      if (word & ~Word<W>::kBiased) {
+        x = x > 0.f ? __fdiv_rn(x, rules.repetition) : __fmul_rn(x, rules.repetition);
+        const uint32_t made = word & Word<W>::kCount;
+        if (made != 0) {
+          x = __fsub_rn(x, __fmul_rn(rules.frequency, static_cast<float>(made)));
+          x = __fsub_rn(x, rules.presence);
+        }
+      }
+      if (word & Word<W>::kBiased) {
+        float sum = 0.f;
+        for (int k = 0; k < a.n_bias; ++k)
+          if (ids[k] == token) sum = __fadd_rn(sum, values[k]);
+        x = __fadd_rn(x, sum);
+      }
+      if (allowed && !((allowed[token >> 5] >> (token & 31)) & 1u)) x = -INFINITY;
       if (out) out[token] = x;
       const uint64_t key = order_key(x, token);
       best = key > best ? key : best;
@@ -200,6 +239,19 @@ logit_rules_kernel(const dkv_logits_args a) {
   cluster_sync_all();  // no CTA leaves while its key is read
 }
 
+template <int DT, typename W>
+int launch_rules(const dkv_logits_args& a, cudaStream_t stream) {
+  // Every touched token of a slice has a place in the list.
+  const int64_t touched = static_cast<int64_t>(a.capacity) + a.n_bias;
+  const int room = static_cast<int>(touched < kSlice ? touched : kSlice);
+  const int bytes = (kSlice + 32) * static_cast<int>(sizeof(W)) + (room * 2 + 15) / 16 * 16;
+  auto kernel = logit_rules_kernel<DT, W>;
+  static std::atomic<uint64_t> done{0};
+  if (!allow_shared(kernel, (kSlice + 32) * (static_cast<int>(sizeof(W)) + 2), done)) return DKV_ERR_CUDA;
+  kernel<<<a.n_rows * kRuleSplits, kRuleThreads, bytes, stream>>>(a);
+  return cudaGetLastError() == cudaSuccess ? DKV_OK : DKV_ERR_CUDA;
+}
+
 }  // namespace
 }  // namespace dkv
 
@@ -214,10 +266,13 @@ extern "C" int dkv_logit_rules(const dkv_logits_args* a, void* stream) {
   if (a->n_bias > dkv::kMaxBias || a->vocab > (1 << 30) || a->n_rows > (INT32_MAX / dkv::kRuleSplits))
     return DKV_ERR_CONFIG;
   if (a->n_rows == 0) return DKV_OK;
-  auto kernel = a->dtype == 0 ? dkv::logit_rules_kernel<0> : a->dtype == 1 ? dkv::logit_rules_kernel<1> : dkv::logit_rules_kernel<2>;
-  const int bytes = dkv::kSlice * (a->n_bias ? 8 : 4);
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, dkv::kSlice * 8) != cudaSuccess)
-    return DKV_ERR_CUDA;
-  kernel<<<a->n_rows * dkv::kRuleSplits, dkv::kRuleThreads, bytes, static_cast<cudaStream_t>(stream)>>>(*a);
-  return cudaGetLastError() == cudaSuccess ? DKV_OK : DKV_ERR_CUDA;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // 14 bits count what a history of at most 16383 tokens can repeat; the halved words leave room for twice the CTAs.
+  if (a->capacity <= 16383)
+    return a->dtype == 0   ? dkv::launch_rules<0, uint16_t>(*a, st)
+           : a->dtype == 1 ? dkv::launch_rules<1, uint16_t>(*a, st)
+                           : dkv::launch_rules<2, uint16_t>(*a, st);
+  return a->dtype == 0   ? dkv::launch_rules<0, uint32_t>(*a, st)
+         : a->dtype == 1 ? dkv::launch_rules<1, uint32_t>(*a, st)
+                         : dkv::launch_rules<2, uint32_t>(*a, st);
 }

@@ -27,6 +27,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "dkv_launch.h"
 #include "dkv_ptx.cuh"
 #include "q4_cells.cuh"
 
@@ -763,18 +764,12 @@ q4_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int 
   store_out4<F16>(a, to, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
 int rows_of(const dkv_q4_attend_args& a) { return a.q_len * (a.n_q_heads / a.n_kv_heads); }
 int tiles_of(const dkv_q4_attend_args& a) { return rows_of(a) <= 8 ? 1 : 2; }  // of 8 query rows that a warp holds
 
 int64_t floats_of(const dkv_q4_attend_args& a) {
   const int rows = rows_of(a), held = rows < 8 * tiles_of(a) ? rows : 8 * tiles_of(a);
-  return 2 * static_cast<int64_t>(sm_count() * 3 * kWarps) * slot_floats(held, a.head_dim);
+  return 2 * static_cast<int64_t>(device_sms() * 3 * kWarps) * slot_floats(held, a.head_dim);
 }
 
 template <int D, int NT, bool F16>
@@ -783,12 +778,13 @@ int launch_decode(const dkv_q4_attend_args& a, int append, cudaStream_t stream) 
   if (static_cast<int64_t>(a.n_kv_heads) > 65535) return DKV_ERR_CONFIG;
   // At most one worker per page that there can be.
   const int64_t pages = static_cast<int64_t>((a.len_bound + q4::kPage - 1) / q4::kPage) * a.n_seq * a.n_kv_heads * chunks;
-  const int most = sm_count() * Decode<D, NT>::kBlocksPerSm;
+  const int most = device_sms() * Decode<D, NT>::kBlocksPerSm;
   const int ctas = pages < most ? (pages < 1 ? 1 : static_cast<int>(pages)) : most;
   const int workers = ctas * kWarps;
   auto kernel = q4_decode_kernel<D, NT, F16>;
   constexpr int bytes = Decode<D, NT>::kBytes;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return DKV_ERR_CUDA;
+  static std::atomic<uint64_t> done{0};
+  if (!allow_shared(kernel, bytes, done)) return DKV_ERR_CUDA;
   kernel<<<ctas, kThreads, bytes, stream>>>(a, chunks, workers, append);
   if (cudaGetLastError() != cudaSuccess) return DKV_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};

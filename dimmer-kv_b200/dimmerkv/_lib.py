@@ -253,18 +253,33 @@ DEVICE_SITES = {1: "key_scores_pair", 2: "key_scores", 3: "value_weights", 4: "v
                 6: "key_scores_dense", 7: "q4_attend", 8: "q4_append / q4_read", 9: "page tables"}
 
 
-def launch(name: str, args, device) -> None:
-    """Enqueue entry point ``name`` on the current stream of ``device``, whichever device is current."""
+_ENTRY: dict = {}
+
+
+def _raw_stream(index: int) -> int:
     import torch
 
-    fn = getattr(lib(), name)
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
-        rc = fn(args, stream)
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+def launch(name: str, args, device) -> None:
+    """Enqueue entry point ``name`` on the current stream of ``device``, whichever device is current."""
+    entry = _ENTRY.get(name)
+    if entry is None:
+        import torch
+
+        # the stream's handle without a Stream object around it, where this torch has that
+        stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+        entry = _ENTRY[name] = (getattr(lib(), name), torch.cuda.current_device, stream, torch.cuda.device)
+    fn, current, stream, switch = entry
+    index = device.index
+    if current() == index:
+        rc = fn(args, stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(args, stream)
-    check(rc, name)
+        with switch(index):
+            rc = fn(args, stream(index))
+    if rc != DKV_OK:
+        check(rc, name)
 
 
 def cuda_device(device):

@@ -91,7 +91,7 @@ class Q4Batch:
         a.fp16, a.blocks, a.max_blocks = r.fp16, self.table.blocks.data_ptr(), self.table.max_blocks
         a.lengths, a.starts, a.n_seq = self.table.lengths.data_ptr(), self.table.starts.data_ptr(), n_seq
         a.status = self.status.data_ptr()
-        self._floats: dict[int, int] = {}  # workspace of dkv_q4_attend by q_len
+        self._calls: dict[tuple, _lib.Q4AttendArgs] = {}
         self._layer_bytes = self.cells[0].numel()
         self._cells_ptr = self.cells.data_ptr()
 
@@ -120,22 +120,24 @@ class Q4Batch:
             raise ValueError(f"layer {layer} of {self.layers}")
         return self._cells_ptr + layer * self._layer_bytes
 
-    def _tensor(self, name: str, x: torch.Tensor, heads: int, rows: int) -> torch.Tensor:
+    def _tensor(self, name: str, x: torch.Tensor, heads: int, rows: int):
+        """x [n_seq, heads, rows, head_dim] as the kernels take it, and its strides."""
         if x.shape != (self.n_seq, heads, rows, self.head_dim):
             raise ValueError(f"{name} {tuple(x.shape)} is not [{self.n_seq}, {heads}, {rows}, {self.head_dim}]")
         if x.device != self.device:
             raise ValueError(f"{name} is on {x.device}, the cache on {self.device}")
-        if x.dtype != self.dtype:
+        if x.dtype is not self.dtype:
             x = x.to(self.dtype)
-        if x.data_ptr() % 16 or any(x.stride(d) % 8 and x.shape[d] > 1 for d in range(3)) or x.stride(3) != 1:
-            x = x.contiguous()
-            if x.data_ptr() % 16:
-                x = x.clone()
-        return x
-
-    @staticmethod
-    def _strides(x: torch.Tensor):
-        return tuple(x.stride(d) if x.shape[d] > 1 else 0 for d in range(3))
+        strides = x.stride()
+        if strides[3] != 1 or (strides[0] | strides[1] | strides[2]) % 8 or x.data_ptr() % 16:
+            # the stride of a dimension of one is free
+            strides = tuple(s if n > 1 else 0 for s, n in zip(strides, x.shape[:3])) + (strides[3],)
+            if strides[3] != 1 or (strides[0] | strides[1] | strides[2]) % 8 or x.data_ptr() % 16:
+                x = x.contiguous()
+                if x.data_ptr() % 16:
+                    x = x.clone()
+                strides = x.stride()
+        return x, strides[:3]
 
     def append(self, layer: int, key: torch.Tensor, value: torch.Tensor) -> None:
         """Store key / value [n_seq, kv_heads, q_len, head_dim] of the planned tokens in one layer's cells."""
@@ -143,12 +145,11 @@ class Q4Batch:
             raise RuntimeError("append needs the slots of a plan")
         cells = self._layer(layer)
         q_len = self._slots.shape[1]
-        key = self._tensor("key", key, self.kv_heads, q_len)
-        value = self._tensor("value", value, self.kv_heads, q_len)
         a = _lib.Q4RowsArgs.from_buffer_copy(self._rows)
+        key, a.k_stride = self._tensor("key", key, self.kv_heads, q_len)
+        value, a.v_stride = self._tensor("value", value, self.kv_heads, q_len)
         a.cells, a.slots, a.q_len = cells, self._slots.data_ptr(), q_len
         a.key, a.value = key.data_ptr(), value.data_ptr()
-        a.k_stride, a.v_stride = self._strides(key), self._strides(value)
         _lib.launch("dkv_q4_append", a, self.device)
 
     def read(self, layer: int, slots: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -166,7 +167,7 @@ class Q4Batch:
                                  device=self.device).unbind(0)
         a.cells, a.slots, a.q_len = self._layer(layer), slots.data_ptr(), n
         a.key, a.value = key.data_ptr(), value.data_ptr()
-        a.k_stride = a.v_stride = self._strides(key)
+        a.k_stride = a.v_stride = key.stride()[:3]
         _lib.launch("dkv_q4_read", a, self.device)
         return key, value
 
@@ -185,22 +186,29 @@ class Q4Batch:
         if self._slots is None:
             raise RuntimeError("attend_layer needs a plan")
         q_len = self._slots.shape[1]
-        query = self._tensor("query", query, self.q_heads, q_len)
-        out = torch.empty(self.n_seq, q_len, self.q_heads, self.head_dim, dtype=out_dtype, device=self.device)
-        a = _lib.Q4AttendArgs.from_buffer_copy(self._attend)
-        a.cells, a.q_len, a.len_bound = self._layer(layer), q_len, self.table.bound
-        a.query, a.q_stride, a.scaling = query.data_ptr(), self._strides(query), float(scaling)
+        query, q_stride = self._tensor("query", query, self.q_heads, q_len)
+        strides = (q_len, out_dtype, q_stride)
         if key is not None:
-            key = self._tensor("key", key, self.kv_heads, q_len)
-            value = self._tensor("value", value, self.kv_heads, q_len)
+            key, k_stride = self._tensor("key", key, self.kv_heads, q_len)
+            value, v_stride = self._tensor("value", value, self.kv_heads, q_len)
+            strides += (k_stride, v_stride)
+        made = self._calls.get(strides)
+        if made is None:  # what stays the same from call to call of this form
+            made = _lib.Q4AttendArgs.from_buffer_copy(self._attend)
+            made.q_len, made.q_stride, made.out_f32 = q_len, q_stride, int(out_dtype == torch.float32)
+            if key is not None:
+                made.k_stride, made.v_stride = k_stride, v_stride
+            made.workspace_floats = int(self.lib.dkv_q4_attend_floats(made))
+            if len(self._calls) > 64:
+                self._calls.clear()
+            self._calls[strides] = made
+        a = _lib.Q4AttendArgs.from_buffer_copy(made)
+        out = torch.empty((self.n_seq, q_len, self.q_heads, self.head_dim), dtype=out_dtype, device=self.device)
+        workspace = torch.empty(a.workspace_floats, dtype=torch.float32, device=self.device)
+        a.cells, a.len_bound, a.scaling = self._layer(layer), self.table.bound, scaling
+        a.query, a.out, a.workspace = query.data_ptr(), out.data_ptr(), workspace.data_ptr()
+        if key is not None:
             a.key, a.value, a.slots = key.data_ptr(), value.data_ptr(), self._slots.data_ptr()
-            a.k_stride, a.v_stride = self._strides(key), self._strides(value)
-        a.out, a.out_f32 = out.data_ptr(), int(out_dtype == torch.float32)
-        floats = self._floats.get(q_len)
-        if floats is None:
-            floats = self._floats[q_len] = int(self.lib.dkv_q4_attend_floats(a))
-        workspace = torch.empty(floats, dtype=torch.float32, device=self.device)
-        a.workspace, a.workspace_floats = workspace.data_ptr(), floats
         _lib.launch("dkv_q4_attend", a, self.device)
         return out
 
