@@ -1,7 +1,7 @@
 // logits.cu — the choice of the next token (dkv_logit_rules): penalties for repeated tokens, biases and a grammar
 // mask on a row of logits, and its largest entry.
 //
-// Eight CTAs of a cluster share a row, each a slice of the vocabulary. The few tokens that a rule touches (those of
+// The four or eight CTAs of a cluster share a row, each a slice of the vocabulary. The few tokens that a rule touches (those of
 // the history, and the biased ones) are separated from the many that none does: a CTA counts its slice's in
 // shared memory (a few flag bits and the times generated in one word per token; integer atomics, so their order
 // does not matter) and lists each at its first count. Then one pass over the slice, loaded ahead of the counting,
@@ -22,10 +22,10 @@ namespace dkv {
 namespace {
 
 constexpr int kRuleThreads = 512;
-constexpr int kRuleSplits = 8;       // CTAs of a row
+constexpr int kMaxSplits = 8;        // CTAs of a row
 constexpr int kVec = 8;              // tokens that a thread loads at a time
-constexpr int kHeld = 4;             // such loads that it holds
-constexpr int kSlice = kRuleThreads * kVec * kHeld - 32;  // tokens that a CTA takes at a time (a multiple of 32)
+constexpr int kMaxSlice = 32768;     // tokens that a CTA takes at a time, at most
+constexpr int kPast = 8;             // tokens of the history that a thread holds
 constexpr int kMaxBias = 1024;
 
 // A token's word: seen in the prompt, biased, and the times generated. 16 bits where the history is short enough.
@@ -48,11 +48,28 @@ __device__ __forceinline__ uint64_t order_key(float x, uint32_t token) {
   return static_cast<uint64_t>(b) << 32 | (0xffffffffu - token);
 }
 
+__device__ __forceinline__ float max_nan(float x, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+
 template <int DT>
 __device__ __forceinline__ float logit_at(const void* p, int64_t i) {
   if constexpr (DT == 0) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
   if constexpr (DT == 1) return __half2float(static_cast<const __half*>(p)[i]);
   return static_cast<const float*>(p)[i];
+}
+
+// The places of the lanes with `fresh` go to the end of the list, with one addition for the warp.
+__device__ __forceinline__ void append_place(bool fresh, uint32_t place, uint16_t* list, int* listed) {
+  const uint32_t who = __ballot_sync(0xffffffffu, fresh);
+  if (who == 0) return;
+  const int lane = threadIdx.x & 31;
+  int at = 0;
+  if (lane == 0) at = atomicAdd(listed, __popc(who));
+  at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1));
+  if (fresh) list[at] = static_cast<uint16_t>(place);
 }
 
 struct RowRules {
@@ -71,91 +88,107 @@ struct Raw {  // kVec logits as they lie in memory
 };
 
 template <int DT, typename W>
-__global__ void __cluster_dims__(kRuleSplits, 1, 1) __launch_bounds__(kRuleThreads, 2)
-logit_rules_kernel(const __grid_constant__ dkv_logits_args a) {
+__global__ void __launch_bounds__(kRuleThreads, 2)
+logit_rules_kernel(const __grid_constant__ dkv_logits_args a, int splits, int slice) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ uint64_t keys[kRuleThreads / 32];
   __shared__ uint64_t slice_key;
   __shared__ int listed;
-  constexpr int kWords = kSlice + 32;
-  W* words = reinterpret_cast<W*>(smem);
-  uint16_t* list = reinterpret_cast<uint16_t*>(smem + kWords * sizeof(W));
-  const int row = blockIdx.x / kRuleSplits, rank = blockIdx.x % kRuleSplits;
+  W* words = reinterpret_cast<W*>(smem);  // [slice + 32]
+  uint16_t* list = reinterpret_cast<uint16_t*>(smem + (slice + 32) * sizeof(W));
+  const int row = blockIdx.x / splits, rank = blockIdx.x % splits;
   const int tid = threadIdx.x;
-  constexpr int kSize = DT == 2 ? 4 : 2;
+  constexpr int kSize = DT == 2 ? 4 : 2, kHeld = DT == 2 ? 2 : 4;  // loads that a thread has under way
   const uint8_t* in = static_cast<const uint8_t*>(a.logits) + row * a.row_stride * kSize;
   float* out = a.adjusted ? a.adjusted + static_cast<int64_t>(row) * a.vocab : nullptr;
   const uint32_t* allowed = a.allowed ? a.allowed + static_cast<int64_t>(row) * ((a.vocab + 31) / 32) : nullptr;
-  const int per = ((a.vocab + kRuleSplits - 1) / kRuleSplits + 31) / 32 * 32;  // tokens of a CTA
+  const int per = ((a.vocab + splits - 1) / splits + 31) / 32 * 32;  // tokens of a CTA
   const int end = min(a.vocab, (rank + 1) * per);
-  const bool failed = cta_failed_at_entry(a.status);
   const int length = max(0, min(a.lengths[row], a.capacity));
   const int prompt = a.prompts[row];
   const int32_t* hist = a.history + static_cast<int64_t>(row) * a.capacity;
   const RowRules rules = {a.repetition[row], a.frequency[row], a.presence[row]};
+  // The history comes kPast tokens a thread at a time, all of them under way before the first is counted.
+  int32_t past[kPast];
+  auto fetch_past = [&](int base) {
+#pragma unroll
+    for (int k = 0; k < kPast; ++k) {
+      const int i = base + k * kRuleThreads + tid;
+      past[k] = i < length ? hist[i] : -1;
+    }
+  };
+  fetch_past(0);
+  const bool failed = cta_failed_at_entry(a.status);
   uint64_t best = 0;
-  for (int lo = rank * per; lo < end && !failed; lo += kSlice) {
-    const int n = min(kSlice, end - lo);
+  float top = -INFINITY;  // of the thread's untouched tokens, in ascending order: the first of equal ones stays
+  int top_at = 0;
+  for (int lo = rank * per; lo < end && !failed; lo += slice) {
+    const int n = min(slice, end - lo);
     // Place p of the slice is token lo - pad + p: vectors of kVec places start on 16-byte boundaries of the logits.
     const int pad = static_cast<int>(reinterpret_cast<uintptr_t>(in + static_cast<int64_t>(lo) * kSize) / kSize % kVec);
     const int first = lo - pad, last = pad + n;
     const bool out_wide = out != nullptr && reinterpret_cast<uintptr_t>(out + first) % 16 == 0;
-    // ---- the slice's logits, on their way while the words are made
+    // ---- the first of the slice's logits, on their way while the words are made
     Raw<DT> raw[kHeld];
-#pragma unroll
-    for (int k = 0; k < kHeld; ++k) {
-      const int p = (k * kRuleThreads + tid) * kVec;
+    auto fetch = [&](int p, Raw<DT>& r) {
       if (p >= pad && p + kVec <= last) {
         const uint4* src = reinterpret_cast<const uint4*>(in + static_cast<int64_t>(first + p) * kSize);
 #pragma unroll
-        for (int h = 0; h < (DT == 2 ? 2 : 1); ++h) raw[k].v[h] = src[h];
+        for (int h = 0; h < (DT == 2 ? 2 : 1); ++h) r.v[h] = src[h];
       }
-    }
+    };
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) fetch((k * kRuleThreads + tid) * kVec, raw[k]);
     __syncthreads();
-    constexpr int kFill = kWords * sizeof(W) / 16;
-    for (int i = tid; i < kFill; i += kRuleThreads) reinterpret_cast<uint4*>(words)[i] = make_uint4(0u, 0u, 0u, 0u);
+    const int fill = (n + 32) * static_cast<int>(sizeof(W)) / 16;
+    for (int i = tid; i <= fill; i += kRuleThreads) reinterpret_cast<uint4*>(words)[i] = make_uint4(0u, 0u, 0u, 0u);
     if (tid == 0) listed = 0;
     __syncthreads();
-    for (int i = tid; i < length; i += kRuleThreads) {
-      const uint32_t at = static_cast<uint32_t>(hist[i]) - static_cast<uint32_t>(lo);
-      if (at < static_cast<uint32_t>(n)) {
-        const uint32_t p = at + pad;
-        if (Word<W>::add(words, p, Word<W>::kSeen, i >= prompt)) list[atomicAdd(&listed, 1)] = static_cast<uint16_t>(p);
+    for (int base = 0; base < length; base += kPast * kRuleThreads) {
+      if (base > 0 || lo != rank * per) fetch_past(base);
+#pragma unroll
+      for (int k = 0; k < kPast; ++k) {
+        const uint32_t at = static_cast<uint32_t>(past[k]) - static_cast<uint32_t>(lo);
+        const uint32_t place = at + pad;
+        const bool fresh = at < static_cast<uint32_t>(n) &&
+                           Word<W>::add(words, place, Word<W>::kSeen, base + k * kRuleThreads + tid >= prompt);
+        append_place(fresh, place, list, &listed);
       }
     }
     const int32_t* ids = a.bias_ids + static_cast<int64_t>(row) * a.n_bias;
     const float* values = a.bias_values + static_cast<int64_t>(row) * a.n_bias;
-    for (int i = tid; i < a.n_bias; i += kRuleThreads) {
-      const uint32_t at = static_cast<uint32_t>(ids[i]) - static_cast<uint32_t>(lo);
-      if (at < static_cast<uint32_t>(n)) {
-        const uint32_t p = at + pad;
-        if (Word<W>::add(words, p, Word<W>::kBiased, false)) list[atomicAdd(&listed, 1)] = static_cast<uint16_t>(p);
-      }
+    for (int base = 0; base < a.n_bias; base += kRuleThreads) {
+      const int i = base + tid;
+      const uint32_t at = i < a.n_bias ? static_cast<uint32_t>(ids[i]) - static_cast<uint32_t>(lo) : 0xffffffffu;
+      const uint32_t place = at + pad;
+      const bool fresh = at < static_cast<uint32_t>(n) && Word<W>::add(words, place, Word<W>::kBiased, false);
+      append_place(fresh, place, list, &listed);
     }
     __syncthreads();
     // ---- the untouched tokens (what is written for the others is overwritten below)
+    for (int k0 = 0; k0 * kRuleThreads * kVec < last; k0 += kHeld)
 #pragma unroll
     for (int k = 0; k < kHeld; ++k) {
-      const int p = (k * kRuleThreads + tid) * kVec;
+      const int p = ((k0 + k) * kRuleThreads + tid) * kVec;
       if (p >= last) break;
       const int token = first + p;
       const bool whole = p >= pad && p + kVec <= last;
-      uint32_t ok = 0xffu;
+      float x[kVec];
+      if (whole) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) x[e] = raw[k].get(e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) x[e] = p + e >= pad && p + e < last ? logit_at<DT>(in, token + e) : -INFINITY;
+      }
+      fetch(p + kHeld * kRuleThreads * kVec, raw[k]);
       if (allowed) {
         const int at = max(token, 0), words_in = (a.vocab + 31) / 32;
         const uint32_t w0 = allowed[at >> 5], w1 = (at >> 5) + 1 < words_in ? allowed[(at >> 5) + 1] : 0u;
-        ok = __funnelshift_r(w0, w1, at & 31) << (at - token);
-      }
-      float x[kVec];
-      uint32_t touched = 0;
+        const uint32_t ok = __funnelshift_r(w0, w1, at & 31) << (at - token);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        const bool here = whole || (p + e >= pad && p + e < last);
-        float v = 0.f;
-        if (whole) v = raw[k].get(e);
-        else if (here) v = logit_at<DT>(in, token + e);
-        x[e] = (ok >> e) & 1u ? v : -INFINITY;
-        touched |= (words[p + e] != 0 || !here ? 1u : 0u) << e;
+        for (int e = 0; e < kVec; ++e)
+          if (!(ok & (1u << e))) x[e] = -INFINITY;
       }
       if (whole && out_wide) {
         reinterpret_cast<float4*>(out + token)[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -165,17 +198,32 @@ logit_rules_kernel(const __grid_constant__ dkv_logits_args a) {
         for (int e = 0; e < kVec; ++e)
           if (p + e >= pad && p + e < last) out[token + e] = x[e];
       }
+      uint32_t any = 0;
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        const uint64_t key = (touched >> e) & 1u ? 0ull : order_key(x[e], token + e);
-        best = key > best ? key : best;
+      for (int h = 0; h < static_cast<int>(sizeof(W)) / 2; ++h) {
+        const uint4 w = reinterpret_cast<const uint4*>(words + p)[h];
+        any |= w.x | w.y | w.z | w.w;
+      }
+      if (any != 0) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)
+          if (words[p + e] != 0) x[e] = -INFINITY;
+      }
+      float m = x[0];
+#pragma unroll
+      for (int e = 1; e < kVec; ++e) m = max_nan(m, x[e]);
+      if (!(m <= top)) {  // larger, or a NaN: rare
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)
+          if (top == top && !(x[e] <= top)) {
+            top = x[e];
+            top_at = token + e;
+          }
       }
     }
     __syncthreads();
     // ---- the touched ones
-    for (int i = tid; i < listed; i += kRuleThreads) {
-      const int p = list[i], token = first + p;
-      const uint32_t word = words[p];
+    auto finish = [&](int token, uint32_t word, float bias) {
       float x = logit_at<DT>(in, token);
       if (word & ~Word<W>::kBiased) {
         x = x > 0.f ? __fdiv_rn(x, rules.repetition) : __fmul_rn(x, rules.repetition);
@@ -185,18 +233,36 @@ logit_rules_kernel(const __grid_constant__ dkv_logits_args a) {
           x = __fsub_rn(x, rules.presence);
         }
       }
-      if (word & Word<W>::kBiased) {
-        float sum = 0.f;
-        for (int k = 0; k < a.n_bias; ++k)
-          if (ids[k] == token) sum = __fadd_rn(sum, values[k]);
-        x = __fadd_rn(x, sum);
-      }
+      if (word & Word<W>::kBiased) x = __fadd_rn(x, bias);
       if (allowed && !((allowed[token >> 5] >> (token & 31)) & 1u)) x = -INFINITY;
       if (out) out[token] = x;
       const uint64_t key = order_key(x, token);
       best = key > best ? key : best;
+    };
+    for (int i = tid; i < listed; i += kRuleThreads) {
+      const int p = list[i];
+      const uint32_t word = words[p];
+      if (!(word & Word<W>::kBiased)) finish(first + p, word, 0.f);
+    }
+    // The first entry of a biased token takes it, with the sum of all its entries in their order. The last warps begin:
+    // the list keeps the first ones busy.
+    for (int i = kRuleThreads - 1 - tid; i < a.n_bias; i += kRuleThreads) {
+      const int id = ids[i];
+      const uint32_t at = static_cast<uint32_t>(id) - static_cast<uint32_t>(lo);
+      if (at >= static_cast<uint32_t>(n)) continue;
+      bool before = false;
+      float sum = 0.f;
+#pragma unroll 8
+      for (int k = 0; k < a.n_bias; ++k) {
+        const bool same = ids[k] == id;
+        before = before || (same && k < i);
+        sum = same ? __fadd_rn(sum, values[k]) : sum;
+      }
+      if (!before) finish(id, words[at + pad], sum);
     }
   }
+  const uint64_t top_key = order_key(top, top_at);
+  best = top_key > best ? top_key : best;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) {
     const uint64_t other = __shfl_xor_sync(0xffffffffu, best, d);
@@ -212,7 +278,7 @@ logit_rules_kernel(const __grid_constant__ dkv_logits_args a) {
   cluster_sync_all();  // every CTA's key is there, and every CTA has read the history
   if (rank == 0 && tid < 32) {
     uint64_t key = 0;
-    if (tid < kRuleSplits) {
+    if (tid < splits) {
       const uint32_t addr = mapa_shared(smem_u32(&slice_key), tid);
       asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key) : "r"(addr) : "memory");
     }
@@ -241,15 +307,32 @@ logit_rules_kernel(const __grid_constant__ dkv_logits_args a) {
 
 template <int DT, typename W>
 int launch_rules(const dkv_logits_args& a, cudaStream_t stream) {
+  // Where clusters of eight would come in a second wave of CTAs, clusters of four with slices twice as long do not (two
+  // CTAs per SM), and go through the history half as often: 64 rows of 128256 take 24 us against 34, 40 rows 24
+  // against 31; one row has 8.0 us with eight. 32-bit words allow half the slice.
+  const int splits = a.n_rows * kMaxSplits <= 2 * device_sms() ? kMaxSplits : kMaxSplits / 2;
+  const int most = sizeof(W) == 2 ? kMaxSlice : kMaxSlice / 2;
+  const int per = ((a.vocab + splits - 1) / splits + 31) / 32 * 32;
+  const int slice = per < most ? per : most;
   // Every touched token of a slice has a place in the list.
   const int64_t touched = static_cast<int64_t>(a.capacity) + a.n_bias;
-  const int room = static_cast<int>(touched < kSlice ? touched : kSlice);
-  const int bytes = (kSlice + 32) * static_cast<int>(sizeof(W)) + (room * 2 + 15) / 16 * 16;
+  const int room = static_cast<int>(touched < slice ? touched : slice);
   auto kernel = logit_rules_kernel<DT, W>;
   static std::atomic<uint64_t> done{0};
-  if (!allow_shared(kernel, (kSlice + 32) * (static_cast<int>(sizeof(W)) + 2), done)) return DKV_ERR_CUDA;
-  kernel<<<a.n_rows * kRuleSplits, kRuleThreads, bytes, stream>>>(a);
-  return cudaGetLastError() == cudaSuccess ? DKV_OK : DKV_ERR_CUDA;
+  if (!allow_shared(kernel, (most + 40) * static_cast<int>(sizeof(W)) + most * 2 + 16, done)) return DKV_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.n_rows * splits);
+  cfg.blockDim = dim3(kRuleThreads);
+  cfg.dynamicSmemBytes = (slice + 32) * static_cast<int>(sizeof(W)) + (room * 2 + 15) / 16 * 16 + 16;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a, splits, slice) == cudaSuccess ? DKV_OK : DKV_ERR_CUDA;
 }
 
 }  // namespace
@@ -263,7 +346,7 @@ extern "C" int dkv_logit_rules(const dkv_logits_args* a, void* stream) {
   if (a->n_rows < 0 || a->vocab < 1 || a->capacity < 1 || a->n_bias < 0 || a->row_stride < 0 || a->dtype < 0 ||
       a->dtype > 2 || (a->n_bias > 0 && (a->bias_ids == nullptr || a->bias_values == nullptr)))
     return DKV_ERR_ARGS;
-  if (a->n_bias > dkv::kMaxBias || a->vocab > (1 << 30) || a->n_rows > (INT32_MAX / dkv::kRuleSplits))
+  if (a->n_bias > dkv::kMaxBias || a->vocab > (1 << 30) || a->n_rows > (INT32_MAX / dkv::kMaxSplits))
     return DKV_ERR_CONFIG;
   if (a->n_rows == 0) return DKV_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -17,9 +17,9 @@
 //
 // Quantising: eight lanes hold a group of 64 dimensions, eight each; minimum and maximum are three shuffles, a
 // lane's eight key codes are exactly one word of the key cell, its value codes the halves of two words of the pair's.
-// The code is the nearest whole number to the true quotient (x - low) / scale, not to its float32 rounding: the
-// float32 quotient, off by less than 2^-18, decides unless it lies within 2^-16 of a half; then the border
-// low + (c + 1/2) * scale, which float64 holds exactly (two float16 numbers, exponents -25 .. 15, and 5 bits),
+// The code is the nearest whole number to the true quotient (x - low) / scale, ties to even, not to its float32
+// rounding: the float32 quotient, off by less than 2^-18, decides unless it lies within 2^-16 of a half; then the
+// border low + (c + 1/2) * scale, which float64 holds exactly (two float16 numbers, exponents -25 .. 15, and 5 bits),
 // is compared with x. So the codes do not depend on how a device rounds a division.
 #pragma once
 #include <cstdint>
@@ -71,56 +71,79 @@ __device__ __forceinline__ uint16_t to16(float v) {
   return F16 ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
 }
 
-// Nearest whole number of 0..15 to (x - low) / scale, ties to even; inv = 1 / scale to float32 accuracy.
-__device__ __forceinline__ uint32_t code_of(float x, float low, float scale, float inv) {
-  const float q = __fmul_rn(__fsub_rn(x, low), inv);
-  float c = rintf(q);
+// The same for a quotient next to a border: q in float32 as quantise8 has it.
+static __device__ __noinline__ uint32_t code_at_border(float x, float low, float scale, float q) {
   const float below = floorf(q);
-  if (fabsf(q - below - 0.5f) < 0x1p-16f && q > -1.f && q < 16.f) {
-    const double border = static_cast<double>(low) + (static_cast<double>(below) + 0.5) * static_cast<double>(scale);
-    const double xd = static_cast<double>(x);
-    const bool up = xd > border || (xd == border && (static_cast<int>(below) & 1));
-    c = up ? below + 1.f : below;
-  }
-  return static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f));
+  if (fabsf(q - below - 0.5f) >= 0x1p-15f) return static_cast<uint32_t>(rintf(q));
+  const double border = static_cast<double>(low) + (static_cast<double>(below) + 0.5) * static_cast<double>(scale);
+  const double xd = static_cast<double>(x);
+  const bool up = xd > border || (xd == border && (static_cast<int>(below) & 1));
+  return static_cast<uint32_t>(up ? below + 1.f : below);
 }
 
 struct Cell8 {
   uint32_t codes;  // nibble e: element e of the lane's eight
   uint16_t scale, low;
-  bool fits;       // the lane's elements are finite and within kCellMax
+  bool fits;       // the group is finite and within kCellMax
 };
+
+template <bool F16, bool MAX>
+__device__ __forceinline__ uint32_t extreme2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (F16) {
+    if constexpr (MAX) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  } else {
+    if constexpr (MAX) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  }
+  return r;
+}
 
 // The lane's eight elements of a group that this lane and the 7 beside it hold (all of a warp's lanes call it).
 template <bool F16>
 __device__ __forceinline__ Cell8 quantise8(const uint4& raw) {
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  float x[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = from16<F16>(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1))));
-  float lo = x[0], hi = x[0];
-  Cell8 c;
-  c.fits = true;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    lo = fminf(lo, x[e]);
-    hi = fmaxf(hi, x[e]);
-    c.fits = c.fits && fabsf(x[e]) <= kCellMax;  // false for a NaN
-  }
+  uint32_t least = extreme2<F16, false>(extreme2<F16, false>(w[0], w[1]), extreme2<F16, false>(w[2], w[3]));
+  uint32_t most = extreme2<F16, true>(extreme2<F16, true>(w[0], w[1]), extreme2<F16, true>(w[2], w[3]));
 #pragma unroll
   for (int d = 1; d < 8; d <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+    least = extreme2<F16, false>(least, __shfl_xor_sync(0xffffffffu, least, d));
+    most = extreme2<F16, true>(most, __shfl_xor_sync(0xffffffffu, most, d));
   }
+  least = extreme2<F16, false>(least, least >> 16);
+  most = extreme2<F16, true>(most, most >> 16);
+  const float lo = from16<F16>(static_cast<uint16_t>(least)), hi = from16<F16>(static_cast<uint16_t>(most));
+  Cell8 c;
+  c.fits = lo >= -kCellMax && hi <= kCellMax;  // false for a NaN
   const __half low_h = __float2half_rn(lo);
   const float low = __half2float(low_h);
   const __half scale_h = __float2half_rn(__fdiv_rn(__fsub_rn(hi, low), 15.f));
   const float scale = __half2float(scale_h);
-  const float inv = scale > 0.f ? __fdiv_rn(1.f, scale) : 0.f;
-  c.codes = 0;
+  const float part = scale > 0.f ? __fdiv_rn(0x1.111112p-4f, scale) : 0.f;  // 1 / (15 scale): quotients of 0..1, clamped
+  constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: what is added to it becomes a whole number
+  uint32_t codes = 0;
+  float q[8], off = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) c.codes |= code_of(x[e], low, scale, inv) << (4 * e);
-  if (!(scale > 0.f)) c.codes = 0;
+  for (int e = 0; e < 8; ++e) {
+    const float x = from16<F16>(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1))));
+    q[e] = __saturatef(__fmul_rn(__fsub_rn(x, low), part));
+    const float m = __fmaf_rn(q[e], 15.f, kWhole);
+    off = fmaxf(off, fabsf(__fmaf_rn(q[e], 15.f, kWhole - m)));
+    codes += __float_as_uint(m) << (4 * e);  // the code in the low bits, and what cancels below
+  }
+  codes -= 0x4b400000u * 0x11111111u;
+  if (off > 0.5f - 0x1p-16f) {  // rare: some quotient next to a border
+    codes = 0;
+#pragma unroll 1
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t pair = (e >> 1) == 0 ? raw.x : (e >> 1) == 1 ? raw.y : (e >> 1) == 2 ? raw.z : raw.w;
+      const float x = from16<F16>(static_cast<uint16_t>(pair >> (16 * (e & 1))));
+      const float quotient = __saturatef(__fmul_rn(__fsub_rn(x, low), part)) * 15.f;
+      codes |= code_at_border(x, low, scale, quotient) << (4 * e);
+    }
+  }
+  c.codes = codes;
   c.scale = __half_as_ushort(scale_h);
   c.low = __half_as_ushort(low_h);
   return c;
@@ -135,13 +158,16 @@ __device__ __forceinline__ void store_key8(uint8_t* page, int r, int j, const Ce
         static_cast<uint32_t>(c.scale) | static_cast<uint32_t>(c.low) << 16;
 }
 template <int D>
+__device__ __forceinline__ void store_value_head(uint8_t* page, int r, int j, const Cell8& c) {
+  *reinterpret_cast<uint32_t*>(page + Cells<D>::value_head(r, j / 8)) =
+      static_cast<uint32_t>(c.scale) | static_cast<uint32_t>(c.low) << 16;
+}
+template <int D>
 __device__ __forceinline__ void store_value8(uint8_t* page, int r, int j, const Cell8& c) {
   uint8_t* w = page + Cells<D>::value_words(r >> 1, j) + 2 * (r & 1);
   *reinterpret_cast<uint16_t*>(w) = static_cast<uint16_t>(c.codes);
   *reinterpret_cast<uint16_t*>(w + 4) = static_cast<uint16_t>(c.codes >> 16);
-  if (j % 8 == 0)
-    *reinterpret_cast<uint32_t*>(page + Cells<D>::value_head(r, j / 8)) =
-        static_cast<uint32_t>(c.scale) | static_cast<uint32_t>(c.low) << 16;
+  if (j % 8 == 0) store_value_head<D>(page, r, j, c);
 }
 
 }  // namespace q4

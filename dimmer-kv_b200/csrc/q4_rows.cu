@@ -15,87 +15,108 @@ namespace {
 using q4::Cells;
 constexpr int kRowThreads = 256;
 
-// One lane: 8 dimensions (the j-th eight of its row) of one token's keys (z = 0) or values (z = 1).
-template <int D, bool F16>
-__global__ void __launch_bounds__(kRowThreads) q4_append_kernel(const dkv_q4_rows_args a) {
-  if (__any_sync(0xffffffffu, status_at_entry(a.status) != 0)) return;  // one answer for the warp's shuffles
-  constexpr int kLanes = D / 8;  // lanes of a row
-  using C = Cells<D>;
-  const int64_t rows = static_cast<int64_t>(a.n_seq) * a.q_len * a.n_kv_heads;
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x) / kLanes;
-  const int j = threadIdx.x % kLanes;
-  const bool is_value = blockIdx.y != 0;
-  int slot = -1;
-  int64_t src = 0;
-  int head = 0;
-  if (row < rows) {
-    const int64_t token = row / a.n_kv_heads;
-    head = static_cast<int>(row - token * a.n_kv_heads);
-    const int s = static_cast<int>(token / a.q_len), i = static_cast<int>(token - static_cast<int64_t>(s) * a.q_len);
-    slot = a.slots[token];
-    const int64_t* st = is_value ? a.v_stride : a.k_stride;
-    src = s * st[0] + head * st[1] + i * st[2] + j * 8;
-    if (slot >= a.n_pages * q4::kPage) {
-      record_error(a.status, kSiteQ4Rows + kErrBadDescriptor);
-      slot = -1;
-    }
+// A lane's place: the j-th eight dimensions of token i of a conversation's KV head. Rows run over tokens fastest, so a
+// warp holds neighbouring tokens of one head: whole lines of the key cells, and both tokens of a value pair.
+struct Place {
+  int seq, head, i, j, slot;  // slot -1: no token
+};
+
+template <int D>
+__device__ __forceinline__ Place place_of(const dkv_q4_rows_args& a) {
+  constexpr int kLanes = D / 8;
+  const uint32_t row = (blockIdx.x * kRowThreads + threadIdx.x) / kLanes;
+  const uint32_t q_len = a.q_len, heads = a.n_kv_heads;
+  const uint32_t line = row / q_len;
+  Place p;
+  p.j = threadIdx.x % kLanes;
+  p.i = static_cast<int>(row - line * q_len);
+  p.seq = static_cast<int>(line / heads);
+  p.head = static_cast<int>(line - p.seq * heads);
+  p.slot = p.seq < a.n_seq ? a.slots[static_cast<int64_t>(p.seq) * a.q_len + p.i] : -1;
+  if (p.slot >= a.n_pages * q4::kPage) {
+    record_error(a.status, kSiteQ4Rows + kErrBadDescriptor);
+    p.slot = -1;
   }
-  uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-  if (slot >= 0) raw = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(is_value ? a.value : a.key) + src);
-  const q4::Cell8 c = q4::quantise8<F16>(raw);
-  if (!c.fits) record_error(a.status, kSiteQ4Rows + kErrCellRange);
-  if (slot < 0) return;
-  uint8_t* page = a.cells + (static_cast<int64_t>(slot / q4::kPage) * a.n_kv_heads + head) * C::kBytes;
-  if (is_value) q4::store_value8<D>(page, slot % q4::kPage, j, c);
-  else q4::store_key8<D>(page, slot % q4::kPage, j, c);
+  return p;
 }
 
 template <int D, bool F16>
-__global__ void __launch_bounds__(kRowThreads) q4_read_kernel(const dkv_q4_rows_args a) {
-  constexpr int kLanes = D / 8;
+__global__ void __launch_bounds__(kRowThreads) q4_append_kernel(const __grid_constant__ dkv_q4_rows_args a) {
   using C = Cells<D>;
-  const bool failed = status_at_entry(a.status) != 0;
-  const int64_t rows = static_cast<int64_t>(a.n_seq) * a.q_len * a.n_kv_heads;
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x) / kLanes;
-  const int j = threadIdx.x % kLanes;
-  const bool is_value = blockIdx.y != 0;
-  if (row >= rows) return;
-  // heads outermost: neighbouring rows are neighbouring tokens of one head, as key and value are laid out
-  const int64_t per_seq = static_cast<int64_t>(a.n_kv_heads) * a.q_len;
-  const int s = static_cast<int>(row / per_seq);
-  const int head = static_cast<int>((row - s * per_seq) / a.q_len);
-  const int i = static_cast<int>(row - s * per_seq - static_cast<int64_t>(head) * a.q_len);
-  int slot = a.slots[static_cast<int64_t>(s) * a.q_len + i];
-  if (slot >= a.n_pages * q4::kPage) {
-    record_error(a.status, kSiteQ4Rows + kErrBadDescriptor);
-    slot = -1;
+  constexpr int kLanes = D / 8;
+  const Place p = place_of<D>(a);
+  uint4 key = make_uint4(0u, 0u, 0u, 0u), value = key;
+  if (p.slot >= 0) {
+    key = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.key) + p.seq * a.k_stride[0] +
+                                          p.head * a.k_stride[1] + p.i * a.k_stride[2] + p.j * 8);
+    value = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.value) + p.seq * a.v_stride[0] +
+                                            p.head * a.v_stride[1] + p.i * a.v_stride[2] + p.j * 8);
   }
-  const int64_t* st = is_value ? a.v_stride : a.k_stride;
-  uint16_t* dst = static_cast<uint16_t*>(is_value ? a.value : a.key) + s * st[0] + head * st[1] + i * st[2] + j * 8;
-  uint32_t out[4] = {0u, 0u, 0u, 0u};
-  if (slot >= 0 && !failed) {
-    const uint8_t* page = a.cells + (static_cast<int64_t>(slot / q4::kPage) * a.n_kv_heads + head) * C::kBytes;
-    const int r = slot % q4::kPage;
-    uint32_t codes, scale_low;
-    if (!is_value) {
-      codes = *reinterpret_cast<const uint32_t*>(page + C::key_word(r, j));
-      scale_low = *reinterpret_cast<const uint32_t*>(page + C::key_head(r, j / 8));
-    } else {
-      const uint8_t* w = page + C::value_words(r >> 1, j) + 2 * (r & 1);
-      codes = *reinterpret_cast<const uint16_t*>(w) |
-              static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(w + 4)) << 16;
-      scale_low = *reinterpret_cast<const uint32_t*>(page + C::value_head(r, j / 8));
-    }
-    const float scale = __half2float(__ushort_as_half(static_cast<uint16_t>(scale_low)));
-    const float low = __half2float(__ushort_as_half(static_cast<uint16_t>(scale_low >> 16)));
+  if (__any_sync(0xffffffffu, status_at_entry(a.status) != 0)) return;  // one answer for the warp's shuffles
+  const q4::Cell8 k = q4::quantise8<F16>(key), v = q4::quantise8<F16>(value);
+  if (!k.fits || !v.fits) record_error(a.status, kSiteQ4Rows + kErrCellRange);
+  // the other token of the pair, where the lanes beside hold it
+  const int there = __shfl_xor_sync(0xffffffffu, p.slot, kLanes);
+  const int beside = __shfl_xor_sync(0xffffffffu, p.i, kLanes);
+  const uint32_t codes = __shfl_xor_sync(0xffffffffu, v.codes, kLanes);
+  if (p.slot < 0) return;
+  uint8_t* page = a.cells + (static_cast<int64_t>(p.slot / q4::kPage) * a.n_kv_heads + p.head) * C::kBytes;
+  const int r = p.slot % q4::kPage;
+  q4::store_key8<D>(page, r, p.j, k);
+  const bool low = (threadIdx.x & kLanes) == 0;
+  const int step = low ? 1 : -1;
+  if (there >= 0 && there == p.slot + step && beside == p.i + step && (r & 1) == (low ? 0 : 1)) {
+    const uint32_t word = low ? __byte_perm(v.codes, codes, 0x5410) : __byte_perm(codes, v.codes, 0x7632);
+    *reinterpret_cast<uint32_t*>(page + C::value_words(r >> 1, p.j) + (low ? 0 : 4)) = word;
+    if (p.j % 8 == 0) q4::store_value_head<D>(page, r, p.j, v);
+  } else {
+    q4::store_value8<D>(page, r, p.j, v);
+  }
+}
+
+// 8 codes to the 16-bit values that they stand for.
+template <bool F16>
+__device__ __forceinline__ uint4 values_of(uint32_t codes, uint32_t scale_low) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&scale_low));
+  uint32_t out[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      // code * scale is exact in float32 (4 and 11 bits): one rounding to float32, one to 16 bits
-      const float v = __fmaf_rn(static_cast<float>((codes >> (4 * e)) & 15u), scale, low);
-      out[e >> 1] |= static_cast<uint32_t>(q4::to16<F16>(v)) << (16 * (e & 1));
+  for (int e = 0; e < 4; ++e) {
+    // code * scale is exact in float32 (4 and 11 bits): one rounding to float32, one to 16 bits
+    const float c0 = __uint_as_float(0x4b000000u | ((codes >> (8 * e)) & 15u)) - 8388608.f;
+    const float c1 = __uint_as_float(0x4b000000u | ((codes >> (8 * e + 4)) & 15u)) - 8388608.f;
+    const float x = __fmaf_rn(c0, f.x, f.y), y = __fmaf_rn(c1, f.x, f.y);
+    if constexpr (F16) {
+      const __half2 h = __floats2half2_rn(x, y);
+      out[e] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+      out[e] = *reinterpret_cast<const uint32_t*>(&h);
     }
   }
-  *reinterpret_cast<uint4*>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
+  return make_uint4(out[0], out[1], out[2], out[3]);
+}
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(kRowThreads) q4_read_kernel(const __grid_constant__ dkv_q4_rows_args a) {
+  using C = Cells<D>;
+  const Place p = place_of<D>(a);
+  if (p.seq >= a.n_seq) return;
+  uint4 key = make_uint4(0u, 0u, 0u, 0u), value = key;
+  if (p.slot >= 0 && status_at_entry(a.status) == 0) {
+    const uint8_t* page = a.cells + (static_cast<int64_t>(p.slot / q4::kPage) * a.n_kv_heads + p.head) * C::kBytes;
+    const int r = p.slot % q4::kPage;
+    const uint8_t* w = page + C::value_words(r >> 1, p.j);
+    const uint32_t codes = *reinterpret_cast<const uint32_t*>(page + C::key_word(r, p.j));
+    const uint32_t w0 = *reinterpret_cast<const uint32_t*>(w), w1 = *reinterpret_cast<const uint32_t*>(w + 4);
+    const uint32_t key_head = *reinterpret_cast<const uint32_t*>(page + C::key_head(r, p.j / 8));
+    const uint32_t value_head = *reinterpret_cast<const uint32_t*>(page + C::value_head(r, p.j / 8));
+    key = values_of<F16>(codes, key_head);
+    value = values_of<F16>(__byte_perm(w0, w1, r & 1 ? 0x7632 : 0x5410), value_head);
+  }
+  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.key) + p.seq * a.k_stride[0] + p.head * a.k_stride[1] +
+                            p.i * a.k_stride[2] + p.j * 8) = key;
+  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.value) + p.seq * a.v_stride[0] + p.head * a.v_stride[1] +
+                            p.i * a.v_stride[2] + p.j * 8) = value;
 }
 
 int check_rows(const dkv_q4_rows_args* a) {
@@ -127,8 +148,8 @@ int dkv_q4_append(const dkv_q4_rows_args* a, void* stream) {
   const int64_t lanes = static_cast<int64_t>(a->n_seq) * a->q_len * a->n_kv_heads * (a->head_dim / 8);
   if (lanes == 0) return DKV_OK;
   const int64_t blocks = (lanes + dkv::kRowThreads - 1) / dkv::kRowThreads;
-  if (blocks > INT32_MAX) return DKV_ERR_CONFIG;
-  const dim3 grid(static_cast<unsigned>(blocks), 2);
+  if (lanes > INT32_MAX) return DKV_ERR_CONFIG;
+  const dim3 grid(static_cast<unsigned>(blocks));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto kernel = a->head_dim == 128 ? (a->fp16 ? dkv::q4_append_kernel<128, true> : dkv::q4_append_kernel<128, false>)
                                    : (a->fp16 ? dkv::q4_append_kernel<64, true> : dkv::q4_append_kernel<64, false>);
@@ -142,8 +163,8 @@ int dkv_q4_read(const dkv_q4_rows_args* a, void* stream) {
   const int64_t lanes = static_cast<int64_t>(a->n_seq) * a->q_len * a->n_kv_heads * (a->head_dim / 8);
   if (lanes == 0) return DKV_OK;
   const int64_t blocks = (lanes + dkv::kRowThreads - 1) / dkv::kRowThreads;
-  if (blocks > INT32_MAX) return DKV_ERR_CONFIG;
-  const dim3 grid(static_cast<unsigned>(blocks), 2);
+  if (lanes > INT32_MAX) return DKV_ERR_CONFIG;
+  const dim3 grid(static_cast<unsigned>(blocks));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto kernel = a->head_dim == 128 ? (a->fp16 ? dkv::q4_read_kernel<128, true> : dkv::q4_read_kernel<128, false>)
                                    : (a->fp16 ? dkv::q4_read_kernel<64, true> : dkv::q4_read_kernel<64, false>);
