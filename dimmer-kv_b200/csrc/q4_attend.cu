@@ -27,26 +27,14 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include "dkv_launch.h"
-#include "dkv_ptx.cuh"
-#include "q4_cells.cuh"
+#include "q4_attend.cuh"
 
 namespace dkv {
 namespace {
 
-using q4::Cells;
+using namespace q4;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kBias = 7.f;    // probabilities are scaled by 2^7
-constexpr float kSlack = 8.f;   // the reference maximum may lag by 2^8: 2^(7 + 8) < 65504
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -75,35 +63,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   return r;
 }
 
-__device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
-__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) { return as_u32(__floats2half2_rn(lo, hi)); }
-
-// How the pages of all units are dealt to the workers (warps): worker w takes the pages
-// [total * w / workers, total * (w + 1) / workers) of the line (conversation, KV head, row chunk, page).
-struct Deal {
-  int64_t total;
-  int workers;
-  __device__ __forceinline__ Deal(int64_t total_, int workers_)
-      : total(total_), workers(static_cast<int>(total_ < workers_ ? total_ : workers_)) {}
-  __device__ __forceinline__ int64_t begin(int w) const {
-    const int64_t x = total * w;
-    return x <= 0xffffffffll ? static_cast<uint32_t>(x) / static_cast<uint32_t>(workers) : x / workers;
-  }
-  // The worker that has place x; none is without a place.
-  __device__ __forceinline__ int owner(int64_t x) const {
-    const int64_t y = (x + 1) * workers - 1;
-    return static_cast<int>(y <= 0xffffffffll ? static_cast<uint32_t>(y) / static_cast<uint32_t>(total) : y / total);
-  }
-};
-
-// Tokens that conversation s attends over (0 if it has no new token).
-__device__ __forceinline__ int tokens_of(const dkv_q4_attend_args& a, int s) {
-  const int start = a.starts[s], len = min(a.lengths[s], a.max_blocks * q4::kPage);
-  return start >= 0 && len > start ? len : 0;
-}
-__device__ __forceinline__ int pages_of(int tokens) { return (tokens + q4::kPage - 1) / q4::kPage; }
-
+// The pages of all units are dealt to the workers (warps) in the order (conversation, KV head, row chunk, page).
 __device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
 
 // One warp: pages of all conversations, and of those before `seq`.
@@ -462,19 +422,6 @@ __device__ __noinline__ void store_new(const dkv_q4_attend_args& a, int seq, int
   fence_async_shared();  // the next bulk copy into this place comes after these writes
 }
 
-template <bool F16>
-__device__ __forceinline__ void store_out4(const dkv_q4_attend_args& a, int64_t at, float x, float y, float z, float w) {
-  if (a.out_f32)
-    *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(x, y, z, w);
-  else
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) =
-        make_uint2(static_cast<uint32_t>(q4::to16<F16>(x)) | static_cast<uint32_t>(q4::to16<F16>(y)) << 16,
-                   static_cast<uint32_t>(q4::to16<F16>(z)) | static_cast<uint32_t>(q4::to16<F16>(w)) << 16);
-}
-
-// A partial result in the workspace: per slot (two per worker) [rows][D] of O, then [rows][2] of (m, l).
-__host__ __device__ __forceinline__ int64_t slot_floats(int rows, int d) { return static_cast<int64_t>(rows) * (d + 4); }
-
 template <int D, int NT, bool F16>
 __global__ void __launch_bounds__(kThreads, (Decode<D, NT>::kBlocksPerSm))
 q4_decode_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int workers, int append) {
@@ -764,7 +711,6 @@ q4_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int 
   store_out4<F16>(a, to, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
 }
 
-int rows_of(const dkv_q4_attend_args& a) { return a.q_len * (a.n_q_heads / a.n_kv_heads); }
 int tiles_of(const dkv_q4_attend_args& a) { return rows_of(a) <= 8 ? 1 : 2; }  // of 8 query rows that a warp holds
 
 int64_t floats_of(const dkv_q4_attend_args& a) {
@@ -818,7 +764,8 @@ extern "C" {
 
 int64_t dkv_q4_attend_floats(const dkv_q4_attend_args* a) {
   if (a == nullptr || dkv::check_sizes(a) != DKV_OK) return -1;
-  return a->n_seq == 0 || a->q_len == 0 ? 0 : dkv::floats_of(*a);
+  if (a->n_seq == 0 || a->q_len == 0) return 0;
+  return dkv::q4::prefill_takes(*a) ? dkv::q4::prefill_floats(*a) : dkv::floats_of(*a);
 }
 
 int dkv_q4_attend(const dkv_q4_attend_args* a, void* stream) {
@@ -835,10 +782,11 @@ int dkv_q4_attend(const dkv_q4_attend_args* a, void* stream) {
   for (int k = 0; k < 3; ++k)
     if (a->q_stride[k] % 8 || (a->key != nullptr && (a->k_stride[k] % 8 || a->v_stride[k] % 8))) return DKV_ERR_ARGS;
   if (a->n_seq == 0 || a->q_len == 0) return DKV_OK;
-  if (a->workspace == nullptr || a->workspace_floats < dkv::floats_of(*a)) return DKV_ERR_SCRATCH;
+  if (a->workspace == nullptr || a->workspace_floats < dkv_q4_attend_floats(a)) return DKV_ERR_SCRATCH;
+  const bool prefill = dkv::q4::prefill_takes(*a);
   const int nt = dkv::tiles_of(*a);
   int append = a->key != nullptr;
-  if (append && dkv::rows_of(*a) > 8 * nt) {
+  if (append && (prefill || dkv::q4::rows_of(*a) > 8 * nt)) {
     // Several row chunks read a new token's page: it has to be there before the first of them.
     dkv_q4_rows_args r = {};
     r.cells = a->cells;
@@ -853,6 +801,7 @@ int dkv_q4_attend(const dkv_q4_attend_args* a, void* stream) {
     append = 0;
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (prefill) return dkv::q4::run_prefill(*a, st);
 #define DKV_Q4_DECODE(D, NT) \
   (a->fp16 ? dkv::launch_decode<D, NT, true>(*a, append, st) : dkv::launch_decode<D, NT, false>(*a, append, st))
   if (a->head_dim == 128) return nt == 1 ? DKV_Q4_DECODE(128, 1) : DKV_Q4_DECODE(128, 2);

@@ -1,0 +1,781 @@
+// q4_prefill.cu — causal attention over the paged 4-bit cache for many query rows per KV head (a question, a prompt's
+// chunk): dkv_q4_attend's matrix-product form, on tcgen05.
+//
+// Bound by the exponentials and the two products, which are about even: a tile of 128 rows x 128 tokens takes 1024
+// cycles of the SM's exponential units and, at head_dim 128, 2 x 512 of its tensor core. Everything else has to hide
+// behind these: a CTA has two tiles of 128 query rows (the rows of a KV head's query heads, token after token), so
+// that one is in the tensor core while the other is in its softmax, and both use the same unpacked keys and values.
+//
+//   warps 0-3, 4-7   softmax of the first and the second tile, one row per thread: scores from TMEM, probabilities
+//                    back into TMEM (over the scores they come from), where the second product takes them
+//   warps 8-11       unpack 128 tokens (two pages) of cells, one token per thread, into float16 tiles with the 128-byte
+//                    swizzle, keys as rows, values as the rows of the contraction
+//   warp 12          issues the products: per step P V of a tile, then at once the next Q K of it
+//
+// TMEM: two score tiles, two outputs, 512 columns. The rows' references (running maxima) lag by up to 2^8, so that
+// outputs are scaled down in TMEM only when a row's maximum has grown past that; a score tile that is complete means
+// that the product issued before it is too, so nothing else has to be waited for.
+//
+// Keys and values are rounded to float16 (2^-11 at most of each), probabilities likewise; for float16 caches, whose
+// outputs show that, what the rounding of keys and values lacks forms second tiles that go through second products.
+//
+// The 128-token steps of all (conversation, KV head, 256-row block) units form one line that is cut evenly over one CTA per
+// SM; blocks that several CTAs share leave partial results in the workspace, which q4_prefill_combine_kernel joins.
+#include "q4_attend.cuh"
+
+namespace dkv {
+namespace q4 {
+namespace {
+
+constexpr int kStep = 128;           // tokens of a step: two pages
+constexpr int kRows = 128;           // query rows of a tile
+constexpr int kBlock = 2 * kRows;    // of a unit
+constexpr int kSoftWarps = 8, kUnpackWarps = 4;
+constexpr int kMmaWarp = kSoftWarps + kUnpackWarps;
+constexpr int kThreads = (kMmaWarp + 1) * 32;
+
+template <int D, bool F16>
+struct Shared {
+  using C = Cells<D>;
+  static constexpr int kPart = kStep * 128;           // 128 rows of 64 dimensions in float16
+  static constexpr int kTile = D / 64 * kPart;
+  static constexpr int kRawStages = F16 ? 1 : 2;
+  static constexpr int kQ = 0;                        // two tiles
+  static constexpr int kK = kQ + 2 * kTile;
+  static constexpr int kV = kK + kTile;
+  static constexpr int kKLow = kV + kTile;            // what the rounding lacks (float16 caches)
+  static constexpr int kVLow = kKLow + (F16 ? kTile : 0);
+  static constexpr int kRaw = kVLow + (F16 ? kTile : 0);
+  static constexpr int kBars = kRaw + kRawStages * 2 * C::kBytes;
+  static constexpr int kNumBars = 2 * kRawStages + 4 + 2 * 4 + 1;
+  static constexpr int kBytes = kBars + kNumBars * 8 + 16;
+  static constexpr int kAlloc = kBytes + 1024;        // the tiles begin on a 1024-byte boundary
+};
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+      "%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// After tmem_ld_wait: no use of the registers may be scheduled before it.
+__device__ __forceinline__ void tmem_fence32(uint32_t (&r)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D[tmem] (+)= A[tmem] * B[smem]: A's rows are TMEM lanes, two float16 of the contraction per 32-bit column.
+__device__ __forceinline__ void mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// ---------------------------------------------------------------- the line of steps
+struct Seq {
+  int start, fresh, rows, blocks;  // rows: new tokens' rows of a KV head
+};
+__device__ __forceinline__ Seq seq_of(const dkv_q4_attend_args& a, int s, int share) {
+  Seq q;
+  const int tokens = tokens_of(a, s);
+  q.start = a.starts[s];
+  q.fresh = tokens == 0 ? 0 : min(tokens - q.start, a.q_len);
+  q.rows = q.fresh * share;
+  q.blocks = (q.rows + kBlock - 1) / kBlock;
+  return q;
+}
+// Tokens that the rows of block b see, and steps to go through them.
+__device__ __forceinline__ int seen_by(const Seq& q, int b, int share) {
+  return q.start + min(((b + 1) * kBlock - 1) / share, q.fresh - 1) + 1;
+}
+__device__ __forceinline__ int steps_of(const Seq& q, int b, int share) {
+  return (seen_by(q, b, share) + kStep - 1) / kStep;
+}
+__device__ __forceinline__ int64_t seq_steps(const Seq& q, int share) {  // of one KV head
+  int64_t n = 0;
+  for (int b = 0; b < q.blocks; ++b) n += steps_of(q, b, share);
+  return n;
+}
+
+__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+
+// One warp: steps of all conversations, and of those before `seq`.
+__device__ __forceinline__ int64_t count_steps(const dkv_q4_attend_args& a, int share, int seq, int64_t& before) {
+  int64_t total = 0;
+  before = 0;
+  for (int base = 0; base < a.n_seq; base += 32) {
+    const int s = base + (threadIdx.x & 31);
+    const int64_t n = s < a.n_seq ? seq_steps(seq_of(a, s, share), share) * a.n_kv_heads : 0;
+    total += warp_sum64(n);
+    before += warp_sum64(s < seq ? n : 0);
+  }
+  return total;
+}
+
+// A CTA's piece of the line, unit by unit. Every warp goes through it on its own (all lanes alike).
+struct Walk {
+  const dkv_q4_attend_args& a;
+  int share;
+  int64_t at, end;      // places left
+  int seq, head, block;
+  Seq q;
+  int first, last, steps;  // this unit's steps [first, last) of `steps`
+  bool opened;
+
+  __device__ __forceinline__ Walk(const dkv_q4_attend_args& a_, int share_, int64_t begin_, int64_t end_)
+      : a(a_), share(share_), at(begin_), end(end_), opened(false) {
+    // the conversation of `begin`
+    const int lane = threadIdx.x & 31;
+    int64_t line = 0;
+    seq = a.n_seq;
+    for (int base = 0; base < a.n_seq; base += 32) {
+      const int s = base + lane;
+      const int64_t own = s < a.n_seq ? seq_steps(seq_of(a, s, share), share) * a.n_kv_heads : 0;
+      int64_t incl = own;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += y;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, line + incl > at);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        seq = base + l;
+        line += __shfl_sync(0xffffffffu, incl - own, l);
+        break;
+      }
+      line += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (seq >= a.n_seq) {  // not reached: begin lies on the line
+      at = end;
+      return;
+    }
+    q = seq_of(a, seq, share);
+    const int64_t per_head = seq_steps(q, share);
+    int64_t rest = at - line;
+    head = static_cast<int>(rest / per_head);
+    rest -= head * per_head;
+    block = 0;
+    while (rest >= steps_of(q, block, share)) rest -= steps_of(q, block++, share);
+    first = static_cast<int>(rest);
+  }
+  // The next unit; false behind the last.
+  __device__ __forceinline__ bool next() {
+    if (opened) {
+      first = 0;
+      if (++block == q.blocks) {
+        block = 0;
+        if (++head == a.n_kv_heads) {
+          head = 0;
+          if (at < end) {
+            do q = seq_of(a, ++seq, share);
+            while (q.blocks == 0);
+          }
+        }
+      }
+    }
+    opened = true;
+    if (at >= end) return false;
+    steps = steps_of(q, block, share);
+    last = static_cast<int>(min(static_cast<int64_t>(steps), first + (end - at)));
+    at += last - first;
+    return true;
+  }
+  __device__ __forceinline__ bool whole() const { return first == 0 && last == steps; }
+  __device__ __forceinline__ bool two() const { return q.rows - block * kBlock > kRows; }  // the second tile has rows
+};
+
+// ---------------------------------------------------------------- unpacking
+// Eight codes (nibbles of w) to eight float16 values scale * c + low in the order 0 4 1 5 2 6 3 7, each rounded once; with
+// LOW also what the rounding lacks.
+template <bool LOW>
+__device__ __forceinline__ uint4 unpack8(uint32_t w, __half2 scale, __half2 low, uint4& lack) {
+  const __half2 k1024 = as_half2(0x64006400u), k16th = as_half2(0x2c002c00u), k64 = as_half2(0xd400d400u);
+  uint32_t v[4], r[4];
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const uint32_t u = b ? w >> 8 : w;
+    const __half2 even = __hsub2(as_half2((u & 0x000f000fu) | 0x64006400u), k1024);
+    const __half2 odd = __hfma2(as_half2((u & 0x00f000f0u) | 0x64006400u), k16th, k64);
+    const __half2 x = __hfma2(even, scale, low), y = __hfma2(odd, scale, low);
+    v[2 * b] = as_u32(x);
+    v[2 * b + 1] = as_u32(y);
+    if constexpr (LOW) {
+      const float s = __low2float(scale), l = __low2float(low);
+      const float2 e = __half22float2(even), o = __half22float2(odd), xf = __half22float2(x), yf = __half22float2(y);
+      r[2 * b] = pack_half2(fmaf(e.x, s, l) - xf.x, fmaf(e.y, s, l) - xf.y);
+      r[2 * b + 1] = pack_half2(fmaf(o.x, s, l) - yf.x, fmaf(o.y, s, l) - yf.y);
+    }
+  }
+  if constexpr (LOW) lack = make_uint4(r[0], r[1], r[2], r[3]);
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+// Place p of a chunk of 8 holds dimension kOrder[p].
+__device__ constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(kThreads, 1)
+q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int slot_rows) {
+  using S = Shared<D, F16>;
+  using C = Cells<D>;
+  constexpr int kGroups = C::kGroups;
+  extern __shared__ uint8_t smem_raw[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  uint8_t* smem = smem_raw + (1024 - smem_u32(smem_raw) % 1024) % 1024;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
+  uint64_t* raw_full = bars;                     // bulk copies of a step's pages
+  uint64_t* raw_free = raw_full + S::kRawStages; // unpacked
+  uint64_t* k_full = raw_free + S::kRawStages;
+  uint64_t* v_full = k_full + 1;
+  uint64_t* k_free = v_full + 1;                 // products that read the tile are complete
+  uint64_t* v_free = k_free + 1;
+  uint64_t* q_full = v_free + 1;                 // [2], by tile
+  uint64_t* s_full = q_full + 2;                 // [2] scores complete
+  uint64_t* p_full = s_full + 2;                 // [2] probabilities in TMEM
+  uint64_t* o_full = p_full + 2;                 // [2] a unit's last product complete
+  uint64_t* drain = o_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + S::kNumBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = warp_id(), lane = threadIdx.x & 31;
+  const int share = a.n_q_heads / a.n_kv_heads;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kRawStages; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_free[i], kUnpackWarps);
+    }
+    mbar_init(k_full, kUnpackWarps);
+    mbar_init(v_full, kUnpackWarps);
+    mbar_init(k_free, 1);
+    mbar_init(v_free, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 4);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  const bool failed = cta_failed_at_entry(a.status);  // a barrier of the CTA
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  int64_t unused;
+  const Deal deal(count_steps(a, share, 0, unused), workers);
+  int64_t begin = 0, end = 0;
+  if (!failed && static_cast<int>(blockIdx.x) < deal.workers) {
+    begin = deal.begin(blockIdx.x);
+    end = deal.begin(blockIdx.x + 1);
+  }
+  // scores of tile i: columns 128 i .. (its probabilities in the first 64 of them); outputs: columns 256 + 128 i ..
+  if (begin < end) {
+    Walk walk(a, share, begin, end);
+    if (warp < kSoftWarps) {
+      // ------------------------------------------------------------ softmax
+      const int tile = warp >> 2, row_in_tile = (warp & 3) * 32 + lane;
+      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const uint32_t s_at = tmem + lanes + tile * 128, o_at = tmem + lanes + 256 + tile * 128;
+      uint32_t s_iter = 0, units = 0;
+      bool ok = true;
+      int64_t place = begin;
+      while (ok && walk.next()) {
+        const int64_t unit_begin = place;
+        place += walk.last - walk.first;
+        if (tile == 1 && !walk.two()) continue;
+        const Seq& q = walk.q;
+        const int row0 = walk.block * kBlock + tile * kRows, r = row0 + row_in_tile, i = r / share;
+        const bool real = r < q.rows;
+        // ---- the row into shared memory, by a power of two that brings its largest element to [2^13, 2^14)
+        float factor;
+        {
+          const uint16_t* src = static_cast<const uint16_t*>(a.query) + walk.seq * a.q_stride[0] +
+                                (walk.head * share + r - i * share) * a.q_stride[1] + i * a.q_stride[2];
+          float big = 0.f;
+          if (real)
+            for (int c = 0; c < D / 8; ++c) {
+              const uint4 u = *reinterpret_cast<const uint4*>(src + c * 8);
+              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(from16<F16>(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1))))));
+            }
+          const int ex = (__float_as_uint(big) >> 23) & 255;
+          const float up = __uint_as_float(static_cast<uint32_t>(min(254, max(1, 267 - ex))) << 23);
+          // a negative scaling goes into the query, so that the largest product is the largest score
+          const float f = a.scaling < 0.f ? -up : up;
+          factor = fabsf(a.scaling) * kLog2e / up;
+#pragma unroll 4
+          for (int c = 0; c < D / 8; ++c) {
+            uint4 u = make_uint4(0u, 0u, 0u, 0u);
+            if (real) u = *reinterpret_cast<const uint4*>(src + c * 8);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = from16<F16>(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)))) * f;
+            *reinterpret_cast<uint4*>(smem + S::kQ + tile * S::kTile + (c >> 3) * S::kPart + sw128_offset(row_in_tile, c & 7)) =
+                make_uint4(pack_half2(x[0], x[4]), pack_half2(x[1], x[5]), pack_half2(x[2], x[6]), pack_half2(x[3], x[7]));
+          }
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&q_full[tile]);
+        }
+        const int limit = real ? q.start + i + 1 : 0;
+        const int full_below = q.start + row0 / share + 1;  // tokens below it are seen by every row of the tile
+        float ref = 0.f, l = 0.f;
+        bool known = false;
+        for (int t = walk.first; t < walk.last; ++t) {
+          ok = warp_wait(&s_full[tile], s_iter & 1, a.status, kSiteQ4Attend + kErrWaitAccum, abort_flag);
+          ++s_iter;
+          if (!ok) break;
+          tc_fence_after();
+          const int base = t * kStep;
+          const bool edge = base + kStep > full_below;
+          float top = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < kStep / 32; ++c) {
+            uint32_t s[32];
+            tmem_ld32(s_at + c * 32, s);
+            tmem_ld_wait();
+            tmem_fence32(s);
+            if (edge) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) top = fmaxf(top, base + c * 32 + e < limit ? __uint_as_float(s[e]) : -INFINITY);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(s[e]));
+            }
+          }
+          top *= factor;
+          const bool first = !known && top > -INFINITY;  // the row's first tokens set the reference wherever they are
+          const bool raise = first || (known && top > ref + kSlack);
+          if (__any_sync(0xffffffffu, raise)) {
+            const float down = raise ? (first ? 0.f : exp2_fast(ref - top)) : 1.f;
+            if (raise) {
+              ref = top;
+              l *= down;
+              known = true;
+            }
+            if (t > walk.first) {
+#pragma unroll
+              for (int c = 0; c < D / 16; ++c) {
+                uint32_t x[16];
+                tmem_ld16(o_at + c * 16, x);
+                tmem_ld_wait();
+                tmem_reg_fence(x);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * down);
+                tmem_st16(o_at + c * 16, x);
+              }
+            }
+          }
+          const float off = kBias - ref;
+#pragma unroll
+          for (int c = 0; c < kStep / 32; ++c) {
+            uint32_t s[32], p[16];
+            tmem_ld32(s_at + c * 32, s);
+            tmem_ld_wait();
+            tmem_fence32(s);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              float x = fmaf(__uint_as_float(s[e]), factor, off);
+              if (edge && base + c * 32 + e >= limit) x = -INFINITY;
+              x = exp2_fast(x);
+              l += x;
+              s[e] = __float_as_uint(x);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) p[e] = pack_half2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
+            tmem_st16(s_at + c * 16, p);
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[tile]);
+        }
+        if (!ok) break;
+        ok = warp_wait(&o_full[tile], units & 1, a.status, kSiteQ4Attend + kErrWaitAccum, abort_flag);
+        ++units;
+        if (!ok) break;
+        tc_fence_after();
+        const bool whole = walk.whole();
+        const float inv = !whole ? 1.f : l != 0.f ? 1.f / l : 0.f;
+        const int64_t to = ((static_cast<int64_t>(walk.seq) * a.q_len + i) * a.n_q_heads + walk.head * share + r - i * share) * D;
+        const int row = tile * kRows + row_in_tile;  // of the block
+        float* slot = a.workspace + (2 * static_cast<int64_t>(blockIdx.x) + (unit_begin == begin ? 0 : 1)) * slot_floats(slot_rows, D);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t x[32];
+          __syncwarp();
+          tmem_ld32(o_at + c * 32, x);
+          tmem_ld_wait();
+          tmem_fence32(x);
+#pragma unroll
+          for (int h = 0; h < 4 && real; ++h) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[kOrder[e]] = __uint_as_float(x[h * 8 + e]) * inv;
+            const int dim = c * 32 + h * 8;
+            if (whole) {
+              store_out4<F16>(a, to + dim, y[0], y[1], y[2], y[3]);
+              store_out4<F16>(a, to + dim + 4, y[4], y[5], y[6], y[7]);
+            } else {
+              *reinterpret_cast<float4*>(slot + row * D + dim) = make_float4(y[0], y[1], y[2], y[3]);
+              *reinterpret_cast<float4*>(slot + row * D + dim + 4) = make_float4(y[4], y[5], y[6], y[7]);
+            }
+          }
+        }
+        if (!whole && real) *reinterpret_cast<float2*>(slot + slot_rows * D + row * 4) = make_float2(ref, l);
+        tc_fence_before();
+      }
+      if (!ok) *abort_flag = 1;
+    } else if (warp < kMmaWarp) {
+      // ------------------------------------------------------------ unpacking
+      const int token = threadIdx.x - kSoftWarps * 32;  // of the step
+      const int64_t page_stride = static_cast<int64_t>(a.n_kv_heads) * C::kBytes;
+      uint32_t issued = 0, iter = 0;
+      bool ok = true;
+      // The copies run ahead of the unpacking, over unit boundaries: a second walk, of the first warp alone.
+      Walk ahead(a, share, begin, end);
+      int ahead_t = 0;
+      bool ahead_on = ahead.next();
+      if (ahead_on) ahead_t = ahead.first;
+      auto issue = [&]() {
+        const uint32_t stage = issued % S::kRawStages;
+        if (issued >= S::kRawStages &&
+            !warp_wait(&raw_free[stage], ((issued / S::kRawStages) - 1) & 1, a.status, kSiteQ4Attend + kErrWaitEmpty, abort_flag))
+          return false;
+        if (lane == 0) {
+          const int seen = seen_by(ahead.q, ahead.block, share);
+          const int32_t* table = a.blocks + static_cast<int64_t>(ahead.seq) * a.max_blocks;
+          const uint8_t* cells = a.cells + static_cast<int64_t>(ahead.head) * C::kBytes;
+          const int pages = min(2, pages_of(seen) - 2 * ahead_t);
+          mbar_arrive_expect_tx(&raw_full[stage], pages * C::kBytes);
+          for (int k = 0; k < pages; ++k) {
+            int id = table[2 * ahead_t + k];
+            if (id < 0 || id >= a.n_pages) {  // recorded, and a page that exists read in its place
+              record_error(a.status, kSiteQ4Attend + kErrBadDescriptor);
+              id = 0;
+            }
+            bulk_load(smem + S::kRaw + (stage * 2 + k) * C::kBytes, cells + id * page_stride, C::kBytes, &raw_full[stage]);
+          }
+        }
+        __syncwarp();
+        ++issued;
+        if (++ahead_t == ahead.last) {
+          ahead_on = ahead.next();
+          if (ahead_on) ahead_t = ahead.first;
+        }
+        return true;
+      };
+      if (warp == kSoftWarps)
+        for (int k = 0; k < S::kRawStages && ok && ahead_on; ++k) ok = issue();
+      while (ok && walk.next()) {
+        const int seen = seen_by(walk.q, walk.block, share);
+        for (int t = walk.first; t < walk.last && ok; ++t, ++iter) {
+          const uint32_t stage = iter % S::kRawStages;
+          ok = warp_wait(&raw_full[stage], (iter / S::kRawStages) & 1, a.status, kSiteQ4Attend + kErrWaitCodes, abort_flag) &&
+               (iter == 0 || warp_wait(k_free, (iter - 1) & 1, a.status, kSiteQ4Attend + kErrWaitEmpty, abort_flag));
+          if (!ok) break;
+          const uint8_t* page = smem + S::kRaw + (stage * 2 + token / kPage) * C::kBytes;
+          const int r = token % kPage;
+          // a token that no row sees may never have been written: zeros, no NaN of its
+          const bool there = t * kStep + token < seen;
+          uint32_t head[2 * kGroups];
+#pragma unroll
+          for (int k = 0; k < 2 * kGroups; ++k)
+            head[k] = there ? *reinterpret_cast<const uint32_t*>(page + C::kHeads + r * C::kHeadBytes + k * 4) : 0u;
+          // ---- keys: the token's four pieces, in an order that keeps the lanes on different banks
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int piece = (k + (D == 128 ? r >> 1 : r >> 2)) & 3;
+            uint32_t w[D / 32];
+            const uint8_t* src = page + C::kKeyCodes + r * (D / 2) + piece * (D / 8);
+            if constexpr (D == 128) {
+              const uint4 u = *reinterpret_cast<const uint4*>(src);
+              w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+            } else {
+              const uint2 u = *reinterpret_cast<const uint2*>(src);
+              w[0] = u.x, w[1] = u.y;
+            }
+#pragma unroll
+            for (int e = 0; e < D / 32; ++e) {
+              const int gr = e >> 1, chunk = piece * 2 + (e & 1);
+              const __half2 h = as_half2(head[gr]);
+              uint4 lack;
+              const uint4 x = unpack8<F16>(w[e], __low2half2(h), __high2half2(h), lack);
+              const uint32_t to = gr * S::kPart + sw128_offset(token, chunk);
+              *reinterpret_cast<uint4*>(smem + S::kK + to) = x;
+              if constexpr (F16) *reinterpret_cast<uint4*>(smem + S::kKLow + to) = lack;
+            }
+          }
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(k_full);
+          // ---- values: the pair's eight pieces, this token's halves of them
+          if (iter > 0 && !warp_wait(v_free, (iter - 1) & 1, a.status, kSiteQ4Attend + kErrWaitEmpty, abort_flag)) {
+            ok = false;
+            break;
+          }
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            uint32_t w[D / 32];
+            const uint8_t* src = page + C::value_piece(r >> 1, g);
+            if constexpr (D == 128) {
+              const uint4 u = *reinterpret_cast<const uint4*>(src);
+              w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+            } else {
+              const uint2 u = *reinterpret_cast<const uint2*>(src);
+              w[0] = u.x, w[1] = u.y;
+            }
+#pragma unroll
+            for (int gr = 0; gr < kGroups; ++gr) {
+              const __half2 h = as_half2(head[kGroups + gr]);
+              uint4 lack;
+              const uint4 x = unpack8<F16>(__byte_perm(w[2 * gr], w[2 * gr + 1], r & 1 ? 0x7632 : 0x5410), __low2half2(h),
+                                           __high2half2(h), lack);
+              const uint32_t to = gr * S::kPart + sw128_offset(token, g);
+              *reinterpret_cast<uint4*>(smem + S::kV + to) = x;
+              if constexpr (F16) *reinterpret_cast<uint4*>(smem + S::kVLow + to) = lack;
+            }
+          }
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(v_full);
+            mbar_arrive(&raw_free[stage]);
+          }
+          if (warp == kSoftWarps && ahead_on) ok = issue();
+        }
+      }
+      if (!ok) *abort_flag = 1;
+      // No copy is in flight when the CTA leaves.
+      if (warp == kSoftWarps)
+        for (uint32_t n = issued - min(issued, static_cast<uint32_t>(S::kRawStages)); n < issued; ++n)
+          warp_wait(&raw_full[n % S::kRawStages], (n / S::kRawStages) & 1, a.status, kSiteQ4Attend + kErrWaitDrain, nullptr);
+    } else {
+      // ------------------------------------------------------------ products
+      constexpr uint32_t kQk = idesc_f16(kRows, kStep, false, false, false);
+      constexpr uint32_t kPv = idesc_f16(kRows, D, false, false, true);
+      const uint32_t k_at = smem_u32(smem + S::kK), v_at = smem_u32(smem + S::kV);
+      uint32_t iter = 0, p_iter[2] = {0, 0}, units[2] = {0, 0};
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity, int err) {
+        ok = ok && warp_wait(bar, parity, a.status, kSiteQ4Attend + err, abort_flag);
+        return ok;
+      };
+      auto scores = [&](int tile) {  // Q K of the tile
+        if (lane == 0) {
+          const uint32_t q_at = smem_u32(smem + S::kQ + tile * S::kTile);
+#pragma unroll
+          for (int part = 0; part < (F16 ? 2 : 1); ++part)
+#pragma unroll
+            for (int gr = 0; gr < kGroups; ++gr)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mma_f16(tmem + tile * 128, smem_desc_sw128(q_at + gr * S::kPart + 32 * k, 16, 1024),
+                        smem_desc_sw128(k_at + (part ? S::kKLow - S::kK : 0) + gr * S::kPart + 32 * k, 16, 1024), kQk,
+                        part > 0 || gr > 0 || k > 0);
+          mma_commit(&s_full[tile]);
+        }
+        __syncwarp();
+      };
+      auto outputs = [&](int tile, bool first) {  // P V of the tile
+        if (lane == 0) {
+#pragma unroll
+          for (int part = 0; part < (F16 ? 2 : 1); ++part)
+#pragma unroll
+            for (int k = 0; k < kStep / 16; ++k)
+              mma_f16_ta(tmem + 256 + tile * 128, tmem + tile * 128 + 8 * k,
+                         smem_desc_sw128(v_at + (part ? S::kVLow - S::kV : 0) + 2048 * k, S::kPart, 1024), kPv,
+                         !first || part > 0 || k > 0);
+        }
+        __syncwarp();
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (lane == 0) mma_commit(bar);
+        __syncwarp();
+      };
+      bool more = walk.next();
+      while (ok && more) {
+        const bool two = walk.two();
+        const int n = walk.last - walk.first;
+        // the unit's first scores
+        if (!wait(k_full, iter & 1, kErrWaitA)) break;
+        for (int tile = 0; tile < (two ? 2 : 1); ++tile) {
+          if (!wait(&q_full[tile], units[tile] & 1, kErrWaitA)) break;
+          tc_fence_after();
+          scores(tile);
+        }
+        if (!ok) break;
+        commit(k_free);
+        for (int t = 0; t < n && ok; ++t, ++iter) {
+          for (int tile = 0; tile < (two ? 2 : 1); ++tile) {
+            if (!wait(&p_full[tile], p_iter[tile] & 1, kErrWaitA)) break;
+            ++p_iter[tile];
+            if (tile == 0 && !wait(v_full, iter & 1, kErrWaitA)) break;
+            tc_fence_after();
+            outputs(tile, t == 0);
+            if (tile == (two ? 1 : 0)) commit(v_free);
+            if (t + 1 == n) {
+              commit(&o_full[tile]);
+              ++units[tile];
+            } else {
+              if (tile == 0 && !wait(k_full, (iter + 1) & 1, kErrWaitA)) break;
+              tc_fence_after();
+              scores(tile);
+            }
+          }
+          if (!ok) break;
+          if (t + 1 < n) commit(k_free);
+        }
+        more = walk.next();
+      }
+      if (!ok) *abort_flag = 1;
+      // Every product is complete before TMEM is given back.
+      commit(drain);
+      warp_wait(drain, 0, a.status, kSiteQ4Attend + kErrWaitDrain, nullptr);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+}
+
+// Joins the blocks that several CTAs share and writes the zeros of the rows behind the new tokens: a warp per row.
+constexpr int kCombineWarps = 8, kCombineRows = 32;
+template <int D, bool F16>
+__global__ void __launch_bounds__(kCombineWarps * 32)
+q4_prefill_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int slot_rows) {
+  __shared__ int64_t line[2];
+  const int share = a.n_q_heads / a.n_kv_heads;
+  const int head = blockIdx.y, seq = blockIdx.z, warp = warp_id(), lane = threadIdx.x & 31;
+  const Seq q = seq_of(a, seq, share);
+  if (warp == 0) {
+    int64_t before;
+    const int64_t all = count_steps(a, share, seq, before);
+    if (lane == 0) line[0] = all, line[1] = before;
+  }
+  __syncthreads();
+  const int64_t per_head = seq_steps(q, share);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const bool failed = cta_failed_at_entry(a.status);
+  const int rows = a.q_len * share;
+  constexpr int kPer = D / 32;  // dimensions of a lane
+  for (int k = warp; k < kCombineRows; k += kCombineWarps) {
+    const int r = blockIdx.x * kCombineRows + k, i = r / share;
+    if (r >= rows) break;
+    const int64_t to =
+        ((static_cast<int64_t>(seq) * a.q_len + i) * a.n_q_heads + head * share + r - i * share) * D + lane * kPer;
+    float sum[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) sum[e] = 0.f;
+    if (r < q.rows && !failed) {
+      const int block = r / kBlock, row = r - block * kBlock;
+      const Deal deal(line[0], workers);
+      int64_t unit = line[1] + head * per_head;
+      for (int b = 0; b < block; ++b) unit += steps_of(q, b, share);
+      const int w0 = deal.owner(unit), w1 = deal.owner(unit + steps_of(q, block, share) - 1);
+      if (w0 == w1) continue;  // one CTA had the whole block
+      const int64_t stride = slot_floats(slot_rows, D);
+      const float* first = a.workspace + (2 * static_cast<int64_t>(w0) + (deal.begin(w0) < unit ? 1 : 0)) * stride;
+      const float* rest = a.workspace + 2 * static_cast<int64_t>(w0) * stride;
+      float den = 0.f, ref = -INFINITY;
+#pragma unroll 4
+      for (int w = 0; w <= w1 - w0; ++w) {
+        const float* slot = w == 0 ? first : rest + 2 * w * stride;
+        const float2 s = *reinterpret_cast<const float2*>(slot + slot_rows * D + row * 4);
+        float o[kPer];
+        if constexpr (kPer == 4) {
+          const float4 u = *reinterpret_cast<const float4*>(slot + row * D + lane * 4);
+          o[0] = u.x, o[1] = u.y, o[2] = u.z, o[3] = u.w;
+        } else {
+          const float2 u = *reinterpret_cast<const float2*>(slot + row * D + lane * 2);
+          o[0] = u.x, o[1] = u.y;
+        }
+        const bool none = s.y == 0.f;  // it saw no token of this row
+        const float now = none ? ref : fmaxf(ref, s.x);
+        const float keep = ref == -INFINITY ? 0.f : exp2_fast(ref - now), add = none ? 0.f : exp2_fast(s.x - now);
+        den = fmaf(s.y, add, den * keep);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) sum[e] = fmaf(o[e], add, sum[e] * keep);
+        ref = now;
+      }
+      const float inv = den != 0.f ? 1.f / den : 0.f;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) sum[e] *= inv;
+    }
+    if constexpr (kPer == 4) {
+      store_out4<F16>(a, to, sum[0], sum[1], sum[2], sum[3]);
+    } else if (a.out_f32) {
+      *reinterpret_cast<float2*>(static_cast<float*>(a.out) + to) = make_float2(sum[0], sum[1]);
+    } else {
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + to) =
+          static_cast<uint32_t>(to16<F16>(sum[0])) | static_cast<uint32_t>(to16<F16>(sum[1])) << 16;
+    }
+  }
+}
+
+int slot_rows_of(const dkv_q4_attend_args& a) { return rows_of(a) < kBlock ? rows_of(a) : kBlock; }
+
+template <int D, bool F16>
+int launch_prefill(const dkv_q4_attend_args& a, cudaStream_t stream) {
+  auto kernel = q4_prefill_kernel<D, F16>;
+  static std::atomic<uint64_t> done{0};
+  if (!allow_shared(kernel, Shared<D, F16>::kAlloc, done)) return DKV_ERR_CUDA;
+  const int workers = device_sms(), slot_rows = slot_rows_of(a);
+  kernel<<<workers, kThreads, Shared<D, F16>::kAlloc, stream>>>(a, workers, slot_rows);
+  if (cudaGetLastError() != cudaSuccess) return DKV_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((rows_of(a) + kCombineRows - 1) / kCombineRows, a.n_kv_heads, a.n_seq);
+  cfg.blockDim = dim3(kCombineWarps * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, q4_prefill_combine_kernel<D, F16>, a, workers, slot_rows) == cudaSuccess ? DKV_OK
+                                                                                                          : DKV_ERR_CUDA;
+}
+
+}  // namespace
+
+bool prefill_takes(const dkv_q4_attend_args& a) { return rows_of(a) > 32; }
+
+int64_t prefill_floats(const dkv_q4_attend_args& a) {
+  return 2 * static_cast<int64_t>(device_sms()) * slot_floats(slot_rows_of(a), a.head_dim);
+}
+
+int run_prefill(const dkv_q4_attend_args& a, cudaStream_t stream) {
+  if (a.head_dim == 128) return a.fp16 ? launch_prefill<128, true>(a, stream) : launch_prefill<128, false>(a, stream);
+  return a.fp16 ? launch_prefill<64, true>(a, stream) : launch_prefill<64, false>(a, stream);
+}
+
+}  // namespace q4
+}  // namespace dkv

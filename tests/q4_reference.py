@@ -45,22 +45,29 @@ def attend64(query, key, value, held, scaling):
     return (p @ v).transpose(0, 1), parts
 
 
-def attend_tolerance(out, parts, dtype, out_dtype):
-    """Largest error of dkv_q4_attend against attend64, for a cache of ``dtype``.
+def attend_tolerance(out, parts, dtype, out_dtype, rows=1):
+    """Largest error of dkv_q4_attend against attend64, for a cache of ``dtype`` and ``rows`` query rows per KV head.
 
-    p * scale is rounded to float16 (half a step: 2^-11) in front of its code, or, for float16 caches, to two float16
-    numbers (2^-21 between them): that much of the sum of p * scale * code. Below 2^-14 the half step is 2^-25
-    instead, of p * 2^7 * scale / 2^k with 2^k at most 4 times the largest scale, times a code of at most 15: 2^-26
-    of the largest scale for every token. A score, a float32 sum of absolute terms ``terms`` in at most 2 * 128
-    additions whose operands the tensor core may cut at 2^-22, is off by at most 2^-17 of them in all, which moves
-    numerator and denominator by that much each. The float32 sums over tokens, chains of at most four products that
-    the tensor core may cut at 2^-22 each and float32 additions of their sums, a few hundred per warp, are good to
-    2^-16 of their absolute terms. The output is
-    rounded once, to half a step of its type."""
+    Up to 32 rows: p * scale is rounded to float16 (half a step: 2^-11) in front of its code, or, for float16 caches, to
+    two float16 numbers (2^-21 between them): that much of the sum of p * scale * code. Below 2^-14 the half step is
+    2^-25 instead, of p * 2^7 * scale / 2^k with 2^k at most 4 times the largest scale, times a code of at most 15:
+    2^-26 of the largest scale for every token.
+    More rows: keys, values and probabilities are rounded to float16, for float16 caches keys and values to two
+    numbers: a score moves by 2^-11 (2^-21) of its absolute terms, numerator and denominator by that; the sum by 2^-11
+    for the probabilities and 2^-11 (2^-21) for the values, and a probability below 2^-14 of 2^7 by 2^-32 of the
+    largest value (15 scales and a low) for every token.
+    A score, a float32 sum of absolute terms ``terms`` in at most 2 * 128 additions whose operands the tensor core may
+    cut at 2^-22, is off by at most 2^-17 of them in all, which moves numerator and denominator by that much each. The
+    float32 sums over tokens, chains of at most four products that the tensor core may cut at 2^-22 each and float32
+    additions of their sums, a few hundred per warp, are good to 2^-16 of their absolute terms (the longer chains of
+    more rows, over values of either sign, to 2^-14). The output is rounded once, to half a step of its type."""
     coded, low, terms, tokens, scale = parts
     step = 2**-11 if dtype == torch.bfloat16 else 2**-21
-    return (coded * step + (coded + low) * (2 * 2**-17 * terms[..., None] + 2**-16) + tokens * 2**-26 * scale
-            + out.abs() * torch.finfo(out_dtype).eps / 2 + 1e-12)
+    if rows <= 32:
+        own = coded * step + (coded + low) * 2**-16 + tokens * 2**-26 * scale
+    else:
+        own = (coded + low) * (2**-11 + step + 2 * step * terms[..., None] + 2**-14) + tokens * 2**-32 * 32 * scale
+    return own + (coded + low) * 2 * 2**-17 * terms[..., None] + out.abs() * torch.finfo(out_dtype).eps / 2 + 1e-12
 
 
 class PlainTable:
