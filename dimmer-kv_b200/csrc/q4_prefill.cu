@@ -9,8 +9,10 @@
 //   warps 0-3, 4-7   softmax of the first and the second tile, one row per thread: scores from TMEM, probabilities
 //                    back into TMEM (over the scores they come from), where the second product takes them
 //   warps 8-11       unpack 128 tokens (two pages) of cells, one token per thread, into float16 tiles with the 128-byte
-//                    swizzle, keys as rows, values as the rows of the contraction
-//   warp 12          issues the products: per step P V of a tile, then at once the next Q K of it
+//                    swizzle, keys as rows, values as the rows of the contraction (8-15, two threads per token, for
+//                    float16 caches, see below)
+//   two more         one issues the products (per step P V of a tile, then at once the next Q K of it), the other the
+//                    bulk copies of the pages
 //
 // TMEM: two score tiles, two outputs, 512 columns. The rows' references (running maxima) lag by up to 2^8, so that
 // outputs are scaled down in TMEM only when a row's maximum has grown past that; a score tile that is complete means
@@ -30,9 +32,16 @@ namespace {
 constexpr int kStep = 128;           // tokens of a step: two pages
 constexpr int kRows = 128;           // query rows of a tile
 constexpr int kBlock = 2 * kRows;    // of a unit
-constexpr int kSoftWarps = 8, kUnpackWarps = 4;
-constexpr int kMmaWarp = kSoftWarps + kUnpackWarps;
-constexpr int kThreads = (kMmaWarp + 1) * 32;
+constexpr int kSoftWarps = 8;
+
+// Float16 caches unpack twice as much; their softmax has the time to go through the scores twice, with fewer registers.
+template <bool F16>
+struct Roles {
+  static constexpr int kUnpackWarps = F16 ? 8 : 4;
+  static constexpr int kMmaWarp = kSoftWarps + kUnpackWarps, kCopyWarp = kMmaWarp + 1;
+  static constexpr int kThreads = (kCopyWarp + 1) * 32;
+  static constexpr bool kOnce = !F16;  // probabilities held in registers until the maximum is known to be in reach
+};
 
 template <int D, bool F16>
 struct Shared {
@@ -235,11 +244,12 @@ __device__ __forceinline__ uint4 unpack8(uint32_t w, __half2 scale, __half2 low,
 __device__ constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
 
 template <int D, bool F16>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Roles<F16>::kThreads, 1)
 q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int slot_rows) {
   using S = Shared<D, F16>;
   using C = Cells<D>;
-  constexpr int kGroups = C::kGroups;
+  constexpr int kGroups = C::kGroups, kUnpackWarps = Roles<F16>::kUnpackWarps;
+  constexpr int kMmaWarp = Roles<F16>::kMmaWarp, kCopyWarp = Roles<F16>::kCopyWarp;
   extern __shared__ uint8_t smem_raw[];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   uint8_t* smem = smem_raw + (1024 - smem_u32(smem_raw) % 1024) % 1024;
@@ -346,7 +356,7 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
         const int limit = real ? q.start + i + 1 : 0;
         const int full_below = q.start + row0 / share + 1;  // tokens below it are seen by every row of the tile
         float ref = 0.f, l = 0.f;
-        bool known = false;
+        bool known = false, settled = false;  // the row has a reference; every row of the warp has
         for (int t = walk.first; t < walk.last; ++t) {
           ok = warp_wait(&s_full[tile], s_iter & 1, a.status, kSiteQ4Attend + kErrWaitAccum, abort_flag);
           ++s_iter;
@@ -354,62 +364,108 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
           tc_fence_after();
           const int base = t * kStep;
           const bool edge = base + kStep > full_below;
-          float top = -INFINITY;
+          bool done = false;
+          if constexpr (Roles<F16>::kOnce) {
+            // ---- every row has a reference and sees all tokens: one pass, and the scores stay until it has held
+            if (settled && !edge) {
+              const uint64_t f2 = f32x2_pack(__float_as_uint(factor), __float_as_uint(factor));
+              const uint64_t o2 = f32x2_pack(__float_as_uint(kBias - ref), __float_as_uint(kBias - ref));
+              uint64_t l2 = 0;
+              float top = -INFINITY;
+              uint32_t p[kStep / 2];
 #pragma unroll
-          for (int c = 0; c < kStep / 32; ++c) {
-            uint32_t s[32];
-            tmem_ld32(s_at + c * 32, s);
-            tmem_ld_wait();
-            tmem_fence32(s);
-            if (edge) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) top = fmaxf(top, base + c * 32 + e < limit ? __uint_as_float(s[e]) : -INFINITY);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(s[e]));
-            }
-          }
-          top *= factor;
-          const bool first = !known && top > -INFINITY;  // the row's first tokens set the reference wherever they are
-          const bool raise = first || (known && top > ref + kSlack);
-          if (__any_sync(0xffffffffu, raise)) {
-            const float down = raise ? (first ? 0.f : exp2_fast(ref - top)) : 1.f;
-            if (raise) {
-              ref = top;
-              l *= down;
-              known = true;
-            }
-            if (t > walk.first) {
-#pragma unroll
-              for (int c = 0; c < D / 16; ++c) {
-                uint32_t x[16];
-                tmem_ld16(o_at + c * 16, x);
+              for (int c = 0; c < kStep / 32; ++c) {
+                uint32_t s[32];
+                tmem_ld32(s_at + c * 32, s);
                 tmem_ld_wait();
-                tmem_reg_fence(x);
+                tmem_fence32(s);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * down);
-                tmem_st16(o_at + c * 16, x);
+                for (int e = 0; e < 16; ++e) {
+                  const uint64_t x = fma_f32x2(f32x2_pack(s[2 * e], s[2 * e + 1]), f2, o2);
+                  const float x0 = __uint_as_float(static_cast<uint32_t>(x)), x1 = __uint_as_float(static_cast<uint32_t>(x >> 32));
+                  top = fmaxf(top, fmaxf(x0, x1));
+                  const float e0 = exp2_fast(x0), e1 = exp2_fast(x1);
+                  l2 = add_f32x2(l2, f32x2_pack(__float_as_uint(e0), __float_as_uint(e1)));
+                  p[c * 16 + e] = pack_half2(e0, e1);
+                }
+              }
+              if (!__any_sync(0xffffffffu, top > kBias + kSlack)) {
+#pragma unroll
+                for (int c = 0; c < kStep / 32; ++c) tmem_st16(s_at + c * 16, reinterpret_cast<const uint32_t(&)[16]>(p[c * 16]));
+                l += f32x2_sum(l2);
+                done = true;
               }
             }
           }
-          const float off = kBias - ref;
+          if (!done) {
+            // ---- the maximum first
+            float top = -INFINITY;
+#pragma unroll 1
+            for (int c = 0; c < kStep / 32; ++c) {
+              uint32_t s[32];
+              tmem_ld32(s_at + c * 32, s);
+              tmem_ld_wait();
+              tmem_fence32(s);
+              const int n = limit - base - c * 32;
+              if (edge) {
 #pragma unroll
-          for (int c = 0; c < kStep / 32; ++c) {
-            uint32_t s[32], p[16];
-            tmem_ld32(s_at + c * 32, s);
-            tmem_ld_wait();
-            tmem_fence32(s);
+                for (int e = 0; e < 32; ++e) top = fmaxf(top, e < n ? __uint_as_float(s[e]) : -INFINITY);
+              } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              float x = fmaf(__uint_as_float(s[e]), factor, off);
-              if (edge && base + c * 32 + e >= limit) x = -INFINITY;
-              x = exp2_fast(x);
-              l += x;
-              s[e] = __float_as_uint(x);
+                for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(s[e]));
+              }
             }
+            top *= factor;
+            const bool first = !known && top > -INFINITY;  // the row's first tokens set the reference wherever they are
+            const bool raise = first || (known && top > ref + kSlack);
+            if (__any_sync(0xffffffffu, raise)) {
+              const float down = raise ? (first ? 0.f : exp2_fast(ref - top)) : 1.f;
+              if (raise) {
+                ref = top;
+                l *= down;
+                known = true;
+              }
+              if (t > walk.first) {
+#pragma unroll 1
+                for (int c = 0; c < D / 16; ++c) {
+                  uint32_t x[16];
+                  tmem_ld16(o_at + c * 16, x);
+                  tmem_ld_wait();
+                  tmem_reg_fence(x);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) p[e] = pack_half2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
-            tmem_st16(s_at + c * 16, p);
+                  for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * down);
+                  tmem_st16(o_at + c * 16, x);
+                }
+              }
+            }
+            settled = __all_sync(0xffffffffu, known);
+            const float off = kBias - ref;
+            const uint64_t f2 = f32x2_pack(__float_as_uint(factor), __float_as_uint(factor));
+            const uint64_t o2 = f32x2_pack(__float_as_uint(off), __float_as_uint(off));
+            uint64_t l2 = 0;
+#pragma unroll 1
+            for (int c = 0; c < kStep / 32; ++c) {
+              uint32_t s[32], p[16];
+              tmem_ld32(s_at + c * 32, s);
+              tmem_ld_wait();
+              tmem_fence32(s);
+              if (edge) {
+                const int n = limit - base - c * 32;
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  s[e] = e < n ? s[e] : 0xff800000u;  // -infinity; the factor is positive
+              }
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const uint64_t x = fma_f32x2(f32x2_pack(s[2 * e], s[2 * e + 1]), f2, o2);
+                const float e0 = exp2_fast(__uint_as_float(static_cast<uint32_t>(x)));
+                const float e1 = exp2_fast(__uint_as_float(static_cast<uint32_t>(x >> 32)));
+                l2 = add_f32x2(l2, f32x2_pack(__float_as_uint(e0), __float_as_uint(e1)));
+                p[e] = pack_half2(e0, e1);
+              }
+              tmem_st16(s_at + c * 16, p);
+            }
+            l += f32x2_sum(l2);
           }
           tmem_st_wait();
           tc_fence_before();
@@ -454,45 +510,11 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
       if (!ok) *abort_flag = 1;
     } else if (warp < kMmaWarp) {
       // ------------------------------------------------------------ unpacking
-      const int token = threadIdx.x - kSoftWarps * 32;  // of the step
-      const int64_t page_stride = static_cast<int64_t>(a.n_kv_heads) * C::kBytes;
-      uint32_t issued = 0, iter = 0;
+      const int token = (threadIdx.x - kSoftWarps * 32) % kStep;  // of the step
+      const int part = (threadIdx.x - kSoftWarps * 32) / kStep;   // which of the kParts shares of it
+      constexpr int kParts = kUnpackWarps / 4;
+      uint32_t iter = 0;
       bool ok = true;
-      // The copies run ahead of the unpacking, over unit boundaries: a second walk, of the first warp alone.
-      Walk ahead(a, share, begin, end);
-      int ahead_t = 0;
-      bool ahead_on = ahead.next();
-      if (ahead_on) ahead_t = ahead.first;
-      auto issue = [&]() {
-        const uint32_t stage = issued % S::kRawStages;
-        if (issued >= S::kRawStages &&
-            !warp_wait(&raw_free[stage], ((issued / S::kRawStages) - 1) & 1, a.status, kSiteQ4Attend + kErrWaitEmpty, abort_flag))
-          return false;
-        if (lane == 0) {
-          const int seen = seen_by(ahead.q, ahead.block, share);
-          const int32_t* table = a.blocks + static_cast<int64_t>(ahead.seq) * a.max_blocks;
-          const uint8_t* cells = a.cells + static_cast<int64_t>(ahead.head) * C::kBytes;
-          const int pages = min(2, pages_of(seen) - 2 * ahead_t);
-          mbar_arrive_expect_tx(&raw_full[stage], pages * C::kBytes);
-          for (int k = 0; k < pages; ++k) {
-            int id = table[2 * ahead_t + k];
-            if (id < 0 || id >= a.n_pages) {  // recorded, and a page that exists read in its place
-              record_error(a.status, kSiteQ4Attend + kErrBadDescriptor);
-              id = 0;
-            }
-            bulk_load(smem + S::kRaw + (stage * 2 + k) * C::kBytes, cells + id * page_stride, C::kBytes, &raw_full[stage]);
-          }
-        }
-        __syncwarp();
-        ++issued;
-        if (++ahead_t == ahead.last) {
-          ahead_on = ahead.next();
-          if (ahead_on) ahead_t = ahead.first;
-        }
-        return true;
-      };
-      if (warp == kSoftWarps)
-        for (int k = 0; k < S::kRawStages && ok && ahead_on; ++k) ok = issue();
       while (ok && walk.next()) {
         const int seen = seen_by(walk.q, walk.block, share);
         for (int t = walk.first; t < walk.last && ok; ++t, ++iter) {
@@ -510,8 +532,8 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
             head[k] = there ? *reinterpret_cast<const uint32_t*>(page + C::kHeads + r * C::kHeadBytes + k * 4) : 0u;
           // ---- keys: the token's four pieces, in an order that keeps the lanes on different banks
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int piece = (k + (D == 128 ? r >> 1 : r >> 2)) & 3;
+          for (int k = 0; k < 4 / kParts; ++k) {
+            const int piece = (k + part * (4 / kParts) + (D == 128 ? r >> 1 : r >> 2)) & 3;
             uint32_t w[D / 32];
             const uint8_t* src = page + C::kKeyCodes + r * (D / 2) + piece * (D / 8);
             if constexpr (D == 128) {
@@ -541,7 +563,8 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
             break;
           }
 #pragma unroll
-          for (int g = 0; g < 8; ++g) {
+          for (int k = 0; k < 8 / kParts; ++k) {
+            const int g = k + part * (8 / kParts);
             uint32_t w[D / 32];
             const uint8_t* src = page + C::value_piece(r >> 1, g);
             if constexpr (D == 128) {
@@ -568,14 +591,47 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
             mbar_arrive(v_full);
             mbar_arrive(&raw_free[stage]);
           }
-          if (warp == kSoftWarps && ahead_on) ok = issue();
+        }
+      }
+      if (!ok) *abort_flag = 1;
+    } else if (warp == kCopyWarp) {
+      // ------------------------------------------------------------ copies of the pages, ahead of the unpacking
+      const int64_t page_stride = static_cast<int64_t>(a.n_kv_heads) * C::kBytes;
+      uint32_t issued = 0;
+      bool ok = true;
+      while (ok && walk.next()) {
+        const int n_pages = pages_of(seen_by(walk.q, walk.block, share));
+        const int32_t* table = a.blocks + static_cast<int64_t>(walk.seq) * a.max_blocks;
+        const uint8_t* cells = a.cells + static_cast<int64_t>(walk.head) * C::kBytes;
+        int ids = 0, ids_at = 2 * walk.first - 32;
+        for (int t = walk.first; t < walk.last && ok; ++t, ++issued) {
+          if (2 * t >= ids_at + 32) {  // the next 32 pages' places, one per lane
+            ids_at = 2 * t;
+            ids = ids_at + lane < n_pages ? table[ids_at + lane] : 0;
+            if (static_cast<unsigned>(ids) >= static_cast<unsigned>(a.n_pages)) {
+              record_error(a.status, kSiteQ4Attend + kErrBadDescriptor);
+              ids = 0;  // recorded, and a page that exists read in its place
+            }
+          }
+          const int id0 = __shfl_sync(0xffffffffu, ids, 2 * t - ids_at), id1 = __shfl_sync(0xffffffffu, ids, 2 * t + 1 - ids_at);
+          const uint32_t stage = issued % S::kRawStages;
+          if (issued >= S::kRawStages)
+            ok = warp_wait(&raw_free[stage], ((issued / S::kRawStages) - 1) & 1, a.status, kSiteQ4Attend + kErrWaitEmpty, abort_flag);
+          if (!ok) break;
+          if (lane == 0) {
+            const bool both = 2 * t + 1 < n_pages;
+            uint8_t* to = smem + S::kRaw + stage * 2 * C::kBytes;
+            mbar_arrive_expect_tx(&raw_full[stage], (both ? 2 : 1) * C::kBytes);
+            bulk_load(to, cells + id0 * page_stride, C::kBytes, &raw_full[stage]);
+            if (both) bulk_load(to + C::kBytes, cells + id1 * page_stride, C::kBytes, &raw_full[stage]);
+          }
+          __syncwarp();
         }
       }
       if (!ok) *abort_flag = 1;
       // No copy is in flight when the CTA leaves.
-      if (warp == kSoftWarps)
-        for (uint32_t n = issued - min(issued, static_cast<uint32_t>(S::kRawStages)); n < issued; ++n)
-          warp_wait(&raw_full[n % S::kRawStages], (n / S::kRawStages) & 1, a.status, kSiteQ4Attend + kErrWaitDrain, nullptr);
+      for (uint32_t n = issued - min(issued, static_cast<uint32_t>(S::kRawStages)); n < issued; ++n)
+        warp_wait(&raw_full[n % S::kRawStages], (n / S::kRawStages) & 1, a.status, kSiteQ4Attend + kErrWaitDrain, nullptr);
     } else {
       // ------------------------------------------------------------ products
       constexpr uint32_t kQk = idesc_f16(kRows, kStep, false, false, false);
@@ -668,10 +724,10 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
 }
 
 // Joins the blocks that several CTAs share and writes the zeros of the rows behind the new tokens: a warp per row.
-constexpr int kCombineWarps = 8, kCombineRows = 32;
+constexpr int kCombineWarps = 8;
 template <int D, bool F16>
 __global__ void __launch_bounds__(kCombineWarps * 32)
-q4_prefill_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int slot_rows) {
+q4_prefill_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int slot_rows, int cta_rows) {
   __shared__ int64_t line[2];
   const int share = a.n_q_heads / a.n_kv_heads;
   const int head = blockIdx.y, seq = blockIdx.z, warp = warp_id(), lane = threadIdx.x & 31;
@@ -687,8 +743,8 @@ q4_prefill_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int work
   const bool failed = cta_failed_at_entry(a.status);
   const int rows = a.q_len * share;
   constexpr int kPer = D / 32;  // dimensions of a lane
-  for (int k = warp; k < kCombineRows; k += kCombineWarps) {
-    const int r = blockIdx.x * kCombineRows + k, i = r / share;
+  for (int k = warp; k < cta_rows; k += kCombineWarps) {
+    const int r = blockIdx.x * cta_rows + k, i = r / share;
     if (r >= rows) break;
     const int64_t to =
         ((static_cast<int64_t>(seq) * a.q_len + i) * a.n_q_heads + head * share + r - i * share) * D + lane * kPer;
@@ -749,10 +805,13 @@ int launch_prefill(const dkv_q4_attend_args& a, cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};
   if (!allow_shared(kernel, Shared<D, F16>::kAlloc, done)) return DKV_ERR_CUDA;
   const int workers = device_sms(), slot_rows = slot_rows_of(a);
-  kernel<<<workers, kThreads, Shared<D, F16>::kAlloc, stream>>>(a, workers, slot_rows);
+  kernel<<<workers, Roles<F16>::kThreads, Shared<D, F16>::kAlloc, stream>>>(a, workers, slot_rows);
   if (cudaGetLastError() != cudaSuccess) return DKV_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((rows_of(a) + kCombineRows - 1) / kCombineRows, a.n_kv_heads, a.n_seq);
+  // Few rows: a warp each, for the joins of a long context are long; many: several each, in about one wave of CTAs.
+  const int64_t rows = static_cast<int64_t>(rows_of(a)) * a.n_kv_heads * a.n_seq;
+  const int cta_rows = rows <= 148 * 8 * kCombineWarps ? kCombineWarps : 4 * kCombineWarps;
+  cfg.gridDim = dim3((rows_of(a) + cta_rows - 1) / cta_rows, a.n_kv_heads, a.n_seq);
   cfg.blockDim = dim3(kCombineWarps * 32);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -760,8 +819,9 @@ int launch_prefill(const dkv_q4_attend_args& a, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, q4_prefill_combine_kernel<D, F16>, a, workers, slot_rows) == cudaSuccess ? DKV_OK
-                                                                                                          : DKV_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, q4_prefill_combine_kernel<D, F16>, a, workers, slot_rows, cta_rows) == cudaSuccess
+             ? DKV_OK
+             : DKV_ERR_CUDA;
 }
 
 }  // namespace
