@@ -8,18 +8,19 @@
 //
 //   warps 0-3, 4-7   softmax of the first and the second tile, one row per thread: scores from TMEM, probabilities
 //                    back into TMEM (over the scores they come from), where the second product takes them
-//   warps 8-11       unpack 128 tokens (two pages) of cells, one token per thread, into float16 tiles with the 128-byte
-//                    swizzle, keys as rows, values as the rows of the contraction (8-15, two threads per token, for
-//                    float16 caches, see below)
-//   two more         one issues the products (per step P V of a tile, then at once the next Q K of it), the other the
-//                    bulk copies of the pages
+//   warps 8-11       unpack the keys of 128 tokens (two pages), one token per thread, into a float16 tile with the
+//                    128-byte swizzle
+//   warps 12-15      the same for the values, which become the rows of the second product's contraction
+//   warp 16, 17      issue the products (per step P V of a tile, then at once the next Q K of it), and the copies of
+//                    the pages
 //
 // TMEM: two score tiles, two outputs, 512 columns. The rows' references (running maxima) lag by up to 2^8, so that
 // outputs are scaled down in TMEM only when a row's maximum has grown past that; a score tile that is complete means
 // that the product issued before it is too, so nothing else has to be waited for.
 //
-// Keys and values are rounded to float16 (2^-11 at most of each), probabilities likewise; for float16 caches, whose
-// outputs show that, what the rounding of keys and values lacks forms second tiles that go through second products.
+// Keys and values are rounded to float16 (2^-11 at most of each), probabilities likewise. For float16 caches, whose
+// outputs show that, what the rounding of keys lacks forms a second tile, and what that of probabilities lacks a second
+// operand beside the first (each 32 columns of scores become 16 of either), that go through second products.
 //
 // The 128-token steps of all (conversation, KV head, 256-row block) units form one line that is cut evenly over one CTA per
 // SM; blocks that several CTAs share leave partial results in the workspace, which q4_prefill_combine_kernel joins.
@@ -34,14 +35,12 @@ constexpr int kRows = 128;           // query rows of a tile
 constexpr int kBlock = 2 * kRows;    // of a unit
 constexpr int kSoftWarps = 8;
 
-// Float16 caches unpack twice as much; their softmax has the time to go through the scores twice, with fewer registers.
-template <bool F16>
-struct Roles {
-  static constexpr int kUnpackWarps = F16 ? 8 : 4;
-  static constexpr int kMmaWarp = kSoftWarps + kUnpackWarps, kCopyWarp = kMmaWarp + 1;
-  static constexpr int kThreads = (kCopyWarp + 1) * 32;
-  static constexpr bool kOnce = !F16;  // probabilities held in registers until the maximum is known to be in reach
-};
+constexpr int kUnpackWarps = 4;  // of the keys, and of the values
+constexpr int kKeyWarp = kSoftWarps, kValueWarp = kKeyWarp + kUnpackWarps, kMmaWarp = kValueWarp + kUnpackWarps,
+              kCopyWarp = kMmaWarp + 1;
+constexpr int kThreads = (kMmaWarp + 4) * 32;  // whole warpgroups: registers are dealt to these
+// Registers per thread: 96 at launch (5 warpgroups, 480 in all), then 2 x 128 + 2 x 72 + 80 = 480.
+constexpr int kSoftRegs = 128, kUnpackRegs = 72, kIssueRegs = 80;
 
 template <int D, bool F16>
 struct Shared {
@@ -51,12 +50,11 @@ struct Shared {
   static constexpr int kRawStages = F16 ? 1 : 2;
   static constexpr int kQ = 0;                        // two tiles
   static constexpr int kK = kQ + 2 * kTile;
-  static constexpr int kV = kK + kTile;
-  static constexpr int kKLow = kV + kTile;            // what the rounding lacks (float16 caches)
-  static constexpr int kVLow = kKLow + (F16 ? kTile : 0);
-  static constexpr int kRaw = kVLow + (F16 ? kTile : 0);
+  static constexpr int kV = kK + kTile;               // two stages: values wait for the whole of a step
+  static constexpr int kKLow = kV + 2 * kTile;        // what the rounding of keys lacks (float16 caches)
+  static constexpr int kRaw = kKLow + (F16 ? kTile : 0);
   static constexpr int kBars = kRaw + kRawStages * 2 * C::kBytes;
-  static constexpr int kNumBars = 2 * kRawStages + 4 + 2 * 4 + 1;
+  static constexpr int kNumBars = 2 * kRawStages + 6 + 2 * 4 + 1;
   static constexpr int kBytes = kBars + kNumBars * 8 + 16;
   static constexpr int kAlloc = kBytes + 1024;        // the tiles begin on a 1024-byte boundary
 };
@@ -244,12 +242,11 @@ __device__ __forceinline__ uint4 unpack8(uint32_t w, __half2 scale, __half2 low,
 __device__ constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
 
 template <int D, bool F16>
-__global__ void __launch_bounds__(Roles<F16>::kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 1)
 q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int slot_rows) {
   using S = Shared<D, F16>;
   using C = Cells<D>;
-  constexpr int kGroups = C::kGroups, kUnpackWarps = Roles<F16>::kUnpackWarps;
-  constexpr int kMmaWarp = Roles<F16>::kMmaWarp, kCopyWarp = Roles<F16>::kCopyWarp;
+  constexpr int kGroups = C::kGroups;
   extern __shared__ uint8_t smem_raw[];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   uint8_t* smem = smem_raw + (1024 - smem_u32(smem_raw) % 1024) % 1024;
@@ -258,9 +255,9 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
   uint64_t* raw_free = raw_full + S::kRawStages; // unpacked
   uint64_t* k_full = raw_free + S::kRawStages;
   uint64_t* v_full = k_full + 1;
-  uint64_t* k_free = v_full + 1;                 // products that read the tile are complete
+  uint64_t* k_free = v_full + 2;                 // products that read the tile are complete
   uint64_t* v_free = k_free + 1;
-  uint64_t* q_full = v_free + 1;                 // [2], by tile
+  uint64_t* q_full = v_free + 2;                 // [2], by tile
   uint64_t* s_full = q_full + 2;                 // [2] scores complete
   uint64_t* p_full = s_full + 2;                 // [2] probabilities in TMEM
   uint64_t* o_full = p_full + 2;                 // [2] a unit's last product complete
@@ -273,13 +270,13 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kRawStages; ++i) {
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_free[i], kUnpackWarps);
+      mbar_init(&raw_free[i], 2 * kUnpackWarps);
     }
     mbar_init(k_full, kUnpackWarps);
-    mbar_init(v_full, kUnpackWarps);
     mbar_init(k_free, 1);
-    mbar_init(v_free, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&v_full[i], kUnpackWarps);
+      mbar_init(&v_free[i], 1);
       mbar_init(&q_full[i], 4);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
@@ -304,8 +301,11 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
   }
   // scores of tile i: columns 128 i .. (its probabilities in the first 64 of them); outputs: columns 256 + 128 i ..
   if (begin < end) {
-    Walk walk(a, share, begin, end);
+    // Every warp of the warpgroups gives or takes its registers at the head of its role (the compiler allots the roles'
+    // code by that), the two without a role as well.
     if (warp < kSoftWarps) {
+      setmaxnreg_inc<kSoftRegs>();
+      Walk walk(a, share, begin, end);
       // ------------------------------------------------------------ softmax
       const int tile = warp >> 2, row_in_tile = (warp & 3) * 32 + lane;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -326,19 +326,22 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
           const uint16_t* src = static_cast<const uint16_t*>(a.query) + walk.seq * a.q_stride[0] +
                                 (walk.head * share + r - i * share) * a.q_stride[1] + i * a.q_stride[2];
           float big = 0.f;
-          if (real)
+          if (real) {
+            for (int c = 0; c < D / 64; ++c) prefetch_l1(src + c * 64);
+#pragma unroll 2
             for (int c = 0; c < D / 8; ++c) {
               const uint4 u = *reinterpret_cast<const uint4*>(src + c * 8);
               const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
               for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(from16<F16>(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1))))));
             }
+          }
           const int ex = (__float_as_uint(big) >> 23) & 255;
           const float up = __uint_as_float(static_cast<uint32_t>(min(254, max(1, 267 - ex))) << 23);
           // a negative scaling goes into the query, so that the largest product is the largest score
           const float f = a.scaling < 0.f ? -up : up;
           factor = fabsf(a.scaling) * kLog2e / up;
-#pragma unroll 4
+#pragma unroll 2
           for (int c = 0; c < D / 8; ++c) {
             uint4 u = make_uint4(0u, 0u, 0u, 0u);
             if (real) u = *reinterpret_cast<const uint4*>(src + c * 8);
@@ -355,8 +358,10 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
         }
         const int limit = real ? q.start + i + 1 : 0;
         const int full_below = q.start + row0 / share + 1;  // tokens below it are seen by every row of the tile
-        float ref = 0.f, l = 0.f;
-        bool known = false, settled = false;  // the row has a reference; every row of the warp has
+        const uint64_t f2 = f32x2_pack(__float_as_uint(factor), __float_as_uint(factor));
+        float ref = 0.f;
+        uint64_t l2 = 0;     // two sums, of the even and the odd tokens
+        bool known = false;  // the row has a reference
         for (int t = walk.first; t < walk.last; ++t) {
           ok = warp_wait(&s_full[tile], s_iter & 1, a.status, kSiteQ4Attend + kErrWaitAccum, abort_flag);
           ++s_iter;
@@ -364,108 +369,77 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
           tc_fence_after();
           const int base = t * kStep;
           const bool edge = base + kStep > full_below;
-          bool done = false;
-          if constexpr (Roles<F16>::kOnce) {
-            // ---- every row has a reference and sees all tokens: one pass, and the scores stay until it has held
-            if (settled && !edge) {
-              const uint64_t f2 = f32x2_pack(__float_as_uint(factor), __float_as_uint(factor));
-              const uint64_t o2 = f32x2_pack(__float_as_uint(kBias - ref), __float_as_uint(kBias - ref));
-              uint64_t l2 = 0;
-              float top = -INFINITY;
-              uint32_t p[kStep / 2];
-#pragma unroll
-              for (int c = 0; c < kStep / 32; ++c) {
-                uint32_t s[32];
-                tmem_ld32(s_at + c * 32, s);
-                tmem_ld_wait();
-                tmem_fence32(s);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  const uint64_t x = fma_f32x2(f32x2_pack(s[2 * e], s[2 * e + 1]), f2, o2);
-                  const float x0 = __uint_as_float(static_cast<uint32_t>(x)), x1 = __uint_as_float(static_cast<uint32_t>(x >> 32));
-                  top = fmaxf(top, fmaxf(x0, x1));
-                  const float e0 = exp2_fast(x0), e1 = exp2_fast(x1);
-                  l2 = add_f32x2(l2, f32x2_pack(__float_as_uint(e0), __float_as_uint(e1)));
-                  p[c * 16 + e] = pack_half2(e0, e1);
-                }
-              }
-              if (!__any_sync(0xffffffffu, top > kBias + kSlack)) {
-#pragma unroll
-                for (int c = 0; c < kStep / 32; ++c) tmem_st16(s_at + c * 16, reinterpret_cast<const uint32_t(&)[16]>(p[c * 16]));
-                l += f32x2_sum(l2);
-                done = true;
-              }
-            }
-          }
-          if (!done) {
-            // ---- the maximum first
-            float top = -INFINITY;
+          // 32 scores at a time become 16 columns of probabilities (and 16 of what their rounding lacks) in their place. The
+          // loop stays rolled: five roles share the instruction cache.
 #pragma unroll 1
-            for (int c = 0; c < kStep / 32; ++c) {
-              uint32_t s[32];
-              tmem_ld32(s_at + c * 32, s);
-              tmem_ld_wait();
-              tmem_fence32(s);
+          for (int c = 0; c < kStep / 32; ++c) {
+            uint32_t s[32];
+            tmem_ld32(s_at + c * 32, s);
+            tmem_ld_wait();
+            tmem_fence32(s);
+            if (edge) {
               const int n = limit - base - c * 32;
-              if (edge) {
 #pragma unroll
-                for (int e = 0; e < 32; ++e) top = fmaxf(top, e < n ? __uint_as_float(s[e]) : -INFINITY);
-              } else {
-#pragma unroll
-                for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(s[e]));
-              }
+              for (int e = 0; e < 32; ++e) s[e] = e < n ? s[e] : 0xff800000u;  // -infinity; the factor is positive
             }
-            top *= factor;
-            const bool first = !known && top > -INFINITY;  // the row's first tokens set the reference wherever they are
-            const bool raise = first || (known && top > ref + kSlack);
+            const uint64_t o2 = f32x2_pack(__float_as_uint(kBias - ref), __float_as_uint(kBias - ref));
+            float top = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const uint64_t x = fma_f32x2(f32x2_pack(s[2 * e], s[2 * e + 1]), f2, o2);
+              s[2 * e] = static_cast<uint32_t>(x);
+              s[2 * e + 1] = static_cast<uint32_t>(x >> 32);
+              top = fmaxf(top, fmaxf(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])));
+            }
+            const bool raise = known ? top > kBias + kSlack : top > -INFINITY;
             if (__any_sync(0xffffffffu, raise)) {
-              const float down = raise ? (first ? 0.f : exp2_fast(ref - top)) : 1.f;
-              if (raise) {
-                ref = top;
-                l *= down;
-                known = true;
-              }
+              // ---- a row's first tokens set its reference, a maximum beyond the slack moves it: by a whole number, so that
+              // what is scaled down for it (the output, this step's probabilities so far) loses nothing
+              const float up = raise ? ceilf(top - kBias) : 0.f;
+              const float down = !raise ? 1.f : known ? exp2_fast(-up) : 0.f;
+              ref += up;
+              known = known || raise;
+              l2 = mul_f32x2(l2, f32x2_pack(__float_as_uint(down), __float_as_uint(down)));
+#pragma unroll
+              for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) - up);
               if (t > walk.first) {
 #pragma unroll 1
-                for (int c = 0; c < D / 16; ++c) {
+                for (int k = 0; k < D / 16; ++k) {
                   uint32_t x[16];
-                  tmem_ld16(o_at + c * 16, x);
+                  tmem_ld16(o_at + k * 16, x);
                   tmem_ld_wait();
                   tmem_reg_fence(x);
 #pragma unroll
                   for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * down);
-                  tmem_st16(o_at + c * 16, x);
+                  tmem_st16(o_at + k * 16, x);
                 }
               }
-            }
-            settled = __all_sync(0xffffffffu, known);
-            const float off = kBias - ref;
-            const uint64_t f2 = f32x2_pack(__float_as_uint(factor), __float_as_uint(factor));
-            const uint64_t o2 = f32x2_pack(__float_as_uint(off), __float_as_uint(off));
-            uint64_t l2 = 0;
+              const __half2 d2 = __float2half2_rn(down);
 #pragma unroll 1
-            for (int c = 0; c < kStep / 32; ++c) {
-              uint32_t s[32], p[16];
-              tmem_ld32(s_at + c * 32, s);
-              tmem_ld_wait();
-              tmem_fence32(s);
-              if (edge) {
-                const int n = limit - base - c * 32;
+              for (int k = 0; k < (F16 ? 2 : 1) * c; ++k) {
+                uint32_t x[16];
+                const uint32_t at = s_at + (F16 ? k * 16 : k * 32);
+                tmem_ld16(at, x);
+                tmem_ld_wait();
+                tmem_reg_fence(x);
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  s[e] = e < n ? s[e] : 0xff800000u;  // -infinity; the factor is positive
+                for (int e = 0; e < 16; ++e) x[e] = as_u32(__hmul2(as_half2(x[e]), d2));
+                tmem_st16(at, x);
               }
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const uint64_t x = fma_f32x2(f32x2_pack(s[2 * e], s[2 * e + 1]), f2, o2);
-                const float e0 = exp2_fast(__uint_as_float(static_cast<uint32_t>(x)));
-                const float e1 = exp2_fast(__uint_as_float(static_cast<uint32_t>(x >> 32)));
-                l2 = add_f32x2(l2, f32x2_pack(__float_as_uint(e0), __float_as_uint(e1)));
-                p[e] = pack_half2(e0, e1);
-              }
-              tmem_st16(s_at + c * 16, p);
             }
-            l += f32x2_sum(l2);
+            uint32_t p[16], lack[F16 ? 16 : 1];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float e0 = exp2_fast(__uint_as_float(s[2 * e])), e1 = exp2_fast(__uint_as_float(s[2 * e + 1]));
+              l2 = add_f32x2(l2, f32x2_pack(__float_as_uint(e0), __float_as_uint(e1)));
+              p[e] = pack_half2(e0, e1);
+              if constexpr (F16) {
+                const float2 back = __half22float2(as_half2(p[e]));
+                lack[e] = pack_half2(e0 - back.x, e1 - back.y);
+              }
+            }
+            tmem_st16(s_at + c * 32, p);
+            if constexpr (F16) tmem_st16(s_at + c * 32 + 16, lack);
           }
           tmem_st_wait();
           tc_fence_before();
@@ -477,12 +451,17 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
         ++units;
         if (!ok) break;
         tc_fence_after();
+        const float l = f32x2_sum(l2);
         const bool whole = walk.whole();
         const float inv = !whole ? 1.f : l != 0.f ? 1.f / l : 0.f;
         const int64_t to = ((static_cast<int64_t>(walk.seq) * a.q_len + i) * a.n_q_heads + walk.head * share + r - i * share) * D;
         const int row = tile * kRows + row_in_tile;  // of the block
         float* slot = a.workspace + (2 * static_cast<int64_t>(blockIdx.x) + (unit_begin == begin ? 0 : 1)) * slot_floats(slot_rows, D);
-#pragma unroll
+        const unsigned reals = __ballot_sync(0xffffffffu, real);
+        // 32 dimensions of the warp's 32 rows at a time through shared memory (the tile's queries are done with), so that
+        // eight lanes write a row's 128 bytes
+        float* box = reinterpret_cast<float*>(smem + S::kQ + tile * S::kTile) + (warp & 3) * 1024;
+#pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t x[32];
           __syncwarp();
@@ -490,111 +469,115 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
           tmem_ld_wait();
           tmem_fence32(x);
 #pragma unroll
-          for (int h = 0; h < 4 && real; ++h) {
+          for (int h = 0; h < 4; ++h) {
             float y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[kOrder[e]] = __uint_as_float(x[h * 8 + e]) * inv;
-            const int dim = c * 32 + h * 8;
-            if (whole) {
-              store_out4<F16>(a, to + dim, y[0], y[1], y[2], y[3]);
-              store_out4<F16>(a, to + dim + 4, y[4], y[5], y[6], y[7]);
-            } else {
-              *reinterpret_cast<float4*>(slot + row * D + dim) = make_float4(y[0], y[1], y[2], y[3]);
-              *reinterpret_cast<float4*>(slot + row * D + dim + 4) = make_float4(y[4], y[5], y[6], y[7]);
+            *reinterpret_cast<float4*>(box + lane * 32 + ((2 * h) ^ (lane & 7)) * 4) = make_float4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<float4*>(box + lane * 32 + ((2 * h + 1) ^ (lane & 7)) * 4) = make_float4(y[4], y[5], y[6], y[7]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int from = k * 4 + (lane >> 3), dim = c * 32 + (lane & 7) * 4;  // the row's lane, the dimension
+            const float4 v = *reinterpret_cast<const float4*>(box + from * 32 + ((lane & 7) ^ (from & 7)) * 4);
+            const int64_t at = __shfl_sync(0xffffffffu, to, from);
+            if ((reals >> from) & 1u) {
+              if (whole) store_out4<F16>(a, at + dim, v.x, v.y, v.z, v.w);
+              else *reinterpret_cast<float4*>(slot + (row - lane + from) * D + dim) = v;
             }
           }
         }
+        fence_async_shared();  // the next unit's queries come after these
         if (!whole && real) *reinterpret_cast<float2*>(slot + slot_rows * D + row * 4) = make_float2(ref, l);
         tc_fence_before();
       }
       if (!ok) *abort_flag = 1;
     } else if (warp < kMmaWarp) {
       // ------------------------------------------------------------ unpacking
-      const int token = (threadIdx.x - kSoftWarps * 32) % kStep;  // of the step
-      const int part = (threadIdx.x - kSoftWarps * 32) / kStep;   // which of the kParts shares of it
-      constexpr int kParts = kUnpackWarps / 4;
+      setmaxnreg_dec<kUnpackRegs>();
+      Walk walk(a, share, begin, end);
+      const bool values = warp >= kValueWarp;
+      const int token = threadIdx.x % kStep;  // of the step
+      const int r = token % kPage;
       uint32_t iter = 0;
       bool ok = true;
       while (ok && walk.next()) {
         const int seen = seen_by(walk.q, walk.block, share);
-        for (int t = walk.first; t < walk.last && ok; ++t, ++iter) {
+        for (int t = walk.first; t < walk.last; ++t, ++iter) {
           const uint32_t stage = iter % S::kRawStages;
           ok = warp_wait(&raw_full[stage], (iter / S::kRawStages) & 1, a.status, kSiteQ4Attend + kErrWaitCodes, abort_flag) &&
-               (iter == 0 || warp_wait(k_free, (iter - 1) & 1, a.status, kSiteQ4Attend + kErrWaitEmpty, abort_flag));
+               (values ? iter < 2 || warp_wait(&v_free[iter & 1], ((iter >> 1) - 1) & 1, a.status,
+                                               kSiteQ4Attend + kErrWaitEmpty, abort_flag)
+                       : iter == 0 || warp_wait(k_free, (iter - 1) & 1, a.status, kSiteQ4Attend + kErrWaitEmpty, abort_flag));
           if (!ok) break;
           const uint8_t* page = smem + S::kRaw + (stage * 2 + token / kPage) * C::kBytes;
-          const int r = token % kPage;
           // a token that no row sees may never have been written: zeros, no NaN of its
           const bool there = t * kStep + token < seen;
-          uint32_t head[2 * kGroups];
+          __half2 scale[kGroups], low[kGroups];
 #pragma unroll
-          for (int k = 0; k < 2 * kGroups; ++k)
-            head[k] = there ? *reinterpret_cast<const uint32_t*>(page + C::kHeads + r * C::kHeadBytes + k * 4) : 0u;
-          // ---- keys: the token's four pieces, in an order that keeps the lanes on different banks
-#pragma unroll
-          for (int k = 0; k < 4 / kParts; ++k) {
-            const int piece = (k + part * (4 / kParts) + (D == 128 ? r >> 1 : r >> 2)) & 3;
-            uint32_t w[D / 32];
-            const uint8_t* src = page + C::kKeyCodes + r * (D / 2) + piece * (D / 8);
-            if constexpr (D == 128) {
-              const uint4 u = *reinterpret_cast<const uint4*>(src);
-              w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-            } else {
-              const uint2 u = *reinterpret_cast<const uint2*>(src);
-              w[0] = u.x, w[1] = u.y;
-            }
-#pragma unroll
-            for (int e = 0; e < D / 32; ++e) {
-              const int gr = e >> 1, chunk = piece * 2 + (e & 1);
-              const __half2 h = as_half2(head[gr]);
-              uint4 lack;
-              const uint4 x = unpack8<F16>(w[e], __low2half2(h), __high2half2(h), lack);
-              const uint32_t to = gr * S::kPart + sw128_offset(token, chunk);
-              *reinterpret_cast<uint4*>(smem + S::kK + to) = x;
-              if constexpr (F16) *reinterpret_cast<uint4*>(smem + S::kKLow + to) = lack;
-            }
+          for (int gr = 0; gr < kGroups; ++gr) {
+            const __half2 h = as_half2(
+                there ? *reinterpret_cast<const uint32_t*>(page + (values ? C::value_head(r, gr) : C::key_head(r, gr))) : 0u);
+            scale[gr] = __low2half2(h);
+            low[gr] = __high2half2(h);
           }
-          fence_async_shared();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(k_full);
-          // ---- values: the pair's eight pieces, this token's halves of them
-          if (iter > 0 && !warp_wait(v_free, (iter - 1) & 1, a.status, kSiteQ4Attend + kErrWaitEmpty, abort_flag)) {
-            ok = false;
-            break;
-          }
+          if (!values) {
+            // the token's four pieces, in an order that keeps the lanes on different banks
+#pragma unroll 2
+            for (int k = 0; k < 4; ++k) {
+              const int piece = (k + (D == 128 ? r >> 1 : r >> 2)) & 3;
+              uint32_t w[D / 32];
+              const uint8_t* src = page + C::kKeyCodes + r * (D / 2) + piece * (D / 8);
+              if constexpr (D == 128) {
+                const uint4 u = *reinterpret_cast<const uint4*>(src);
+                w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+              } else {
+                const uint2 u = *reinterpret_cast<const uint2*>(src);
+                w[0] = u.x, w[1] = u.y;
+              }
 #pragma unroll
-          for (int k = 0; k < 8 / kParts; ++k) {
-            const int g = k + part * (8 / kParts);
-            uint32_t w[D / 32];
-            const uint8_t* src = page + C::value_piece(r >> 1, g);
-            if constexpr (D == 128) {
-              const uint4 u = *reinterpret_cast<const uint4*>(src);
-              w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-            } else {
-              const uint2 u = *reinterpret_cast<const uint2*>(src);
-              w[0] = u.x, w[1] = u.y;
+              for (int e = 0; e < D / 32; ++e) {
+                uint4 lack;
+                const uint4 x = unpack8<F16>(w[e], scale[e >> 1], low[e >> 1], lack);
+                const uint32_t to = (e >> 1) * S::kPart + sw128_offset(token, piece * 2 + (e & 1));
+                *reinterpret_cast<uint4*>(smem + S::kK + to) = x;
+                if constexpr (F16) *reinterpret_cast<uint4*>(smem + S::kKLow + to) = lack;
+              }
             }
+          } else {
+            // the pair's eight pieces, this token's halves of them
+#pragma unroll 4
+            for (int g = 0; g < 8; ++g) {
+              uint32_t w[D / 32];
+              const uint8_t* src = page + C::value_piece(r >> 1, g);
+              if constexpr (D == 128) {
+                const uint4 u = *reinterpret_cast<const uint4*>(src);
+                w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+              } else {
+                const uint2 u = *reinterpret_cast<const uint2*>(src);
+                w[0] = u.x, w[1] = u.y;
+              }
 #pragma unroll
-            for (int gr = 0; gr < kGroups; ++gr) {
-              const __half2 h = as_half2(head[kGroups + gr]);
-              uint4 lack;
-              const uint4 x = unpack8<F16>(__byte_perm(w[2 * gr], w[2 * gr + 1], r & 1 ? 0x7632 : 0x5410), __low2half2(h),
-                                           __high2half2(h), lack);
-              const uint32_t to = gr * S::kPart + sw128_offset(token, g);
-              *reinterpret_cast<uint4*>(smem + S::kV + to) = x;
-              if constexpr (F16) *reinterpret_cast<uint4*>(smem + S::kVLow + to) = lack;
+              for (int gr = 0; gr < kGroups; ++gr) {
+                uint4 none;
+                *reinterpret_cast<uint4*>(smem + S::kV + (iter & 1) * S::kTile + gr * S::kPart + sw128_offset(token, g)) =
+                    unpack8<false>(__byte_perm(w[2 * gr], w[2 * gr + 1], r & 1 ? 0x7632 : 0x5410), scale[gr], low[gr], none);
+              }
             }
           }
           fence_async_shared();
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(v_full);
+            mbar_arrive(values ? &v_full[iter & 1] : k_full);
             mbar_arrive(&raw_free[stage]);
           }
         }
       }
       if (!ok) *abort_flag = 1;
     } else if (warp == kCopyWarp) {
+      setmaxnreg_dec<kIssueRegs>();
+      Walk walk(a, share, begin, end);
       // ------------------------------------------------------------ copies of the pages, ahead of the unpacking
       const int64_t page_stride = static_cast<int64_t>(a.n_kv_heads) * C::kBytes;
       uint32_t issued = 0;
@@ -632,7 +615,11 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
       // No copy is in flight when the CTA leaves.
       for (uint32_t n = issued - min(issued, static_cast<uint32_t>(S::kRawStages)); n < issued; ++n)
         warp_wait(&raw_full[n % S::kRawStages], (n / S::kRawStages) & 1, a.status, kSiteQ4Attend + kErrWaitDrain, nullptr);
+    } else if (warp > kCopyWarp) {
+      setmaxnreg_dec<kIssueRegs>();
     } else {
+      setmaxnreg_dec<kIssueRegs>();
+      Walk walk(a, share, begin, end);
       // ------------------------------------------------------------ products
       constexpr uint32_t kQk = idesc_f16(kRows, kStep, false, false, false);
       constexpr uint32_t kPv = idesc_f16(kRows, D, false, false, true);
@@ -643,31 +630,40 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
         ok = ok && warp_wait(bar, parity, a.status, kSiteQ4Attend + err, abort_flag);
         return ok;
       };
+      // A step of 16 dimensions is 32 bytes further in a row, one of 64 the next part; 16 tokens are 2048 bytes further.
       auto scores = [&](int tile) {  // Q K of the tile
         if (lane == 0) {
           const uint32_t q_at = smem_u32(smem + S::kQ + tile * S::kTile);
-#pragma unroll
+          uint32_t on = 0;
+#pragma unroll 1
           for (int part = 0; part < (F16 ? 2 : 1); ++part)
+#pragma unroll 1
+            for (int gr = 0; gr < kGroups; ++gr) {
+              const uint64_t q_desc = smem_desc_sw128(q_at + gr * S::kPart, 16, 1024);
+              const uint64_t k_desc = smem_desc_sw128(k_at + (part ? S::kKLow - S::kK : 0) + gr * S::kPart, 16, 1024);
 #pragma unroll
-            for (int gr = 0; gr < kGroups; ++gr)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                mma_f16(tmem + tile * 128, smem_desc_sw128(q_at + gr * S::kPart + 32 * k, 16, 1024),
-                        smem_desc_sw128(k_at + (part ? S::kKLow - S::kK : 0) + gr * S::kPart + 32 * k, 16, 1024), kQk,
-                        part > 0 || gr > 0 || k > 0);
+              for (int k = 0; k < 4; ++k) {
+                mma_f16(tmem + tile * 128, q_desc + 2 * k, k_desc + 2 * k, kQk, on);
+                on = 1;
+              }
+            }
           mma_commit(&s_full[tile]);
         }
         __syncwarp();
       };
-      auto outputs = [&](int tile, bool first) {  // P V of the tile
+      auto outputs = [&](int tile, bool first, uint32_t stage) {  // P V of the tile
         if (lane == 0) {
+          uint32_t on = first ? 0u : 1u;
+#pragma unroll 1
+          for (int part = 0; part < (F16 ? 2 : 1); ++part) {
+            const uint32_t p_at = tmem + tile * 128 + part * 16;
+            const uint64_t v_desc = smem_desc_sw128(v_at + stage * S::kTile, S::kPart, 1024);
 #pragma unroll
-          for (int part = 0; part < (F16 ? 2 : 1); ++part)
-#pragma unroll
-            for (int k = 0; k < kStep / 16; ++k)
-              mma_f16_ta(tmem + 256 + tile * 128, tmem + tile * 128 + 8 * k,
-                         smem_desc_sw128(v_at + (part ? S::kVLow - S::kV : 0) + 2048 * k, S::kPart, 1024), kPv,
-                         !first || part > 0 || k > 0);
+            for (int k = 0; k < kStep / 16; ++k) {
+              mma_f16_ta(tmem + 256 + tile * 128, p_at + (k >> 1) * 32 + (k & 1) * 8, v_desc + 128 * k, kPv, on);
+              on = 1;
+            }
+          }
         }
         __syncwarp();
       };
@@ -692,10 +688,10 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
           for (int tile = 0; tile < (two ? 2 : 1); ++tile) {
             if (!wait(&p_full[tile], p_iter[tile] & 1, kErrWaitA)) break;
             ++p_iter[tile];
-            if (tile == 0 && !wait(v_full, iter & 1, kErrWaitA)) break;
+            if (tile == 0 && !wait(&v_full[iter & 1], (iter >> 1) & 1, kErrWaitA)) break;
             tc_fence_after();
-            outputs(tile, t == 0);
-            if (tile == (two ? 1 : 0)) commit(v_free);
+            outputs(tile, t == 0, iter & 1);
+            if (tile == (two ? 1 : 0)) commit(&v_free[iter & 1]);
             if (t + 1 == n) {
               commit(&o_full[tile]);
               ++units[tile];
@@ -805,7 +801,7 @@ int launch_prefill(const dkv_q4_attend_args& a, cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};
   if (!allow_shared(kernel, Shared<D, F16>::kAlloc, done)) return DKV_ERR_CUDA;
   const int workers = device_sms(), slot_rows = slot_rows_of(a);
-  kernel<<<workers, Roles<F16>::kThreads, Shared<D, F16>::kAlloc, stream>>>(a, workers, slot_rows);
+  kernel<<<workers, kThreads, Shared<D, F16>::kAlloc, stream>>>(a, workers, slot_rows);
   if (cudaGetLastError() != cudaSuccess) return DKV_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   // Few rows: a warp each, for the joins of a long context are long; many: several each, in about one wave of CTAs.
