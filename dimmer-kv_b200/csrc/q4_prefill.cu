@@ -325,27 +325,26 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
         {
           const uint16_t* src = static_cast<const uint16_t*>(a.query) + walk.seq * a.q_stride[0] +
                                 (walk.head * share + r - i * share) * a.q_stride[1] + i * a.q_stride[2];
-          float big = 0.f;
-          if (real) {
-            for (int c = 0; c < D / 64; ++c) prefetch_l1(src + c * 64);
-#pragma unroll 2
-            for (int c = 0; c < D / 8; ++c) {
-              const uint4 u = *reinterpret_cast<const uint4*>(src + c * 8);
-              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+          uint4 raw[D / 8];  // the row, all of its loads under way at once
 #pragma unroll
-              for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(from16<F16>(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1))))));
-            }
+          for (int c = 0; c < D / 8; ++c)
+            raw[c] = real ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+          uint32_t most = 0;
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) {
+            const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) most = extreme2<F16, true>(most, w[e] & 0x7fff7fffu);
           }
+          const float big = fmaxf(from16<F16>(static_cast<uint16_t>(most)), from16<F16>(static_cast<uint16_t>(most >> 16)));
           const int ex = (__float_as_uint(big) >> 23) & 255;
           const float up = __uint_as_float(static_cast<uint32_t>(min(254, max(1, 267 - ex))) << 23);
           // a negative scaling goes into the query, so that the largest product is the largest score
           const float f = a.scaling < 0.f ? -up : up;
           factor = fabsf(a.scaling) * kLog2e / up;
-#pragma unroll 2
+#pragma unroll
           for (int c = 0; c < D / 8; ++c) {
-            uint4 u = make_uint4(0u, 0u, 0u, 0u);
-            if (real) u = *reinterpret_cast<const uint4*>(src + c * 8);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = from16<F16>(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)))) * f;
@@ -370,7 +369,8 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
           const int base = t * kStep;
           const bool edge = base + kStep > full_below;
           // 32 scores at a time become 16 columns of probabilities (and 16 of what their rounding lacks) in their place. The
-          // loop stays rolled: five roles share the instruction cache.
+          // loop stays rolled: five roles share the instruction cache (and with the next scores loaded ahead, the registers
+          // that these take cost as much as the wait for them).
 #pragma unroll 1
           for (int c = 0; c < kStep / 32; ++c) {
             uint32_t s[32];
@@ -757,26 +757,39 @@ q4_prefill_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int work
       const int64_t stride = slot_floats(slot_rows, D);
       const float* first = a.workspace + (2 * static_cast<int64_t>(w0) + (deal.begin(w0) < unit ? 1 : 0)) * stride;
       const float* rest = a.workspace + 2 * static_cast<int64_t>(w0) * stride;
+      auto slot = [&](int w) { return w == 0 ? first : rest + 2 * w * stride; };
       float den = 0.f, ref = -INFINITY;
-#pragma unroll 4
-      for (int w = 0; w <= w1 - w0; ++w) {
-        const float* slot = w == 0 ? first : rest + 2 * w * stride;
-        const float2 s = *reinterpret_cast<const float2*>(slot + slot_rows * D + row * 4);
-        float o[kPer];
-        if constexpr (kPer == 4) {
-          const float4 u = *reinterpret_cast<const float4*>(slot + row * D + lane * 4);
-          o[0] = u.x, o[1] = u.y, o[2] = u.z, o[3] = u.w;
-        } else {
-          const float2 u = *reinterpret_cast<const float2*>(slot + row * D + lane * 2);
-          o[0] = u.x, o[1] = u.y;
-        }
-        const bool none = s.y == 0.f;  // it saw no token of this row
-        const float now = none ? ref : fmaxf(ref, s.x);
-        const float keep = ref == -INFINITY ? 0.f : exp2_fast(ref - now), add = none ? 0.f : exp2_fast(s.x - now);
-        den = fmaf(s.y, add, den * keep);
+      for (int base = 0; base <= w1 - w0; base += 32) {
+        // the factors of 32 CTAs, one per lane, then their sums with no load waiting for another
+        const int n = min(32, w1 - w0 + 1 - base);
+        const float2 s = lane < n ? *reinterpret_cast<const float2*>(slot(base + lane) + slot_rows * D + row * 4)
+                                  : make_float2(0.f, 0.f);
+        const float mine = s.y == 0.f ? -INFINITY : s.x;  // one that saw no token of this row
+        float now = fmaxf(ref, mine);
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) sum[e] = fmaf(o[e], add, sum[e] * keep);
+        for (int d = 16; d > 0; d >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
+        const float f = mine == -INFINITY ? 0.f : exp2_fast(mine - now);
+        float add = s.y * f;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
+        const float keep = ref == -INFINITY ? 0.f : exp2_fast(ref - now);
+        den = fmaf(den, keep, add);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) sum[e] *= keep;
         ref = now;
+#pragma unroll 8
+        for (int w = 0; w < n; ++w) {
+          const float* o = slot(base + w) + row * D + lane * kPer;
+          const float fw = __shfl_sync(0xffffffffu, f, w);
+          if constexpr (kPer == 4) {
+            const float4 u = *reinterpret_cast<const float4*>(o);
+            sum[0] = fmaf(u.x, fw, sum[0]), sum[1] = fmaf(u.y, fw, sum[1]);
+            sum[2] = fmaf(u.z, fw, sum[2]), sum[3] = fmaf(u.w, fw, sum[3]);
+          } else {
+            const float2 u = *reinterpret_cast<const float2*>(o);
+            sum[0] = fmaf(u.x, fw, sum[0]), sum[1] = fmaf(u.y, fw, sum[1]);
+          }
+        }
       }
       const float inv = den != 0.f ? 1.f / den : 0.f;
 #pragma unroll
