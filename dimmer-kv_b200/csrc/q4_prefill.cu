@@ -835,7 +835,10 @@ int launch_prefill(const dkv_q4_attend_args& a, cudaStream_t stream) {
 
 }  // namespace
 
-bool prefill_takes(const dkv_q4_attend_args& a) { return rows_of(a) > 32; }
+// Up to 64 rows q4_decode_kernel, which takes 16 at a time, is the faster one: over 4 contexts of 3K to 9K tokens, 24 / 8
+// heads of 128, bf16, 48 rows take 54 us there and 60 here, 72 rows 69 and 60 (64 rows of heads of 64: 48 and 51, 96: 61
+// and 52).
+bool prefill_takes(const dkv_q4_attend_args& a) { return rows_of(a) > 64; }
 
 int64_t prefill_floats(const dkv_q4_attend_args& a) {
   return 2 * static_cast<int64_t>(device_sms()) * slot_floats(slot_rows_of(a), a.head_dim);

@@ -48,7 +48,7 @@ def attend64(query, key, value, held, scaling):
 def attend_tolerance(out, parts, dtype, out_dtype, rows=1):
     """Largest error of dkv_q4_attend against attend64, for a cache of ``dtype`` and ``rows`` query rows per KV head.
 
-    Up to 32 rows: p * scale is rounded to float16 (half a step: 2^-11) in front of its code, or, for float16 caches, to
+    Up to 64 rows: p * scale is rounded to float16 (half a step: 2^-11) in front of its code, or, for float16 caches, to
     two float16 numbers (2^-21 between them): that much of the sum of p * scale * code. Below 2^-14 the half step is
     2^-25 instead, of p * 2^7 * scale / 2^k with 2^k at most 4 times the largest scale, times a code of at most 15:
     2^-26 of the largest scale for every token.
@@ -63,7 +63,7 @@ def attend_tolerance(out, parts, dtype, out_dtype, rows=1):
     more rows, over values of either sign, to 2^-14). The output is rounded once, to half a step of its type."""
     coded, low, terms, tokens, scale = parts
     step = 2**-11 if dtype == torch.bfloat16 else 2**-21
-    if rows <= 32:
+    if rows <= 64:
         own = coded * step + (coded + low) * 2**-16 + tokens * 2**-26 * scale
     else:
         own = (coded + low) * (2**-11 + step + 2 * step * terms[..., None] + 2**-14) + tokens * 2**-32 * 32 * scale

@@ -245,6 +245,9 @@ CASES = [
     (32, 8, 64, [20000], [1], 1),
     (24, 8, 128, [0], [11], 11),
     (4, 4, 64, [127, 1], [33, 32], 33),
+    (8, 8, 128, [100, 64], [64, 1], 64),
+    (8, 8, 128, [100, 64], [65, 1], 65),
+    (4, 4, 64, [500], [129], 129),
     (32, 8, 64, [0, 3000, 64], [300, 0, 257], 300),
     (24, 8, 128, [9000, 65], [86, 171], 171),
 ]
