@@ -79,55 +79,80 @@ __device__ __forceinline__ int64_t count_pages(const dkv_q4_attend_args& a, int 
   return total;
 }
 
+// How a warp holds its query rows: NT tiles of 8 columns, two columns per lane; or, NT = 0, up to 4 rows, each on the
+// even column of a pair, so that a lane has one row to do the softmax of and the odd column takes what the rounding of
+// the row's probabilities lacks.
 template <int D, int NT>
 struct Decode {
   using C = Cells<D>;
-  static constexpr int kRows = 8 * NT;
+  static constexpr bool kPair = NT == 0;
+  static constexpr int kTilesN = kPair ? 1 : NT;
+  static constexpr int kCols = kPair ? 1 : 2;    // of a lane, per tile
+  static constexpr int kRows = kPair ? 4 : 8 * NT;
   static constexpr int kStages = D == 128 ? 2 : 4;
-  static constexpr int kTiles = NT == 1 ? 2 : 1;  // of 16 tokens at a time, for the latencies to overlap
+  static constexpr int kTiles = NT <= 1 ? 2 : 1;  // of 16 tokens at a time, for the latencies to overlap
   static constexpr int kBlocksPerSm = D == 128 && NT == 2 ? 2 : 3;  // two accumulators of 128 need the registers
   static constexpr int kWarpBytes = kStages * C::kBytes;
   static constexpr int kBars = kWarps * kWarpBytes;
   static constexpr int kBytes = kBars + kWarps * kStages * 8;
+  // The row of column c of tile nt that lane t = 0..3 has.
+  static __device__ __forceinline__ int row(int nt, int t, int c) { return kPair ? t : nt * 8 + 2 * t + c; }
 };
 
 // A unit's query rows as the second operand, and the factors of their scores.
 template <int D, int NT>
 struct Query {
+  using S = Decode<D, NT>;
   static constexpr int kGroups = Cells<D>::kGroups;
-  uint32_t frag[D / 16][NT][2];
-  float factor[NT][2], sum[NT][2][kGroups];
-  int limit[NT][2];  // tokens below it are seen (0: no row)
+  uint32_t frag[D / 16][S::kTilesN][2];
+  float factor[S::kTilesN][S::kCols], sum[S::kTilesN][S::kCols][kGroups];
+  int limit[S::kTilesN][S::kCols];  // tokens below it are seen (0: no row)
+};
+// The rows as they lie in memory: a lane has 16 dimensions of each group of the row of column g.
+template <int D, int NT>
+struct RawQuery {
+  uint4 v[Decode<D, NT>::kTilesN][Cells<D>::kGroups][2];
 };
 
-template <int D, int NT, bool F16>
-__device__ __forceinline__ void load_query(const dkv_q4_attend_args& a, int seq, int head, int row0, int share, int start,
-                                           int fresh, Query<D, NT>& q) {
-  constexpr int kGroups = Cells<D>::kGroups;
+template <int D, int NT>
+__device__ __forceinline__ void fetch_query(const dkv_q4_attend_args& a, int seq, int head, int row0, int share, int fresh,
+                                            RawQuery<D, NT>& raw) {
+  using S = Decode<D, NT>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = row0 + nt * 8 + g;
-    const int i = r / share;
-    const bool real = r < a.q_len * share && i < fresh;
+  for (int nt = 0; nt < S::kTilesN; ++nt) {
+    const int r = row0 + (S::kPair ? g >> 1 : nt * 8 + g), i = r / share;
+    const bool real = r < a.q_len * share && i < fresh && !(S::kPair && (g & 1));
+    const uint16_t* src = static_cast<const uint16_t*>(a.query) + seq * a.q_stride[0] +
+                          (head * share + r - i * share) * a.q_stride[1] + i * a.q_stride[2] + t * 16;
+#pragma unroll
+    for (int gr = 0; gr < Cells<D>::kGroups; ++gr)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        raw.v[nt][gr][h] = real ? *reinterpret_cast<const uint4*>(src + gr * 64 + h * 8) : make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+template <int D, int NT, bool F16>
+__device__ __forceinline__ void make_query(const dkv_q4_attend_args& a, int row0, int share, int start, int fresh,
+                                           const RawQuery<D, NT>& raw, Query<D, NT>& q) {
+  using S = Decode<D, NT>;
+  constexpr int kGroups = Cells<D>::kGroups;
+  const int lane = threadIdx.x & 31, t = lane & 3;
+#pragma unroll
+  for (int nt = 0; nt < S::kTilesN; ++nt) {
     float x[kGroups][16];
     float big = 0.f, sum[kGroups];
 #pragma unroll
     for (int gr = 0; gr < kGroups; ++gr) {
-      uint4 raw[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-      if (real) {
-        const uint16_t* src = static_cast<const uint16_t*>(a.query) + seq * a.q_stride[0] +
-                              (head * share + r - i * share) * a.q_stride[1] + i * a.q_stride[2] + gr * 64 + t * 16;
-        raw[0] = *reinterpret_cast<const uint4*>(src);
-        raw[1] = *reinterpret_cast<const uint4*>(src + 8);
-      }
       sum[gr] = 0.f;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t w[4] = {raw[h].x, raw[h].y, raw[h].z, raw[h].w};
+        const uint4 u = raw.v[nt][gr][h];
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float v = q4::from16<F16>(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1))));
+          const float v = from16<F16>(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1))));
           x[gr][h * 8 + e] = v;
           big = fmaxf(big, fabsf(v));
           sum[gr] += v;
@@ -155,13 +180,13 @@ __device__ __forceinline__ void load_query(const dkv_q4_attend_args& a, int seq,
     const float scale = a.scaling * kLog2e;
     const float fac = scale * (16777216.f / up);
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int from = (2 * t + c) * 4;
+    for (int c = 0; c < S::kCols; ++c) {
+      const int from = (2 * t + c) * 4;  // a lane of the column's row
       q.factor[nt][c] = __shfl_sync(0xffffffffu, fac, from);
 #pragma unroll
       for (int gr = 0; gr < kGroups; ++gr) q.sum[nt][c][gr] = __shfl_sync(0xffffffffu, sum[gr] * scale, from);
-      const int rc = row0 + nt * 8 + 2 * t + c, ic = rc / share;
-      q.limit[nt][c] = (rc < a.q_len * share && ic < fresh) ? start + ic + 1 : 0;
+      const int r = row0 + S::row(nt, t, c), i = r / share;
+      q.limit[nt][c] = (r < a.q_len * share && i < fresh) ? start + i + 1 : 0;
     }
   }
 }
@@ -170,17 +195,49 @@ __device__ __forceinline__ void load_query(const dkv_q4_attend_args& a, int seq,
 // over the codes in units of 2^k * 2^-24 (even dimensions) or 2^-20 (odd ones).
 template <int D, int NT>
 struct State {
-  float o[D / 16][NT][4];
-  float l[NT][2], neg[NT][2], low[NT][2][Cells<D>::kGroups];
-  float unit;      // 2^-k: scales so far times it are at most 1
-  uint32_t known;  // bit 2 nt + c: the column has a reference
+  using S = Decode<D, NT>;
+  float o[D / 16][S::kTilesN][2 * S::kCols];  // [column] of dimension row g, then of g + 8
+  float l[S::kTilesN][S::kCols], neg[S::kTilesN][S::kCols], low[S::kTilesN][S::kCols][Cells<D>::kGroups];
+  float unit;      // 2^-k
+  uint32_t cap;    // 2^k as float16 bits: no scale so far is above it
+  uint32_t known;  // bit kCols nt + c: the column has a reference
   bool open;       // some column has none yet (warp-uniform)
 };
 
-// 2^-k for the largest scale: scale * 2^-k in [1/4, 1/2).
-__device__ __forceinline__ float unit_for(float scale) {
-  const int ex = (__float_as_uint(scale) >> 23) & 255;
-  return scale > 0.f ? __uint_as_float(static_cast<uint32_t>(252 - ex) << 23) : 0x1p24f;
+// Before a page's tokens: the unit for their value scales (tokens from `seen` on are not looked at).
+template <int D, int NT>
+__device__ __forceinline__ void fit_unit(const uint8_t* page, int base, int seen, State<D, NT>& st) {
+  using C = Cells<D>;
+  using S = Decode<D, NT>;
+  const int lane = threadIdx.x & 31;
+  uint32_t most = 0;  // scales are not negative: ordered as their bits
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = lane + 32 * h;
+    const uint8_t* hp = page + C::value_head(r, 0);
+    uint32_t top;
+    if constexpr (C::kGroups == 2) {
+      const uint2 u = *reinterpret_cast<const uint2*>(hp);
+      top = max(u.x & 0xffffu, u.y & 0xffffu);
+    } else {
+      top = *reinterpret_cast<const uint32_t*>(hp) & 0xffffu;
+    }
+    if (base + r < seen) most = max(most, top);
+  }
+  if (!__any_sync(0xffffffffu, most > st.cap)) return;
+  most = __reduce_max_sync(0xffffffffu, most);
+  // a power of two at least twice the largest scale, so that it seldom has to move
+  const int ex = (__float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(most)))) >> 23) & 255;
+  const float unit = __uint_as_float(static_cast<uint32_t>(252 - ex) << 23);
+  st.cap = __half_as_ushort(__float2half_rn(1.f / unit));
+  const float shrink = unit / st.unit;
+  st.unit = unit;
+#pragma unroll
+  for (int mt = 0; mt < D / 16; ++mt)
+#pragma unroll
+    for (int nt = 0; nt < S::kTilesN; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2 * S::kCols; ++e) st.o[mt][nt][e] *= shrink;
 }
 
 // 16 * TT tokens of a page in shared memory (rows 16 * tile ..), the first of them token `base` of the conversation.
@@ -189,16 +246,17 @@ template <int D, int NT, int TT, bool F16, bool EDGE>
 __device__ __forceinline__ void attend(const uint8_t* page, int tile, int base, int seen, const Query<D, NT>& q,
                                        State<D, NT>& st) {
   using C = Cells<D>;
-  constexpr int kGroups = C::kGroups;
+  using S = Decode<D, NT>;
+  constexpr int kGroups = C::kGroups, kN = S::kTilesN, kCols = S::kCols;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  float p[TT][NT][4];
+  float p[TT][kN][2][kCols];  // [tokens g, g + 8][column]
   __half2 vhead[TT][2][kGroups];
   bool rise = EDGE || st.open;
 #pragma unroll
   for (int tt = 0; tt < TT; ++tt) {
     // ---- scores of tokens g and g + 8
     const int row = (tile + tt) * 16 + g;
-    float acc[kGroups][NT][4];
+    float acc[kGroups][kN][4];
     const uint8_t* kr = page + C::kKeyCodes + row * (D / 2) + t * (D / 8);
     uint32_t x[2 * kGroups], y[2 * kGroups];
     if constexpr (D == 128) {
@@ -219,7 +277,7 @@ __device__ __forceinline__ void attend(const uint8_t* page, int tile, int base, 
         for (int odd = 0; odd < 2; ++odd) {
           const uint32_t mask = odd ? 0x00f000f0u : 0x000f000fu;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
+          for (int nt = 0; nt < kN; ++nt) {
             const uint32_t* b = q.frag[gr * 4 + w * 2 + odd][nt];
             if (w == 0 && odd == 0) mma16816_first(acc[gr][nt], u & mask, v & mask, u8 & mask, v8 & mask, b[0], b[1]);
             else mma16816(acc[gr][nt], u & mask, v & mask, u8 & mask, v8 & mask, b[0], b[1]);
@@ -247,12 +305,11 @@ __device__ __forceinline__ void attend(const uint8_t* page, int tile, int base, 
         kl[gr] = f.y;
         // tokens that no row sees may never have been written: no NaN of theirs into the sums
         vhead[tt][h][gr] = as_half2(gone ? 0u : hd[kGroups + gr]);
-        rise = rise || __low2float(vhead[tt][h][gr]) * st.unit > 1.f;
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < kN; ++nt)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < kCols; ++c) {
           float dot = ks[0] * acc[0][nt][2 * h + c];
           float s = fmaf(kl[0], q.sum[nt][c][0], st.neg[nt][c]);
           if constexpr (kGroups == 2) {
@@ -263,42 +320,28 @@ __device__ __forceinline__ void attend(const uint8_t* page, int tile, int base, 
           if constexpr (EDGE) {
             if (base + tt * 16 + g + 8 * h >= q.limit[nt][c]) s = -INFINITY;
           }
-          p[tt][nt][2 * h + c] = s;
+          p[tt][nt][h][c] = s;
           rise = rise || s > kBias + kSlack;
         }
     }
   }
   if (__any_sync(0xffffffffu, rise)) {
-    // ---- a score above the reference's slack, a scale above the unit, or a column without a reference: references
-    // move up to the columns' maxima, and what is summed so far scales down
-    float big = 0.f;
-#pragma unroll
-    for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int gr = 0; gr < kGroups; ++gr) big = fmaxf(big, __low2float(vhead[tt][h][gr]));
-    big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));  // not negative: ordered as its bits
-    float shrink = 1.f;
-    if (big * st.unit > 1.f) {
-      const float unit = unit_for(big);
-      shrink = unit / st.unit;
-      st.unit = unit;
-    }
+    // ---- a score above the reference's slack, or a column without a reference: references move up to the columns'
+    // maxima, and what is summed so far scales down
     bool open = false;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float f[2];
+    for (int nt = 0; nt < kN; ++nt) {
+      float f[kCols];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < kCols; ++c) {
         float top = -INFINITY;
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt) top = fmaxf(top, fmaxf(p[tt][nt][c], p[tt][nt][c + 2]));
+        for (int tt = 0; tt < TT; ++tt) top = fmaxf(top, fmaxf(p[tt][nt][0][c], p[tt][nt][1][c]));
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         // a column's first tokens set the reference wherever they are; later ones raise it, and only from beyond the
         // slack, so that a row's result does not depend on the rows beside it
-        const uint32_t bit = 1u << (2 * nt + c);
+        const uint32_t bit = 1u << (kCols * nt + c);
         const bool first = (st.known & bit) == 0, none = first && top == -INFINITY;
         const float move = none ? 0.f : first || top > kBias + kSlack ? top - kBias : 0.f;
         st.known |= none ? 0u : bit;
@@ -309,20 +352,22 @@ __device__ __forceinline__ void attend(const uint8_t* page, int tile, int base, 
         for (int gr = 0; gr < kGroups; ++gr) st.low[nt][c][gr] *= f[c];
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) {
-          p[tt][nt][c] -= move;
-          p[tt][nt][c + 2] -= move;
+          p[tt][nt][0][c] -= move;
+          p[tt][nt][1][c] -= move;
         }
-        f[c] *= shrink;
         open = open || none;
       }
 #pragma unroll
       for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) st.o[mt][nt][e] *= f[e & 1];
+        for (int e = 0; e < 2 * kCols; ++e) st.o[mt][nt][e] *= f[e % kCols];
     }
     st.open = __any_sync(0xffffffffu, open);
   }
-  uint32_t pf[TT][kGroups][NT][2], pr[F16 ? TT : 1][kGroups][NT][2], v[TT][2][D / 32];
+  // Second operands: with a column per row what a float16 rounding lacks takes products of its own, with a pair of
+  // columns it is the second column's.
+  constexpr bool kMore = F16 && !S::kPair;
+  uint32_t pf[TT][kGroups][kN][2], pr[kMore ? TT : 1][kGroups][kN][2], v[TT][2][D / 32];
 #pragma unroll
   for (int tt = 0; tt < TT; ++tt) {
 #pragma unroll
@@ -335,20 +380,30 @@ __device__ __forceinline__ void attend(const uint8_t* page, int tile, int base, 
         vl[gr] = f.y;
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float e0 = exp2_fast(p[tt][nt][2 * h]), e1 = exp2_fast(p[tt][nt][2 * h + 1]);
-        st.l[nt][0] += e0;
-        st.l[nt][1] += e1;
+      for (int nt = 0; nt < kN; ++nt) {
+        float e[kCols];
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          e[c] = exp2_fast(p[tt][nt][h][c]);
+          st.l[nt][c] += e[c];
+#pragma unroll
+          for (int gr = 0; gr < kGroups; ++gr) st.low[nt][c][gr] = fmaf(e[c], vl[gr], st.low[nt][c][gr]);
+        }
 #pragma unroll
         for (int gr = 0; gr < kGroups; ++gr) {
-          st.low[nt][0][gr] = fmaf(e0, vl[gr], st.low[nt][0][gr]);
-          st.low[nt][1][gr] = fmaf(e1, vl[gr], st.low[nt][1][gr]);
-          const float w0 = e0 * vs[gr], w1 = e1 * vs[gr];
-          const uint32_t hi = pack_half2(w0, w1);
-          pf[tt][gr][nt][h] = transpose8(hi);
-          if constexpr (F16) {
-            const float2 back = __half22float2(as_half2(hi));
-            pr[tt][gr][nt][h] = transpose8(pack_half2(w0 - back.x, w1 - back.y));
+          const float w0 = e[0] * vs[gr];
+          if constexpr (S::kPair) {
+            uint32_t hi = pack_half2(w0, 0.f);
+            if constexpr (F16) hi = pack_half2(w0, w0 - __low2float(as_half2(hi)));
+            pf[tt][gr][nt][h] = transpose8(hi);
+          } else {
+            const float w1 = e[kCols - 1] * vs[gr];
+            const uint32_t hi = pack_half2(w0, w1);
+            pf[tt][gr][nt][h] = transpose8(hi);
+            if constexpr (kMore) {
+              const float2 back = __half22float2(as_half2(hi));
+              pr[tt][gr][nt][h] = transpose8(pack_half2(w0 - back.x, w1 - back.y));
+            }
           }
         }
       }
@@ -374,7 +429,7 @@ __device__ __forceinline__ void attend(const uint8_t* page, int tile, int base, 
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < kN; ++nt) {
         float sum[4];
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) {
@@ -383,11 +438,16 @@ __device__ __forceinline__ void attend(const uint8_t* page, int tile, int base, 
           const uint32_t* hi = pf[tt][i >> 1][nt];
           if (tt == 0) mma16816_first(sum, u0, u1, w0, w1, hi[0], hi[1]);
           else mma16816(sum, u0, u1, w0, w1, hi[0], hi[1]);
-          if constexpr (F16) mma16816(sum, u0, u1, w0, w1, pr[tt][i >> 1][nt][0], pr[tt][i >> 1][nt][1]);
+          if constexpr (kMore) mma16816(sum, u0, u1, w0, w1, pr[tt][i >> 1][nt][0], pr[tt][i >> 1][nt][1]);
         }
         float* o = st.o[i * 2 + b][nt];
-        add2(o[0], o[1], sum[0], sum[1]);
-        add2(o[2], o[3], sum[2], sum[3]);
+        if constexpr (S::kPair) {
+          if constexpr (F16) add2(sum[0], sum[2], sum[1], sum[3]);
+          add2(o[0], o[1], sum[0], sum[2]);
+        } else {
+          add2(o[0], o[1], sum[0], sum[1]);
+          add2(o[2], o[3], sum[2], sum[3]);
+        }
       }
 }
 
@@ -491,17 +551,20 @@ q4_decode_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int w
     const int64_t page_stride = static_cast<int64_t>(a.n_kv_heads) * C::kBytes;
     uint8_t* cells = a.cells + static_cast<int64_t>(head) * C::kBytes;
 
-    int ids = 0, ids_at = p0 - 32;
+    // The pages' places, one per lane, 32 at a time, the next 32 on their way.
+    int ids_at = p0, ids = p0 + lane < p1 ? table[p0 + lane] : 0, ids_next = p0 + 32 + lane < p1 ? table[p0 + 32 + lane] : 0;
+    RawQuery<D, NT> raw;
+    fetch_query<D, NT>(a, seq, head, row0, share, fresh, raw);  // ahead of the pages, which would keep it waiting
     auto page_id = [&](int p) {
       if (p >= ids_at + 32) {
-        ids_at = p;
-        ids = p + lane < p1 ? table[p + lane] : 0;
-        if (static_cast<unsigned>(ids) >= static_cast<unsigned>(a.n_pages)) {
-          record_error(a.status, kSiteQ4Attend + kErrBadDescriptor);
-          ids = -1;
-        }
+        ids_at += 32;
+        ids = ids_next;
+        ids_next = ids_at + 32 + lane < p1 ? table[ids_at + 32 + lane] : 0;
       }
-      return __shfl_sync(0xffffffffu, ids, p - ids_at);
+      const int id = __shfl_sync(0xffffffffu, ids, p - ids_at);
+      if (static_cast<unsigned>(id) < static_cast<unsigned>(a.n_pages)) return id;
+      record_error(a.status, kSiteQ4Attend + kErrBadDescriptor);
+      return -1;
     };
     const uint32_t copies0 = copies;  // page p is copy copies0 + p - p0
     auto fetch = [&](int p) {
@@ -518,20 +581,24 @@ q4_decode_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int w
     for (int p = p0; p < min(pe, p0 + S::kStages); ++p) fetch(p);
 
     Query<D, NT> q;
-    load_query<D, NT, F16>(a, seq, head, row0, share, start, fresh, q);
+    make_query<D, NT, F16>(a, row0, share, start, fresh, raw, q);
     State<D, NT> st;
     st.open = true;
     st.known = 0;
-    st.unit = 0x1p24f;
+    st.unit = 1.f;
+    st.cap = 0;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      st.l[nt][0] = st.l[nt][1] = st.neg[nt][0] = st.neg[nt][1] = 0.f;
+    for (int nt = 0; nt < S::kTilesN; ++nt) {
 #pragma unroll
-      for (int gr = 0; gr < C::kGroups; ++gr) st.low[nt][0][gr] = st.low[nt][1][gr] = 0.f;
+      for (int c = 0; c < S::kCols; ++c) {
+        st.l[nt][c] = st.neg[nt][c] = 0.f;
+#pragma unroll
+        for (int gr = 0; gr < C::kGroups; ++gr) st.low[nt][c][gr] = 0.f;
+      }
 #pragma unroll
       for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) st.o[mt][nt][e] = 0.f;
+        for (int e = 0; e < 2 * S::kCols; ++e) st.o[mt][nt][e] = 0.f;
     }
 
     bool ok = true;
@@ -547,6 +614,7 @@ q4_decode_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int w
           store_new<D, F16>(a, seq, head, start, max(start, base), min(start + fresh, base + q4::kPage), page,
                             cells + id * page_stride);
       }
+      fit_unit<D, NT>(page, base, seen, st);
       if (base + q4::kPage <= full_below) {
         for (int tile = 0; tile < q4::kPage / 16; tile += S::kTiles)
           attend<D, NT, S::kTiles, F16, false>(page, tile, base + tile * 16, seen, q, st);
@@ -569,9 +637,9 @@ q4_decode_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int w
     float* slot = a.workspace + (worker * 2 + (at == begin ? 0 : 1)) * slot_floats(rows, D);
     const float even = 0x1p24f / st.unit, odd = 0x1p20f / st.unit;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < S::kTilesN; ++nt)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < S::kCols; ++c) {
         float sum = st.l[nt][c], low[C::kGroups];
 #pragma unroll
         for (int gr = 0; gr < C::kGroups; ++gr) low[gr] = st.low[nt][c][gr];
@@ -581,16 +649,16 @@ q4_decode_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int w
 #pragma unroll
           for (int gr = 0; gr < C::kGroups; ++gr) low[gr] += __shfl_xor_sync(0xffffffffu, low[gr], d);
         }
-        const int col = nt * 8 + 2 * t + c, r = row0 + col, i = r / share;
+        const int col = S::row(nt, t, c), r = row0 + col, i = r / share;
         if (r >= a.q_len * share || i >= fresh) continue;  // q4_combine_kernel writes the zeros behind the new tokens
         const float inv = sum != 0.f ? 1.f / sum : 0.f;
         const int64_t to =
             ((static_cast<int64_t>(seq) * a.q_len + i) * a.n_q_heads + head * share + r - i * share) * D + g * 8;
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) {
-          const float y0 = fmaf(st.o[2 * k][nt][c], even, low[k >> 1]), y1 = fmaf(st.o[2 * k][nt][c + 2], odd, low[k >> 1]);
+          const float y0 = fmaf(st.o[2 * k][nt][c], even, low[k >> 1]), y1 = fmaf(st.o[2 * k][nt][c + S::kCols], odd, low[k >> 1]);
           const float y2 = fmaf(st.o[2 * k + 1][nt][c], even, low[k >> 1]),
-                      y3 = fmaf(st.o[2 * k + 1][nt][c + 2], odd, low[k >> 1]);
+                      y3 = fmaf(st.o[2 * k + 1][nt][c + S::kCols], odd, low[k >> 1]);
           const int dim = (k >> 1) * 64 + (k & 1) * 4;
           if (whole) store_out4<F16>(a, to + dim, y0 * inv, y1 * inv, y2 * inv, y3 * inv);
           else *reinterpret_cast<float4*>(slot + col * D + g * 8 + dim) = make_float4(y0, y1, y2, y3);
@@ -619,9 +687,10 @@ q4_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int 
   __shared__ float factor[kFactors];
   __shared__ float warp_ref[kCombineThreads / 32], warp_den[kCombineThreads / 32];
   const int share = a.n_q_heads / a.n_kv_heads;
-  const int rows = min(8 * NT, a.q_len * share);
+  constexpr int kRows = Decode<D, NT>::kRows;
+  const int rows = min(kRows, a.q_len * share);
   const int r = blockIdx.x, head = blockIdx.y, seq = blockIdx.z;
-  const int chunk = r / (8 * NT), col = r - chunk * 8 * NT, i = r / share;
+  const int chunk = r / kRows, col = r - chunk * kRows, i = r / share;
   const int tid = threadIdx.x, x = tid % kLanes, slice = tid / kLanes;
   const int tokens = tokens_of(a, seq), n_pages = pages_of(tokens);
   const int fresh = tokens == 0 ? 0 : min(tokens - a.starts[seq], a.q_len);
@@ -711,16 +780,18 @@ q4_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int 
   store_out4<F16>(a, to, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
 }
 
-int tiles_of(const dkv_q4_attend_args& a) { return rows_of(a) <= 8 ? 1 : 2; }  // of 8 query rows that a warp holds
+// NT of q4_decode_kernel, and the query rows that a warp then holds.
+int tiles_of(const dkv_q4_attend_args& a) { return rows_of(a) <= 4 ? 0 : rows_of(a) <= 8 ? 1 : 2; }
+int held_rows(int nt) { return nt == 0 ? 4 : 8 * nt; }
 
 int64_t floats_of(const dkv_q4_attend_args& a) {
-  const int rows = rows_of(a), held = rows < 8 * tiles_of(a) ? rows : 8 * tiles_of(a);
+  const int rows = rows_of(a), most = held_rows(tiles_of(a)), held = rows < most ? rows : most;
   return 2 * static_cast<int64_t>(device_sms() * 3 * kWarps) * slot_floats(held, a.head_dim);
 }
 
 template <int D, int NT, bool F16>
 int launch_decode(const dkv_q4_attend_args& a, int append, cudaStream_t stream) {
-  const int rows = rows_of(a), chunks = (rows + 8 * NT - 1) / (8 * NT);
+  const int rows = rows_of(a), held = held_rows(NT), chunks = (rows + held - 1) / held;
   if (static_cast<int64_t>(a.n_kv_heads) > 65535) return DKV_ERR_CONFIG;
   // At most one worker per page that there can be.
   const int64_t pages = static_cast<int64_t>((a.len_bound + q4::kPage - 1) / q4::kPage) * a.n_seq * a.n_kv_heads * chunks;
@@ -786,7 +857,7 @@ int dkv_q4_attend(const dkv_q4_attend_args* a, void* stream) {
   const bool prefill = dkv::q4::prefill_takes(*a);
   const int nt = dkv::tiles_of(*a);
   int append = a->key != nullptr;
-  if (append && (prefill || dkv::q4::rows_of(*a) > 8 * nt)) {
+  if (append && (prefill || dkv::q4::rows_of(*a) > dkv::held_rows(nt))) {
     // Several row chunks read a new token's page: it has to be there before the first of them.
     dkv_q4_rows_args r = {};
     r.cells = a->cells;
@@ -804,8 +875,8 @@ int dkv_q4_attend(const dkv_q4_attend_args* a, void* stream) {
   if (prefill) return dkv::q4::run_prefill(*a, st);
 #define DKV_Q4_DECODE(D, NT) \
   (a->fp16 ? dkv::launch_decode<D, NT, true>(*a, append, st) : dkv::launch_decode<D, NT, false>(*a, append, st))
-  if (a->head_dim == 128) return nt == 1 ? DKV_Q4_DECODE(128, 1) : DKV_Q4_DECODE(128, 2);
-  return nt == 1 ? DKV_Q4_DECODE(64, 1) : DKV_Q4_DECODE(64, 2);
+  if (a->head_dim == 128) return nt == 0 ? DKV_Q4_DECODE(128, 0) : nt == 1 ? DKV_Q4_DECODE(128, 1) : DKV_Q4_DECODE(128, 2);
+  return nt == 0 ? DKV_Q4_DECODE(64, 0) : nt == 1 ? DKV_Q4_DECODE(64, 1) : DKV_Q4_DECODE(64, 2);
 #undef DKV_Q4_DECODE
 }
 
