@@ -501,9 +501,13 @@ q4_decode_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int w
   }
   const int failed = status_at_entry(a.status);
   const int worker = warp * gridDim.x + blockIdx.x;  // neighbours in the line on different SMs
-  int64_t unused;
   const int units = a.n_kv_heads * chunks;  // of a conversation
-  const Deal deal(count_pages(a, 0, unused) * units, workers);
+  // Pages of the 32 conversations from `base` on, one per lane; the first 32 are kept for the search below.
+  auto lane_pages = [&](int base) { return base + lane < a.n_seq ? pages_of(tokens_of(a, base + lane)) : 0; };
+  const int kept = lane_pages(0);
+  int64_t all = warp_sum(kept);
+  for (int base = 32; base < a.n_seq; base += 32) all += warp_sum(lane_pages(base));
+  const Deal deal(all * units, workers);
   if (__any_sync(0xffffffffu, failed != 0)) return;
   if (worker >= deal.workers) return;
   const int64_t begin = deal.begin(worker), end = deal.begin(worker + 1);
@@ -511,24 +515,22 @@ q4_decode_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int w
   // the conversation of the first page
   int seq = 0;
   int64_t seq_at = 0;  // its first place in the line
-  for (int base = 0;; base += 32) {
-    const int s = base + lane;
-    int64_t incl = s < a.n_seq ? static_cast<int64_t>(pages_of(tokens_of(a, s))) * units : 0;
-    const int64_t own = incl;
+  for (int base = 0; base < a.n_seq; base += 32) {
+    const int own = base == 0 ? kept : lane_pages(base);
+    int incl = own;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, incl, d);
+      const int y = __shfl_up_sync(0xffffffffu, incl, d);
       if (lane >= d) incl += y;
     }
-    const unsigned past = __ballot_sync(0xffffffffu, seq_at + incl > begin);
+    const unsigned past = __ballot_sync(0xffffffffu, seq_at + static_cast<int64_t>(incl) * units > begin);
     if (past) {
       const int first = __ffs(past) - 1;
       seq = base + first;
-      seq_at += __shfl_sync(0xffffffffu, incl - own, first);
+      seq_at += static_cast<int64_t>(__shfl_sync(0xffffffffu, incl - own, first)) * units;
       break;
     }
-    seq_at += __shfl_sync(0xffffffffu, incl, 31);
-    if (base + 32 >= a.n_seq) return;  // not reached: begin lies on the line
+    seq_at += static_cast<int64_t>(__shfl_sync(0xffffffffu, incl, 31)) * units;
   }
 
   uint32_t copies = 0;  // issued by this warp so far: stage copies % kStages, phase copies / kStages
@@ -538,7 +540,8 @@ q4_decode_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int w
     int tokens = tokens_of(a, seq);
     while (tokens == 0) tokens = tokens_of(a, ++seq);
     const int n_pages = pages_of(tokens);
-    const int unit = static_cast<int>((at - seq_at) / n_pages);
+    const int64_t off = at - seq_at;
+    const int unit = static_cast<int>(off <= 0xffffffffll ? static_cast<uint32_t>(off) / static_cast<uint32_t>(n_pages) : off / n_pages);
     const int64_t unit_at = seq_at + static_cast<int64_t>(unit) * n_pages;
     const int p0 = static_cast<int>(at - unit_at);
     const int p1 = static_cast<int>(min(static_cast<int64_t>(n_pages), end - unit_at));
