@@ -17,16 +17,17 @@
 //
 // Quantising: eight lanes hold a group of 64 dimensions, eight each; minimum and maximum are three shuffles, a
 // lane's eight key codes are exactly one word of the key cell, its value codes the halves of two words of the pair's.
-// The code is the nearest whole number to the true quotient (x - low) / scale, ties to even, not to its float32
-// rounding: the float32 quotient, off by less than 2^-18, decides unless it lies within 2^-16 of a half; then the
-// border low + (c + 1/2) * scale, which float64 holds exactly (two float16 numbers, exponents -25 .. 15, and 5 bits),
-// is compared with x. So the codes do not depend on how a device rounds a division.
+// The code is the nearest whole number to the true quotient (x - low) / scale, ties to even, not to a float32
+// rounding of it: the float32 quotient, by the hardware's reciprocal off by less than 2^-18, decides unless it lies
+// within 2^-16 of a half; then the border low + (c + 1/2) * scale, which float64 holds exactly (two float16 numbers,
+// exponents -25 .. 15, and 5 bits), is compared with x. So the codes do not depend on how a device divides.
 #pragma once
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "../../include/dimmer_kv.h"
+#include "dkv_ptx.cuh"
 
 namespace dkv {
 namespace q4 {
@@ -71,14 +72,26 @@ __device__ __forceinline__ uint16_t to16(float v) {
   return F16 ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
 }
 
-// The same for a quotient next to a border: q in float32 as quantise8 has it.
-static __device__ __noinline__ uint32_t code_at_border(float x, float low, float scale, float q) {
-  const float below = floorf(q);
-  if (fabsf(q - below - 0.5f) >= 0x1p-15f) return static_cast<uint32_t>(rintf(q));
-  const double border = static_cast<double>(low) + (static_cast<double>(below) + 0.5) * static_cast<double>(scale);
-  const double xd = static_cast<double>(x);
-  const bool up = xd > border || (xd == border && (static_cast<int>(below) & 1));
-  return static_cast<uint32_t>(up ? below + 1.f : below);
+// Codes of a lane whose quotients go beyond 0 .. 15 or come close to a border between two codes: rare.
+template <bool F16>
+static __device__ __noinline__ uint32_t codes_with_care(uint4 raw, float low, float scale, float part) {
+  uint32_t codes = 0;
+#pragma unroll 1
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t pair = (e >> 1) == 0 ? raw.x : (e >> 1) == 1 ? raw.y : (e >> 1) == 2 ? raw.z : raw.w;
+    const float x = from16<F16>(static_cast<uint16_t>(pair >> (16 * (e & 1))));
+    const float q = fminf(fmaxf(__fmul_rn(__fsub_rn(x, low), part), 0.f), 15.f);
+    const float below = floorf(q);
+    uint32_t code = static_cast<uint32_t>(rintf(q));
+    if (fabsf(q - below - 0.5f) < 0x1p-15f) {
+      const double border = static_cast<double>(low) + (static_cast<double>(below) + 0.5) * static_cast<double>(scale);
+      const double xd = static_cast<double>(x);
+      const bool up = xd > border || (xd == border && (static_cast<int>(below) & 1));
+      code = static_cast<uint32_t>(up ? below + 1.f : below);
+    }
+    codes |= code << (4 * e);
+  }
+  return codes;
 }
 
 struct Cell8 {
@@ -120,29 +133,28 @@ __device__ __forceinline__ Cell8 quantise8(const uint4& raw) {
   const float low = __half2float(low_h);
   const __half scale_h = __float2half_rn(__fdiv_rn(__fsub_rn(hi, low), 15.f));
   const float scale = __half2float(scale_h);
-  const float part = scale > 0.f ? __fdiv_rn(0x1.111112p-4f, scale) : 0.f;  // 1 / (15 scale): quotients of 0..1, clamped
+  float part;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(part) : "f"(scale));
+  part = scale > 0.f ? part : 0.f;
   constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: what is added to it becomes a whole number
+  const uint64_t low2 = f32x2_pack(__float_as_uint(-low), __float_as_uint(-low));
+  const uint64_t part2 = f32x2_pack(__float_as_uint(part), __float_as_uint(part));
+  const uint64_t whole2 = f32x2_pack(__float_as_uint(kWhole), __float_as_uint(kWhole));
+  const uint64_t minus2 = f32x2_pack(0xbf800000u, 0xbf800000u);
   uint32_t codes = 0;
-  float q[8], off = 0.f;
+  float off = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float x = from16<F16>(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1))));
-    q[e] = __saturatef(__fmul_rn(__fsub_rn(x, low), part));
-    const float m = __fmaf_rn(q[e], 15.f, kWhole);
-    off = fmaxf(off, fabsf(__fmaf_rn(q[e], 15.f, kWhole - m)));
-    codes += __float_as_uint(m) << (4 * e);  // the code in the low bits, and what cancels below
+  for (int e = 0; e < 4; ++e) {
+    const float x0 = from16<F16>(static_cast<uint16_t>(w[e])), x1 = from16<F16>(static_cast<uint16_t>(w[e] >> 16));
+    const uint64_t d = add_f32x2(f32x2_pack(__float_as_uint(x0), __float_as_uint(x1)), low2);
+    const uint64_t m = fma_f32x2(d, part2, whole2);
+    const uint64_t r = fma_f32x2(d, part2, fma_f32x2(m, minus2, whole2));  // quotient - code
+    off = fmaxf(off, fmaxf(fabsf(__uint_as_float(static_cast<uint32_t>(r))), fabsf(__uint_as_float(static_cast<uint32_t>(r >> 32)))));
+    codes += (static_cast<uint32_t>(m) << (8 * e)) + (static_cast<uint32_t>(m >> 32) << (8 * e + 4));
   }
-  codes -= 0x4b400000u * 0x11111111u;
-  if (off > 0.5f - 0x1p-16f) {  // rare: some quotient next to a border
-    codes = 0;
-#pragma unroll 1
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t pair = (e >> 1) == 0 ? raw.x : (e >> 1) == 1 ? raw.y : (e >> 1) == 2 ? raw.z : raw.w;
-      const float x = from16<F16>(static_cast<uint16_t>(pair >> (16 * (e & 1))));
-      const float quotient = __saturatef(__fmul_rn(__fsub_rn(x, low), part)) * 15.f;
-      codes |= code_at_border(x, low, scale, quotient) << (4 * e);
-    }
-  }
+  codes -= 0x4b400000u * 0x11111111u;  // the constant's own bits under the codes
+  const bool inside = (lo - low) * part > -0.49f && (hi - low) * part < 15.49f;  // false where low's rounding is coarse
+  if (!inside || off > 0.5f - 0x1p-16f) codes = codes_with_care<F16>(raw, low, scale, part);
   c.codes = codes;
   c.scale = __half_as_ushort(scale_h);
   c.low = __half_as_ushort(low_h);

@@ -52,7 +52,8 @@ __global__ void __launch_bounds__(kRowThreads) q4_append_kernel(const __grid_con
     value = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.value) + p.seq * a.v_stride[0] +
                                             p.head * a.v_stride[1] + p.i * a.v_stride[2] + p.j * 8);
   }
-  if (__any_sync(0xffffffffu, status_at_entry(a.status) != 0)) return;  // one answer for the warp's shuffles
+  // one answer for the warp's shuffles: nothing to do for it, or nothing to be done
+  if (__all_sync(0xffffffffu, p.slot < 0) || __any_sync(0xffffffffu, status_at_entry(a.status) != 0)) return;
   const q4::Cell8 k = q4::quantise8<F16>(key), v = q4::quantise8<F16>(value);
   if (!k.fits || !v.fits) record_error(a.status, kSiteQ4Rows + kErrCellRange);
   // the other token of the pair, where the lanes beside hold it
