@@ -456,25 +456,28 @@ __device__ __forceinline__ void attend(const uint8_t* page, int tile, int base, 
 template <int D, bool F16>
 __device__ __noinline__ void store_new(const dkv_q4_attend_args& a, int seq, int head, int start, int first, int last,
                                        uint8_t* copy, uint8_t* cell) {
-  constexpr int kLanes = D / 8, kPer = 32 / (2 * kLanes);  // lanes of a row; tokens (key and value row) at a time
+  constexpr int kLanes = D / 16, kPer = 32 / (2 * kLanes);  // lanes of a row; tokens (key and value row) at a time
   const int lane = threadIdx.x & 31;
   const int j = lane % kLanes, is_value = (lane / kLanes) & 1, sub = lane / (2 * kLanes);
   const int64_t* sd = is_value ? a.v_stride : a.k_stride;
-  const uint16_t* src = static_cast<const uint16_t*>(is_value ? a.value : a.key) + seq * sd[0] + head * sd[1] + j * 8;
+  const uint16_t* src = static_cast<const uint16_t*>(is_value ? a.value : a.key) + seq * sd[0] + head * sd[1] + j * 16;
   for (int tok = first; tok < last; tok += kPer) {
     const int mine = tok + sub;
-    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-    if (mine < last) raw = *reinterpret_cast<const uint4*>(src + (mine - start) * sd[2]);
-    const q4::Cell8 c = q4::quantise8<F16>(raw);
+    uint4 raw[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+    if (mine < last) {
+      const uint4* from = reinterpret_cast<const uint4*>(src + (mine - start) * sd[2]);
+      raw[0] = from[0], raw[1] = from[1];
+    }
+    const q4::Cell16 c = q4::quantise16<F16>(raw);
     if (!c.fits) record_error(a.status, kSiteQ4Rows + kErrCellRange);
     if (mine < last) {
       const int r = mine % q4::kPage;
       if (is_value) {
-        q4::store_value8<D>(copy, r, j, c);
-        q4::store_value8<D>(cell, r, j, c);
+        q4::store_value16<D>(copy, r, j, c);
+        q4::store_value16<D>(cell, r, j, c);
       } else {
-        q4::store_key8<D>(copy, r, j, c);
-        q4::store_key8<D>(cell, r, j, c);
+        q4::store_key16<D>(copy, r, j, c);
+        q4::store_key16<D>(cell, r, j, c);
       }
     }
   }

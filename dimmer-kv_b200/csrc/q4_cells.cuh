@@ -15,8 +15,8 @@
 //     64: lanes t = 0..3 read four pairs at once, a multiple of 64 bytes apart, and would share banks otherwise.
 //   headers: float16 (scale, low) of a token's key groups, then of its value groups: one load per token.
 //
-// Quantising: eight lanes hold a group of 64 dimensions, eight each; minimum and maximum are three shuffles, a
-// lane's eight key codes are exactly one word of the key cell, its value codes the halves of two words of the pair's.
+// Quantising: four lanes hold a group of 64 dimensions, sixteen each (two 16-byte loads); minimum and maximum are two
+// shuffles, eight key codes are exactly one word of the key cell, eight value codes the halves of two words of the pair's.
 // The code is the nearest whole number to the true quotient (x - low) / scale, ties to even, not to a float32
 // rounding of it: the float32 quotient, by the hardware's reciprocal off by less than 2^-18, decides unless it lies
 // within 2^-16 of a half; then the border low + (c + 1/2) * scale, which float64 holds exactly (two float16 numbers,
@@ -94,10 +94,10 @@ static __device__ __noinline__ uint32_t codes_with_care(uint4 raw, float low, fl
   return codes;
 }
 
-struct Cell8 {
-  uint32_t codes;  // nibble e: element e of the lane's eight
+struct Cell16 {
+  uint32_t codes[2];  // of the lane's first and second eight elements, nibble e: element e
   uint16_t scale, low;
-  bool fits;       // the group is finite and within kCellMax
+  bool fits;          // the group is finite and within kCellMax
 };
 
 template <bool F16, bool MAX>
@@ -113,21 +113,25 @@ __device__ __forceinline__ uint32_t extreme2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// The lane's eight elements of a group that this lane and the 7 beside it hold (all of a warp's lanes call it).
+// The lane's sixteen elements of a group that this lane and the 3 beside it hold (all of a warp's lanes call it).
 template <bool F16>
-__device__ __forceinline__ Cell8 quantise8(const uint4& raw) {
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  uint32_t least = extreme2<F16, false>(extreme2<F16, false>(w[0], w[1]), extreme2<F16, false>(w[2], w[3]));
-  uint32_t most = extreme2<F16, true>(extreme2<F16, true>(w[0], w[1]), extreme2<F16, true>(w[2], w[3]));
+__device__ __forceinline__ Cell16 quantise16(const uint4 (&raw)[2]) {
+  const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+  uint32_t least = w[0], most = w[0];
 #pragma unroll
-  for (int d = 1; d < 8; d <<= 1) {
+  for (int e = 1; e < 8; ++e) {
+    least = extreme2<F16, false>(least, w[e]);
+    most = extreme2<F16, true>(most, w[e]);
+  }
+#pragma unroll
+  for (int d = 1; d < 4; d <<= 1) {
     least = extreme2<F16, false>(least, __shfl_xor_sync(0xffffffffu, least, d));
     most = extreme2<F16, true>(most, __shfl_xor_sync(0xffffffffu, most, d));
   }
   least = extreme2<F16, false>(least, least >> 16);
   most = extreme2<F16, true>(most, most >> 16);
   const float lo = from16<F16>(static_cast<uint16_t>(least)), hi = from16<F16>(static_cast<uint16_t>(most));
-  Cell8 c;
+  Cell16 c;
   c.fits = lo >= -kCellMax && hi <= kCellMax;  // false for a NaN
   const __half low_h = __float2half_rn(lo);
   const float low = __half2float(low_h);
@@ -141,45 +145,51 @@ __device__ __forceinline__ Cell8 quantise8(const uint4& raw) {
   const uint64_t part2 = f32x2_pack(__float_as_uint(part), __float_as_uint(part));
   const uint64_t whole2 = f32x2_pack(__float_as_uint(kWhole), __float_as_uint(kWhole));
   const uint64_t minus2 = f32x2_pack(0xbf800000u, 0xbf800000u);
-  uint32_t codes = 0;
-  float off = 0.f;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float x0 = from16<F16>(static_cast<uint16_t>(w[e])), x1 = from16<F16>(static_cast<uint16_t>(w[e] >> 16));
-    const uint64_t d = add_f32x2(f32x2_pack(__float_as_uint(x0), __float_as_uint(x1)), low2);
-    const uint64_t m = fma_f32x2(d, part2, whole2);
-    const uint64_t r = fma_f32x2(d, part2, fma_f32x2(m, minus2, whole2));  // quotient - code
-    off = fmaxf(off, fmaxf(fabsf(__uint_as_float(static_cast<uint32_t>(r))), fabsf(__uint_as_float(static_cast<uint32_t>(r >> 32)))));
-    codes += (static_cast<uint32_t>(m) << (8 * e)) + (static_cast<uint32_t>(m >> 32) << (8 * e + 4));
-  }
-  codes -= 0x4b400000u * 0x11111111u;  // the constant's own bits under the codes
   const bool inside = (lo - low) * part > -0.49f && (hi - low) * part < 15.49f;  // false where low's rounding is coarse
-  if (!inside || off > 0.5f - 0x1p-16f) codes = codes_with_care<F16>(raw, low, scale, part);
-  c.codes = codes;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t codes = 0;
+    float off = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t u = w[4 * h + e];
+      const float x0 = from16<F16>(static_cast<uint16_t>(u)), x1 = from16<F16>(static_cast<uint16_t>(u >> 16));
+      const uint64_t d = add_f32x2(f32x2_pack(__float_as_uint(x0), __float_as_uint(x1)), low2);
+      const uint64_t m = fma_f32x2(d, part2, whole2);
+      const uint64_t r = fma_f32x2(d, part2, fma_f32x2(m, minus2, whole2));  // quotient - code
+      off = fmaxf(off, fmaxf(fabsf(__uint_as_float(static_cast<uint32_t>(r))), fabsf(__uint_as_float(static_cast<uint32_t>(r >> 32)))));
+      codes += (static_cast<uint32_t>(m) << (8 * e)) + (static_cast<uint32_t>(m >> 32) << (8 * e + 4));
+    }
+    c.codes[h] = codes - 0x4b400000u * 0x11111111u;  // the constant's own bits under the codes
+    if (!inside || off > 0.5f - 0x1p-16f) c.codes[h] = codes_with_care<F16>(raw[h], low, scale, part);
+  }
   c.scale = __half_as_ushort(scale_h);
   c.low = __half_as_ushort(low_h);
   return c;
 }
 
-// The j-th eight dimensions of token r of a page, written into it (in shared or in global memory).
+// The j-th sixteen dimensions of token r of a page, written into it (in shared or in global memory).
 template <int D>
-__device__ __forceinline__ void store_key8(uint8_t* page, int r, int j, const Cell8& c) {
-  *reinterpret_cast<uint32_t*>(page + Cells<D>::key_word(r, j)) = c.codes;
-  if (j % 8 == 0)
-    *reinterpret_cast<uint32_t*>(page + Cells<D>::key_head(r, j / 8)) =
+__device__ __forceinline__ void store_key16(uint8_t* page, int r, int j, const Cell16& c) {
+  *reinterpret_cast<uint2*>(page + Cells<D>::key_word(r, 2 * j)) = make_uint2(c.codes[0], c.codes[1]);
+  if (j % 4 == 0)
+    *reinterpret_cast<uint32_t*>(page + Cells<D>::key_head(r, j / 4)) =
         static_cast<uint32_t>(c.scale) | static_cast<uint32_t>(c.low) << 16;
 }
 template <int D>
-__device__ __forceinline__ void store_value_head(uint8_t* page, int r, int j, const Cell8& c) {
-  *reinterpret_cast<uint32_t*>(page + Cells<D>::value_head(r, j / 8)) =
+__device__ __forceinline__ void store_value_head(uint8_t* page, int r, int j, const Cell16& c) {
+  *reinterpret_cast<uint32_t*>(page + Cells<D>::value_head(r, j / 4)) =
       static_cast<uint32_t>(c.scale) | static_cast<uint32_t>(c.low) << 16;
 }
 template <int D>
-__device__ __forceinline__ void store_value8(uint8_t* page, int r, int j, const Cell8& c) {
-  uint8_t* w = page + Cells<D>::value_words(r >> 1, j) + 2 * (r & 1);
-  *reinterpret_cast<uint16_t*>(w) = static_cast<uint16_t>(c.codes);
-  *reinterpret_cast<uint16_t*>(w + 4) = static_cast<uint16_t>(c.codes >> 16);
-  if (j % 8 == 0) store_value_head<D>(page, r, j, c);
+__device__ __forceinline__ void store_value16(uint8_t* page, int r, int j, const Cell16& c) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint8_t* w = page + Cells<D>::value_words(r >> 1, 2 * j + h) + 2 * (r & 1);
+    *reinterpret_cast<uint16_t*>(w) = static_cast<uint16_t>(c.codes[h]);
+    *reinterpret_cast<uint16_t*>(w + 4) = static_cast<uint16_t>(c.codes[h] >> 16);
+  }
+  if (j % 4 == 0) store_value_head<D>(page, r, j, c);
 }
 
 }  // namespace q4

@@ -1,7 +1,7 @@
 // q4_rows.cu — keys and values into the cells of the paged 4-bit cache, and back (dkv_q4_append, dkv_q4_read).
 //
-// A lane takes eight dimensions of a token (one 16-byte load or store; q4_cells.cuh quantises). Memory bound: 2
-// bytes read and 0.56 written per element, and the reverse.
+// A lane takes sixteen dimensions of a token's key and value (q4_cells.cuh quantises). 2 bytes are read and 0.56 written
+// per element, and the reverse.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -15,7 +15,7 @@ namespace {
 using q4::Cells;
 constexpr int kRowThreads = 256;
 
-// A lane's place: the j-th eight dimensions of token i of a conversation's KV head. Rows run over tokens fastest, so a
+// A lane's place: the j-th sixteen dimensions of token i of a conversation's KV head. Rows run over tokens fastest, so a
 // warp holds neighbouring tokens of one head: whole lines of the key cells, and both tokens of a value pair.
 struct Place {
   int seq, head, i, j, slot;  // slot -1: no token
@@ -23,7 +23,7 @@ struct Place {
 
 template <int D>
 __device__ __forceinline__ Place place_of(const dkv_q4_rows_args& a) {
-  constexpr int kLanes = D / 8;
+  constexpr int kLanes = D / 16;
   const uint32_t row = (blockIdx.x * kRowThreads + threadIdx.x) / kLanes;
   const uint32_t q_len = a.q_len, heads = a.n_kv_heads;
   const uint32_t line = row / q_len;
@@ -43,35 +43,38 @@ __device__ __forceinline__ Place place_of(const dkv_q4_rows_args& a) {
 template <int D, bool F16>
 __global__ void __launch_bounds__(kRowThreads) q4_append_kernel(const __grid_constant__ dkv_q4_rows_args a) {
   using C = Cells<D>;
-  constexpr int kLanes = D / 8;
+  constexpr int kLanes = D / 16;
   const Place p = place_of<D>(a);
-  uint4 key = make_uint4(0u, 0u, 0u, 0u), value = key;
+  uint4 key[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)}, value[2] = {key[0], key[0]};
   if (p.slot >= 0) {
-    key = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.key) + p.seq * a.k_stride[0] +
-                                          p.head * a.k_stride[1] + p.i * a.k_stride[2] + p.j * 8);
-    value = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.value) + p.seq * a.v_stride[0] +
-                                            p.head * a.v_stride[1] + p.i * a.v_stride[2] + p.j * 8);
+    const uint4* ks = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.key) + p.seq * a.k_stride[0] +
+                                                     p.head * a.k_stride[1] + p.i * a.k_stride[2] + p.j * 16);
+    const uint4* vs = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.value) + p.seq * a.v_stride[0] +
+                                                     p.head * a.v_stride[1] + p.i * a.v_stride[2] + p.j * 16);
+    key[0] = ks[0], key[1] = ks[1], value[0] = vs[0], value[1] = vs[1];
   }
   // one answer for the warp's shuffles: nothing to do for it, or nothing to be done
   if (__all_sync(0xffffffffu, p.slot < 0) || __any_sync(0xffffffffu, status_at_entry(a.status) != 0)) return;
-  const q4::Cell8 k = q4::quantise8<F16>(key), v = q4::quantise8<F16>(value);
+  const q4::Cell16 k = q4::quantise16<F16>(key), v = q4::quantise16<F16>(value);
   if (!k.fits || !v.fits) record_error(a.status, kSiteQ4Rows + kErrCellRange);
   // the other token of the pair, where the lanes beside hold it
   const int there = __shfl_xor_sync(0xffffffffu, p.slot, kLanes);
   const int beside = __shfl_xor_sync(0xffffffffu, p.i, kLanes);
-  const uint32_t codes = __shfl_xor_sync(0xffffffffu, v.codes, kLanes);
+  const uint32_t other[2] = {__shfl_xor_sync(0xffffffffu, v.codes[0], kLanes), __shfl_xor_sync(0xffffffffu, v.codes[1], kLanes)};
   if (p.slot < 0) return;
   uint8_t* page = a.cells + (static_cast<int64_t>(p.slot / q4::kPage) * a.n_kv_heads + p.head) * C::kBytes;
   const int r = p.slot % q4::kPage;
-  q4::store_key8<D>(page, r, p.j, k);
-  const bool low = (threadIdx.x & kLanes) == 0;
-  const int step = low ? 1 : -1;
-  if (there >= 0 && there == p.slot + step && beside == p.i + step && (r & 1) == (low ? 0 : 1)) {
-    const uint32_t word = low ? __byte_perm(v.codes, codes, 0x5410) : __byte_perm(codes, v.codes, 0x7632);
-    *reinterpret_cast<uint32_t*>(page + C::value_words(r >> 1, p.j) + (low ? 0 : 4)) = word;
-    if (p.j % 8 == 0) q4::store_value_head<D>(page, r, p.j, v);
+  q4::store_key16<D>(page, r, p.j, k);
+  const bool first = (threadIdx.x & kLanes) == 0;
+  const int step = first ? 1 : -1;
+  if (there >= 0 && there == p.slot + step && beside == p.i + step && (r & 1) == (first ? 0 : 1)) {
+    // the even token's lane writes the first eight dimensions of both, the odd one's the second
+    const uint32_t even = first ? v.codes[0] : other[1], odd = first ? other[0] : v.codes[1];
+    *reinterpret_cast<uint2*>(page + C::value_words(r >> 1, 2 * p.j + (first ? 0 : 1))) =
+        make_uint2(__byte_perm(even, odd, 0x5410), __byte_perm(even, odd, 0x7632));
+    if (p.j % 4 == 0) q4::store_value_head<D>(page, r, p.j, v);
   } else {
-    q4::store_value8<D>(page, r, p.j, v);
+    q4::store_value16<D>(page, r, p.j, v);
   }
 }
 
@@ -102,22 +105,27 @@ __global__ void __launch_bounds__(kRowThreads) q4_read_kernel(const __grid_const
   using C = Cells<D>;
   const Place p = place_of<D>(a);
   if (p.seq >= a.n_seq) return;
-  uint4 key = make_uint4(0u, 0u, 0u, 0u), value = key;
+  uint4 key[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)}, value[2] = {key[0], key[0]};
   if (p.slot >= 0 && status_at_entry(a.status) == 0) {
     const uint8_t* page = a.cells + (static_cast<int64_t>(p.slot / q4::kPage) * a.n_kv_heads + p.head) * C::kBytes;
     const int r = p.slot % q4::kPage;
-    const uint8_t* w = page + C::value_words(r >> 1, p.j);
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(page + C::key_word(r, p.j));
-    const uint32_t w0 = *reinterpret_cast<const uint32_t*>(w), w1 = *reinterpret_cast<const uint32_t*>(w + 4);
-    const uint32_t key_head = *reinterpret_cast<const uint32_t*>(page + C::key_head(r, p.j / 8));
-    const uint32_t value_head = *reinterpret_cast<const uint32_t*>(page + C::value_head(r, p.j / 8));
-    key = values_of<F16>(codes, key_head);
-    value = values_of<F16>(__byte_perm(w0, w1, r & 1 ? 0x7632 : 0x5410), value_head);
+    const uint2 codes = *reinterpret_cast<const uint2*>(page + C::key_word(r, 2 * p.j));
+    const uint32_t key_head = *reinterpret_cast<const uint32_t*>(page + C::key_head(r, p.j / 4));
+    const uint32_t value_head = *reinterpret_cast<const uint32_t*>(page + C::value_head(r, p.j / 4));
+    const uint32_t half = r & 1 ? 0x7632 : 0x5410;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint2 w = *reinterpret_cast<const uint2*>(page + C::value_words(r >> 1, 2 * p.j + h));
+      value[h] = values_of<F16>(__byte_perm(w.x, w.y, half), value_head);
+    }
+    key[0] = values_of<F16>(codes.x, key_head);
+    key[1] = values_of<F16>(codes.y, key_head);
   }
-  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.key) + p.seq * a.k_stride[0] + p.head * a.k_stride[1] +
-                            p.i * a.k_stride[2] + p.j * 8) = key;
-  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.value) + p.seq * a.v_stride[0] + p.head * a.v_stride[1] +
-                            p.i * a.v_stride[2] + p.j * 8) = value;
+  uint4* ks = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.key) + p.seq * a.k_stride[0] + p.head * a.k_stride[1] +
+                                       p.i * a.k_stride[2] + p.j * 16);
+  uint4* vs = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.value) + p.seq * a.v_stride[0] + p.head * a.v_stride[1] +
+                                       p.i * a.v_stride[2] + p.j * 16);
+  ks[0] = key[0], ks[1] = key[1], vs[0] = value[0], vs[1] = value[1];
 }
 
 int check_rows(const dkv_q4_rows_args* a) {
@@ -146,7 +154,7 @@ int64_t dkv_q4_page_bytes(int32_t head_dim) {
 int dkv_q4_append(const dkv_q4_rows_args* a, void* stream) {
   const int rc = dkv::check_rows(a);
   if (rc != DKV_OK) return rc;
-  const int64_t lanes = static_cast<int64_t>(a->n_seq) * a->q_len * a->n_kv_heads * (a->head_dim / 8);
+  const int64_t lanes = static_cast<int64_t>(a->n_seq) * a->q_len * a->n_kv_heads * (a->head_dim / 16);
   if (lanes == 0) return DKV_OK;
   const int64_t blocks = (lanes + dkv::kRowThreads - 1) / dkv::kRowThreads;
   if (lanes > INT32_MAX) return DKV_ERR_CONFIG;
@@ -161,7 +169,7 @@ int dkv_q4_append(const dkv_q4_rows_args* a, void* stream) {
 int dkv_q4_read(const dkv_q4_rows_args* a, void* stream) {
   const int rc = dkv::check_rows(a);
   if (rc != DKV_OK) return rc;
-  const int64_t lanes = static_cast<int64_t>(a->n_seq) * a->q_len * a->n_kv_heads * (a->head_dim / 8);
+  const int64_t lanes = static_cast<int64_t>(a->n_seq) * a->q_len * a->n_kv_heads * (a->head_dim / 16);
   if (lanes == 0) return DKV_OK;
   const int64_t blocks = (lanes + dkv::kRowThreads - 1) / dkv::kRowThreads;
   if (lanes > INT32_MAX) return DKV_ERR_CONFIG;
