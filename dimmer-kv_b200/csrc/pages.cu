@@ -20,6 +20,7 @@ namespace {
 
 constexpr int kPage = DKV_PAGE_TOKENS;
 constexpr int kPlanThreads = 1024;
+constexpr int kBatch = 4;
 constexpr int kMaxSeq = 8192;           // conversations of one table (offsets held in shared memory)
 constexpr int64_t kSlotsInPlan = 8192;  // slots that the plan's CTA writes itself
 
@@ -47,18 +48,8 @@ __device__ __forceinline__ int cta_scan(int v, int* scratch, int& total) {
   return x + before;
 }
 
-__device__ __forceinline__ void write_slots(const dkv_page_args& a, const int* starts, int64_t first, int64_t step) {
-  const int64_t n = static_cast<int64_t>(a.n_seq) * a.q_len;
-  for (int64_t e = first; e < n; e += step) {
-    const int s = static_cast<int>(e / a.q_len), i = static_cast<int>(e - static_cast<int64_t>(s) * a.q_len);
-    int slot = -1;
-    if (i < a.counts[s]) {
-      const int at = starts[s] + i;
-      slot = a.blocks[static_cast<int64_t>(s) * a.max_blocks + at / kPage] * kPage + at % kPage;
-    }
-    a.slots[e] = slot;
-  }
-}
+// The slot of token `at` of a conversation whose blocks are `row`.
+__device__ __forceinline__ int slot_of(const int32_t* row, int at) { return row[at / kPage] * kPage + at % kPage; }
 
 __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const dkv_page_args a, int slots_here) {
   __shared__ int offset[kMaxSeq];
@@ -69,6 +60,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const dkv_page_
   bool bad = tid == 0 && status_at_entry(a.status) != 0;
   bool counts_bad = false;
   int64_t taken = 0;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   for (int base = 0; base < a.n_seq; base += kPlanThreads) {
     const int s = base + tid;
     int take = 0;
@@ -98,37 +90,57 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const dkv_page_
     const int len = a.lengths[s];
     const int have = pages_of(len), need = pages_of(len + a.counts[s]);
     int* row = a.blocks + static_cast<int64_t>(s) * a.max_blocks;
-    for (int j = have + lane; j < need; j += 32) row[j] = a.free_pages[n_free - 1 - (offset[s] + j - have)];
+    const int32_t* from = a.free_pages + n_free - 1 - offset[s] + have;  // page j is from[-j]
+    for (int j = have + lane; j < need; j += 32 * kBatch) {
+      int page[kBatch];  // kBatch loads under way at a time
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) page[k] = j + 32 * k < need ? __ldg(from - (j + 32 * k)) : 0;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k)
+        if (j + 32 * k < need) row[j + 32 * k] = page[k];
+    }
     if (lane == 0) a.starts[s] = len;
   }
   __syncthreads();
-  if (slots_here) write_slots(a, a.starts, tid, kPlanThreads);
+  if (slots_here) {
+    const int n = a.n_seq * a.q_len;
+    for (int e = tid; e < n; e += kPlanThreads) {
+      const int s = e / a.q_len, i = e - s * a.q_len;
+      a.slots[e] = i < a.counts[s] ? slot_of(a.blocks + static_cast<int64_t>(s) * a.max_blocks, a.starts[s] + i) : -1;
+    }
+  }
   for (int s = tid; s < a.n_seq; s += kPlanThreads) a.lengths[s] = a.starts[s] + a.counts[s];
   if (tid == 0) a.n_free[0] = n_free - static_cast<int>(taken);
 }
 
-// Slots of tokens starts[s] .. starts[s] + counts[s] - 1. The table is read only: any number of CTAs. `checked`:
-// the plan that ran before has checked the counts (a failed one left the status word set).
-__global__ void __launch_bounds__(256) page_slots_kernel(const dkv_page_args a, int planned) {
-  if (status_at_entry(a.status) != 0) {
-    if (planned) return;  // the plan wrote -1
-    const int64_t n = static_cast<int64_t>(a.n_seq) * a.q_len;
-    for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < n; e += 256ll * gridDim.x) a.slots[e] = -1;
+// Slots of tokens starts[s] .. starts[s] + counts[s] - 1: a CTA takes kSlotTile rows of one conversation, a thread four.
+// The table is read only. `planned`: the plan that ran before (this launch begins under its end) has checked the counts;
+// a failed one left the status word set and every slot -1.
+constexpr int kSlotThreads = 256, kSlotTile = 4 * kSlotThreads;
+__global__ void __launch_bounds__(kSlotThreads) page_slots_kernel(const dkv_page_args a, int planned) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int tiles = (a.q_len + kSlotTile - 1) / kSlotTile;
+  const int s = blockIdx.x / tiles, i0 = (blockIdx.x - s * tiles) * kSlotTile + threadIdx.x * 4;
+  const bool failed = status_at_entry(a.status) != 0;
+  if (i0 >= a.q_len || (failed && planned)) return;
+  const int start = a.starts[s], count = a.counts[s], len = a.lengths[s];
+  const int32_t* row = a.blocks + static_cast<int64_t>(s) * a.max_blocks;
+  int32_t* out = a.slots + static_cast<int64_t>(s) * a.q_len + i0;
+  const int n = min(4, a.q_len - i0);
+  if (!failed && count > i0 && (start < 0 || start > len || min(count, i0 + n) > len - start)) {
+    record_error(a.status, kSitePages + kErrCounts);
+    for (int k = 0; k < n; ++k) out[k] = -1;
     return;
   }
-  const int64_t n = static_cast<int64_t>(a.n_seq) * a.q_len;
-  for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < n; e += 256ll * gridDim.x) {
-    const int s = static_cast<int>(e / a.q_len), i = static_cast<int>(e - static_cast<int64_t>(s) * a.q_len);
-    int slot = -1;
-    if (i < a.counts[s]) {
-      const int at = a.starts[s] + i;
-      if (at < 0 || at >= a.lengths[s]) {
-        record_error(a.status, kSitePages + kErrCounts);
-      } else {
-        slot = a.blocks[static_cast<int64_t>(s) * a.max_blocks + at / kPage] * kPage + at % kPage;
-      }
-    }
-    a.slots[e] = slot;
+  int slot[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) slot[k] = !failed && k < n && i0 + k < count ? slot_of(row, start + i0 + k) : -1;
+  if (n == 4 && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
+    *reinterpret_cast<int4*>(out) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < n) out[k] = slot[k];
   }
 }
 
@@ -167,9 +179,17 @@ __global__ void __launch_bounds__(kPlanThreads) page_trim_kernel(const dkv_page_
     const int len = a.lengths[s], kept = min(len, a.counts[s]);
     const int first = pages_of(kept), have = pages_of(len);
     int* row = a.blocks + static_cast<int64_t>(s) * a.max_blocks;
-    for (int j = first + lane; j < have; j += 32) {
-      a.free_pages[top - (offset[s] + j - first)] = row[j];
-      row[j] = -1;
+    int32_t* to = a.free_pages + top - offset[s] + first;  // block j goes to to[-j]
+    for (int j = first + lane; j < have; j += 32 * kBatch) {
+      int page[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) page[k] = j + 32 * k < have ? row[j + 32 * k] : 0;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k)
+        if (j + 32 * k < have) {
+          to[-(j + 32 * k)] = page[k];
+          row[j + 32 * k] = -1;
+        }
     }
     __syncwarp();
     if (lane == 0) {
@@ -195,9 +215,19 @@ int check_pool(const dkv_page_args* a) {
   return DKV_OK;
 }
 
-int slots_grid(int64_t n) {
-  const int64_t g = (n + 1023) / 1024;
-  return static_cast<int>(g < 1 ? 1 : (g > 148 * 8 ? 148 * 8 : g));
+int launch_slots(const dkv_page_args& a, int planned, cudaStream_t stream) {
+  const int64_t ctas = static_cast<int64_t>(a.n_seq) * ((a.q_len + kSlotTile - 1) / kSlotTile);
+  if (ctas > INT32_MAX) return DKV_ERR_CONFIG;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(kSlotThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = planned ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, page_slots_kernel, a, planned) == cudaSuccess ? DKV_OK : DKV_ERR_CUDA;
 }
 
 }  // namespace
@@ -215,8 +245,8 @@ int dkv_page_plan(const dkv_page_args* a, void* stream) {
   const int here = n <= dkv::kSlotsInPlan;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   dkv::page_plan_kernel<<<1, dkv::kPlanThreads, 0, st>>>(*a, here);
-  if (!here) dkv::page_slots_kernel<<<dkv::slots_grid(n), 256, 0, st>>>(*a, 1);
-  return cudaGetLastError() == cudaSuccess ? DKV_OK : DKV_ERR_CUDA;
+  if (cudaGetLastError() != cudaSuccess) return DKV_ERR_CUDA;
+  return here ? DKV_OK : dkv::launch_slots(*a, 1, st);
 }
 
 int dkv_page_trim(const dkv_page_args* a, void* stream) {
@@ -232,10 +262,8 @@ int dkv_page_slots(const dkv_page_args* a, void* stream) {
   const int rc = dkv::check_pages(a);
   if (rc != DKV_OK) return rc;
   if (a->q_len < 0 || (a->slots == nullptr && a->q_len > 0)) return DKV_ERR_ARGS;
-  const int64_t n = static_cast<int64_t>(a->n_seq) * a->q_len;
-  if (n == 0) return DKV_OK;
-  dkv::page_slots_kernel<<<dkv::slots_grid(n), 256, 0, static_cast<cudaStream_t>(stream)>>>(*a, 0);
-  return cudaGetLastError() == cudaSuccess ? DKV_OK : DKV_ERR_CUDA;
+  if (a->n_seq == 0 || a->q_len == 0) return DKV_OK;
+  return dkv::launch_slots(*a, 0, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
