@@ -76,7 +76,7 @@ class LogitRules:
     def load(self, history: torch.Tensor, lengths=None, prompts=None) -> None:
         """The tokens so far: ``history`` [n_rows, n], of which row r has ``lengths[r]`` (default: all n), the first
         ``prompts[r]`` of them its prompt (default: all), the others generated."""
-        n = history.shape[1]
+        n = history.shape[-1]
         if history.dim() != 2 or history.shape[0] != self.n_rows or n > self.capacity:
             raise ValueError(f"history must be [{self.n_rows}, at most {self.capacity}]")
         self.history[:, :n] = history.to(self.history)

@@ -61,7 +61,10 @@ class PageTable:
         """int32 [n_seq] of ``count`` everywhere (kept: the same tensor for the same count)."""
         t = self._even.get(count)
         if t is None:
-            t = self._even[count] = torch.full((self.n_seq,), count, dtype=torch.int32, device=self.device)
+            t = torch.full((self.n_seq,), count, dtype=torch.int32, device=self.device)
+            # one made in a capture is filled when the graph runs, and lives in the graph's memory
+            if not torch.cuda.is_current_stream_capturing():
+                self._even[count] = t
         return t
 
     def _counts(self, counts) -> torch.Tensor:

@@ -250,6 +250,11 @@ CASES = [
     (4, 4, 64, [500], [129], 129),
     (32, 8, 64, [0, 3000, 64], [300, 0, 257], 300),
     (24, 8, 128, [9000, 65], [86, 171], 171),
+    (16, 1, 64, [200, 3], [1, 1], 1),
+    (4, 4, 128, [70, 0], [4, 4], 4),
+    # more conversations than a warp has lanes, some without a new token
+    (4, 2, 64, [(37 * s) % 301 for s in range(70)], [s % 3 > 0 for s in range(70)], 1),
+    (4, 2, 64, [(53 * s) % 200 for s in range(45)], [(7 * s) % 41 for s in range(45)], 40),
 ]
 
 
@@ -257,6 +262,7 @@ CASES = [
 @pytest.mark.parametrize("case", CASES, ids=[f"{c[0]}x{c[1]}x{c[2]}-{max(c[3])}+{c[5]}" for c in CASES])
 def test_attention_over_cells(case, dtype):
     q_heads, kv_heads, dim, held, counts, q_len = case
+    counts = [int(c) for c in counts]
     batch, query, k, v, keys, values = _filled(len(held), q_heads, kv_heads, dim, dtype, held, counts, q_len)
     scaling = dim ** -0.5
     out = batch.attend_layer(0, query, k, v, scaling)
@@ -360,6 +366,60 @@ def test_strides_offsets_streams_and_graphs():
     for x, y in zip(fresh, got):
         assert torch.equal(y[1], dequantise4(*quantise4(x[1])).to(x.dtype))
     batch.check_status()
+
+
+@pytest.mark.parametrize("q_len", [3, 40, 9000])
+def test_captured_steps_of_any_length(q_len):
+    """Plans (the larger ones with a second kernel) and attention of every form in a graph, the first call of their kind
+    there; replays advance the tables, eager calls follow."""
+    dim, kv, hq, n = 64, 2, 8, 2
+    batch = Q4Batch(n, layers=1, kv_heads=kv, q_heads=hq, head_dim=dim, max_tokens=4 * q_len + 128)
+    data = [[_rows(n, h, q_len, dim, torch.bfloat16, 10 * i + j) for j, h in enumerate((hq, kv, kv))] for i in range(3)]
+    counts = torch.tensor([q_len, q_len - 1], dtype=torch.int32, device=DEV)
+    static = [x.clone() for x in data[0]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        slots = batch.plan(counts, q_len)
+        out = batch.attend_layer(0, *static, 0.125)
+        batch.plan(None, 2)
+        batch.trim(batch.table.starts)
+    torch.cuda.current_stream().wait_stream(side)
+    outs = []
+    for x in data[:2]:
+        for a, b in zip(static, x):
+            a.copy_(b)
+        graph.replay()
+        outs.append((out.clone(), slots.clone()))
+    assert batch.lengths.tolist() == [2 * q_len, 2 * q_len - 2]
+    batch.plan(counts, q_len)
+    last = batch.attend_layer(0, *data[2], 0.125)
+    again = Q4Batch(n, layers=1, kv_heads=kv, q_heads=hq, head_dim=dim, max_tokens=4 * q_len + 128)
+    for x, got in zip(data, outs + [(last, None)]):
+        s = again.plan(counts, q_len)
+        assert torch.equal(again.attend_layer(0, *x, 0.125), got[0])
+        assert got[1] is None or torch.equal(s, got[1])
+    batch.plan(None, 2)  # its even counts were first made in the capture
+    assert batch.lengths.tolist() == [3 * q_len + 2, 3 * q_len - 1]
+    batch.check_status()
+    again.check_status()
+
+
+def test_two_readers_at_once():
+    """Attention without new tokens only reads: two streams at a time, several calls each, the same answers."""
+    held = [5000, 700, 64]
+    batch, query, k, v, keys, values = _filled(3, 24, 8, 128, torch.bfloat16, held, [1] * 3, 1, seed=3)
+    want = batch.attend_layer(0, query, k, v, 0.09)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(20):
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append(batch.attend_layer(0, query, None, None, 0.09))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
 
 
 def test_far_pages_of_a_large_pool():

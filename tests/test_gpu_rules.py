@@ -74,6 +74,46 @@ def test_rules_follow_the_formulas(rows, vocab, n, n_bias, grammar, dtype):
     rules.check_status()
 
 
+def test_long_histories_and_many_rows():
+    """Counts beyond 14 bits (histories with room for more than 16383 tokens), and rows enough for the longer slices."""
+    rows, vocab = 2, 140003
+    g = torch.Generator(device=DEV).manual_seed(4)
+    x = torch.randn(rows, vocab, generator=g, device=DEV)
+    history = torch.full((rows, 20000), 5, dtype=torch.int32, device=DEV)
+    history[:, :4000] = torch.randint(0, vocab, (rows, 4000), generator=g, device=DEV, dtype=torch.int32)
+    rules = LogitRules(rows, vocab, capacity=20001, repetition=1.25, frequency=0.0625, presence=0.5)
+    rules.load(history, prompts=[3000, 0])
+    out, token = rules.apply(x)
+    count = torch.zeros(rows, vocab, device=DEV)
+    seen = torch.zeros(rows, vocab, dtype=torch.bool, device=DEV)
+    for r, p in enumerate((3000, 0)):
+        count[r] = torch.bincount(history[r, p:].long(), minlength=vocab)
+        seen[r] = torch.bincount(history[r].long(), minlength=vocab) > 0
+    pen = torch.full((rows, 1), 1.25, device=DEV)  # a tensor: torch divides by a number as a product with its reciprocal
+    want = torch.where(seen, torch.where(x > 0, x / pen, x * pen), x)
+    want = torch.where(count > 0, (want - 0.0625 * count) - 0.5, want)  # the same float32 steps: the same bits
+    assert torch.equal(out, want) and torch.equal(token, _first_best(want))
+    assert float(count[:, 5].min()) >= 16000
+    rows = 60
+    x = torch.randn(rows, vocab, generator=g, device=DEV).bfloat16()
+    rules = LogitRules(rows, vocab, capacity=64, repetition=torch.linspace(1, 2, rows), presence=0.25)
+    history = torch.randint(0, vocab, (rows, 50), generator=g, device=DEV, dtype=torch.int32)
+    rules.load(history, prompts=[r % 50 for r in range(rows)])
+    allowed = torch.randint(-2**31, 2**31, (rows, (vocab + 31) // 32), generator=g, device=DEV, dtype=torch.int64).to(torch.int32)
+    out, token = rules.apply(x, allowed)
+    seen = torch.zeros(rows, vocab, dtype=torch.bool, device=DEV).scatter_(1, history.long(), True)
+    made = torch.zeros(rows, vocab, dtype=torch.bool, device=DEV)
+    for r in range(rows):
+        made[r, history[r, r % 50:].long()] = True
+    pen = torch.linspace(1, 2, rows, device=DEV)[:, None]
+    want = torch.where(seen, torch.where(x > 0, x.float() / pen, x.float() * pen), x.float())
+    want = torch.where(made, want - 0.25, want)
+    at = torch.arange(vocab, device=DEV)
+    want = torch.where((allowed[:, at // 32] >> (at % 32)) & 1 != 0, want, -float("inf"))
+    assert torch.equal(out, want) and torch.equal(token, _first_best(want))
+    rules.check_status()
+
+
 def test_choice_at_ties_and_ends():
     x = torch.full((6, 300), -2.0, device=DEV)
     x[0, [17, 200]] = 1.5                      # equal: the lowest
