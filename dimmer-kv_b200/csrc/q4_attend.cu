@@ -15,8 +15,8 @@
 // q4_decode_kernel: few query rows per KV head (one token, or a short draft). Bound by the cells' bytes, and close to it
 // by unpacking them (the integer pipe runs at half rate). The pages of all (conversation, KV head, row chunk) units
 // form one line, cut into equal pieces, one per WARP, so that any mix of lengths, heads and conversations fills the
-// GPU evenly; a unit that several warps share leaves partial (m, l, O) in the workspace, which q4_combine_kernel
-// joins. A page of one KV head is one contiguous block: each warp keeps a ring of bulk copies of its own and meets no
+// GPU evenly; a unit that several warps share leaves partial (m, l, O) in the workspace, which the join
+// kernels put together. A page of one KV head is one contiguous block: each warp keeps a ring of bulk copies of its own and meets no
 // other warp. It contracts tokens as the 16 rows of m16n8k16 and query rows as its 8 columns (3 or 4 heads that share a
 // KV head are the rule), S^T = C Q^T, then O^T = C^T P^T; P^T in the layout of the second product is one 8 x 8
 // transpose per 8 tokens (movmatrix). A code pair of a word is a float16 pair after ONE mask: the 4 bits are a
@@ -544,7 +544,7 @@ q4_decode_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int w
     while (tokens == 0) tokens = tokens_of(a, ++seq);
     const int n_pages = pages_of(tokens);
     const int64_t off = at - seq_at;
-    const int unit = static_cast<int>(off <= 0xffffffffll ? static_cast<uint32_t>(off) / static_cast<uint32_t>(n_pages) : off / n_pages);
+    const int unit = static_cast<int>(divide<true>(off, n_pages));
     const int64_t unit_at = seq_at + static_cast<int64_t>(unit) * n_pages;
     const int p0 = static_cast<int>(at - unit_at);
     const int p1 = static_cast<int>(min(static_cast<int64_t>(n_pages), end - unit_at));
@@ -656,7 +656,7 @@ q4_decode_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int w
           for (int gr = 0; gr < C::kGroups; ++gr) low[gr] += __shfl_xor_sync(0xffffffffu, low[gr], d);
         }
         const int col = S::row(nt, t, c), r = row0 + col, i = r / share;
-        if (r >= a.q_len * share || i >= fresh) continue;  // q4_combine_kernel writes the zeros behind the new tokens
+        if (r >= a.q_len * share || i >= fresh) continue;  // the joins write the zeros behind the new tokens
         const float inv = sum != 0.f ? 1.f / sum : 0.f;
         const int64_t to =
             ((static_cast<int64_t>(seq) * a.q_len + i) * a.n_q_heads + head * share + r - i * share) * D + g * 8;
@@ -679,62 +679,105 @@ q4_decode_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int w
   }
 }
 
-// Joins the partial results of the units that several workers share, and writes the zeros of the rows behind the new
-// tokens. One CTA per (query row of a KV head, KV head, conversation): the workers' factors first, then D / 4 lanes of
-// 4 dimensions in kSlices slices over the workers, with nothing that one load has to wait for another.
-constexpr int kCombineThreads = 256;
-constexpr int kFactors = 512;  // workers of a unit whose factors are held at a time
+// The joins write the rows of the units that several workers share, and the zeros of the rows behind the new tokens.
+struct JoinRow {
+  int seq, head, r, i;
+  int64_t to;  // where the row's output begins
+  __device__ __forceinline__ JoinRow(const dkv_q4_attend_args& a, int id, int share, int d) {
+    const int rows = a.q_len * share;
+    const int line = id / rows;
+    r = id - line * rows;
+    seq = line / a.n_kv_heads;
+    head = line - seq * a.n_kv_heads;
+    i = r / share;
+    to = ((static_cast<int64_t>(seq) * a.q_len + i) * a.n_q_heads + head * share + r - i * share) * d;
+  }
+};
+
+// Many rows, of few pieces each: a warp per row.
+constexpr int kJoinWarps = 8;
 template <int D, int NT, bool F16>
-__global__ void __launch_bounds__(kCombineThreads)
-q4_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int workers) {
-  constexpr int kLanes = D / 4, kSlices = kCombineThreads / kLanes;
-  __shared__ int64_t line[2];
-  __shared__ float4 part[kSlices][kLanes];
-  __shared__ float factor[kFactors];
-  __shared__ float warp_ref[kCombineThreads / 32], warp_den[kCombineThreads / 32];
-  const int share = a.n_q_heads / a.n_kv_heads;
+__global__ void __launch_bounds__(kJoinWarps * 32)
+q4_join_rows_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int workers) {
   constexpr int kRows = Decode<D, NT>::kRows;
-  const int rows = min(kRows, a.q_len * share);
-  const int r = blockIdx.x, head = blockIdx.y, seq = blockIdx.z;
-  const int chunk = r / kRows, col = r - chunk * kRows, i = r / share;
-  const int tid = threadIdx.x, x = tid % kLanes, slice = tid / kLanes;
-  const int tokens = tokens_of(a, seq), n_pages = pages_of(tokens);
-  const int fresh = tokens == 0 ? 0 : min(tokens - a.starts[seq], a.q_len);
+  const int share = a.n_q_heads / a.n_kv_heads, rows = a.q_len * share, units = a.n_kv_heads * chunks;
+  const int id = blockIdx.x * kJoinWarps + warp_id();
+  if (id >= rows * a.n_kv_heads * a.n_seq) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
+  const JoinRow row(a, id, share, D);
+  const int tokens = tokens_of(a, row.seq), n_pages = pages_of(tokens);
+  const bool real = tokens > 0 && row.i < min(tokens - a.starts[row.seq], a.q_len);
+  const int chunk = row.r / kRows;
+  int64_t before;
+  const int64_t all = count_pages(a, row.seq, before);
+  Pieces pieces;
+  if (real)
+    pieces = Pieces(a, Deal(all * units, workers), before * units + static_cast<int64_t>(row.head * chunks + chunk) * n_pages,
+                    n_pages, min(kRows, rows), D);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // what is above does not depend on the main kernel
+  float sum[D / 32];
+#pragma unroll
+  for (int e = 0; e < D / 32; ++e) sum[e] = 0.f;
+  const int failed = status_at_entry(a.status);
+  if (real) {
+    if (pieces.n == 1 && !__any_sync(0xffffffffu, failed != 0)) return;  // one worker had the whole unit
+    if (pieces.n > 1) join_row<D, -1, 8>(pieces, min(kRows, rows), row.r - chunk * kRows, sum);
+  }
+  if (__any_sync(0xffffffffu, failed != 0)) {
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) sum[e] = 0.f;
+  }
+  store_row<D, F16>(a, row.to, sum);
+}
+
+// Few rows, of many pieces: a CTA per row and 32 dimensions; the pieces' factors first, then 8 lanes of 4 dimensions in
+// kSlices slices over the pieces, with nothing that one load has to wait for another.
+constexpr int kPartThreads = 256;
+constexpr int kFactors = 512;  // pieces whose factors are held at a time
+template <int D, int NT, bool F16>
+__global__ void __launch_bounds__(kPartThreads)
+q4_join_parts_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int workers) {
+  constexpr int kRows = Decode<D, NT>::kRows, kParts = D / 32, kSlices = kPartThreads / 8;
+  __shared__ int64_t line[2];
+  __shared__ float4 part[kPartThreads / 32][8];
+  __shared__ float factor[kFactors];
+  __shared__ float warp_ref[kPartThreads / 32], warp_den[kPartThreads / 32];
+  const int share = a.n_q_heads / a.n_kv_heads, rows = min(kRows, a.q_len * share), units = a.n_kv_heads * chunks;
+  const JoinRow row(a, blockIdx.x / kParts, share, D);
+  const int tid = threadIdx.x, slice = tid / 8, dim = (blockIdx.x % kParts) * 32 + (tid % 8) * 4;
+  const int tokens = tokens_of(a, row.seq), n_pages = pages_of(tokens);
+  const int chunk = row.r / kRows, col = row.r - chunk * kRows;
   if (tid < 32) {
     int64_t before;
-    const int64_t all = count_pages(a, seq, before);
+    const int64_t all = count_pages(a, row.seq, before);
     if (tid == 0) line[0] = all, line[1] = before;
   }
   __syncthreads();
-  const int units = a.n_kv_heads * chunks;
-  const int64_t to = ((static_cast<int64_t>(seq) * a.q_len + i) * a.n_q_heads + head * share + r - i * share) * D + x * 4;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  // The main kernel of this call may have set the status word while others of its warps finished: the CTA's one answer.
-  if (i >= fresh || cta_failed_at_entry(a.status)) {
-    if (slice == 0) store_out4<F16>(a, to, 0.f, 0.f, 0.f, 0.f);
+  const bool real = tokens > 0 && row.i < min(tokens - a.starts[row.seq], a.q_len);
+  Pieces pieces;
+  if (real)
+    pieces = Pieces(a, Deal(line[0] * units, workers), line[1] * units + static_cast<int64_t>(row.head * chunks + chunk) * n_pages,
+                    n_pages, rows, D);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // what is above does not depend on the main kernel
+  // That one may have set the status word while others of its warps finished: the CTA's one answer.
+  if (cta_failed_at_entry(a.status) || !real) {
+    if (slice == 0) store_out4<F16>(a, row.to + dim, 0.f, 0.f, 0.f, 0.f);
     return;
   }
-  const Deal deal(line[0] * units, workers);
-  const int64_t unit_at = line[1] * units + static_cast<int64_t>(head * chunks + chunk) * n_pages;
-  const int w0 = deal.owner(unit_at), w1 = deal.owner(unit_at + n_pages - 1);
-  if (w0 == w1) return;  // one worker had the whole unit
-  const int64_t stride = slot_floats(rows, D);
-  // the unit is the last segment of w0 unless w0 begins with it, and the first segment of the others
-  const float* first = a.workspace + (2 * static_cast<int64_t>(w0) + (deal.begin(w0) < unit_at ? 1 : 0)) * stride;
-  const float* rest = a.workspace + 2 * static_cast<int64_t>(w0) * stride;
-  auto slot = [&](int k) { return k == 0 ? first : rest + 2 * k * stride; };
+  if (pieces.n == 1) return;  // one worker had the whole unit
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   float den = 0.f, ref = INFINITY;  // sums are relative to 2^-ref; the smallest ref is the largest maximum
-  const int n = w1 - w0 + 1;
-  for (int base = 0; base < n; base += kFactors) {
-    const int m = min(kFactors, n - base);
-    float mine[kFactors / kCombineThreads], weight[kFactors / kCombineThreads];
+  for (int base = 0; base < pieces.n; base += kFactors) {
+    const int m = min(kFactors, pieces.n - base);
+    float mine[kFactors / kPartThreads], weight[kFactors / kPartThreads];
     float low = INFINITY;
 #pragma unroll
-    for (int k = 0; k < kFactors / kCombineThreads; ++k) {
-      const int w = k * kCombineThreads + tid;
-      const float2 s = w < m ? *reinterpret_cast<const float2*>(slot(base + w) + rows * D + col * 4) : make_float2(0.f, 0.f);
-      mine[k] = s.y == 0.f ? INFINITY : s.x;  // a worker that saw no token of this row
+    for (int k = 0; k < kFactors / kPartThreads; ++k) {
+      const int w = k * kPartThreads + tid;
+      const float2 s = w < m ? *reinterpret_cast<const float2*>(pieces.slot(base + w) + rows * D + col * 4) : make_float2(0.f, 0.f);
+      mine[k] = s.y == 0.f ? INFINITY : s.x;  // a piece that saw no token of this row
       weight[k] = s.y;
       low = fminf(low, mine[k]);
     }
@@ -744,11 +787,11 @@ q4_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int 
     __syncthreads();
     float now = ref;
 #pragma unroll
-    for (int k = 0; k < kCombineThreads / 32; ++k) now = fminf(now, warp_ref[k]);
+    for (int k = 0; k < kPartThreads / 32; ++k) now = fminf(now, warp_ref[k]);
     float add = 0.f;
 #pragma unroll
-    for (int k = 0; k < kFactors / kCombineThreads; ++k) {
-      const int w = k * kCombineThreads + tid;
+    for (int k = 0; k < kFactors / kPartThreads; ++k) {
+      const int w = k * kPartThreads + tid;
       const float f = mine[k] == INFINITY ? 0.f : exp2_fast(now - mine[k]);
       if (w < m) factor[w] = f;
       add = fmaf(weight[k], f, add);
@@ -760,12 +803,12 @@ q4_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int 
     const float keep = ref == INFINITY ? 0.f : exp2_fast(now - ref);
     den *= keep;
 #pragma unroll
-    for (int k = 0; k < kCombineThreads / 32; ++k) den += warp_den[k];
+    for (int k = 0; k < kPartThreads / 32; ++k) den += warp_den[k];
     sum.x *= keep, sum.y *= keep, sum.z *= keep, sum.w *= keep;
     ref = now;
 #pragma unroll 8
     for (int w = slice; w < m; w += kSlices) {
-      const float4 o = *reinterpret_cast<const float4*>(slot(base + w) + col * D + x * 4);
+      const float4 o = *reinterpret_cast<const float4*>(pieces.slot(base + w) + col * D + dim);
       const float f = factor[w];
       sum.x = fmaf(o.x, f, sum.x);
       sum.y = fmaf(o.y, f, sum.y);
@@ -774,16 +817,24 @@ q4_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int 
     }
     __syncthreads();
   }
-  part[slice][x] = sum;
+  // the slices' sums: four of a warp's by shuffles, the warps' through shared memory
+#pragma unroll
+  for (int d = 8; d < 32; d <<= 1) {
+    sum.x += __shfl_xor_sync(0xffffffffu, sum.x, d);
+    sum.y += __shfl_xor_sync(0xffffffffu, sum.y, d);
+    sum.z += __shfl_xor_sync(0xffffffffu, sum.z, d);
+    sum.w += __shfl_xor_sync(0xffffffffu, sum.w, d);
+  }
+  if ((tid & 31) < 8) part[tid >> 5][tid & 7] = sum;
   __syncthreads();
   if (slice != 0) return;
 #pragma unroll
-  for (int k = 1; k < kSlices; ++k) {
-    const float4 o = part[k][x];
+  for (int k = 1; k < kPartThreads / 32; ++k) {
+    const float4 o = part[k][tid];
     sum.x += o.x, sum.y += o.y, sum.z += o.z, sum.w += o.w;
   }
   const float inv = den != 0.f ? 1.f / den : 0.f;
-  store_out4<F16>(a, to, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+  store_out4<F16>(a, row.to + dim, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
 }
 
 // NT of q4_decode_kernel, and the query rows that a warp then holds.
@@ -810,16 +861,23 @@ int launch_decode(const dkv_q4_attend_args& a, int append, cudaStream_t stream) 
   if (!allow_shared(kernel, bytes, done)) return DKV_ERR_CUDA;
   kernel<<<ctas, kThreads, bytes, stream>>>(a, chunks, workers, append);
   if (cudaGetLastError() != cudaSuccess) return DKV_ERR_CUDA;
+  // Many rows have few pieces each and a warp does for one; of few rows each has the pieces of many workers. 24 heads of
+  // 128 over 4K-16K tokens: 64 conversations 127 us with a warp per row, 156 with CTAs; 16: 48 and 52; 8: 38 and 34.
+  const int64_t joins = static_cast<int64_t>(rows) * a.n_kv_heads * a.n_seq;
+  const bool many = joins >= 256;
+  const int64_t grid = many ? (joins + kJoinWarps - 1) / kJoinWarps : joins * (D / 32);
+  if (joins * (D / 32) > INT32_MAX) return DKV_ERR_CONFIG;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(rows, a.n_kv_heads, a.n_seq);
-  cfg.blockDim = dim3(kCombineThreads);
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(many ? kJoinWarps * 32 : kPartThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, q4_combine_kernel<D, NT, F16>, a, chunks, workers) == cudaSuccess ? DKV_OK : DKV_ERR_CUDA;
+  auto join = many ? q4_join_rows_kernel<D, NT, F16> : q4_join_parts_kernel<D, NT, F16>;
+  return cudaLaunchKernelEx(&cfg, join, a, chunks, workers) == cudaSuccess ? DKV_OK : DKV_ERR_CUDA;
 }
 
 int check_sizes(const dkv_q4_attend_args* a) {

@@ -32,22 +32,28 @@ __device__ __forceinline__ int tokens_of(const dkv_q4_attend_args& a, int s) {
 }
 __device__ __forceinline__ int pages_of(int tokens) { return (tokens + kPage - 1) / kPage; }
 
+// a / b: lines shorter than 2^32 / workers, all but the largest, do with 32 bits; the others' division is kept out of line
+// (CALL), for kernels of a few microseconds wait for their code, but for the kernel that deals out registers: a call in it
+// would hold every role to the registers of the launch (q4_prefill_kernel: 74 us without, 81 with).
+static __device__ __noinline__ int64_t divide64(int64_t a, int64_t b) { return a / b; }
+template <bool CALL>
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  if (a <= 0xffffffffll && b <= 0xffffffffll) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return CALL ? divide64(a, b) : a / b;
+}
+
 // How a line of `total` places is dealt to the workers: worker w has [total * w / workers, total * (w + 1) / workers).
-struct Deal {
+template <bool CALL>
+struct DealOf {
   int64_t total;
   int workers;
-  __device__ __forceinline__ Deal(int64_t total_, int workers_)
+  __device__ __forceinline__ DealOf(int64_t total_, int workers_)
       : total(total_), workers(static_cast<int>(total_ < workers_ ? total_ : workers_)) {}
-  __device__ __forceinline__ int64_t begin(int w) const {
-    const int64_t x = total * w;
-    return x <= 0xffffffffll ? static_cast<uint32_t>(x) / static_cast<uint32_t>(workers) : x / workers;
-  }
+  __device__ __forceinline__ int64_t begin(int w) const { return divide<CALL>(total * w, workers); }
   // The worker that has place x; none is without a place.
-  __device__ __forceinline__ int owner(int64_t x) const {
-    const int64_t y = (x + 1) * workers - 1;
-    return static_cast<int>(y <= 0xffffffffll ? static_cast<uint32_t>(y) / static_cast<uint32_t>(total) : y / total);
-  }
+  __device__ __forceinline__ int owner(int64_t x) const { return static_cast<int>(divide<CALL>((x + 1) * workers - 1, total)); }
 };
+using Deal = DealOf<true>;
 
 template <bool F16>
 __device__ __forceinline__ void store_out4(const dkv_q4_attend_args& a, int64_t at, float x, float y, float z, float w) {
@@ -61,6 +67,82 @@ __device__ __forceinline__ void store_out4(const dkv_q4_attend_args& a, int64_t 
 
 // A partial result in the workspace: per slot (two per worker) [rows][D] of O, then [rows][4] with (reference, l).
 __host__ __device__ __forceinline__ int64_t slot_floats(int rows, int d) { return static_cast<int64_t>(rows) * (d + 4); }
+
+// The partial results of one unit: worker w0 + k left the unit's piece in slot(k). The unit is the last segment of w0 unless
+// w0 begins with it (its second slot), and the first segment of the others.
+struct Pieces {
+  const float *first = nullptr, *rest = nullptr;
+  int64_t stride = 0;
+  int n = 0;
+  __device__ __forceinline__ Pieces() {}
+  __device__ __forceinline__ Pieces(const dkv_q4_attend_args& a, const Deal& deal, int64_t unit, int places, int rows, int d) {
+    const int w0 = deal.owner(unit), w1 = deal.owner(unit + places - 1);
+    stride = slot_floats(rows, d);
+    n = w1 - w0 + 1;
+    first = a.workspace + (2 * static_cast<int64_t>(w0) + (deal.begin(w0) < unit ? 1 : 0)) * stride;
+    rest = a.workspace + 2 * static_cast<int64_t>(w0) * stride;
+  }
+  __device__ __forceinline__ const float* slot(int k) const { return k == 0 ? first : rest + 2 * k * stride; }
+};
+
+// Joins the pieces of row `row` of a unit: a warp, D / 32 dimensions per lane. References are where the sums' factor is
+// 2^-reference (SIGN = 1: q4_prefill's maxima) or 2^reference (-1: q4_decode's negated ones).
+template <int D, int SIGN, int UNROLL>
+__device__ __forceinline__ void join_row(const Pieces& p, int rows, int row, float (&sum)[D / 32]) {
+  constexpr int kPer = D / 32;
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) sum[e] = 0.f;
+  float den = 0.f, ref = -INFINITY;
+  for (int base = 0; base < p.n; base += 32) {
+    // the factors of 32 pieces, one per lane, then their sums with no load waiting for another
+    const int n = min(32, p.n - base);
+    const float2 s = lane < n ? *reinterpret_cast<const float2*>(p.slot(base + lane) + rows * D + row * 4) : make_float2(0.f, 0.f);
+    const float mine = s.y == 0.f ? -INFINITY : SIGN * s.x;  // a piece that saw no token of this row has no say
+    float now = fmaxf(ref, mine);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
+    const float f = mine == -INFINITY ? 0.f : exp2_fast(mine - now);
+    float add = s.y * f;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
+    const float keep = ref == -INFINITY ? 0.f : exp2_fast(ref - now);
+    den = fmaf(den, keep, add);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) sum[e] *= keep;
+    ref = now;
+#pragma unroll UNROLL
+    for (int w = 0; w < n; ++w) {
+      const float* o = p.slot(base + w) + row * D + lane * kPer;
+      const float fw = __shfl_sync(0xffffffffu, f, w);
+      if constexpr (kPer == 4) {
+        const float4 u = *reinterpret_cast<const float4*>(o);
+        sum[0] = fmaf(u.x, fw, sum[0]), sum[1] = fmaf(u.y, fw, sum[1]);
+        sum[2] = fmaf(u.z, fw, sum[2]), sum[3] = fmaf(u.w, fw, sum[3]);
+      } else {
+        const float2 u = *reinterpret_cast<const float2*>(o);
+        sum[0] = fmaf(u.x, fw, sum[0]), sum[1] = fmaf(u.y, fw, sum[1]);
+      }
+    }
+  }
+  const float inv = den != 0.f ? 1.f / den : 0.f;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) sum[e] *= inv;
+}
+
+// A lane's D / 32 dimensions of an output row that begins at `at`.
+template <int D, bool F16>
+__device__ __forceinline__ void store_row(const dkv_q4_attend_args& a, int64_t at, const float (&v)[D / 32]) {
+  at += (threadIdx.x & 31) * (D / 32);
+  if constexpr (D == 128) {
+    store_out4<F16>(a, at, v[0], v[1], v[2], v[3]);
+  } else if (a.out_f32) {
+    *reinterpret_cast<float2*>(static_cast<float*>(a.out) + at) = make_float2(v[0], v[1]);
+  } else {
+    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at) =
+        static_cast<uint32_t>(to16<F16>(v[0])) | static_cast<uint32_t>(to16<F16>(v[1])) << 16;
+  }
+}
 
 // Query rows of a KV head (all new tokens' rows of its query heads).
 inline int rows_of(const dkv_q4_attend_args& a) { return a.q_len * (a.n_q_heads / a.n_kv_heads); }

@@ -181,7 +181,7 @@ struct Walk {
     q = seq_of(a, seq, share);
     const int64_t per_head = seq_steps(q, share);
     int64_t rest = at - line;
-    head = static_cast<int>(rest / per_head);
+    head = static_cast<int>(divide<false>(rest, per_head));
     rest -= head * per_head;
     block = 0;
     while (rest >= steps_of(q, block, share)) rest -= steps_of(q, block++, share);
@@ -293,7 +293,7 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
   const uint32_t tmem = *tmem_slot;
 
   int64_t unused;
-  const Deal deal(count_steps(a, share, 0, unused), workers);
+  const DealOf<false> deal(count_steps(a, share, 0, unused), workers);
   int64_t begin = 0, end = 0;
   if (!failed && static_cast<int>(blockIdx.x) < deal.workers) {
     begin = deal.begin(blockIdx.x);
@@ -719,7 +719,8 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
   if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
-// Joins the blocks that several CTAs share and writes the zeros of the rows behind the new tokens: a warp per row.
+// Joins the blocks that several CTAs share and writes the zeros of the rows behind the new tokens: cta_rows (which divides
+// kBlock) rows of one block per CTA, a warp per row.
 constexpr int kCombineWarps = 8;
 template <int D, bool F16>
 __global__ void __launch_bounds__(kCombineWarps * 32)
@@ -728,81 +729,31 @@ q4_prefill_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int work
   const int share = a.n_q_heads / a.n_kv_heads;
   const int head = blockIdx.y, seq = blockIdx.z, warp = warp_id(), lane = threadIdx.x & 31;
   const Seq q = seq_of(a, seq, share);
+  const int rows = a.q_len * share, r0 = blockIdx.x * cta_rows, block = r0 / kBlock;
   if (warp == 0) {
     int64_t before;
     const int64_t all = count_steps(a, share, seq, before);
-    if (lane == 0) line[0] = all, line[1] = before;
+    int64_t unit = before + head * seq_steps(q, share);
+    for (int b = 0; b < min(block, q.blocks); ++b) unit += steps_of(q, b, share);
+    if (lane == 0) line[0] = all, line[1] = unit;
   }
   __syncthreads();
-  const int64_t per_head = seq_steps(q, share);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  Pieces pieces;
+  if (r0 < q.rows) pieces = Pieces(a, Deal(line[0], workers), line[1], steps_of(q, block, share), slot_rows, D);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // what is above does not depend on the main kernel
   const bool failed = cta_failed_at_entry(a.status);
-  const int rows = a.q_len * share;
-  constexpr int kPer = D / 32;  // dimensions of a lane
   for (int k = warp; k < cta_rows; k += kCombineWarps) {
-    const int r = blockIdx.x * cta_rows + k, i = r / share;
+    const int r = r0 + k, i = r / share;
     if (r >= rows) break;
-    const int64_t to =
-        ((static_cast<int64_t>(seq) * a.q_len + i) * a.n_q_heads + head * share + r - i * share) * D + lane * kPer;
-    float sum[kPer];
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) sum[e] = 0.f;
+    float sum[D / 32];
     if (r < q.rows && !failed) {
-      const int block = r / kBlock, row = r - block * kBlock;
-      const Deal deal(line[0], workers);
-      int64_t unit = line[1] + head * per_head;
-      for (int b = 0; b < block; ++b) unit += steps_of(q, b, share);
-      const int w0 = deal.owner(unit), w1 = deal.owner(unit + steps_of(q, block, share) - 1);
-      if (w0 == w1) continue;  // one CTA had the whole block
-      const int64_t stride = slot_floats(slot_rows, D);
-      const float* first = a.workspace + (2 * static_cast<int64_t>(w0) + (deal.begin(w0) < unit ? 1 : 0)) * stride;
-      const float* rest = a.workspace + 2 * static_cast<int64_t>(w0) * stride;
-      auto slot = [&](int w) { return w == 0 ? first : rest + 2 * w * stride; };
-      float den = 0.f, ref = -INFINITY;
-      for (int base = 0; base <= w1 - w0; base += 32) {
-        // the factors of 32 CTAs, one per lane, then their sums with no load waiting for another
-        const int n = min(32, w1 - w0 + 1 - base);
-        const float2 s = lane < n ? *reinterpret_cast<const float2*>(slot(base + lane) + slot_rows * D + row * 4)
-                                  : make_float2(0.f, 0.f);
-        const float mine = s.y == 0.f ? -INFINITY : s.x;  // one that saw no token of this row
-        float now = fmaxf(ref, mine);
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
-        const float f = mine == -INFINITY ? 0.f : exp2_fast(mine - now);
-        float add = s.y * f;
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
-        const float keep = ref == -INFINITY ? 0.f : exp2_fast(ref - now);
-        den = fmaf(den, keep, add);
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) sum[e] *= keep;
-        ref = now;
-#pragma unroll 8
-        for (int w = 0; w < n; ++w) {
-          const float* o = slot(base + w) + row * D + lane * kPer;
-          const float fw = __shfl_sync(0xffffffffu, f, w);
-          if constexpr (kPer == 4) {
-            const float4 u = *reinterpret_cast<const float4*>(o);
-            sum[0] = fmaf(u.x, fw, sum[0]), sum[1] = fmaf(u.y, fw, sum[1]);
-            sum[2] = fmaf(u.z, fw, sum[2]), sum[3] = fmaf(u.w, fw, sum[3]);
-          } else {
-            const float2 u = *reinterpret_cast<const float2*>(o);
-            sum[0] = fmaf(u.x, fw, sum[0]), sum[1] = fmaf(u.y, fw, sum[1]);
-          }
-        }
-      }
-      const float inv = den != 0.f ? 1.f / den : 0.f;
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) sum[e] *= inv;
-    }
-    if constexpr (kPer == 4) {
-      store_out4<F16>(a, to, sum[0], sum[1], sum[2], sum[3]);
-    } else if (a.out_f32) {
-      *reinterpret_cast<float2*>(static_cast<float*>(a.out) + to) = make_float2(sum[0], sum[1]);
+      if (pieces.n == 1) continue;  // one CTA had the whole block
+      join_row<D, 1, 16>(pieces, slot_rows, r - block * kBlock, sum);
     } else {
-      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + to) =
-          static_cast<uint32_t>(to16<F16>(sum[0])) | static_cast<uint32_t>(to16<F16>(sum[1])) << 16;
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) sum[e] = 0.f;
     }
+    store_row<D, F16>(a, ((static_cast<int64_t>(seq) * a.q_len + i) * a.n_q_heads + head * share + r - i * share) * D, sum);
   }
 }
 
