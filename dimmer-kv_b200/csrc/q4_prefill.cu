@@ -3,26 +3,26 @@
 //
 // Bound by the exponentials and the two products, which are about even: a tile of 128 rows x 128 tokens takes 1024
 // cycles of the SM's exponential units and, at head_dim 128, 2 x 512 of its tensor core. Everything else has to hide
-// behind these: a CTA has two tiles of 128 query rows (the rows of a KV head's query heads, token after token), so
-// that one is in the tensor core while the other is in its softmax, and both use the same unpacked keys and values.
+// behind these: a CTA has two tiles of 128 query rows (the rows of a KV head's query heads, token after token), which
+// use the same unpacked keys and values, and two buffers of scores for each: a step is one page, 64 tokens, and a tile's
+// next scores are made while the softmax of the last is under way, so that neither waits for the other's latency.
 //
 //   warps 0-3, 4-7   softmax of the first and the second tile, one row per thread: scores from TMEM, probabilities
 //                    back into TMEM (over the scores they come from), where the second product takes them
-//   warps 8-11       unpack the keys of 128 tokens (two pages), one token per thread, into a float16 tile with the
-//                    128-byte swizzle
+//   warps 8-11       unpack the keys of a page, two threads per token, into a float16 tile with the 128-byte swizzle
 //   warps 12-15      the same for the values, which become the rows of the second product's contraction
-//   warp 16, 17      issue the products (per step P V of a tile, then at once the next Q K of it), and the copies of
-//                    the pages
+//   warps 16, 17     issue the products of a tile each (per step the next Q K, then P V)
+//   warp 18          issues the copies of the pages
 //
-// TMEM: two score tiles, two outputs, 512 columns. The rows' references (running maxima) lag by up to 2^8, so that
-// outputs are scaled down in TMEM only when a row's maximum has grown past that; a score tile that is complete means
-// that the product issued before it is too, so nothing else has to be waited for.
+// TMEM: two score buffers of 64 columns and an output per tile, 512 columns. The rows' references (running maxima) lag by
+// up to 2^8, so that outputs are scaled down in TMEM (once the products on them are complete) only when a row's maximum
+// has grown past that.
 //
 // Keys and values are rounded to float16 (2^-11 at most of each), probabilities likewise. For float16 caches, whose
 // outputs show that, what the rounding of keys lacks forms a second tile, and what that of probabilities lacks a second
 // operand beside the first (each 32 columns of scores become 16 of either), that go through second products.
 //
-// The 128-token steps of all (conversation, KV head, 256-row block) units form one line that is cut evenly over one CTA per
+// The steps of all (conversation, KV head, 256-row block) units form one line that is cut evenly over one CTA per
 // SM; blocks that several CTAs share leave partial results in the workspace, which q4_prefill_combine_kernel joins.
 #include "q4_attend.cuh"
 
@@ -30,14 +30,14 @@ namespace dkv {
 namespace q4 {
 namespace {
 
-constexpr int kStep = 128;           // tokens of a step: two pages
+constexpr int kStep = kPage;         // tokens of a step
 constexpr int kRows = 128;           // query rows of a tile
 constexpr int kBlock = 2 * kRows;    // of a unit
 constexpr int kSoftWarps = 8;
 
 constexpr int kUnpackWarps = 4;  // of the keys, and of the values
 constexpr int kKeyWarp = kSoftWarps, kValueWarp = kKeyWarp + kUnpackWarps, kMmaWarp = kValueWarp + kUnpackWarps,
-              kCopyWarp = kMmaWarp + 1;
+              kCopyWarp = kMmaWarp + 2;
 constexpr int kThreads = (kMmaWarp + 4) * 32;  // whole warpgroups: registers are dealt to these
 // Registers per thread: 96 at launch (5 warpgroups, 480 in all), then 2 x 128 + 2 x 72 + 80 = 480.
 constexpr int kSoftRegs = 128, kUnpackRegs = 72, kIssueRegs = 80;
@@ -45,16 +45,16 @@ constexpr int kSoftRegs = 128, kUnpackRegs = 72, kIssueRegs = 80;
 template <int D, bool F16>
 struct Shared {
   using C = Cells<D>;
-  static constexpr int kPart = kStep * 128;           // 128 rows of 64 dimensions in float16
-  static constexpr int kTile = D / 64 * kPart;
-  static constexpr int kRawStages = F16 ? 1 : 2;
+  static constexpr int kQPart = kRows * 128, kPart = kStep * 128;  // 64 dimensions of 128 rows, of 64 tokens, in float16
+  static constexpr int kQTile = D / 64 * kQPart, kTile = D / 64 * kPart;
+  static constexpr int kRawStages = 4, kStages = 2;
   static constexpr int kQ = 0;                        // two tiles
-  static constexpr int kK = kQ + 2 * kTile;
-  static constexpr int kV = kK + kTile;               // two stages: values wait for the whole of a step
-  static constexpr int kKLow = kV + 2 * kTile;        // what the rounding of keys lacks (float16 caches)
-  static constexpr int kRaw = kKLow + (F16 ? kTile : 0);
-  static constexpr int kBars = kRaw + kRawStages * 2 * C::kBytes;
-  static constexpr int kNumBars = 2 * kRawStages + 6 + 2 * 4 + 1;
+  static constexpr int kK = kQ + 2 * kQTile;          // kStages of each
+  static constexpr int kV = kK + kStages * kTile;
+  static constexpr int kKLow = kV + kStages * kTile;  // what the rounding of keys lacks (float16 caches)
+  static constexpr int kRaw = kKLow + (F16 ? kStages * kTile : 0);
+  static constexpr int kBars = kRaw + kRawStages * C::kBytes;
+  static constexpr int kNumBars = 2 * kRawStages + 4 * kStages + 2 + 4 + 4 + 2 + 2 + 2;
   static constexpr int kBytes = kBars + kNumBars * 8 + 16;
   static constexpr int kAlloc = kBytes + 1024;        // the tiles begin on a 1024-byte boundary
 };
@@ -93,6 +93,14 @@ __device__ __forceinline__ void mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uin
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+
+// One lane of a warp whose lanes are together, the same one every time; a branch on it keeps the warp's uniform registers,
+// in which tcgen05 takes its operands, where one on the lane's number moves every operand there again.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t lead;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}\n" : "=r"(lead));
+  return lead != 0;
 }
 
 // ---------------------------------------------------------------- the line of steps
@@ -253,15 +261,16 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
   uint64_t* raw_full = bars;                     // bulk copies of a step's pages
   uint64_t* raw_free = raw_full + S::kRawStages; // unpacked
-  uint64_t* k_full = raw_free + S::kRawStages;
-  uint64_t* v_full = k_full + 1;
-  uint64_t* k_free = v_full + 2;                 // products that read the tile are complete
-  uint64_t* v_free = k_free + 1;
-  uint64_t* q_full = v_free + 2;                 // [2], by tile
-  uint64_t* s_full = q_full + 2;                 // [2] scores complete
-  uint64_t* p_full = s_full + 2;                 // [2] probabilities in TMEM
-  uint64_t* o_full = p_full + 2;                 // [2] a unit's last product complete
-  uint64_t* drain = o_full + 2;
+  uint64_t* k_full = raw_free + S::kRawStages;   // [kStages] each
+  uint64_t* v_full = k_full + S::kStages;
+  uint64_t* k_free = v_full + S::kStages;        // products that read the tile are complete
+  uint64_t* v_free = k_free + S::kStages;
+  uint64_t* q_full = v_free + S::kStages;        // [2], by tile
+  uint64_t* s_full = q_full + 2;                 // [tile][buffer]: scores complete
+  uint64_t* p_full = s_full + 4;                 // [tile][buffer]: probabilities in TMEM
+  uint64_t* o_done = p_full + 4;                 // [tile]: a step's product on the output complete
+  uint64_t* o_full = o_done + 2;                 // [tile]: a unit's output complete
+  uint64_t* drain = o_full + 2;                  // [tile]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + S::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -272,17 +281,22 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
       mbar_init(&raw_full[i], 1);
       mbar_init(&raw_free[i], 2 * kUnpackWarps);
     }
-    mbar_init(k_full, kUnpackWarps);
-    mbar_init(k_free, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(&k_full[i], kUnpackWarps);
       mbar_init(&v_full[i], kUnpackWarps);
-      mbar_init(&v_free[i], 1);
+      mbar_init(&k_free[i], 2);
+      mbar_init(&v_free[i], 2);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 4);
+      mbar_init(&o_done[i], 1);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&drain[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
-      mbar_init(&o_full[i], 1);
     }
-    mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -299,7 +313,7 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
     begin = deal.begin(blockIdx.x);
     end = deal.begin(blockIdx.x + 1);
   }
-  // scores of tile i: columns 128 i .. (its probabilities in the first 64 of them); outputs: columns 256 + 128 i ..
+  // scores of tile i, buffer b: columns 128 i + 64 b .. (its probabilities in their place); outputs: columns 256 + 128 i ..
   if (begin < end) {
     // Every warp of the warpgroups gives or takes its registers at the head of its role (the compiler allots the roles'
     // code by that), the two without a role as well.
@@ -309,8 +323,8 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
       // ------------------------------------------------------------ softmax
       const int tile = warp >> 2, row_in_tile = (warp & 3) * 32 + lane;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-      const uint32_t s_at = tmem + lanes + tile * 128, o_at = tmem + lanes + 256 + tile * 128;
-      uint32_t s_iter = 0, units = 0;
+      const uint32_t o_at = tmem + lanes + 256 + tile * 128;
+      uint32_t count = 0, units = 0;  // this tile's steps and units so far
       bool ok = true;
       int64_t place = begin;
       while (ok && walk.next()) {
@@ -348,7 +362,7 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = from16<F16>(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)))) * f;
-            *reinterpret_cast<uint4*>(smem + S::kQ + tile * S::kTile + (c >> 3) * S::kPart + sw128_offset(row_in_tile, c & 7)) =
+            *reinterpret_cast<uint4*>(smem + S::kQ + tile * S::kQTile + (c >> 3) * S::kQPart + sw128_offset(row_in_tile, c & 7)) =
                 make_uint4(pack_half2(x[0], x[4]), pack_half2(x[1], x[5]), pack_half2(x[2], x[6]), pack_half2(x[3], x[7]));
           }
           fence_async_shared();
@@ -361,9 +375,10 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
         float ref = 0.f;
         uint64_t l2 = 0;     // two sums, of the even and the odd tokens
         bool known = false;  // the row has a reference
-        for (int t = walk.first; t < walk.last; ++t) {
-          ok = warp_wait(&s_full[tile], s_iter & 1, a.status, kSiteQ4Attend + kErrWaitAccum, abort_flag);
-          ++s_iter;
+        for (int t = walk.first; t < walk.last && ok; ++t, ++count) {
+          const int bar = tile * 2 + (count & 1);
+          const uint32_t s_at = tmem + lanes + bar * 64;
+          ok = warp_wait(&s_full[bar], (count >> 1) & 1, a.status, kSiteQ4Attend + kErrWaitAccum, abort_flag);
           if (!ok) break;
           tc_fence_after();
           const int base = t * kStep;
@@ -403,6 +418,9 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
 #pragma unroll
               for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) - up);
               if (t > walk.first) {
+                // these scores came after the product of the step before the last, so one phase at most is open
+                ok = ok && warp_wait(&o_done[tile], (count - 1) & 1, a.status, kSiteQ4Attend + kErrWaitAccum, abort_flag);
+                tc_fence_after();
 #pragma unroll 1
                 for (int k = 0; k < D / 16; ++k) {
                   uint32_t x[16];
@@ -444,11 +462,10 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[tile]);
+          if (lane == 0) mbar_arrive(&p_full[bar]);
         }
         if (!ok) break;
-        ok = warp_wait(&o_full[tile], units & 1, a.status, kSiteQ4Attend + kErrWaitAccum, abort_flag);
-        ++units;
+        ok = warp_wait(&o_full[tile], units++ & 1, a.status, kSiteQ4Attend + kErrWaitAccum, abort_flag);
         if (!ok) break;
         tc_fence_after();
         const float l = f32x2_sum(l2);
@@ -460,7 +477,7 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
         const unsigned reals = __ballot_sync(0xffffffffu, real);
         // 32 dimensions of the warp's 32 rows at a time through shared memory (the tile's queries are done with), so that
         // eight lanes write a row's 128 bytes
-        float* box = reinterpret_cast<float*>(smem + S::kQ + tile * S::kTile) + (warp & 3) * 1024;
+        float* box = reinterpret_cast<float*>(smem + S::kQ + tile * S::kQTile) + (warp & 3) * 1024;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t x[32];
@@ -498,22 +515,20 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
       setmaxnreg_dec<kUnpackRegs>();
       Walk walk(a, share, begin, end);
       const bool values = warp >= kValueWarp;
-      const int token = threadIdx.x % kStep;  // of the step
-      const int r = token % kPage;
+      const int r = threadIdx.x % kStep, half = (threadIdx.x / kStep) & 1;  // the token of the page, which half of it
       uint32_t iter = 0;
       bool ok = true;
       while (ok && walk.next()) {
         const int seen = seen_by(walk.q, walk.block, share);
         for (int t = walk.first; t < walk.last; ++t, ++iter) {
-          const uint32_t stage = iter % S::kRawStages;
-          ok = warp_wait(&raw_full[stage], (iter / S::kRawStages) & 1, a.status, kSiteQ4Attend + kErrWaitCodes, abort_flag) &&
-               (values ? iter < 2 || warp_wait(&v_free[iter & 1], ((iter >> 1) - 1) & 1, a.status,
-                                               kSiteQ4Attend + kErrWaitEmpty, abort_flag)
-                       : iter == 0 || warp_wait(k_free, (iter - 1) & 1, a.status, kSiteQ4Attend + kErrWaitEmpty, abort_flag));
+          const uint32_t raw = iter % S::kRawStages, stage = iter % S::kStages, turn = iter / S::kStages;
+          ok = warp_wait(&raw_full[raw], (iter / S::kRawStages) & 1, a.status, kSiteQ4Attend + kErrWaitCodes, abort_flag) &&
+               (turn == 0 || warp_wait(values ? &v_free[stage] : &k_free[stage], (turn - 1) & 1, a.status,
+                                       kSiteQ4Attend + kErrWaitEmpty, abort_flag));
           if (!ok) break;
-          const uint8_t* page = smem + S::kRaw + (stage * 2 + token / kPage) * C::kBytes;
+          const uint8_t* page = smem + S::kRaw + raw * C::kBytes;
           // a token that no row sees may never have been written: zeros, no NaN of its
-          const bool there = t * kStep + token < seen;
+          const bool there = t * kStep + r < seen;
           __half2 scale[kGroups], low[kGroups];
 #pragma unroll
           for (int gr = 0; gr < kGroups; ++gr) {
@@ -523,10 +538,10 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
             low[gr] = __high2half2(h);
           }
           if (!values) {
-            // the token's four pieces, in an order that keeps the lanes on different banks
+            // two of the token's four pieces, in an order that keeps the lanes on different banks
 #pragma unroll 2
-            for (int k = 0; k < 4; ++k) {
-              const int piece = (k + (D == 128 ? r >> 1 : r >> 2)) & 3;
+            for (int k = 0; k < 2; ++k) {
+              const int piece = (k + 2 * half + (D == 128 ? r >> 1 : r >> 2)) & 3;
               uint32_t w[D / 32];
               const uint8_t* src = page + C::kKeyCodes + r * (D / 2) + piece * (D / 8);
               if constexpr (D == 128) {
@@ -540,15 +555,16 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
               for (int e = 0; e < D / 32; ++e) {
                 uint4 lack;
                 const uint4 x = unpack8<F16>(w[e], scale[e >> 1], low[e >> 1], lack);
-                const uint32_t to = (e >> 1) * S::kPart + sw128_offset(token, piece * 2 + (e & 1));
+                const uint32_t to = stage * S::kTile + (e >> 1) * S::kPart + sw128_offset(r, piece * 2 + (e & 1));
                 *reinterpret_cast<uint4*>(smem + S::kK + to) = x;
                 if constexpr (F16) *reinterpret_cast<uint4*>(smem + S::kKLow + to) = lack;
               }
             }
           } else {
-            // the pair's eight pieces, this token's halves of them
-#pragma unroll 4
-            for (int g = 0; g < 8; ++g) {
+            // four of the pair's eight pieces, this token's halves of them
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int g = 4 * half + k;
               uint32_t w[D / 32];
               const uint8_t* src = page + C::value_piece(r >> 1, g);
               if constexpr (D == 128) {
@@ -561,7 +577,7 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
 #pragma unroll
               for (int gr = 0; gr < kGroups; ++gr) {
                 uint4 none;
-                *reinterpret_cast<uint4*>(smem + S::kV + (iter & 1) * S::kTile + gr * S::kPart + sw128_offset(token, g)) =
+                *reinterpret_cast<uint4*>(smem + S::kV + stage * S::kTile + gr * S::kPart + sw128_offset(r, g)) =
                     unpack8<false>(__byte_perm(w[2 * gr], w[2 * gr + 1], r & 1 ? 0x7632 : 0x5410), scale[gr], low[gr], none);
               }
             }
@@ -569,8 +585,8 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
           fence_async_shared();
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(values ? &v_full[iter & 1] : k_full);
-            mbar_arrive(&raw_free[stage]);
+            mbar_arrive(values ? &v_full[stage] : &k_full[stage]);
+            mbar_arrive(&raw_free[raw]);
           }
         }
       }
@@ -586,27 +602,24 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
         const int n_pages = pages_of(seen_by(walk.q, walk.block, share));
         const int32_t* table = a.blocks + static_cast<int64_t>(walk.seq) * a.max_blocks;
         const uint8_t* cells = a.cells + static_cast<int64_t>(walk.head) * C::kBytes;
-        int ids = 0, ids_at = 2 * walk.first - 32;
+        int ids = 0, ids_at = walk.first - 32;
         for (int t = walk.first; t < walk.last && ok; ++t, ++issued) {
-          if (2 * t >= ids_at + 32) {  // the next 32 pages' places, one per lane
-            ids_at = 2 * t;
-            ids = ids_at + lane < n_pages ? table[ids_at + lane] : 0;
+          if (t >= ids_at + 32) {  // the next 32 pages' places, one per lane
+            ids_at = t;
+            ids = t + lane < n_pages ? table[t + lane] : 0;
             if (static_cast<unsigned>(ids) >= static_cast<unsigned>(a.n_pages)) {
               record_error(a.status, kSiteQ4Attend + kErrBadDescriptor);
               ids = 0;  // recorded, and a page that exists read in its place
             }
           }
-          const int id0 = __shfl_sync(0xffffffffu, ids, 2 * t - ids_at), id1 = __shfl_sync(0xffffffffu, ids, 2 * t + 1 - ids_at);
-          const uint32_t stage = issued % S::kRawStages;
+          const int id = __shfl_sync(0xffffffffu, ids, t - ids_at);
+          const uint32_t raw = issued % S::kRawStages;
           if (issued >= S::kRawStages)
-            ok = warp_wait(&raw_free[stage], ((issued / S::kRawStages) - 1) & 1, a.status, kSiteQ4Attend + kErrWaitEmpty, abort_flag);
+            ok = warp_wait(&raw_free[raw], ((issued / S::kRawStages) - 1) & 1, a.status, kSiteQ4Attend + kErrWaitEmpty, abort_flag);
           if (!ok) break;
           if (lane == 0) {
-            const bool both = 2 * t + 1 < n_pages;
-            uint8_t* to = smem + S::kRaw + stage * 2 * C::kBytes;
-            mbar_arrive_expect_tx(&raw_full[stage], (both ? 2 : 1) * C::kBytes);
-            bulk_load(to, cells + id0 * page_stride, C::kBytes, &raw_full[stage]);
-            if (both) bulk_load(to + C::kBytes, cells + id1 * page_stride, C::kBytes, &raw_full[stage]);
+            mbar_arrive_expect_tx(&raw_full[raw], C::kBytes);
+            bulk_load(smem + S::kRaw + raw * C::kBytes, cells + id * page_stride, C::kBytes, &raw_full[raw]);
           }
           __syncwarp();
         }
@@ -623,93 +636,73 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
       // ------------------------------------------------------------ products
       constexpr uint32_t kQk = idesc_f16(kRows, kStep, false, false, false);
       constexpr uint32_t kPv = idesc_f16(kRows, D, false, false, true);
-      const uint32_t k_at = smem_u32(smem + S::kK), v_at = smem_u32(smem + S::kV);
-      uint32_t iter = 0, p_iter[2] = {0, 0}, units[2] = {0, 0};
+      const int tile = warp - kMmaWarp;
+      const uint32_t q_at = smem_u32(smem + S::kQ + tile * S::kQTile), k_at = smem_u32(smem + S::kK), v_at = smem_u32(smem + S::kV);
+      const uint32_t s_at = __shfl_sync(0xffffffffu, tmem, 0) + tile * 128, o_at = s_at + 256;
+      uint32_t iter = 0, made = 0, used = 0, units = 0;  // steps, of them with scores made, probabilities used
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity, int err) {
         ok = ok && warp_wait(bar, parity, a.status, kSiteQ4Attend + err, abort_flag);
         return ok;
       };
-      // A step of 16 dimensions is 32 bytes further in a row, one of 64 the next part; 16 tokens are 2048 bytes further.
-      auto scores = [&](int tile) {  // Q K of the tile
-        if (lane == 0) {
-          const uint32_t q_at = smem_u32(smem + S::kQ + tile * S::kTile);
-          uint32_t on = 0;
-#pragma unroll 1
-          for (int part = 0; part < (F16 ? 2 : 1); ++part)
-#pragma unroll 1
-            for (int gr = 0; gr < kGroups; ++gr) {
-              const uint64_t q_desc = smem_desc_sw128(q_at + gr * S::kPart, 16, 1024);
-              const uint64_t k_desc = smem_desc_sw128(k_at + (part ? S::kKLow - S::kK : 0) + gr * S::kPart, 16, 1024);
+      // Q K of step `step` (a dimension step of 16 is 32 bytes further in a row, one of 64 the next part). A buffer is free
+      // once the product on its probabilities is issued: a warp's products complete in order.
+      auto scores = [&](uint32_t step, bool mine) {
+        const uint32_t stage = step % S::kStages;
+        if (!wait(&k_full[stage], (step / S::kStages) & 1, kErrWaitA)) return;
+        tc_fence_after();
+        const uint32_t bar = made & 1;
+        const uint64_t q_desc = smem_desc_sw128(q_at, 16, 1024), k_desc = smem_desc_sw128(k_at + stage * S::kTile, 16, 1024);
+        if (elect_lane()) {
+          if (mine) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                mma_f16(tmem + tile * 128, q_desc + 2 * k, k_desc + 2 * k, kQk, on);
-                on = 1;
-              }
+            for (int k = 0; k < (F16 ? 2 : 1) * D / 16; ++k) {
+              const int part = k / (D / 16), gr = k / 4 % kGroups, at = 2 * (k % 4);
+              mma_f16(s_at + bar * 64, q_desc + gr * (S::kQPart / 16) + at,
+                      k_desc + part * ((S::kKLow - S::kK) / 16) + gr * (S::kPart / 16) + at, kQk, k > 0);
             }
-          mma_commit(&s_full[tile]);
-        }
-        __syncwarp();
-      };
-      auto outputs = [&](int tile, bool first, uint32_t stage) {  // P V of the tile
-        if (lane == 0) {
-          uint32_t on = first ? 0u : 1u;
-#pragma unroll 1
-          for (int part = 0; part < (F16 ? 2 : 1); ++part) {
-            const uint32_t p_at = tmem + tile * 128 + part * 16;
-            const uint64_t v_desc = smem_desc_sw128(v_at + stage * S::kTile, S::kPart, 1024);
-#pragma unroll
-            for (int k = 0; k < kStep / 16; ++k) {
-              mma_f16_ta(tmem + 256 + tile * 128, p_at + (k >> 1) * 32 + (k & 1) * 8, v_desc + 128 * k, kPv, on);
-              on = 1;
-            }
+            mma_commit(&s_full[tile * 2 + bar]);
           }
+          mma_commit(&k_free[stage]);
         }
         __syncwarp();
-      };
-      auto commit = [&](uint64_t* bar) {
-        if (lane == 0) mma_commit(bar);
-        __syncwarp();
+        made += mine;
       };
       bool more = walk.next();
       while (ok && more) {
-        const bool two = walk.two();
-        const int n = walk.last - walk.first;
-        // the unit's first scores
-        if (!wait(k_full, iter & 1, kErrWaitA)) break;
-        for (int tile = 0; tile < (two ? 2 : 1); ++tile) {
-          if (!wait(&q_full[tile], units[tile] & 1, kErrWaitA)) break;
-          tc_fence_after();
-          scores(tile);
-        }
-        if (!ok) break;
-        commit(k_free);
+        const bool mine = tile == 0 || walk.two();
+        const int n = __shfl_sync(0xffffffffu, walk.last - walk.first, 0);
+        if (mine) wait(&q_full[tile], units++ & 1, kErrWaitA);
+        if (ok) scores(iter, mine);
         for (int t = 0; t < n && ok; ++t, ++iter) {
-          for (int tile = 0; tile < (two ? 2 : 1); ++tile) {
-            if (!wait(&p_full[tile], p_iter[tile] & 1, kErrWaitA)) break;
-            ++p_iter[tile];
-            if (tile == 0 && !wait(&v_full[iter & 1], (iter >> 1) & 1, kErrWaitA)) break;
-            tc_fence_after();
-            outputs(tile, t == 0, iter & 1);
-            if (tile == (two ? 1 : 0)) commit(&v_free[iter & 1]);
-            if (t + 1 == n) {
-              commit(&o_full[tile]);
-              ++units[tile];
-            } else {
-              if (tile == 0 && !wait(k_full, (iter + 1) & 1, kErrWaitA)) break;
-              tc_fence_after();
-              scores(tile);
+          if (t + 1 < n) scores(iter + 1, mine);
+          const uint32_t stage = iter % S::kStages, bar = used & 1;
+          if (mine && !wait(&p_full[tile * 2 + bar], (used >> 1) & 1, kErrWaitA)) break;
+          if (!wait(&v_full[stage], (iter / S::kStages) & 1, kErrWaitA)) break;
+          tc_fence_after();
+          const uint64_t v_desc = smem_desc_sw128(v_at + stage * S::kTile, S::kPart, 1024);
+          if (elect_lane()) {
+            if (mine) {  // P V; 16 tokens are 2048 bytes further
+#pragma unroll
+              for (int k = 0; k < (F16 ? 2 : 1) * kStep / 16; ++k) {
+                const int part = k / (kStep / 16), at = k % (kStep / 16);
+                mma_f16_ta(o_at, s_at + bar * 64 + part * 16 + (at >> 1) * 32 + (at & 1) * 8, v_desc + 128 * at, kPv, t > 0 || k > 0);
+              }
+              mma_commit(&o_done[tile]);
+              if (t + 1 == n) mma_commit(&o_full[tile]);
             }
+            mma_commit(&v_free[stage]);
           }
-          if (!ok) break;
-          if (t + 1 < n) commit(k_free);
+          __syncwarp();
+          used += mine;
         }
         more = walk.next();
       }
       if (!ok) *abort_flag = 1;
       // Every product is complete before TMEM is given back.
-      commit(drain);
-      warp_wait(drain, 0, a.status, kSiteQ4Attend + kErrWaitDrain, nullptr);
+      if (elect_lane()) mma_commit(&drain[tile]);
+      __syncwarp();
+      warp_wait(&drain[tile], 0, a.status, kSiteQ4Attend + kErrWaitDrain, nullptr);
     }
   }
   __syncwarp();
