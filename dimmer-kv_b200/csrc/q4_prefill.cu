@@ -9,8 +9,8 @@
 //
 //   warps 0-3, 4-7   softmax of the first and the second tile, one row per thread: scores from TMEM, probabilities
 //                    back into TMEM (over the scores they come from), where the second product takes them
-//   warps 8-11       unpack the keys of a page, two threads per token, into a float16 tile with the 128-byte swizzle
-//   warps 12-15      the same for the values, which become the rows of the second product's contraction
+//   warps 8-15       unpack a page, four threads per token: the keys into a float16 tile with the 128-byte swizzle, the
+//                    values into one whose rows are those of the second product's contraction
 //   warps 16, 17     issue the products of a tile each (per step the next Q K, then P V)
 //   warp 18          issues the copies of the pages
 //
@@ -35,9 +35,8 @@ constexpr int kRows = 128;           // query rows of a tile
 constexpr int kBlock = 2 * kRows;    // of a unit
 constexpr int kSoftWarps = 8;
 
-constexpr int kUnpackWarps = 4;  // of the keys, and of the values
-constexpr int kKeyWarp = kSoftWarps, kValueWarp = kKeyWarp + kUnpackWarps, kMmaWarp = kValueWarp + kUnpackWarps,
-              kCopyWarp = kMmaWarp + 2;
+constexpr int kUnpackWarps = 8;
+constexpr int kMmaWarp = kSoftWarps + kUnpackWarps, kCopyWarp = kMmaWarp + 2;
 constexpr int kThreads = (kMmaWarp + 4) * 32;  // whole warpgroups: registers are dealt to these
 // Registers per thread: 96 at launch (5 warpgroups, 480 in all), then 2 x 128 + 2 x 72 + 80 = 480.
 constexpr int kSoftRegs = 128, kUnpackRegs = 72, kIssueRegs = 80;
@@ -148,6 +147,53 @@ __device__ __forceinline__ int64_t count_steps(const dkv_q4_attend_args& a, int 
   return total;
 }
 
+// Where a CTA's piece of the line begins and ends, and the step of `begin`.
+struct Start {
+  int64_t begin, end;
+  Seq q;
+  int seq, head, block, first;
+};
+// One warp, all lanes alike: 64-bit divisions and two rounds of loads, of which every role's warp would take its share of
+// the SM's time.
+__device__ __forceinline__ Start find_start(const dkv_q4_attend_args& a, int share, int workers) {
+  const int lane = threadIdx.x & 31;
+  auto steps_at = [&](int s) { return s < a.n_seq ? seq_steps(seq_of(a, s, share), share) * a.n_kv_heads : 0; };
+  const int64_t own0 = steps_at(lane);  // the first 32 conversations'
+  int64_t total = warp_sum64(own0);
+  for (int base = 32; base < a.n_seq; base += 32) total += warp_sum64(steps_at(base + lane));
+  const DealOf<false> deal(total, workers);
+  Start at = {};
+  if (static_cast<int>(blockIdx.x) >= deal.workers) return at;
+  at.begin = deal.begin(blockIdx.x);
+  at.end = deal.begin(blockIdx.x + 1);
+  int64_t line = 0;
+  for (int base = 0; base < a.n_seq; base += 32) {  // the conversation of `begin`
+    const int64_t own = base == 0 ? own0 : steps_at(base + lane);
+    int64_t incl = own;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += y;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, line + incl > at.begin);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      at.seq = base + l;
+      at.q = seq_of(a, at.seq, share);
+      int64_t rest = at.begin - line - __shfl_sync(0xffffffffu, incl - own, l);
+      const int64_t per_head = seq_steps(at.q, share);
+      at.head = static_cast<int>(divide<false>(rest, per_head));
+      rest -= at.head * per_head;
+      while (rest >= steps_of(at.q, at.block, share)) rest -= steps_of(at.q, at.block++, share);
+      at.first = static_cast<int>(rest);
+      return at;
+    }
+    line += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  at.end = at.begin;  // not reached: begin lies on the line
+  return at;
+}
+
 // A CTA's piece of the line, unit by unit. Every warp goes through it on its own (all lanes alike).
 struct Walk {
   const dkv_q4_attend_args& a;
@@ -158,43 +204,9 @@ struct Walk {
   int first, last, steps;  // this unit's steps [first, last) of `steps`
   bool opened;
 
-  __device__ __forceinline__ Walk(const dkv_q4_attend_args& a_, int share_, int64_t begin_, int64_t end_)
-      : a(a_), share(share_), at(begin_), end(end_), opened(false) {
-    // the conversation of `begin`
-    const int lane = threadIdx.x & 31;
-    int64_t line = 0;
-    seq = a.n_seq;
-    for (int base = 0; base < a.n_seq; base += 32) {
-      const int s = base + lane;
-      const int64_t own = s < a.n_seq ? seq_steps(seq_of(a, s, share), share) * a.n_kv_heads : 0;
-      int64_t incl = own;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += y;
-      }
-      const unsigned past = __ballot_sync(0xffffffffu, line + incl > at);
-      if (past) {
-        const int l = __ffs(past) - 1;
-        seq = base + l;
-        line += __shfl_sync(0xffffffffu, incl - own, l);
-        break;
-      }
-      line += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    if (seq >= a.n_seq) {  // not reached: begin lies on the line
-      at = end;
-      return;
-    }
-    q = seq_of(a, seq, share);
-    const int64_t per_head = seq_steps(q, share);
-    int64_t rest = at - line;
-    head = static_cast<int>(divide<false>(rest, per_head));
-    rest -= head * per_head;
-    block = 0;
-    while (rest >= steps_of(q, block, share)) rest -= steps_of(q, block++, share);
-    first = static_cast<int>(rest);
-  }
+  __device__ __forceinline__ Walk(const dkv_q4_attend_args& a_, int share_, const Start& s)
+      : a(a_), share(share_), at(s.begin), end(s.end), q(s.q), seq(s.seq), head(s.head), block(s.block), first(s.first),
+        opened(false) {}
   // The next unit; false behind the last.
   __device__ __forceinline__ bool next() {
     if (opened) {
@@ -222,6 +234,15 @@ struct Walk {
 };
 
 // ---------------------------------------------------------------- unpacking
+__device__ __forceinline__ uint64_t wide2(__half2 h) {
+  const float2 f = __half22float2(h);
+  return f32x2_pack(__float_as_uint(f.x), __float_as_uint(f.y));
+}
+// What the float16 pair h lacks to x.
+__device__ __forceinline__ uint32_t lack2(uint64_t x, __half2 h) {
+  const uint64_t d = fma_f32x2(wide2(h), f32x2_pack(0xbf800000u, 0xbf800000u), x);
+  return pack_half2(__uint_as_float(static_cast<uint32_t>(d)), __uint_as_float(static_cast<uint32_t>(d >> 32)));
+}
 // Eight codes (nibbles of w) to eight float16 values scale * c + low in the order 0 4 1 5 2 6 3 7, each rounded once; with
 // LOW also what the rounding lacks.
 template <bool LOW>
@@ -237,10 +258,10 @@ __device__ __forceinline__ uint4 unpack8(uint32_t w, __half2 scale, __half2 low,
     v[2 * b] = as_u32(x);
     v[2 * b + 1] = as_u32(y);
     if constexpr (LOW) {
-      const float s = __low2float(scale), l = __low2float(low);
-      const float2 e = __half22float2(even), o = __half22float2(odd), xf = __half22float2(x), yf = __half22float2(y);
-      r[2 * b] = pack_half2(fmaf(e.x, s, l) - xf.x, fmaf(e.y, s, l) - xf.y);
-      r[2 * b + 1] = pack_half2(fmaf(o.x, s, l) - yf.x, fmaf(o.y, s, l) - yf.y);
+      const uint32_t s = __float_as_uint(__low2float(scale)), l = __float_as_uint(__low2float(low));
+      const uint64_t s2 = f32x2_pack(s, s), l2 = f32x2_pack(l, l);
+      r[2 * b] = lack2(fma_f32x2(wide2(even), s2, l2), x);
+      r[2 * b + 1] = lack2(fma_f32x2(wide2(odd), s2, l2), y);
     }
   }
   if constexpr (LOW) lack = make_uint4(r[0], r[1], r[2], r[3]);
@@ -276,10 +297,15 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
 
   const int warp = warp_id(), lane = threadIdx.x & 31;
   const int share = a.n_q_heads / a.n_kv_heads;
+  __shared__ Start start;
+  if (warp == 1) {
+    const Start at = find_start(a, share, workers);
+    if (lane == 0) start = at;
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kRawStages; ++i) {
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_free[i], 2 * kUnpackWarps);
+      mbar_init(&raw_free[i], kUnpackWarps);
     }
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&k_full[i], kUnpackWarps);
@@ -306,20 +332,14 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  int64_t unused;
-  const DealOf<false> deal(count_steps(a, share, 0, unused), workers);
-  int64_t begin = 0, end = 0;
-  if (!failed && static_cast<int>(blockIdx.x) < deal.workers) {
-    begin = deal.begin(blockIdx.x);
-    end = deal.begin(blockIdx.x + 1);
-  }
+  const int64_t begin = start.begin, end = failed ? begin : start.end;
   // scores of tile i, buffer b: columns 128 i + 64 b .. (its probabilities in their place); outputs: columns 256 + 128 i ..
   if (begin < end) {
     // Every warp of the warpgroups gives or takes its registers at the head of its role (the compiler allots the roles'
     // code by that), the two without a role as well.
     if (warp < kSoftWarps) {
       setmaxnreg_inc<kSoftRegs>();
-      Walk walk(a, share, begin, end);
+      Walk walk(a, share, start);
       // ------------------------------------------------------------ softmax
       const int tile = warp >> 2, row_in_tile = (warp & 3) * 32 + lane;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -337,33 +357,52 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
         // ---- the row into shared memory, by a power of two that brings its largest element to [2^13, 2^14)
         float factor;
         {
-          const uint16_t* src = static_cast<const uint16_t*>(a.query) + walk.seq * a.q_stride[0] +
-                                (walk.head * share + r - i * share) * a.q_stride[1] + i * a.q_stride[2];
-          uint4 raw[D / 8];  // the row, all of its loads under way at once
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c)
-            raw[c] = real ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u);
-          uint32_t most = 0;
+          // (rows behind the last load the first element's, and count as zeros)
+          const int64_t src =
+              real ? walk.seq * a.q_stride[0] + (walk.head * share + r - i * share) * a.q_stride[1] + i * a.q_stride[2] : 0;
+          const unsigned reals = __ballot_sync(0xffffffffu, real);
+          uint8_t* own = smem + S::kQ + tile * S::kQTile;
+          uint4 raw[D / 8];
+          constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;  // lanes that load a row, rows of a load: all under way at once
 #pragma unroll
           for (int c = 0; c < D / 8; ++c) {
-            const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+            const int from = c * kAtOnce + lane / kLanes;
+            const int64_t at = __shfl_sync(0xffffffffu, src, from);
+            raw[c] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.query) + at + lane % kLanes * 8);
+          }
+          __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) most = extreme2<F16, true>(most, w[e] & 0x7fff7fffu);
+          for (int c = 0; c < D / 8; ++c) {
+            const int from = c * kAtOnce + lane / kLanes, chunk = lane % kLanes;
+            *reinterpret_cast<uint4*>(own + (chunk >> 3) * S::kQPart + sw128_offset(row_in_tile - lane + from, chunk & 7)) =
+                (reals >> from) & 1u ? raw[c] : make_uint4(0u, 0u, 0u, 0u);
+          }
+          __syncwarp();
+          // (rolled: the code runs once per unit, and comes from L2 when it does)
+          uint32_t most = 0;
+#pragma unroll 4
+          for (int c = 0; c < D / 8; ++c) {
+            const uint4 w = *reinterpret_cast<const uint4*>(own + (c >> 3) * S::kQPart + sw128_offset(row_in_tile, c & 7));
+            most = extreme2<F16, true>(most, w.x & 0x7fff7fffu);
+            most = extreme2<F16, true>(most, w.y & 0x7fff7fffu);
+            most = extreme2<F16, true>(most, w.z & 0x7fff7fffu);
+            most = extreme2<F16, true>(most, w.w & 0x7fff7fffu);
           }
           const float big = fmaxf(from16<F16>(static_cast<uint16_t>(most)), from16<F16>(static_cast<uint16_t>(most >> 16)));
           const int ex = (__float_as_uint(big) >> 23) & 255;
-          const float up = __uint_as_float(static_cast<uint32_t>(min(254, max(1, 267 - ex))) << 23);
+          const uint32_t e_up = static_cast<uint32_t>(min(253, max(1, 267 - ex)));
+          const float up = __uint_as_float(e_up << 23), down = __uint_as_float((254u - e_up) << 23);  // 2^n and 2^-n
           // a negative scaling goes into the query, so that the largest product is the largest score
           const float f = a.scaling < 0.f ? -up : up;
-          factor = fabsf(a.scaling) * kLog2e / up;
-#pragma unroll
+          factor = fabsf(a.scaling) * kLog2e * down;
+#pragma unroll 4
           for (int c = 0; c < D / 8; ++c) {
-            const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+            uint4& at = *reinterpret_cast<uint4*>(own + (c >> 3) * S::kQPart + sw128_offset(row_in_tile, c & 7));
+            const uint32_t w[4] = {at.x, at.y, at.z, at.w};
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = from16<F16>(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)))) * f;
-            *reinterpret_cast<uint4*>(smem + S::kQ + tile * S::kQTile + (c >> 3) * S::kQPart + sw128_offset(row_in_tile, c & 7)) =
-                make_uint4(pack_half2(x[0], x[4]), pack_half2(x[1], x[5]), pack_half2(x[2], x[6]), pack_half2(x[3], x[7]));
+            at = make_uint4(pack_half2(x[0], x[4]), pack_half2(x[1], x[5]), pack_half2(x[2], x[6]), pack_half2(x[3], x[7]));
           }
           fence_async_shared();
           __syncwarp();
@@ -383,78 +422,67 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
           tc_fence_after();
           const int base = t * kStep;
           const bool edge = base + kStep > full_below;
-          // 32 scores at a time become 16 columns of probabilities (and 16 of what their rounding lacks) in their place. The
-          // loop stays rolled: five roles share the instruction cache (and with the next scores loaded ahead, the registers
-          // that these take cost as much as the wait for them).
+          uint32_t s[kStep / 32][32];
+#pragma unroll
+          for (int c = 0; c < kStep / 32; ++c) tmem_ld32(s_at + c * 32, s[c]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < kStep / 32; ++c) tmem_fence32(s[c]);
+          if (edge) {
+            const int n = limit - base;
+#pragma unroll
+            for (int e = 0; e < kStep; ++e) s[e / 32][e % 32] = e < n ? s[e / 32][e % 32] : 0xff800000u;  // -infinity; the factor is positive
+          }
+          const uint64_t o2 = f32x2_pack(__float_as_uint(kBias - ref), __float_as_uint(kBias - ref));
+          float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < kStep; e += 2) {
+            uint32_t &s0 = s[e / 32][e % 32], &s1 = s[e / 32][e % 32 + 1];
+            const uint64_t x = fma_f32x2(f32x2_pack(s0, s1), f2, o2);
+            s0 = static_cast<uint32_t>(x);
+            s1 = static_cast<uint32_t>(x >> 32);
+            float& top = tops[e / 2 % 4];
+            top = fmaxf(top, fmaxf(__uint_as_float(s0), __uint_as_float(s1)));
+          }
+          const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+          const bool raise = known ? top > kBias + kSlack : top > -INFINITY;
+          if (__any_sync(0xffffffffu, raise)) {
+            // ---- a row's first tokens set its reference, a maximum beyond the slack moves it: by a whole number, so that
+            // what is scaled down for it (the output so far) loses nothing
+            const float up = raise ? ceilf(top - kBias) : 0.f;
+            const float down = !raise ? 1.f : known ? exp2_fast(-up) : 0.f;
+            ref += up;
+            known = known || raise;
+            l2 = mul_f32x2(l2, f32x2_pack(__float_as_uint(down), __float_as_uint(down)));
+#pragma unroll
+            for (int e = 0; e < kStep; ++e) s[e / 32][e % 32] = __float_as_uint(__uint_as_float(s[e / 32][e % 32]) - up);
+            if (t > walk.first) {
+              // these scores came after the product of the step before the last, so one phase at most is open
+              ok = ok && warp_wait(&o_done[tile], (count - 1) & 1, a.status, kSiteQ4Attend + kErrWaitAccum, abort_flag);
+              tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < kStep / 32; ++c) {
-            uint32_t s[32];
-            tmem_ld32(s_at + c * 32, s);
-            tmem_ld_wait();
-            tmem_fence32(s);
-            if (edge) {
-              const int n = limit - base - c * 32;
-#pragma unroll
-              for (int e = 0; e < 32; ++e) s[e] = e < n ? s[e] : 0xff800000u;  // -infinity; the factor is positive
-            }
-            const uint64_t o2 = f32x2_pack(__float_as_uint(kBias - ref), __float_as_uint(kBias - ref));
-            float top = -INFINITY;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const uint64_t x = fma_f32x2(f32x2_pack(s[2 * e], s[2 * e + 1]), f2, o2);
-              s[2 * e] = static_cast<uint32_t>(x);
-              s[2 * e + 1] = static_cast<uint32_t>(x >> 32);
-              top = fmaxf(top, fmaxf(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])));
-            }
-            const bool raise = known ? top > kBias + kSlack : top > -INFINITY;
-            if (__any_sync(0xffffffffu, raise)) {
-              // ---- a row's first tokens set its reference, a maximum beyond the slack moves it: by a whole number, so that
-              // what is scaled down for it (the output, this step's probabilities so far) loses nothing
-              const float up = raise ? ceilf(top - kBias) : 0.f;
-              const float down = !raise ? 1.f : known ? exp2_fast(-up) : 0.f;
-              ref += up;
-              known = known || raise;
-              l2 = mul_f32x2(l2, f32x2_pack(__float_as_uint(down), __float_as_uint(down)));
-#pragma unroll
-              for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) - up);
-              if (t > walk.first) {
-                // these scores came after the product of the step before the last, so one phase at most is open
-                ok = ok && warp_wait(&o_done[tile], (count - 1) & 1, a.status, kSiteQ4Attend + kErrWaitAccum, abort_flag);
-                tc_fence_after();
-#pragma unroll 1
-                for (int k = 0; k < D / 16; ++k) {
-                  uint32_t x[16];
-                  tmem_ld16(o_at + k * 16, x);
-                  tmem_ld_wait();
-                  tmem_reg_fence(x);
-#pragma unroll
-                  for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * down);
-                  tmem_st16(o_at + k * 16, x);
-                }
-              }
-              const __half2 d2 = __float2half2_rn(down);
-#pragma unroll 1
-              for (int k = 0; k < (F16 ? 2 : 1) * c; ++k) {
+              for (int k = 0; k < D / 16; ++k) {
                 uint32_t x[16];
-                const uint32_t at = s_at + (F16 ? k * 16 : k * 32);
-                tmem_ld16(at, x);
+                tmem_ld16(o_at + k * 16, x);
                 tmem_ld_wait();
                 tmem_reg_fence(x);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = as_u32(__hmul2(as_half2(x[e]), d2));
-                tmem_st16(at, x);
+                for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * down);
+                tmem_st16(o_at + k * 16, x);
               }
             }
+          }
+          // 32 scores become 16 columns of probabilities (and 16 of what their rounding lacks) in their place
+#pragma unroll
+          for (int c = 0; c < kStep / 32; ++c) {
             uint32_t p[16], lack[F16 ? 16 : 1];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float e0 = exp2_fast(__uint_as_float(s[2 * e])), e1 = exp2_fast(__uint_as_float(s[2 * e + 1]));
-              l2 = add_f32x2(l2, f32x2_pack(__float_as_uint(e0), __float_as_uint(e1)));
+              const float e0 = exp2_fast(__uint_as_float(s[c][2 * e])), e1 = exp2_fast(__uint_as_float(s[c][2 * e + 1]));
+              const uint64_t both = f32x2_pack(__float_as_uint(e0), __float_as_uint(e1));
+              l2 = add_f32x2(l2, both);
               p[e] = pack_half2(e0, e1);
-              if constexpr (F16) {
-                const float2 back = __half22float2(as_half2(p[e]));
-                lack[e] = pack_half2(e0 - back.x, e1 - back.y);
-              }
+              if constexpr (F16) lack[e] = lack2(both, as_half2(p[e]));
             }
             tmem_st16(s_at + c * 32, p);
             if constexpr (F16) tmem_st16(s_at + c * 32 + 16, lack);
@@ -513,79 +541,74 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
     } else if (warp < kMmaWarp) {
       // ------------------------------------------------------------ unpacking
       setmaxnreg_dec<kUnpackRegs>();
-      Walk walk(a, share, begin, end);
-      const bool values = warp >= kValueWarp;
-      const int r = threadIdx.x % kStep, half = (threadIdx.x / kStep) & 1;  // the token of the page, which half of it
+      Walk walk(a, share, start);
+      const int r = threadIdx.x % kStep, part = (threadIdx.x / kStep) & 3;  // the token of the page, which quarter of it
       uint32_t iter = 0;
       bool ok = true;
+      auto load = [&](uint32_t (&w)[D / 32], const uint8_t* src) {
+        if constexpr (D == 128) {
+          const uint4 u = *reinterpret_cast<const uint4*>(src);
+          w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2*>(src);
+          w[0] = u.x, w[1] = u.y;
+        }
+      };
+      auto wait = [&](uint64_t* bar, uint32_t parity, int err) {
+        ok = ok && warp_wait(bar, parity, a.status, kSiteQ4Attend + err, abort_flag);
+        return ok;
+      };
       while (ok && walk.next()) {
         const int seen = seen_by(walk.q, walk.block, share);
         for (int t = walk.first; t < walk.last; ++t, ++iter) {
           const uint32_t raw = iter % S::kRawStages, stage = iter % S::kStages, turn = iter / S::kStages;
-          ok = warp_wait(&raw_full[raw], (iter / S::kRawStages) & 1, a.status, kSiteQ4Attend + kErrWaitCodes, abort_flag) &&
-               (turn == 0 || warp_wait(values ? &v_free[stage] : &k_free[stage], (turn - 1) & 1, a.status,
-                                       kSiteQ4Attend + kErrWaitEmpty, abort_flag));
+          wait(&raw_full[raw], (iter / S::kRawStages) & 1, kErrWaitCodes);
+          if (turn > 0) wait(&k_free[stage], (turn - 1) & 1, kErrWaitEmpty);
           if (!ok) break;
           const uint8_t* page = smem + S::kRaw + raw * C::kBytes;
           // a token that no row sees may never have been written: zeros, no NaN of its
           const bool there = t * kStep + r < seen;
-          __half2 scale[kGroups], low[kGroups];
+          auto header = [&](int at) { return as_half2(there ? *reinterpret_cast<const uint32_t*>(page + at) : 0u); };
+          {
+            // one of the token's four pieces, in an order that keeps the lanes on different banks
+            const int piece = (part + (D == 128 ? r >> 1 : r >> 2)) & 3;
+            uint32_t w[D / 32];
+            load(w, page + C::kKeyCodes + r * (D / 2) + piece * (D / 8));
 #pragma unroll
-          for (int gr = 0; gr < kGroups; ++gr) {
-            const __half2 h = as_half2(
-                there ? *reinterpret_cast<const uint32_t*>(page + (values ? C::value_head(r, gr) : C::key_head(r, gr))) : 0u);
-            scale[gr] = __low2half2(h);
-            low[gr] = __high2half2(h);
-          }
-          if (!values) {
-            // two of the token's four pieces, in an order that keeps the lanes on different banks
-#pragma unroll 2
-            for (int k = 0; k < 2; ++k) {
-              const int piece = (k + 2 * half + (D == 128 ? r >> 1 : r >> 2)) & 3;
-              uint32_t w[D / 32];
-              const uint8_t* src = page + C::kKeyCodes + r * (D / 2) + piece * (D / 8);
-              if constexpr (D == 128) {
-                const uint4 u = *reinterpret_cast<const uint4*>(src);
-                w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-              } else {
-                const uint2 u = *reinterpret_cast<const uint2*>(src);
-                w[0] = u.x, w[1] = u.y;
-              }
+            for (int gr = 0; gr < kGroups; ++gr) {
+              const __half2 h = header(C::key_head(r, gr));
 #pragma unroll
-              for (int e = 0; e < D / 32; ++e) {
+              for (int e = 0; e < 2; ++e) {
                 uint4 lack;
-                const uint4 x = unpack8<F16>(w[e], scale[e >> 1], low[e >> 1], lack);
-                const uint32_t to = stage * S::kTile + (e >> 1) * S::kPart + sw128_offset(r, piece * 2 + (e & 1));
+                const uint4 x = unpack8<F16>(w[2 * gr + e], __low2half2(h), __high2half2(h), lack);
+                const uint32_t to = stage * S::kTile + gr * S::kPart + sw128_offset(r, piece * 2 + e);
                 *reinterpret_cast<uint4*>(smem + S::kK + to) = x;
                 if constexpr (F16) *reinterpret_cast<uint4*>(smem + S::kKLow + to) = lack;
               }
             }
-          } else {
-            // four of the pair's eight pieces, this token's halves of them
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&k_full[stage]);
+          }
+          if (turn > 0 && !wait(&v_free[stage], (turn - 1) & 1, kErrWaitEmpty)) break;
+          // two of the pair's eight pieces, this token's halves of them
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int g = 4 * half + k;
-              uint32_t w[D / 32];
-              const uint8_t* src = page + C::value_piece(r >> 1, g);
-              if constexpr (D == 128) {
-                const uint4 u = *reinterpret_cast<const uint4*>(src);
-                w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-              } else {
-                const uint2 u = *reinterpret_cast<const uint2*>(src);
-                w[0] = u.x, w[1] = u.y;
-              }
+          for (int k = 0; k < 2; ++k) {
+            const int g = 2 * part + k;
+            uint32_t w[D / 32];
+            load(w, page + C::value_piece(r >> 1, g));
 #pragma unroll
-              for (int gr = 0; gr < kGroups; ++gr) {
-                uint4 none;
-                *reinterpret_cast<uint4*>(smem + S::kV + stage * S::kTile + gr * S::kPart + sw128_offset(r, g)) =
-                    unpack8<false>(__byte_perm(w[2 * gr], w[2 * gr + 1], r & 1 ? 0x7632 : 0x5410), scale[gr], low[gr], none);
-              }
+            for (int gr = 0; gr < kGroups; ++gr) {
+              const __half2 h = header(C::value_head(r, gr));
+              uint4 none;
+              *reinterpret_cast<uint4*>(smem + S::kV + stage * S::kTile + gr * S::kPart + sw128_offset(r, g)) =
+                  unpack8<false>(__byte_perm(w[2 * gr], w[2 * gr + 1], r & 1 ? 0x7632 : 0x5410), __low2half2(h), __high2half2(h), none);
             }
           }
           fence_async_shared();
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(values ? &v_full[stage] : &k_full[stage]);
+            mbar_arrive(&v_full[stage]);
             mbar_arrive(&raw_free[raw]);
           }
         }
@@ -593,7 +616,7 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
       if (!ok) *abort_flag = 1;
     } else if (warp == kCopyWarp) {
       setmaxnreg_dec<kIssueRegs>();
-      Walk walk(a, share, begin, end);
+      Walk walk(a, share, start);
       // ------------------------------------------------------------ copies of the pages, ahead of the unpacking
       const int64_t page_stride = static_cast<int64_t>(a.n_kv_heads) * C::kBytes;
       uint32_t issued = 0;
@@ -632,7 +655,7 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
       setmaxnreg_dec<kIssueRegs>();
     } else {
       setmaxnreg_dec<kIssueRegs>();
-      Walk walk(a, share, begin, end);
+      Walk walk(a, share, start);
       // ------------------------------------------------------------ products
       constexpr uint32_t kQk = idesc_f16(kRows, kStep, false, false, false);
       constexpr uint32_t kPv = idesc_f16(kRows, D, false, false, true);
