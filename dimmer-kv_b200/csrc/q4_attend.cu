@@ -712,7 +712,7 @@ q4_join_rows_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, in
   const int chunk = row.r / kRows;
   int64_t before;
   const int64_t all = count_pages(a, row.seq, before);
-  Pieces pieces;
+  Pieces pieces = {};
   if (real)
     pieces = Pieces(a, Deal(all * units, workers), before * units + static_cast<int64_t>(row.head * chunks + chunk) * n_pages,
                     n_pages, min(kRows, rows), D);
@@ -756,7 +756,7 @@ q4_join_parts_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, i
   }
   __syncthreads();
   const bool real = tokens > 0 && row.i < min(tokens - a.starts[row.seq], a.q_len);
-  Pieces pieces;
+  Pieces pieces = {};
   if (real)
     pieces = Pieces(a, Deal(line[0] * units, workers), line[1] * units + static_cast<int64_t>(row.head * chunks + chunk) * n_pages,
                     n_pages, rows, D);

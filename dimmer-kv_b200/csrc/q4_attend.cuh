@@ -71,10 +71,10 @@ __host__ __device__ __forceinline__ int64_t slot_floats(int rows, int d) { retur
 // The partial results of one unit: worker w0 + k left the unit's piece in slot(k). The unit is the last segment of w0 unless
 // w0 begins with it (its second slot), and the first segment of the others.
 struct Pieces {
-  const float *first = nullptr, *rest = nullptr;
-  int64_t stride = 0;
-  int n = 0;
-  __device__ __forceinline__ Pieces() {}
+  const float *first, *rest;
+  int64_t stride;
+  int n;
+  Pieces() = default;
   __device__ __forceinline__ Pieces(const dkv_q4_attend_args& a, const Deal& deal, int64_t unit, int places, int rows, int d) {
     const int w0 = deal.owner(unit), w1 = deal.owner(unit + places - 1);
     stride = slot_floats(rows, d);
@@ -128,6 +128,17 @@ __device__ __forceinline__ void join_row(const Pieces& p, int rows, int row, flo
   const float inv = den != 0.f ? 1.f / den : 0.f;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) sum[e] *= inv;
+}
+
+template <int N>
+__device__ __forceinline__ void load_row(const float* at, float (&x)[N]) {
+  if constexpr (N == 4) {
+    const float4 u = *reinterpret_cast<const float4*>(at);
+    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+  } else {
+    const float2 u = *reinterpret_cast<const float2*>(at);
+    x[0] = u.x, x[1] = u.y;
+  }
 }
 
 // A lane's D / 32 dimensions of an output row that begins at `at`.

@@ -134,17 +134,13 @@ __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
   return v;
 }
 
-// One warp: steps of all conversations, and of those before `seq`.
-__device__ __forceinline__ int64_t count_steps(const dkv_q4_attend_args& a, int share, int seq, int64_t& before) {
-  int64_t total = 0;
-  before = 0;
-  for (int base = 0; base < a.n_seq; base += 32) {
-    const int s = base + (threadIdx.x & 31);
-    const int64_t n = s < a.n_seq ? seq_steps(seq_of(a, s, share), share) * a.n_kv_heads : 0;
-    total += warp_sum64(n);
-    before += warp_sum64(s < seq ? n : 0);
-  }
-  return total;
+int slot_rows_of(const dkv_q4_attend_args& a) { return rows_of(a) < kBlock ? rows_of(a) : kBlock; }
+
+// Behind the slots: the slot of a unit's first piece, and the CTA of its last.
+__device__ __forceinline__ int2* unit_record(const dkv_q4_attend_args& a, int workers, int slot_rows, int seq, int head, int block) {
+  const int blocks = (a.q_len * (a.n_q_heads / a.n_kv_heads) + kBlock - 1) / kBlock;
+  return reinterpret_cast<int2*>(a.workspace + 2 * static_cast<int64_t>(workers) * slot_floats(slot_rows, a.head_dim)) +
+         (static_cast<int64_t>(seq) * a.n_kv_heads + head) * blocks + block;
 }
 
 // Where a CTA's piece of the line begins and ends, and the step of `begin`.
@@ -350,6 +346,11 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
       while (ok && walk.next()) {
         const int64_t unit_begin = place;
         place += walk.last - walk.first;
+        if (threadIdx.x == 0) {
+          int2* by = unit_record(a, workers, slot_rows, walk.seq, walk.head, walk.block);
+          if (walk.first == 0) by->x = 2 * blockIdx.x + (unit_begin == begin ? 0 : 1);
+          if (walk.last == walk.steps) by->y = blockIdx.x;
+        }
         if (tile == 1 && !walk.two()) continue;
         const Seq& q = walk.q;
         const int row0 = walk.block * kBlock + tile * kRows, r = row0 + row_in_tile, i = r / share;
@@ -736,44 +737,83 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
 }
 
 // Joins the blocks that several CTAs share and writes the zeros of the rows behind the new tokens: cta_rows (which divides
-// kBlock) rows of one block per CTA, a warp per row.
-constexpr int kCombineWarps = 8;
+// kBlock) rows of one block per CTA. A row of many pieces, as few long contexts leave them, has a warp that takes the pieces'
+// factors in its lanes; of few pieces, a warp takes kAtOnce rows together, with all of their loads under way (4 x 512 rows of
+// 24 heads of 128 in two or three pieces: 25 us one row after another).
+constexpr int kCombineWarps = 8, kAtOnce = 4, kFewPieces = 4;
 template <int D, bool F16>
 __global__ void __launch_bounds__(kCombineWarps * 32)
 q4_prefill_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int slot_rows, int cta_rows) {
-  __shared__ int64_t line[2];
   const int share = a.n_q_heads / a.n_kv_heads;
   const int head = blockIdx.y, seq = blockIdx.z, warp = warp_id(), lane = threadIdx.x & 31;
   const Seq q = seq_of(a, seq, share);
   const int rows = a.q_len * share, r0 = blockIdx.x * cta_rows, block = r0 / kBlock;
-  if (warp == 0) {
-    int64_t before;
-    const int64_t all = count_steps(a, share, seq, before);
-    int64_t unit = before + head * seq_steps(q, share);
-    for (int b = 0; b < min(block, q.blocks); ++b) unit += steps_of(q, b, share);
-    if (lane == 0) line[0] = all, line[1] = unit;
-  }
-  __syncthreads();
-  Pieces pieces;
-  if (r0 < q.rows) pieces = Pieces(a, Deal(line[0], workers), line[1], steps_of(q, block, share), slot_rows, D);
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // what is above does not depend on the main kernel
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const bool failed = cta_failed_at_entry(a.status);
-  for (int k = warp; k < cta_rows; k += kCombineWarps) {
-    const int r = r0 + k, i = r / share;
-    if (r >= rows) break;
-    float sum[D / 32];
-    if (r < q.rows && !failed) {
-      if (pieces.n == 1) continue;  // one CTA had the whole block
+  Pieces pieces = {};
+  if (r0 < q.rows && !failed) {
+    const int2 by = *unit_record(a, workers, slot_rows, seq, head, block);
+    pieces.stride = slot_floats(slot_rows, D);
+    pieces.first = a.workspace + by.x * pieces.stride;
+    pieces.rest = a.workspace + (by.x & ~1) * pieces.stride;
+    pieces.n = by.y - (by.x >> 1) + 1;
+    if (by.x < 0 || by.y >= workers || pieces.n < 1) pieces.n = 0;
+  }
+  constexpr int kPer = D / 32;
+  const int end = min(r0 + cta_rows, rows);  // of the CTA
+  auto place = [&](int r) {
+    const int i = r / share;
+    return ((static_cast<int64_t>(seq) * a.q_len + i) * a.n_q_heads + head * share + r - i * share) * D;
+  };
+  const float zeros[kPer] = {};
+  for (int r = max(r0, failed ? 0 : q.rows) + warp; r < end; r += kCombineWarps) store_row<D, F16>(a, place(r), zeros);
+  if (pieces.n <= 1) return;  // one CTA had the whole block, or it has no row
+  const int last = min(end, q.rows);
+  if (pieces.n > kFewPieces) {
+    for (int r = r0 + warp; r < last; r += kCombineWarps) {
+      float sum[kPer];
       join_row<D, 1, 16>(pieces, slot_rows, r - block * kBlock, sum);
-    } else {
-#pragma unroll
-      for (int e = 0; e < D / 32; ++e) sum[e] = 0.f;
+      store_row<D, F16>(a, place(r), sum);
     }
-    store_row<D, F16>(a, ((static_cast<int64_t>(seq) * a.q_len + i) * a.n_q_heads + head * share + r - i * share) * D, sum);
+    return;
+  }
+  for (int first = r0 + warp * kAtOnce; first < last; first += kCombineWarps * kAtOnce) {
+    float o[kFewPieces][kAtOnce][kPer];
+    float2 s[kFewPieces][kAtOnce];
+#pragma unroll
+    for (int w = 0; w < kFewPieces; ++w)
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const float* slot = pieces.slot(min(w, pieces.n - 1));
+        const int row = min(first + k, last - 1) - block * kBlock;
+        if (w < pieces.n) {
+          load_row<kPer>(slot + row * D + lane * kPer, o[w][k]);
+          s[w][k] = *reinterpret_cast<const float2*>(slot + slot_rows * D + row * 4);
+        } else {
+          for (float& x : o[w][k]) x = 0.f;
+          s[w][k] = make_float2(0.f, 0.f);
+        }
+      }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      float ref = -INFINITY, den = 0.f, sum[kPer] = {};
+#pragma unroll
+      for (int w = 0; w < kFewPieces; ++w) ref = s[w][k].y == 0.f ? ref : fmaxf(ref, s[w][k].x);
+#pragma unroll
+      for (int w = 0; w < kFewPieces; ++w) {
+        // a piece that saw no token of this row has no say
+        const float f = s[w][k].y == 0.f ? 0.f : exp2_fast(s[w][k].x - ref);
+        den = fmaf(s[w][k].y, f, den);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) sum[e] = fmaf(o[w][k][e], f, sum[e]);
+      }
+      const float inv = den != 0.f ? 1.f / den : 0.f;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) sum[e] *= inv;
+      if (first + k < last) store_row<D, F16>(a, place(first + k), sum);
+    }
   }
 }
-
-int slot_rows_of(const dkv_q4_attend_args& a) { return rows_of(a) < kBlock ? rows_of(a) : kBlock; }
 
 template <int D, bool F16>
 int launch_prefill(const dkv_q4_attend_args& a, cudaStream_t stream) {
@@ -786,7 +826,7 @@ int launch_prefill(const dkv_q4_attend_args& a, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   // Few rows: a warp each, for the joins of a long context are long; many: several each, in about one wave of CTAs.
   const int64_t rows = static_cast<int64_t>(rows_of(a)) * a.n_kv_heads * a.n_seq;
-  const int cta_rows = rows <= 148 * 8 * kCombineWarps ? kCombineWarps : 4 * kCombineWarps;
+  const int cta_rows = rows <= 148 * 8 * kCombineWarps ? kCombineWarps : 8 * kCombineWarps;
   cfg.gridDim = dim3((rows_of(a) + cta_rows - 1) / cta_rows, a.n_kv_heads, a.n_seq);
   cfg.blockDim = dim3(kCombineWarps * 32);
   cfg.stream = stream;
@@ -808,7 +848,8 @@ int launch_prefill(const dkv_q4_attend_args& a, cudaStream_t stream) {
 bool prefill_takes(const dkv_q4_attend_args& a) { return rows_of(a) > 64; }
 
 int64_t prefill_floats(const dkv_q4_attend_args& a) {
-  return 2 * static_cast<int64_t>(device_sms()) * slot_floats(slot_rows_of(a), a.head_dim);
+  const int64_t units = static_cast<int64_t>(a.n_seq) * a.n_kv_heads * ((rows_of(a) + kBlock - 1) / kBlock);
+  return 2 * static_cast<int64_t>(device_sms()) * slot_floats(slot_rows_of(a), a.head_dim) + 2 * units;
 }
 
 int run_prefill(const dkv_q4_attend_args& a, cudaStream_t stream) {
