@@ -91,7 +91,7 @@ struct Decode {
   static constexpr int kRows = kPair ? 4 : 8 * NT;
   static constexpr int kStages = D == 128 ? 2 : 4;
   static constexpr int kTiles = NT <= 1 ? 2 : 1;  // of 16 tokens at a time, for the latencies to overlap
-  static constexpr int kBlocksPerSm = D == 128 && NT == 2 ? 2 : 3;  // two accumulators of 128 need the registers
+  static constexpr int kBlocksPerSm = D * NT > 128 ? 2 : 3;  // the accumulators need the registers
   static constexpr int kWarpBytes = kStages * C::kBytes;
   static constexpr int kBars = kWarps * kWarpBytes;
   static constexpr int kBytes = kBars + kWarps * kStages * 8;
@@ -838,7 +838,11 @@ q4_join_parts_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, i
 }
 
 // NT of q4_decode_kernel, and the query rows that a warp then holds.
-int tiles_of(const dkv_q4_attend_args& a) { return rows_of(a) <= 4 ? 0 : rows_of(a) <= 8 ? 1 : 2; }
+int tiles_of(const dkv_q4_attend_args& a) {
+  const int rows = rows_of(a);
+  // 17 to 24 rows of heads of 64 go through the pages once, in three tiles (a third one of 128 leaves no registers).
+  return rows <= 4 ? 0 : rows <= 8 ? 1 : rows > 16 && rows <= 24 && a.head_dim == 64 ? 3 : 2;
+}
 int held_rows(int nt) { return nt == 0 ? 4 : 8 * nt; }
 
 int64_t floats_of(const dkv_q4_attend_args& a) {
@@ -940,7 +944,7 @@ int dkv_q4_attend(const dkv_q4_attend_args* a, void* stream) {
 #define DKV_Q4_DECODE(D, NT) \
   (a->fp16 ? dkv::launch_decode<D, NT, true>(*a, append, st) : dkv::launch_decode<D, NT, false>(*a, append, st))
   if (a->head_dim == 128) return nt == 0 ? DKV_Q4_DECODE(128, 0) : nt == 1 ? DKV_Q4_DECODE(128, 1) : DKV_Q4_DECODE(128, 2);
-  return nt == 0 ? DKV_Q4_DECODE(64, 0) : nt == 1 ? DKV_Q4_DECODE(64, 1) : DKV_Q4_DECODE(64, 2);
+  return nt == 0 ? DKV_Q4_DECODE(64, 0) : nt == 1 ? DKV_Q4_DECODE(64, 1) : nt == 2 ? DKV_Q4_DECODE(64, 2) : DKV_Q4_DECODE(64, 3);
 #undef DKV_Q4_DECODE
 }
 
