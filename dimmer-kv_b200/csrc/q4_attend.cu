@@ -66,19 +66,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 // The pages of all units are dealt to the workers (warps) in the order (conversation, KV head, row chunk, page).
 __device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
 
-// One warp: pages of all conversations, and of those before `seq`.
-__device__ __forceinline__ int64_t count_pages(const dkv_q4_attend_args& a, int seq, int64_t& before) {
-  int64_t total = 0;
-  before = 0;
-  for (int base = 0; base < a.n_seq; base += 32) {
-    const int s = base + (threadIdx.x & 31);
-    const int p = s < a.n_seq ? pages_of(tokens_of(a, s)) : 0;
-    total += warp_sum(p);
-    before += warp_sum(s < seq ? p : 0);
-  }
-  return total;
-}
-
 // How a warp holds its query rows: NT tiles of 8 columns, two columns per lane; or, NT = 0, up to 4 rows, each on the
 // even column of a pair, so that a lane has one row to do the softmax of and the odd column takes what the rounding of
 // the row's probabilities lacks.
@@ -553,6 +540,9 @@ q4_decode_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int w
     const int last_i = min((min(row0 + S::kRows, a.q_len * share) - 1) / share, fresh - 1);
     const int seen = row0 / share < fresh ? start + last_i + 1 : 0;
     const int full_below = start + row0 / share + 1;  // tokens below it are seen by every row
+    if (lane == 0)
+      record_unit(unit_record(a, workers, rows, static_cast<int64_t>(seq) * units + unit), worker, at != begin, p0 == 0,
+                  p1 == n_pages);
     const int32_t* table = a.blocks + static_cast<int64_t>(seq) * a.max_blocks;
     const int64_t page_stride = static_cast<int64_t>(a.n_kv_heads) * C::kBytes;
     uint8_t* cells = a.cells + static_cast<int64_t>(head) * C::kBytes;
@@ -707,27 +697,18 @@ q4_join_rows_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, in
     return;
   }
   const JoinRow row(a, id, share, D);
-  const int tokens = tokens_of(a, row.seq), n_pages = pages_of(tokens);
+  const int tokens = tokens_of(a, row.seq), held = min(kRows, rows), chunk = row.r / kRows;
   const bool real = tokens > 0 && row.i < min(tokens - a.starts[row.seq], a.q_len);
-  const int chunk = row.r / kRows;
-  int64_t before;
-  const int64_t all = count_pages(a, row.seq, before);
-  Pieces pieces = {};
-  if (real)
-    pieces = Pieces(a, Deal(all * units, workers), before * units + static_cast<int64_t>(row.head * chunks + chunk) * n_pages,
-                    n_pages, min(kRows, rows), D);
   asm volatile("griddepcontrol.wait;" ::: "memory");  // what is above does not depend on the main kernel
+  const int2 by = *unit_record(a, workers, held, static_cast<int64_t>(row.seq) * units + row.head * chunks + chunk);
+  const int failed = status_at_entry(a.status);
   float sum[D / 32];
 #pragma unroll
   for (int e = 0; e < D / 32; ++e) sum[e] = 0.f;
-  const int failed = status_at_entry(a.status);
-  if (real) {
-    if (pieces.n == 1 && !__any_sync(0xffffffffu, failed != 0)) return;  // one worker had the whole unit
-    if (pieces.n > 1) join_row<D, -1, 8>(pieces, min(kRows, rows), row.r - chunk * kRows, sum);
-  }
-  if (__any_sync(0xffffffffu, failed != 0)) {
-#pragma unroll
-    for (int e = 0; e < D / 32; ++e) sum[e] = 0.f;
+  if (real && !__any_sync(0xffffffffu, failed != 0)) {
+    const Pieces pieces(a, by, workers, held, D);
+    if (pieces.n == 1) return;  // one worker had the whole unit
+    join_row<D, -1, 16>(pieces, held, row.r - chunk * kRows, sum);
   }
   store_row<D, F16>(a, row.to, sum);
 }
@@ -740,32 +721,22 @@ template <int D, int NT, bool F16>
 __global__ void __launch_bounds__(kPartThreads)
 q4_join_parts_kernel(const __grid_constant__ dkv_q4_attend_args a, int chunks, int workers) {
   constexpr int kRows = Decode<D, NT>::kRows, kParts = D / 32, kSlices = kPartThreads / 8;
-  __shared__ int64_t line[2];
   __shared__ float4 part[kPartThreads / 32][8];
   __shared__ float factor[kFactors];
   __shared__ float warp_ref[kPartThreads / 32], warp_den[kPartThreads / 32];
   const int share = a.n_q_heads / a.n_kv_heads, rows = min(kRows, a.q_len * share), units = a.n_kv_heads * chunks;
   const JoinRow row(a, blockIdx.x / kParts, share, D);
   const int tid = threadIdx.x, slice = tid / 8, dim = (blockIdx.x % kParts) * 32 + (tid % 8) * 4;
-  const int tokens = tokens_of(a, row.seq), n_pages = pages_of(tokens);
-  const int chunk = row.r / kRows, col = row.r - chunk * kRows;
-  if (tid < 32) {
-    int64_t before;
-    const int64_t all = count_pages(a, row.seq, before);
-    if (tid == 0) line[0] = all, line[1] = before;
-  }
-  __syncthreads();
+  const int tokens = tokens_of(a, row.seq), chunk = row.r / kRows, col = row.r - chunk * kRows;
   const bool real = tokens > 0 && row.i < min(tokens - a.starts[row.seq], a.q_len);
-  Pieces pieces = {};
-  if (real)
-    pieces = Pieces(a, Deal(line[0] * units, workers), line[1] * units + static_cast<int64_t>(row.head * chunks + chunk) * n_pages,
-                    n_pages, rows, D);
   asm volatile("griddepcontrol.wait;" ::: "memory");  // what is above does not depend on the main kernel
+  const int2 by = *unit_record(a, workers, rows, static_cast<int64_t>(row.seq) * units + row.head * chunks + chunk);
   // That one may have set the status word while others of its warps finished: the CTA's one answer.
   if (cta_failed_at_entry(a.status) || !real) {
     if (slice == 0) store_out4<F16>(a, row.to + dim, 0.f, 0.f, 0.f, 0.f);
     return;
   }
+  const Pieces pieces(a, by, workers, rows, D);
   if (pieces.n == 1) return;  // one worker had the whole unit
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   float den = 0.f, ref = INFINITY;  // sums are relative to 2^-ref; the smallest ref is the largest maximum
@@ -847,7 +818,8 @@ int held_rows(int nt) { return nt == 0 ? 4 : 8 * nt; }
 
 int64_t floats_of(const dkv_q4_attend_args& a) {
   const int rows = rows_of(a), most = held_rows(tiles_of(a)), held = rows < most ? rows : most;
-  return 2 * static_cast<int64_t>(device_sms() * 3 * kWarps) * slot_floats(held, a.head_dim);
+  const int64_t units = static_cast<int64_t>(a.n_seq) * a.n_kv_heads * ((rows + most - 1) / most);
+  return 2 * static_cast<int64_t>(device_sms() * 3 * kWarps) * slot_floats(held, a.head_dim) + 2 * units;
 }
 
 template <int D, int NT, bool F16>

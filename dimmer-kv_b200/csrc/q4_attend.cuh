@@ -50,8 +50,6 @@ struct DealOf {
   __device__ __forceinline__ DealOf(int64_t total_, int workers_)
       : total(total_), workers(static_cast<int>(total_ < workers_ ? total_ : workers_)) {}
   __device__ __forceinline__ int64_t begin(int w) const { return divide<CALL>(total * w, workers); }
-  // The worker that has place x; none is without a place.
-  __device__ __forceinline__ int owner(int64_t x) const { return static_cast<int>(divide<CALL>((x + 1) * workers - 1, total)); }
 };
 using Deal = DealOf<true>;
 
@@ -68,6 +66,15 @@ __device__ __forceinline__ void store_out4(const dkv_q4_attend_args& a, int64_t 
 // A partial result in the workspace: per slot (two per worker) [rows][D] of O, then [rows][4] with (reference, l).
 __host__ __device__ __forceinline__ int64_t slot_floats(int rows, int d) { return static_cast<int64_t>(rows) * (d + 4); }
 
+// Behind the slots, per unit: the slot of its first piece, written by the worker that has it, and the worker of its last.
+__device__ __forceinline__ int2* unit_record(const dkv_q4_attend_args& a, int workers, int rows, int64_t unit) {
+  return reinterpret_cast<int2*>(a.workspace + 2 * static_cast<int64_t>(workers) * slot_floats(rows, a.head_dim)) + unit;
+}
+__device__ __forceinline__ void record_unit(int2* by, int worker, bool second_slot, bool begins, bool ends) {
+  if (begins) by->x = 2 * worker + second_slot;
+  if (ends) by->y = worker;
+}
+
 // The partial results of one unit: worker w0 + k left the unit's piece in slot(k). The unit is the last segment of w0 unless
 // w0 begins with it (its second slot), and the first segment of the others.
 struct Pieces {
@@ -75,12 +82,11 @@ struct Pieces {
   int64_t stride;
   int n;
   Pieces() = default;
-  __device__ __forceinline__ Pieces(const dkv_q4_attend_args& a, const Deal& deal, int64_t unit, int places, int rows, int d) {
-    const int w0 = deal.owner(unit), w1 = deal.owner(unit + places - 1);
+  __device__ __forceinline__ Pieces(const dkv_q4_attend_args& a, int2 by, int workers, int rows, int d) {
     stride = slot_floats(rows, d);
-    n = w1 - w0 + 1;
-    first = a.workspace + (2 * static_cast<int64_t>(w0) + (deal.begin(w0) < unit ? 1 : 0)) * stride;
-    rest = a.workspace + 2 * static_cast<int64_t>(w0) * stride;
+    first = a.workspace + by.x * stride;
+    rest = a.workspace + (by.x & ~1) * stride;
+    n = by.x >= 0 && by.y < workers ? max(0, by.y - (by.x >> 1) + 1) : 0;  // (unwritten records only after an error)
   }
   __device__ __forceinline__ const float* slot(int k) const { return k == 0 ? first : rest + 2 * k * stride; }
 };

@@ -136,11 +136,9 @@ __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
 
 int slot_rows_of(const dkv_q4_attend_args& a) { return rows_of(a) < kBlock ? rows_of(a) : kBlock; }
 
-// Behind the slots: the slot of a unit's first piece, and the CTA of its last.
-__device__ __forceinline__ int2* unit_record(const dkv_q4_attend_args& a, int workers, int slot_rows, int seq, int head, int block) {
+__device__ __forceinline__ int64_t unit_of(const dkv_q4_attend_args& a, int seq, int head, int block) {
   const int blocks = (a.q_len * (a.n_q_heads / a.n_kv_heads) + kBlock - 1) / kBlock;
-  return reinterpret_cast<int2*>(a.workspace + 2 * static_cast<int64_t>(workers) * slot_floats(slot_rows, a.head_dim)) +
-         (static_cast<int64_t>(seq) * a.n_kv_heads + head) * blocks + block;
+  return (static_cast<int64_t>(seq) * a.n_kv_heads + head) * blocks + block;
 }
 
 // Where a CTA's piece of the line begins and ends, and the step of `begin`.
@@ -346,11 +344,9 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
       while (ok && walk.next()) {
         const int64_t unit_begin = place;
         place += walk.last - walk.first;
-        if (threadIdx.x == 0) {
-          int2* by = unit_record(a, workers, slot_rows, walk.seq, walk.head, walk.block);
-          if (walk.first == 0) by->x = 2 * blockIdx.x + (unit_begin == begin ? 0 : 1);
-          if (walk.last == walk.steps) by->y = blockIdx.x;
-        }
+        if (threadIdx.x == 0)
+          record_unit(unit_record(a, workers, slot_rows, unit_of(a, walk.seq, walk.head, walk.block)), blockIdx.x,
+                      unit_begin != begin, walk.first == 0, walk.last == walk.steps);
         if (tile == 1 && !walk.two()) continue;
         const Seq& q = walk.q;
         const int row0 = walk.block * kBlock + tile * kRows, r = row0 + row_in_tile, i = r / share;
@@ -751,14 +747,8 @@ q4_prefill_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int work
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const bool failed = cta_failed_at_entry(a.status);
   Pieces pieces = {};
-  if (r0 < q.rows && !failed) {
-    const int2 by = *unit_record(a, workers, slot_rows, seq, head, block);
-    pieces.stride = slot_floats(slot_rows, D);
-    pieces.first = a.workspace + by.x * pieces.stride;
-    pieces.rest = a.workspace + (by.x & ~1) * pieces.stride;
-    pieces.n = by.y - (by.x >> 1) + 1;
-    if (by.x < 0 || by.y >= workers || pieces.n < 1) pieces.n = 0;
-  }
+  if (r0 < q.rows && !failed)
+    pieces = Pieces(a, *unit_record(a, workers, slot_rows, unit_of(a, seq, head, block)), workers, slot_rows, D);
   constexpr int kPer = D / 32;
   const int end = min(r0 + cta_rows, rows);  // of the CTA
   auto place = [&](int r) {
