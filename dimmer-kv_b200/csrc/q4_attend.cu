@@ -912,7 +912,7 @@ int dkv_q4_attend(const dkv_q4_attend_args* a, void* stream) {
     append = 0;
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (prefill) return dkv::q4::run_prefill(*a, st);
+  if (prefill) return dkv::q4::run_prefill(*a, a->key != nullptr, st);
 #define DKV_Q4_DECODE(D, NT) \
   (a->fp16 ? dkv::launch_decode<D, NT, true>(*a, append, st) : dkv::launch_decode<D, NT, false>(*a, append, st))
   if (a->head_dim == 128) return nt == 0 ? DKV_Q4_DECODE(128, 0) : nt == 1 ? DKV_Q4_DECODE(128, 1) : DKV_Q4_DECODE(128, 2);

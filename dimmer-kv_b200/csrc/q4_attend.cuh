@@ -167,7 +167,7 @@ inline int rows_of(const dkv_q4_attend_args& a) { return a.q_len * (a.n_q_heads 
 // q4_prefill.cu
 bool prefill_takes(const dkv_q4_attend_args& a);
 int64_t prefill_floats(const dkv_q4_attend_args& a);
-int run_prefill(const dkv_q4_attend_args& a, cudaStream_t stream);
+int run_prefill(const dkv_q4_attend_args& a, bool appended, cudaStream_t stream);
 
 }  // namespace q4
 }  // namespace dkv

@@ -1,17 +1,20 @@
 // q4_prefill.cu — causal attention over the paged 4-bit cache for many query rows per KV head (a question, a prompt's
 // chunk): dkv_q4_attend's matrix-product form, on tcgen05.
 //
-// Bound by the exponentials and the two products, which are about even: a tile of 128 rows x 128 tokens takes 1024
-// cycles of the SM's exponential units and, at head_dim 128, 2 x 512 of its tensor core. Everything else has to hide
-// behind these: a CTA has two tiles of 128 query rows (the rows of a KV head's query heads, token after token), which
-// use the same unpacked keys and values, and two buffers of scores for each: a step is one page, 64 tokens, and a tile's
-// next scores are made while the softmax of the last is under way, so that neither waits for the other's latency.
+// A CTA has two tiles of 128 query rows (the rows of a KV head's query heads, token after token), which use the same
+// unpacked keys and values, and two buffers of scores for each: a step is one page, 64 tokens, and a tile's next scores
+// are made while the softmax of the last is under way. At head_dim 128 a step of both tiles takes at least 1024 cycles of
+// the SM's exponential units, 1024 of its tensor core and about 1300 of its shared memory's bandwidth (of that of
+// float16 caches, below, 2048 and 2500); measured are 2300 for bfloat16, where the softmax's latencies, two warps
+// to a scheduler, are the bound, and 3100 for float16, where the products are. Steps of 128 tokens with one buffer, which
+// have fewer and wider products, took 5500 and 8000.
 //
 //   warps 0-3, 4-7   softmax of the first and the second tile, one row per thread: scores from TMEM, probabilities
 //                    back into TMEM (over the scores they come from), where the second product takes them
 //   warps 8-15       unpack a page, four threads per token: the keys into a float16 tile with the 128-byte swizzle, the
 //                    values into one whose rows are those of the second product's contraction
-//   warps 16, 17     issue the products of a tile each (per step the next Q K, then P V)
+//   warps 16, 17     issue the products of a tile each (per step the next Q K, then P V; one warp for both tiles, which
+//                    waits for each in turn, took 299 us where two take 224)
 //   warp 18          issues the copies of the pages
 //
 // TMEM: two score buffers of 64 columns and an output per tile, 512 columns. The rows' references (running maxima) lag by
@@ -24,6 +27,9 @@
 //
 // The steps of all (conversation, KV head, 256-row block) units form one line that is cut evenly over one CTA per
 // SM; blocks that several CTAs share leave partial results in the workspace, which q4_prefill_combine_kernel joins.
+//
+// 24 / 8 heads of 128: 4 x 512 tokens over 2K to 8K, float16, 205 us with the store and the joins, 64 tokens over 32K,
+// bfloat16, 61 us.
 #include "q4_attend.cuh"
 
 namespace dkv {
@@ -322,6 +328,7 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
   }
   if (warp == kMmaWarp) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the new tokens' cells; what is above reads lengths alone
   const bool failed = cta_failed_at_entry(a.status);  // a barrier of the CTA
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
@@ -734,8 +741,8 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
 
 // Joins the blocks that several CTAs share and writes the zeros of the rows behind the new tokens: cta_rows (which divides
 // kBlock) rows of one block per CTA. A row of many pieces, as few long contexts leave them, has a warp that takes the pieces'
-// factors in its lanes; of few pieces, a warp takes kAtOnce rows together, with all of their loads under way (4 x 512 rows of
-// 24 heads of 128 in two or three pieces: 25 us one row after another).
+// factors in its lanes; of few pieces, a warp takes kAtOnce rows together, with all of their loads under way (the
+// 49152 rows of 4 x 512 tokens of 24 heads of 128, in two or three pieces: 15 us, one row after another 20).
 constexpr int kCombineWarps = 8, kAtOnce = 4, kFewPieces = 4;
 template <int D, bool F16>
 __global__ void __launch_bounds__(kCombineWarps * 32)
@@ -806,24 +813,30 @@ q4_prefill_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int work
 }
 
 template <int D, bool F16>
-int launch_prefill(const dkv_q4_attend_args& a, cudaStream_t stream) {
+int launch_prefill(const dkv_q4_attend_args& a, bool appended, cudaStream_t stream) {
   auto kernel = q4_prefill_kernel<D, F16>;
   static std::atomic<uint64_t> done{0};
   if (!allow_shared(kernel, Shared<D, F16>::kAlloc, done)) return DKV_ERR_CUDA;
   const int workers = device_sms(), slot_rows = slot_rows_of(a);
-  kernel<<<workers, kThreads, Shared<D, F16>::kAlloc, stream>>>(a, workers, slot_rows);
-  if (cudaGetLastError() != cudaSuccess) return DKV_ERR_CUDA;
-  cudaLaunchConfig_t cfg = {};
-  // Few rows: a warp each, for the joins of a long context are long; many: several each, in about one wave of CTAs.
-  const int64_t rows = static_cast<int64_t>(rows_of(a)) * a.n_kv_heads * a.n_seq;
-  const int cta_rows = rows <= 148 * 8 * kCombineWarps ? kCombineWarps : 8 * kCombineWarps;
-  cfg.gridDim = dim3((rows_of(a) + cta_rows - 1) / cta_rows, a.n_kv_heads, a.n_seq);
-  cfg.blockDim = dim3(kCombineWarps * 32);
-  cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(workers);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Shared<D, F16>::kAlloc;
+  cfg.stream = stream;
   cfg.attrs = attr;
+  // Right behind the kernel that stores the new tokens, which writes nothing that is read before the wait for it; behind
+  // any other, whose writes are not known, in its turn.
+  cfg.numAttrs = appended ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kernel, a, workers, slot_rows) != cudaSuccess) return DKV_ERR_CUDA;
+  // Few rows: a warp each, for the joins of a long context are long; many: several each, in about one wave of CTAs.
+  const int64_t rows = static_cast<int64_t>(rows_of(a)) * a.n_kv_heads * a.n_seq;
+  const int cta_rows = rows <= workers * 8 * kCombineWarps ? kCombineWarps : 8 * kCombineWarps;
+  cfg.gridDim = dim3((rows_of(a) + cta_rows - 1) / cta_rows, a.n_kv_heads, a.n_seq);
+  cfg.blockDim = dim3(kCombineWarps * 32);
+  cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, q4_prefill_combine_kernel<D, F16>, a, workers, slot_rows, cta_rows) == cudaSuccess
              ? DKV_OK
@@ -833,8 +846,8 @@ int launch_prefill(const dkv_q4_attend_args& a, cudaStream_t stream) {
 }  // namespace
 
 // Up to 64 rows q4_decode_kernel, which takes 16 at a time, is the faster one: over 4 contexts of 3K to 9K tokens, 24 / 8
-// heads of 128, bf16, 48 rows take 54 us there and 60 here, 72 rows 69 and 60 (64 rows of heads of 64: 48 and 51, 96: 61
-// and 52).
+// heads of 128, bf16, 48 rows take 47 us there and 50 here, 63 rows 50 and 47 (64 rows of heads of 64: 41 and 42, 84: 45
+// and 39); over 32 such contexts 48 rows 174 and 215.
 bool prefill_takes(const dkv_q4_attend_args& a) { return rows_of(a) > 64; }
 
 int64_t prefill_floats(const dkv_q4_attend_args& a) {
@@ -842,9 +855,10 @@ int64_t prefill_floats(const dkv_q4_attend_args& a) {
   return 2 * static_cast<int64_t>(device_sms()) * slot_floats(slot_rows_of(a), a.head_dim) + 2 * units;
 }
 
-int run_prefill(const dkv_q4_attend_args& a, cudaStream_t stream) {
-  if (a.head_dim == 128) return a.fp16 ? launch_prefill<128, true>(a, stream) : launch_prefill<128, false>(a, stream);
-  return a.fp16 ? launch_prefill<64, true>(a, stream) : launch_prefill<64, false>(a, stream);
+int run_prefill(const dkv_q4_attend_args& a, bool appended, cudaStream_t stream) {
+  if (a.head_dim == 128)
+    return a.fp16 ? launch_prefill<128, true>(a, appended, stream) : launch_prefill<128, false>(a, appended, stream);
+  return a.fp16 ? launch_prefill<64, true>(a, appended, stream) : launch_prefill<64, false>(a, appended, stream);
 }
 
 }  // namespace q4

@@ -44,6 +44,7 @@ template <int D, bool F16>
 __global__ void __launch_bounds__(kRowThreads) q4_append_kernel(const __grid_constant__ dkv_q4_rows_args a) {
   using C = Cells<D>;
   constexpr int kLanes = D / 16;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // an attention that reads these cells begins to set up
   const Place p = place_of<D>(a);
   uint4 key[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)}, value[2] = {key[0], key[0]};
   if (p.slot >= 0) {
