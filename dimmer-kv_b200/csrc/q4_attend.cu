@@ -457,16 +457,16 @@ __device__ __noinline__ void store_new(const dkv_q4_attend_args& a, int seq, int
       const uint4* from = reinterpret_cast<const uint4*>(src + (mine - start) * sd[2]);
       raw[0] = from[0], raw[1] = from[1];
     }
-    const q4::Cell16 c = q4::quantise16<F16>(raw);
+    const q4::CellPart<2> c = q4::quantise<F16>(raw);
     if (!c.fits) record_error(a.status, kSiteQ4Rows + kErrCellRange);
     if (mine < last) {
       const int r = mine % q4::kPage;
       if (is_value) {
-        q4::store_value16<D>(copy, r, j, c);
-        q4::store_value16<D>(cell, r, j, c);
+        q4::store_value<D>(copy, r, j, c);
+        q4::store_value<D>(cell, r, j, c);
       } else {
-        q4::store_key16<D>(copy, r, j, c);
-        q4::store_key16<D>(cell, r, j, c);
+        q4::store_key<D>(copy, r, j, c);
+        q4::store_key<D>(cell, r, j, c);
       }
     }
   }

@@ -15,8 +15,8 @@
 //     64: lanes t = 0..3 read four pairs at once, a multiple of 64 bytes apart, and would share banks otherwise.
 //   headers: float16 (scale, low) of a token's key groups, then of its value groups: one load per token.
 //
-// Quantising: four lanes hold a group of 64 dimensions, sixteen each (two 16-byte loads); minimum and maximum are two
-// shuffles, eight key codes are exactly one word of the key cell, eight value codes the halves of two words of the pair's.
+// Quantising: 8 / H lanes hold a group of 64 dimensions, 8 H each (H 16-byte loads); minimum and maximum are a shuffle
+// or two, eight key codes are exactly one word of the key cell, eight value codes the halves of two words of the pair's.
 // The code is the nearest whole number to the true quotient (x - low) / scale, ties to even, not to a float32
 // rounding of it: the float32 quotient, by the hardware's reciprocal off by less than 2^-18, decides unless it lies
 // within 2^-16 of a half; then the border low + (c + 1/2) * scale, which float64 holds exactly (two float16 numbers,
@@ -94,8 +94,9 @@ static __device__ __noinline__ uint32_t codes_with_care(uint4 raw, float low, fl
   return codes;
 }
 
-struct Cell16 {
-  uint32_t codes[2];  // of the lane's first and second eight elements, nibble e: element e
+template <int H>
+struct CellPart {
+  uint32_t codes[H];  // of the lane's eights of elements, nibble e: element e
   uint16_t scale, low;
   bool fits;          // the group is finite and within kCellMax
 };
@@ -113,25 +114,27 @@ __device__ __forceinline__ uint32_t extreme2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// The lane's sixteen elements of a group that this lane and the 3 beside it hold (all of a warp's lanes call it).
-template <bool F16>
-__device__ __forceinline__ Cell16 quantise16(const uint4 (&raw)[2]) {
-  const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+// The lane's 8 H elements of a group that this lane and those beside it hold (all of a warp's lanes call it).
+template <bool F16, int H>
+__device__ __forceinline__ CellPart<H> quantise(const uint4 (&raw)[H]) {
+  uint32_t w[4 * H];
+#pragma unroll
+  for (int h = 0; h < H; ++h) w[4 * h] = raw[h].x, w[4 * h + 1] = raw[h].y, w[4 * h + 2] = raw[h].z, w[4 * h + 3] = raw[h].w;
   uint32_t least = w[0], most = w[0];
 #pragma unroll
-  for (int e = 1; e < 8; ++e) {
+  for (int e = 1; e < 4 * H; ++e) {
     least = extreme2<F16, false>(least, w[e]);
     most = extreme2<F16, true>(most, w[e]);
   }
 #pragma unroll
-  for (int d = 1; d < 4; d <<= 1) {
+  for (int d = 1; d < 8 / H; d <<= 1) {
     least = extreme2<F16, false>(least, __shfl_xor_sync(0xffffffffu, least, d));
     most = extreme2<F16, true>(most, __shfl_xor_sync(0xffffffffu, most, d));
   }
   least = extreme2<F16, false>(least, least >> 16);
   most = extreme2<F16, true>(most, most >> 16);
   const float lo = from16<F16>(static_cast<uint16_t>(least)), hi = from16<F16>(static_cast<uint16_t>(most));
-  Cell16 c;
+  CellPart<H> c;
   c.fits = lo >= -kCellMax && hi <= kCellMax;  // false for a NaN
   const __half low_h = __float2half_rn(lo);
   const float low = __half2float(low_h);
@@ -147,7 +150,7 @@ __device__ __forceinline__ Cell16 quantise16(const uint4 (&raw)[2]) {
   const uint64_t minus2 = f32x2_pack(0xbf800000u, 0xbf800000u);
   const bool inside = (lo - low) * part > -0.49f && (hi - low) * part < 15.49f;  // false where low's rounding is coarse
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < H; ++h) {
     uint32_t codes = 0;
     float off = 0.f;
 #pragma unroll
@@ -168,28 +171,31 @@ __device__ __forceinline__ Cell16 quantise16(const uint4 (&raw)[2]) {
   return c;
 }
 
-// The j-th sixteen dimensions of token r of a page, written into it (in shared or in global memory).
-template <int D>
-__device__ __forceinline__ void store_key16(uint8_t* page, int r, int j, const Cell16& c) {
-  *reinterpret_cast<uint2*>(page + Cells<D>::key_word(r, 2 * j)) = make_uint2(c.codes[0], c.codes[1]);
-  if (j % 4 == 0)
-    *reinterpret_cast<uint32_t*>(page + Cells<D>::key_head(r, j / 4)) =
+// The j-th 8 H dimensions of token r of a page, written into it (in shared or in global memory).
+template <int D, int H>
+__device__ __forceinline__ void store_key(uint8_t* page, int r, int j, const CellPart<H>& c) {
+#pragma unroll
+  for (int h = 0; h < H; h += 2)
+    *reinterpret_cast<uint2*>(page + Cells<D>::key_word(r, H * j + h)) = make_uint2(c.codes[h], c.codes[h + 1]);
+  if (j % (8 / H) == 0)
+    *reinterpret_cast<uint32_t*>(page + Cells<D>::key_head(r, j / (8 / H))) =
         static_cast<uint32_t>(c.scale) | static_cast<uint32_t>(c.low) << 16;
 }
-template <int D>
-__device__ __forceinline__ void store_value_head(uint8_t* page, int r, int j, const Cell16& c) {
-  *reinterpret_cast<uint32_t*>(page + Cells<D>::value_head(r, j / 4)) =
-      static_cast<uint32_t>(c.scale) | static_cast<uint32_t>(c.low) << 16;
+template <int D, int H>
+__device__ __forceinline__ void store_value_head(uint8_t* page, int r, int j, const CellPart<H>& c) {
+  if (j % (8 / H) == 0)
+    *reinterpret_cast<uint32_t*>(page + Cells<D>::value_head(r, j / (8 / H))) =
+        static_cast<uint32_t>(c.scale) | static_cast<uint32_t>(c.low) << 16;
 }
-template <int D>
-__device__ __forceinline__ void store_value16(uint8_t* page, int r, int j, const Cell16& c) {
+template <int D, int H>
+__device__ __forceinline__ void store_value(uint8_t* page, int r, int j, const CellPart<H>& c) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint8_t* w = page + Cells<D>::value_words(r >> 1, 2 * j + h) + 2 * (r & 1);
+  for (int h = 0; h < H; ++h) {
+    uint8_t* w = page + Cells<D>::value_words(r >> 1, H * j + h) + 2 * (r & 1);
     *reinterpret_cast<uint16_t*>(w) = static_cast<uint16_t>(c.codes[h]);
     *reinterpret_cast<uint16_t*>(w + 4) = static_cast<uint16_t>(c.codes[h] >> 16);
   }
-  if (j % 4 == 0) store_value_head<D>(page, r, j, c);
+  store_value_head<D>(page, r, j, c);
 }
 
 }  // namespace q4

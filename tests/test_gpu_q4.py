@@ -146,6 +146,30 @@ def test_cells_hold_what_the_definition_says(dim, heads, n, q_len, dtype):
     batch.check_status()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,q_len", [(64, 5201), (128, 2601)])
+def test_cells_of_long_prompts(dim, q_len, dtype):
+    """More rows than the GPU takes at once, for which a lane has more of a row."""
+    batch = Q4Batch(2, layers=1, kv_heads=8, q_heads=8, head_dim=dim, max_tokens=q_len + 3, dtype=dtype)
+    batch.plan([3, 0], 3)  # one starts inside a page, at an odd token
+    few = [_rows(2, 8, 3, dim, dtype, s) for s in (8, 9)]
+    batch.append(0, *few)
+    first = batch._slots
+    counts = torch.tensor([q_len, q_len - 334], device=DEV)
+    batch.plan(counts.tolist(), q_len)
+    k, v = _rows(2, 8, q_len, dim, dtype, 1, "key"), _rows(2, 8, q_len, dim, dtype, 2)
+    pad = (torch.arange(q_len, device=DEV) >= counts[:, None])[:, None, :, None]
+    k.masked_fill_(pad, float("nan"))
+    v.masked_fill_(pad, float("inf"))
+    batch.append(0, k, v)
+    for x, y in zip((k, v), batch.read(0)):
+        want = dequantise4(*quantise4(torch.where(pad, 0.0, x.float())))
+        assert torch.equal(y, torch.where(pad, 0.0, want).to(dtype))
+    for x, y in zip(few, batch.read(0, first)):
+        assert torch.equal(y[0], dequantise4(*quantise4(x[0])).to(dtype))
+    batch.check_status()
+
+
 def test_codes_at_the_borders_between_two():
     """x exactly half way between two codes goes to the even one, one 16-bit step beside it to its own side."""
     dim = 64
@@ -271,6 +295,23 @@ def test_attention_over_cells(case, dtype):
     _check(out32, query, keys, values, held, counts, scaling)
     assert torch.equal(out32.to(dtype), out)
     batch.check_status()
+
+
+ROW_CASES = [
+    # three tiles of eight rows, full, with one more than two, and with padding
+    (32, 8, 64, [70, 1000, 64], [6, 6, 6], 6),
+    (17, 1, 64, [300, 0, 63], [1, 1, 0], 1),
+    (8, 1, 64, [129, 40, 9000], [3, 0, 2], 3),
+    # enough rows for a CTA of the joins to take 64, the last of them not a multiple of four
+    (24, 8, 128, [300, 65, 1000, 0, 64], [171, 170, 3, 171, 0], 171),
+    (32, 8, 64, [900, 0, 64, 1], [131, 130, 129, 131], 131),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", ROW_CASES, ids=[f"{c[0]}x{c[1]}x{c[2]}-{max(c[3])}+{c[5]}" for c in ROW_CASES])
+def test_attention_of_row_counts_at_the_borders(case, dtype):
+    test_attention_over_cells(case, dtype)
 
 
 def test_attention_of_peaked_and_flat_rows():
