@@ -94,6 +94,8 @@ logit_rules_kernel(const __grid_constant__ dkv_logits_args a, int splits, int sl
   __shared__ uint64_t keys[kRuleThreads / 32];
   __shared__ uint64_t slice_key;
   __shared__ int listed;
+  __shared__ __align__(16) int32_t ids[kMaxBias];  // the row's biases
+  __shared__ __align__(16) float values[kMaxBias];
   W* words = reinterpret_cast<W*>(smem);  // [slice + 32]
   uint16_t* list = reinterpret_cast<uint16_t*>(smem + (slice + 32) * sizeof(W));
   const int row = blockIdx.x / splits, rank = blockIdx.x % splits;
@@ -118,7 +120,11 @@ logit_rules_kernel(const __grid_constant__ dkv_logits_args a, int splits, int sl
     }
   };
   fetch_past(0);
-  const bool failed = cta_failed_at_entry(a.status);
+  for (int i = tid; i < a.n_bias; i += kRuleThreads) {
+    ids[i] = a.bias_ids[static_cast<int64_t>(row) * a.n_bias + i];
+    values[i] = a.bias_values[static_cast<int64_t>(row) * a.n_bias + i];
+  }
+  const bool failed = cta_failed_at_entry(a.status);  // a barrier of the CTA
   uint64_t best = 0;
   float top = -INFINITY;  // of the thread's untouched tokens, in ascending order: the first of equal ones stays
   int top_at = 0;
@@ -155,8 +161,6 @@ logit_rules_kernel(const __grid_constant__ dkv_logits_args a, int splits, int sl
         append_place(fresh, place, list, &listed);
       }
     }
-    const int32_t* ids = a.bias_ids + static_cast<int64_t>(row) * a.n_bias;
-    const float* values = a.bias_values + static_cast<int64_t>(row) * a.n_bias;
     for (int base = 0; base < a.n_bias; base += kRuleThreads) {
       const int i = base + tid;
       const uint32_t at = i < a.n_bias ? static_cast<uint32_t>(ids[i]) - static_cast<uint32_t>(lo) : 0xffffffffu;
