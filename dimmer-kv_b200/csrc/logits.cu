@@ -97,7 +97,8 @@ logit_rules_kernel(const __grid_constant__ dkv_logits_args a, int splits, int sl
   __shared__ __align__(16) int32_t ids[kMaxBias];  // the row's biases
   __shared__ __align__(16) float values[kMaxBias];
   W* words = reinterpret_cast<W*>(smem);  // [slice + 32]
-  uint16_t* list = reinterpret_cast<uint16_t*>(smem + (slice + 32) * sizeof(W));
+  uint32_t* mask = reinterpret_cast<uint32_t*>(smem + (slice + 32) * sizeof(W));  // [slice / 32 + 4], the slice's grammar
+  uint16_t* list = reinterpret_cast<uint16_t*>(mask + slice / 32 + 4);
   const int row = blockIdx.x / splits, rank = blockIdx.x % splits;
   const int tid = threadIdx.x;
   constexpr int kSize = DT == 2 ? 4 : 2, kHeld = DT == 2 ? 2 : 4;  // loads that a thread has under way
@@ -146,8 +147,10 @@ logit_rules_kernel(const __grid_constant__ dkv_logits_args a, int splits, int sl
 #pragma unroll
     for (int k = 0; k < kHeld; ++k) fetch((k * kRuleThreads + tid) * kVec, raw[k]);
     __syncthreads();
-    const int fill = (n + 32) * static_cast<int>(sizeof(W)) / 16;
-    for (int i = tid; i <= fill; i += kRuleThreads) reinterpret_cast<uint4*>(words)[i] = make_uint4(0u, 0u, 0u, 0u);
+    const int masks = allowed ? (n + 31) / 32 : -1;
+    for (int i = tid; i <= masks; i += kRuleThreads) mask[i] = i < masks ? allowed[lo / 32 + i] : 0u;
+    const int fill = ((n + 32) * static_cast<int>(sizeof(W)) + 15) / 16;
+    for (int i = tid; i < fill; i += kRuleThreads) reinterpret_cast<uint4*>(words)[i] = make_uint4(0u, 0u, 0u, 0u);
     if (tid == 0) listed = 0;
     __syncthreads();
     for (int base = 0; base < length; base += kPast * kRuleThreads) {
@@ -187,9 +190,8 @@ logit_rules_kernel(const __grid_constant__ dkv_logits_args a, int splits, int sl
       }
       fetch(p + kHeld * kRuleThreads * kVec, raw[k]);
       if (allowed) {
-        const int at = max(token, 0), words_in = (a.vocab + 31) / 32;
-        const uint32_t w0 = allowed[at >> 5], w1 = (at >> 5) + 1 < words_in ? allowed[(at >> 5) + 1] : 0u;
-        const uint32_t ok = __funnelshift_r(w0, w1, at & 31) << (at - token);
+        const int at = max(p - pad, 0);
+        const uint32_t ok = __funnelshift_r(mask[at >> 5], mask[(at >> 5) + 1], at & 31) << (at - (p - pad));
 #pragma unroll
         for (int e = 0; e < kVec; ++e)
           if (!(ok & (1u << e))) x[e] = -INFINITY;
@@ -238,7 +240,7 @@ logit_rules_kernel(const __grid_constant__ dkv_logits_args a, int splits, int sl
         }
       }
       if (word & Word<W>::kBiased) x = __fadd_rn(x, bias);
-      if (allowed && !((allowed[token >> 5] >> (token & 31)) & 1u)) x = -INFINITY;
+      if (allowed && !((mask[(token - lo) >> 5] >> (token & 31)) & 1u)) x = -INFINITY;
       if (out) out[token] = x;
       const uint64_t key = order_key(x, token);
       best = key > best ? key : best;
@@ -323,11 +325,11 @@ int launch_rules(const dkv_logits_args& a, cudaStream_t stream) {
   const int room = static_cast<int>(touched < slice ? touched : slice);
   auto kernel = logit_rules_kernel<DT, W>;
   static std::atomic<uint64_t> done{0};
-  if (!allow_shared(kernel, (most + 40) * static_cast<int>(sizeof(W)) + most * 2 + 16, done)) return DKV_ERR_CUDA;
+  if (!allow_shared(kernel, (most + 40) * static_cast<int>(sizeof(W)) + most * 2 + most / 8 + 32, done)) return DKV_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.n_rows * splits);
   cfg.blockDim = dim3(kRuleThreads);
-  cfg.dynamicSmemBytes = (slice + 32) * static_cast<int>(sizeof(W)) + (room * 2 + 15) / 16 * 16 + 16;
+  cfg.dynamicSmemBytes = (slice + 32) * static_cast<int>(sizeof(W)) + slice / 8 + 16 + (room * 2 + 15) / 16 * 16 + 16;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
