@@ -314,7 +314,7 @@ logit_rules_kernel(const __grid_constant__ dkv_logits_args a, int splits, int sl
 template <int DT, typename W>
 int launch_rules(const dkv_logits_args& a, cudaStream_t stream) {
   // Where clusters of eight would come in a second wave of CTAs, clusters of four with slices twice as long do not (two
-  // CTAs per SM), and go through the history half as often: 64 rows of 128256 take 24 us against 34, 40 rows 24
+  // CTAs per SM), and go through the history half as often: 64 rows of 128256 took 24 us against 34, 40 rows 24
   // against 31; one row has 8.0 us with eight. 32-bit words allow half the slice.
   const int splits = a.n_rows * kMaxSplits <= 2 * device_sms() ? kMaxSplits : kMaxSplits / 2;
   const int most = sizeof(W) == 2 ? kMaxSlice : kMaxSlice / 2;
