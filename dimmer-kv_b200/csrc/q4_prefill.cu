@@ -399,6 +399,7 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
           // a negative scaling goes into the query, so that the largest product is the largest score
           const float f = a.scaling < 0.f ? -up : up;
           factor = fabsf(a.scaling) * kLog2e * down;
+          factor = factor < 0x1p-126f ? 0x1p-126f : factor;  // above zero, for what is hidden is infinity times it
 #pragma unroll 4
           for (int c = 0; c < D / 8; ++c) {
             uint4& at = *reinterpret_cast<uint4*>(own + (c >> 3) * S::kQPart + sw128_offset(row_in_tile, c & 7));

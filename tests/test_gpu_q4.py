@@ -297,6 +297,20 @@ def test_attention_over_cells(case, dtype):
     batch.check_status()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("q_len", [1, 2, 5, 40])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_where_every_score_is_nothing(dim, q_len, dtype):
+    """A scaling of zero, or of next to nothing with queries of zero: the mean of the values that a row sees."""
+    held, counts = [70, 0, 300], [q_len, q_len, q_len - 1]
+    batch, query, k, v, keys, values = _filled(3, 4, 2, dim, dtype, held, counts, q_len)
+    out = batch.attend_layer(0, query, k, v, 0.0)
+    _check(out, query, keys, values, held, counts, 0.0)
+    zero = torch.zeros_like(query)
+    for scaling in (1e-30, -1e-30, -0.125):
+        assert torch.equal(batch.attend_layer(0, zero, None, None, scaling), out)
+
+
 ROW_CASES = [
     # three tiles of eight rows, full, with one more than two, and with padding
     (32, 8, 64, [70, 1000, 64], [6, 6, 6], 6),
