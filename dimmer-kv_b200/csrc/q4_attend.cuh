@@ -91,9 +91,20 @@ struct Pieces {
   __device__ __forceinline__ const float* slot(int k) const { return k == 0 ? first : rest + 2 * k * stride; }
 };
 
+template <int N>
+__device__ __forceinline__ void load_row(const float* at, float (&x)[N]) {
+  if constexpr (N == 4) {
+    const float4 u = *reinterpret_cast<const float4*>(at);
+    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+  } else {
+    const float2 u = *reinterpret_cast<const float2*>(at);
+    x[0] = u.x, x[1] = u.y;
+  }
+}
+
 // Joins the pieces of row `row` of a unit: a warp, D / 32 dimensions per lane. References are where the sums' factor is
 // 2^-reference (SIGN = 1: q4_prefill's maxima) or 2^reference (-1: q4_decode's negated ones).
-template <int D, int SIGN, int UNROLL>
+template <int D, int SIGN, int UNROLL, int AHEAD>
 __device__ __forceinline__ void join_row(const Pieces& p, int rows, int row, float (&sum)[D / 32]) {
   constexpr int kPer = D / 32;
   const int lane = threadIdx.x & 31;
@@ -101,8 +112,12 @@ __device__ __forceinline__ void join_row(const Pieces& p, int rows, int row, flo
   for (int e = 0; e < kPer; ++e) sum[e] = 0.f;
   float den = 0.f, ref = -INFINITY;
   for (int base = 0; base < p.n; base += 32) {
-    // the factors of 32 pieces, one per lane, then their sums with no load waiting for another
+    // the factors of 32 pieces, one per lane, then their sums with no load waiting for another; the loads of the first
+    // AHEAD pieces are under way with the factors'
     const int n = min(32, p.n - base);
+    float ahead[AHEAD > 0 ? AHEAD : 1][kPer];
+#pragma unroll
+    for (int w = 0; w < AHEAD; ++w) load_row<kPer>(p.slot(base + min(w, n - 1)) + row * D + lane * kPer, ahead[w]);
     const float2 s = lane < n ? *reinterpret_cast<const float2*>(p.slot(base + lane) + rows * D + row * 4) : make_float2(0.f, 0.f);
     const float mine = s.y == 0.f ? -INFINITY : SIGN * s.x;  // a piece that saw no token of this row has no say
     float now = fmaxf(ref, mine);
@@ -117,34 +132,24 @@ __device__ __forceinline__ void join_row(const Pieces& p, int rows, int row, flo
 #pragma unroll
     for (int e = 0; e < kPer; ++e) sum[e] *= keep;
     ref = now;
-#pragma unroll UNROLL
-    for (int w = 0; w < n; ++w) {
-      const float* o = p.slot(base + w) + row * D + lane * kPer;
+#pragma unroll
+    for (int w = 0; w < AHEAD; ++w) {
       const float fw = __shfl_sync(0xffffffffu, f, w);
-      if constexpr (kPer == 4) {
-        const float4 u = *reinterpret_cast<const float4*>(o);
-        sum[0] = fmaf(u.x, fw, sum[0]), sum[1] = fmaf(u.y, fw, sum[1]);
-        sum[2] = fmaf(u.z, fw, sum[2]), sum[3] = fmaf(u.w, fw, sum[3]);
-      } else {
-        const float2 u = *reinterpret_cast<const float2*>(o);
-        sum[0] = fmaf(u.x, fw, sum[0]), sum[1] = fmaf(u.y, fw, sum[1]);
-      }
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) sum[e] = w < n ? fmaf(ahead[w][e], fw, sum[e]) : sum[e];
+    }
+#pragma unroll UNROLL
+    for (int w = AHEAD; w < n; ++w) {
+      float o[kPer];
+      load_row<kPer>(p.slot(base + w) + row * D + lane * kPer, o);
+      const float fw = __shfl_sync(0xffffffffu, f, w);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) sum[e] = fmaf(o[e], fw, sum[e]);
     }
   }
   const float inv = den != 0.f ? 1.f / den : 0.f;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) sum[e] *= inv;
-}
-
-template <int N>
-__device__ __forceinline__ void load_row(const float* at, float (&x)[N]) {
-  if constexpr (N == 4) {
-    const float4 u = *reinterpret_cast<const float4*>(at);
-    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
-  } else {
-    const float2 u = *reinterpret_cast<const float2*>(at);
-    x[0] = u.x, x[1] = u.y;
-  }
 }
 
 // A lane's D / 32 dimensions of an output row that begins at `at`.

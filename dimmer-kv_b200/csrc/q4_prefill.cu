@@ -770,7 +770,7 @@ q4_prefill_combine_kernel(const __grid_constant__ dkv_q4_attend_args a, int work
   if (pieces.n > kFewPieces) {
     for (int r = r0 + warp; r < last; r += kCombineWarps) {
       float sum[kPer];
-      join_row<D, 1, 16>(pieces, slot_rows, r - block * kBlock, sum);
+      join_row<D, 1, 16, 0>(pieces, slot_rows, r - block * kBlock, sum);
       store_row<D, F16>(a, place(r), sum);
     }
     return;
