@@ -6,8 +6,8 @@
 // are made while the softmax of the last is under way. At head_dim 128 a step of both tiles takes at least 1024 cycles of
 // the SM's exponential units, 1024 of its tensor core and about 1300 of its shared memory's bandwidth (of that of
 // float16 caches, below, 2048 and 2500); measured are 2300 for bfloat16, where the softmax's latencies, two warps
-// to a scheduler, are the bound, and 3100 for float16, where the products are. Steps of 128 tokens with one buffer, which
-// have fewer and wider products, took 5500 and 8000.
+// to a scheduler, are the bound, and 3100 for float16, where the products are. Steps of twice as many tokens with one
+// buffer, of fewer and wider products, took 5500 and 8000.
 //
 //   warps 0-3, 4-7   softmax of the first and the second tile, one row per thread: scores from TMEM, probabilities
 //                    back into TMEM (over the scores they come from), where the second product takes them
