@@ -28,8 +28,8 @@
 // The steps of all (conversation, KV head, 256-row block) units form one line that is cut evenly over one CTA per
 // SM; blocks that several CTAs share leave partial results in the workspace, which q4_prefill_combine_kernel joins.
 //
-// 24 / 8 heads of 128: 4 x 512 tokens over 2K to 8K, float16, 205 us with the store and the joins, 64 tokens over 32K,
-// bfloat16, 61 us.
+// 24 / 8 heads of 128: 4 x 512 tokens over 2K to 8K, float16, 204 us with the store and the joins, 64 tokens over 32K,
+// bfloat16, 60 us.
 #include "q4_attend.cuh"
 
 namespace dkv {
@@ -548,6 +548,11 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
       setmaxnreg_dec<kUnpackRegs>();
       Walk walk(a, share, start);
       const int r = threadIdx.x % kStep, part = (threadIdx.x / kStep) & 3;  // the token of the page, which quarter of it
+      // The one of the token's four pieces of key codes that this thread takes, so that the lanes of a load, and those of a
+      // store into the swizzled tile, lie on different banks: rows 2 i and 2 i + 1 (4 i .. 4 i + 3 of 64 dimensions, where
+      // the piece i itself does) take part ^ f(i), with f(i) and f(i) ^ i both permutations of 0 .. 3.
+      const int i2 = (r >> 1) & 3;
+      const int piece = part ^ (D == 128 ? i2 >> 1 | ((i2 ^ i2 >> 1) & 1) << 1 : (r >> 2) & 3);
       uint32_t iter = 0;
       bool ok = true;
       auto load = [&](uint32_t (&w)[D / 32], const uint8_t* src) {
@@ -573,15 +578,16 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
           const uint8_t* page = smem + S::kRaw + raw * C::kBytes;
           // a token that no row sees may never have been written: zeros, no NaN of its
           const bool there = t * kStep + r < seen;
-          auto header = [&](int at) { return as_half2(there ? *reinterpret_cast<const uint32_t*>(page + at) : 0u); };
+          uint32_t heads[2 * kGroups];  // (scale, low) of the key's groups, of the value's
+          load(heads, page + C::key_head(r, 0));
+#pragma unroll
+          for (int e = 0; e < 2 * kGroups; ++e) heads[e] = there ? heads[e] : 0u;
           {
-            // one of the token's four pieces, in an order that keeps the lanes on different banks
-            const int piece = (part + (D == 128 ? r >> 1 : r >> 2)) & 3;
             uint32_t w[D / 32];
             load(w, page + C::kKeyCodes + r * (D / 2) + piece * (D / 8));
 #pragma unroll
             for (int gr = 0; gr < kGroups; ++gr) {
-              const __half2 h = header(C::key_head(r, gr));
+              const __half2 h = as_half2(heads[gr]);
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 uint4 lack;
@@ -604,7 +610,7 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
             load(w, page + C::value_piece(r >> 1, g));
 #pragma unroll
             for (int gr = 0; gr < kGroups; ++gr) {
-              const __half2 h = header(C::value_head(r, gr));
+              const __half2 h = as_half2(heads[kGroups + gr]);
               uint4 none;
               *reinterpret_cast<uint4*>(smem + S::kV + stage * S::kTile + gr * S::kPart + sw128_offset(r, g)) =
                   unpack8<false>(__byte_perm(w[2 * gr], w[2 * gr + 1], r & 1 ? 0x7632 : 0x5410), __low2half2(h), __high2half2(h), none);
