@@ -477,6 +477,38 @@ def test_two_readers_at_once():
     assert all(torch.equal(g, want) for g in got)
 
 
+@pytest.mark.parametrize("q_len", [1, 5, 90])
+def test_two_batches_on_two_streams(q_len):
+    """Two batches, each stored to and attended by a stream of its own, step after step: as one after the other."""
+    data = [[[_rows(2, h, q_len, 64, torch.float16, 100 * b + 10 * i + j) for j, h in enumerate((16, 4, 4))] for i in range(6)]
+            for b in range(2)]
+    held = [[_rows(2, 4, 700, 64, torch.float16, 900 + 2 * b + j) for j in range(2)] for b in range(2)]
+    batches = []
+    for _ in range(2):
+        for b in range(2):
+            batch = Q4Batch(2, layers=1, kv_heads=4, q_heads=16, head_dim=64, max_tokens=700 + 6 * q_len, dtype=torch.float16)
+            batch.plan([700, 311], 700)
+            batch.append(0, *held[b])
+            batches.append(batch)
+
+    def step(batch, x, i):
+        batch.plan([q_len, q_len - i % 2], q_len)
+        return batch.attend_layer(0, *x, 0.125)
+
+    want = [[step(batches[b], x, i) for i, x in enumerate(data[b])] for b in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for i in range(6):
+        for b in range(2):
+            with torch.cuda.stream(streams[b]):
+                got[b].append(step(batches[2 + b], data[b][i], i))
+    torch.cuda.synchronize()
+    for b in range(2):
+        assert all(torch.equal(x, y) for x, y in zip(want[b], got[b]))
+        batches[2 + b].check_status()
+
+
 def test_far_pages_of_a_large_pool():
     """Cells beyond 2^32 bytes: the pages of one conversation lie at the end of a pool of 5 GB."""
     dim, kv = 128, 8
