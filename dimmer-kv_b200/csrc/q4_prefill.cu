@@ -679,8 +679,11 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
         ok = ok && warp_wait(bar, parity, a.status, kSiteQ4Attend + err, abort_flag);
         return ok;
       };
-      // Q K of step `step` (a dimension step of 16 is 32 bytes further in a row, one of 64 the next part). A buffer is free
-      // once the product on its probabilities is issued: a warp's products complete in order.
+      // Scores go where the product of two steps before had its probabilities, as an operand in TMEM. Products are ordered
+      // among themselves only where accumulator and shape are the same, so that one's completion is waited for: the last
+      // that the warp has issued, before every step, so that no more than one phase of its barrier is ever open.
+      auto last_product = [&](bool mine) { return !mine || used == 0 || wait(&o_done[tile], (used - 1) & 1, kErrWaitAccum); };
+      // Q K of step `step` (a dimension step of 16 is 32 bytes further in a row, one of 64 the next part).
       auto scores = [&](uint32_t step, bool mine) {
         const uint32_t stage = step % S::kStages;
         if (!wait(&k_full[stage], (step / S::kStages) & 1, kErrWaitA)) return;
@@ -707,9 +710,9 @@ q4_prefill_kernel(const __grid_constant__ dkv_q4_attend_args a, int workers, int
         const bool mine = tile == 0 || walk.two();
         const int n = __shfl_sync(0xffffffffu, walk.last - walk.first, 0);
         if (mine) wait(&q_full[tile], units++ & 1, kErrWaitA);
-        if (ok) scores(iter, mine);
+        if (ok && last_product(mine)) scores(iter, mine);
         for (int t = 0; t < n && ok; ++t, ++iter) {
-          if (t + 1 < n) scores(iter + 1, mine);
+          if (last_product(mine) && t + 1 < n) scores(iter + 1, mine);
           const uint32_t stage = iter % S::kStages, bar = used & 1;
           if (mine && !wait(&p_full[tile * 2 + bar], (used >> 1) & 1, kErrWaitA)) break;
           if (!wait(&v_full[stage], (iter / S::kStages) & 1, kErrWaitA)) break;

@@ -328,6 +328,20 @@ def test_attention_of_row_counts_at_the_borders(case, dtype):
     test_attention_over_cells(case, dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("q_heads,kv_heads,dim,counts", [(8, 2, 64, [2500]), (6, 2, 128, [1500, 777]), (4, 4, 128, [2049])])
+def test_attention_of_whole_prompts(q_heads, kv_heads, dim, counts, dtype):
+    """Prompts in one piece: blocks of rows of up to forty steps, whose scores take the places of probabilities in turn."""
+    held, q_len = [0] * len(counts), counts[0]
+    batch, query, k, v, keys, values = _filled(len(counts), q_heads, kv_heads, dim, dtype, held, counts, q_len, seed=21)
+    query *= 4  # rows whose maxima move from page to page
+    out = batch.attend_layer(0, query, k, v, dim ** -0.5)
+    _check(out, query, keys, values, held, counts, dim ** -0.5)
+    for _ in range(3):
+        assert torch.equal(batch.attend_layer(0, query, None, None, dim ** -0.5), out)
+    batch.check_status()
+
+
 def test_attention_of_peaked_and_flat_rows():
     """Scores far apart (one token takes all), equal ones, ones that grow along the context (the running maximum moves
     page after page), and queries of very small and very large size."""
