@@ -199,7 +199,7 @@ __device__ __forceinline__ void fit_unit(const uint8_t* page, int base, int seen
   using C = Cells<D>;
   using S = Decode<D, NT>;
   const int lane = threadIdx.x & 31;
-  uint32_t most = 0;  // scales are not negative: ordered as their bits
+  uint32_t most = 0;  // scales are not negative: ordered as their bits (but for the sign that a zero may have)
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int r = lane + 32 * h;
@@ -207,9 +207,9 @@ __device__ __forceinline__ void fit_unit(const uint8_t* page, int base, int seen
     uint32_t top;
     if constexpr (C::kGroups == 2) {
       const uint2 u = *reinterpret_cast<const uint2*>(hp);
-      top = max(u.x & 0xffffu, u.y & 0xffffu);
+      top = max(u.x & 0x7fffu, u.y & 0x7fffu);
     } else {
-      top = *reinterpret_cast<const uint32_t*>(hp) & 0xffffu;
+      top = *reinterpret_cast<const uint32_t*>(hp) & 0x7fffu;
     }
     if (base + r < seen) most = max(most, top);
   }

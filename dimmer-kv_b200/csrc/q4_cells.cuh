@@ -138,7 +138,8 @@ __device__ __forceinline__ CellPart<H> quantise(const uint4 (&raw)[H]) {
   c.fits = lo >= -kCellMax && hi <= kCellMax;  // false for a NaN
   const __half low_h = __float2half_rn(lo);
   const float low = __half2float(low_h);
-  const __half scale_h = __float2half_rn(__fdiv_rn(__fsub_rn(hi, low), 15.f));
+  // low's rounding may lie above every element (a bfloat16 group of next to nothing): +0 then, never a scale with a sign
+  const __half scale_h = __float2half_rn(__fdiv_rn(fmaxf(__fsub_rn(hi, low), 0.f), 15.f));
   const float scale = __half2float(scale_h);
   float part;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(part) : "f"(scale));

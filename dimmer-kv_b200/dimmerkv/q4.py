@@ -35,7 +35,7 @@ def quantise4(x: torch.Tensor):
     in torch operations, on any device."""
     g = x.float().unflatten(-1, (-1, GROUP))
     low = g.amin(-1).half()
-    scale = ((g.amax(-1) - low.float()) / 15).half()
+    scale = ((g.amax(-1) - low.float()).clamp_min(0.0) / 15).half().abs()  # low may round above the largest: +0
     step = scale.double()[..., None]
     q = (g.double() - low.double()[..., None]) / torch.where(step > 0, step, torch.ones_like(step))
     q = torch.where(step > 0, q.round().clamp(0, 15), torch.zeros_like(q))

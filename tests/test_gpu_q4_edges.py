@@ -1,0 +1,43 @@
+"""The paged 4-bit cache and the logit rules at their edges: cells without a spread, masks, empty calls, captured steps,
+and what the drivers do when something has failed."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import tinymodel as tm
+from dimmerkv import _lib, dimmer
+from dimmerkv.compressed_attention import greedy_answer, greedy_decode_batch
+from dimmerkv.logits import LogitRules
+from dimmerkv.q4 import Q4Batch, Q4Context, restore
+from test_gpu_q4 import _check, _filled, _rows, _Tokens
+from test_gpu_rules import _first_best
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda")
+
+
+@pytest.mark.parametrize("q_len", [1, 5, 12, 90])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_groups_whose_least_value_rounds_above_their_largest(dim, q_len):
+    """bfloat16 groups of next to nothing: low, rounded to float16, lies above every element. Their scale is +0, held
+    and new tokens alike, and the tokens beside them come out as ever."""
+    held, counts, dtype = [130, 64], [q_len, q_len], torch.bfloat16
+    batch, query, _, _, keys, values = _filled(2, 4, 2, dim, dtype, held, counts, q_len, seed=31)
+    batch.trim([0, 0])
+    values[:, :, 3::7, :64] = -1e-8
+    values[:, :, 5::11] = -1.5e-6
+    values[0, :, held[0]] = -1.5e-6  # the first new token of one conversation
+    keys[:, :, 2::9, :64] = -1.5e-6
+    batch.plan(held, held[0])
+    batch.append(0, keys[:, :, :held[0]], values[:, :, :held[0]])
+    batch.plan(counts, q_len)
+    new = [torch.stack([x[s, :, h:h + q_len] for s, h in enumerate(held)]) for x in (keys, values)]
+    out = batch.attend_layer(0, query, *new, dim ** -0.5)
+    _check(out, query, keys, values, held, counts, dim ** -0.5)
+    heads = batch.cells[0, :, :, 64 * dim:].reshape(batch.table.n_pages, 2, 64, -1, 2, 2)  # token, group, (scale, low), bytes
+    slots = batch.table.slots(sum(held[:1]) + q_len)[0].long()
+    high = heads[slots // 64, :, slots % 64, :, 0, 1]
+    assert int(high.max()) < 128  # no sign
+    batch.check_status()

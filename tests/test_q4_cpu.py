@@ -149,3 +149,14 @@ def test_struct_mirrors_of_the_new_entry_points():
         names = [re.sub(r"\[.*?\]", "", f).split()[-1].lstrip("*") for stmt in body.split(";") if stmt.strip()
                  for f in stmt.split(",")]
         assert names == [f[0] for f in mirror._fields_], struct
+
+
+def test_scales_have_no_sign():
+    """Groups whose least value, rounded to float16, lies above their largest: code 0 of a scale of +0."""
+    x = torch.full((3, 64), -1e-8).bfloat16()
+    x[1] = -1.5e-6
+    x[2, ::2] = -1.4e-6
+    codes, scale, low = quantise4(x)
+    assert bool((low.float()[:, 0] >= x.float().amax(-1)).any())
+    assert not scale.signbit().any() and not codes[:2].any()
+    assert torch.equal(dequantise4(codes, scale, low).double(), cells64(x)[0])
