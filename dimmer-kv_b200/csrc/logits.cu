@@ -41,10 +41,12 @@ struct Word {
   }
 };
 
+constexpr uint64_t kFailedKey = ~0ull;  // above every token's key: a CTA that found the status word set and did no work
+
 __device__ __forceinline__ uint64_t order_key(float x, uint32_t token) {
   if (x == -INFINITY) return 0ull;
   uint32_t b = __float_as_uint(x);
-  b = x != x ? 0xffffffffu : (x == 0.f ? 0x80000000u : (b & 0x80000000u ? ~b : b | 0x80000000u));
+  b = x != x ? 0xfffffffeu : (x == 0.f ? 0x80000000u : (b & 0x80000000u ? ~b : b | 0x80000000u));
   return static_cast<uint64_t>(b) << 32 | (0xffffffffu - token);
 }
 
@@ -274,6 +276,9 @@ logit_rules_kernel(const __grid_constant__ dkv_logits_args a, int splits, int sl
     const uint64_t other = __shfl_xor_sync(0xffffffffu, best, d);
     best = other > best ? other : best;
   }
+  // A row of the same launch may have set the status word in between, seen by some CTAs of this row and not by others: one
+  // that did no work leaves the row without a token, for what the others found is of a part of the vocabulary.
+  if (failed) best = kFailedKey;
   if ((tid & 31) == 0) keys[tid >> 5] = best;
   __syncthreads();
   if (tid == 0) {
@@ -294,9 +299,10 @@ logit_rules_kernel(const __grid_constant__ dkv_logits_args a, int splits, int sl
       key = other > key ? other : key;
     }
     if (tid == 0) {
-      const int64_t token = key == 0 ? -1 : static_cast<int64_t>(0xffffffffu - static_cast<uint32_t>(key));
+      const int64_t token =
+          key == 0 || key == kFailedKey ? -1 : static_cast<int64_t>(0xffffffffu - static_cast<uint32_t>(key));
       a.tokens[row] = token;
-      if (a.append && token >= 0 && !failed) {
+      if (a.append && token >= 0) {
         const int at = a.lengths[row];
         if (at >= 0 && at < a.capacity) {
           a.history[static_cast<int64_t>(row) * a.capacity + at] = static_cast<int32_t>(token);

@@ -41,3 +41,23 @@ def test_groups_whose_least_value_rounds_above_their_largest(dim, q_len):
     high = heads[slots // 64, :, slots % 64, :, 0, 1]
     assert int(high.max()) < 128  # no sign
     batch.check_status()
+
+
+@pytest.mark.parametrize("rows,vocab", [(600, 40000), (40, 1000)])
+def test_a_full_history_leaves_the_other_rows_whole(rows, vocab):
+    """A row with no room tells; another row of the call has its own best token, or, where it began after that, none:
+    never the best of a part of the vocabulary, and never one that its history does not have."""
+    g = torch.Generator(device=DEV).manual_seed(7)
+    x = torch.randn(rows, vocab, generator=g, device=DEV)
+    best = x.argmax(-1)
+    for _ in range(30):
+        rules = LogitRules(rows, vocab, capacity=4)
+        rules.lengths[0] = 4
+        token = rules.pick(x)
+        with pytest.raises(_lib.DimmerKVError, match="114"):
+            rules.check_status()
+        assert int(token[0]) in (-1, int(best[0])) and int(rules.lengths[0]) == 4
+        made = token >= 0
+        assert torch.equal(token[made], best[made])
+        assert torch.equal(rules.lengths[1:], made[1:].int())
+        assert torch.equal(rules.history[1:, 0].long(), token[1:])  # -1 where nothing was appended
