@@ -163,8 +163,9 @@ def greedy_decode_batch(model, batch: CompressedBatch, cache, host_ids: torch.Te
 
     ``host_ids`` / ``host_positions``: [B, 1] int64 in (pinned) host memory. Every step copies the
     ids to the device, runs the model with attention over the codes and reads the next ids back, with
-    the batch's status word behind them; the host waits for them at most ``batch.poll_wait_s`` seconds
-    and raises ``DimmerKVError`` on a device error (``CompressedBatch.poll_status``).
+    the batch's status word (and that of the rules) behind them; the host waits for them at most
+    ``batch.poll_wait_s`` seconds and raises ``DimmerKVError`` on a device error (``CompressedBatch.poll_status``),
+    a full history among them.
     Returns (tokens [B, steps] int64 on the host, byte counts of the per-step copies)."""
     if grammar is not None and rules is None:
         raise ValueError("a grammar needs rules (LogitRules)")
@@ -172,6 +173,7 @@ def greedy_decode_batch(model, batch: CompressedBatch, cache, host_ids: torch.Te
     ids_host = host_ids.clone().pin_memory() if not host_ids.is_pinned() else host_ids.clone()
     pos = host_positions.to(device)
     out = torch.empty(ids_host.shape[0], steps, dtype=torch.int64)
+    rules_host = None if rules is None else torch.zeros(1, dtype=torch.int32).pin_memory()
     dimmer.STATE.compressed = batch
     try:
         for i in range(steps):
@@ -183,14 +185,18 @@ def greedy_decode_batch(model, batch: CompressedBatch, cache, host_ids: torch.Te
                 mask = grammar(out[:, i - 1] if i else None) if grammar is not None else None
                 nxt = rules.pick(logits[:, -1], mask)[:, None]
             ids_host.copy_(nxt, non_blocking=True)  # device -> pinned host
-            batch.poll_status(depth=0)  # bounded wait for the ids and the status word behind them
+            if rules is not None:
+                rules_host.copy_(rules.status, non_blocking=True)
+            batch.poll_status(depth=0)  # bounded wait for the ids and the status words behind them
             out[:, i] = ids_host[:, 0]
+            if rules is not None and int(rules_host) != 0:
+                raise _lib.DimmerKVError(_lib.describe_device_error(int(rules_host)))
             if rules is not None and bool((out[:, i] < 0).any()):
-                rules.check_status()
                 rows = (out[:, i] < 0).nonzero().flatten().tolist()
                 raise _lib.DimmerKVError(f"step {i}: no token is allowed in conversations {rows}")
             pos = pos + 1
     finally:
         dimmer.STATE.compressed = None
     nbytes = ids_host.numel() * ids_host.element_size()
-    return out, {"h2d_bytes_per_step": nbytes, "d2h_bytes_per_step": nbytes + batch.status.element_size()}
+    words = batch.status.element_size() + (0 if rules is None else rules.status.element_size())
+    return out, {"h2d_bytes_per_step": nbytes, "d2h_bytes_per_step": nbytes + words}

@@ -61,3 +61,32 @@ def test_a_full_history_leaves_the_other_rows_whole(rows, vocab):
         assert torch.equal(token[made], best[made])
         assert torch.equal(rules.lengths[1:], made[1:].int())
         assert torch.equal(rules.history[1:, 0].long(), token[1:])  # -1 where nothing was appended
+
+
+def _prefilled(model, rows, max_tokens=128):
+    batch = Q4Batch(rows, layers=2, kv_heads=8, q_heads=32, head_dim=64, max_tokens=max_tokens, dtype=model.dtype)
+    ids = tm.context_ids().to(DEV)[0, :rows * 40].view(rows, 40)
+    dimmer.STATE.compressed = batch
+    try:
+        model(input_ids=ids, past_key_values=batch.cache, position_ids=torch.arange(40, device=DEV)[None].expand(rows, -1),
+              use_cache=True)
+    finally:
+        dimmer.STATE.compressed = None
+    return batch
+
+
+def test_the_batch_driver_tells_a_full_history_at_its_last_step():
+    model = tm.build_model(torch.bfloat16, DEV)
+    dimmer.install(model)
+    with torch.inference_mode():
+        for steps, full in ((3, False), (4, True)):
+            rules = LogitRules(2, 1024, capacity=3)
+            args = (torch.tensor([[1], [2]]), torch.full((2, 1), 40), steps)
+            batch = _prefilled(model, 2)
+            if full:
+                with pytest.raises(_lib.DimmerKVError, match="114"):
+                    greedy_decode_batch(model, batch, batch.cache, *args, rules=rules)
+            else:
+                out, moved = greedy_decode_batch(model, batch, batch.cache, *args, rules=rules)
+                assert torch.equal(rules.history.cpu(), out.int())
+                assert moved["d2h_bytes_per_step"] == 2 * 8 + 4 + 4  # the ids and two status words
