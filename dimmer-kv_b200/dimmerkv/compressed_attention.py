@@ -119,6 +119,9 @@ def greedy_answer(model, tokenizer, context, cache, input_ids: torch.Tensor, sta
     ``rules`` (a one-row ``LogitRules``) adjusts the logits of every step before the choice and takes the chosen
     token into its history; ``grammar(last)`` gives that step's mask (``allow_mask``; None: everything) from the
     token before it (None at the first step). A step whose mask leaves nothing ends the answer.
+
+    A ``Q4Context`` whose pass failed (no room for its tokens, a value that no cell holds) raises ``DimmerKVError``
+    at that step: what the model made of it is no answer.
     """
     if grammar is not None and rules is None:
         raise ValueError("a grammar needs rules (LogitRules)")
@@ -141,8 +144,10 @@ def greedy_answer(model, tokenizer, context, cache, input_ids: torch.Tensor, sta
                 mask = grammar(generated[-1] if generated else None) if grammar is not None else None
                 token = int(rules.pick(logits[:, -1], mask)[0])
                 rules.check_status()
-                if token < 0:
-                    break
+            if context is not None and hasattr(context, "check_status"):
+                context.check_status()  # the token's copy has waited for the pass
+            if token < 0:
+                break
             if stop_at_eos and (token == tokenizer.eos_token_id or token in tokenizer.all_special_ids):
                 break
             generated.append(token)

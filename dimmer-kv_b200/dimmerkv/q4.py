@@ -287,6 +287,9 @@ class Q4Context:
     def exact_bytes(self) -> int:
         return 0
 
+    def check_status(self) -> None:
+        self.batch.check_status()
+
     def attend(self, module, query, key, value, attention_mask, scaling):
         return self.batch.attend(module, query, key, value, attention_mask, scaling)
 

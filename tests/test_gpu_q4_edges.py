@@ -90,3 +90,28 @@ def test_the_batch_driver_tells_a_full_history_at_its_last_step():
                 out, moved = greedy_decode_batch(model, batch, batch.cache, *args, rules=rules)
                 assert torch.equal(rules.history.cpu(), out.int())
                 assert moved["d2h_bytes_per_step"] == 2 * 8 + 4 + 4  # the ids and two status words
+
+
+def test_an_answer_over_a_context_without_room_is_no_answer():
+    """Tokens beyond a context's room, or values that no cell holds, end greedy_answer with the error."""
+    model = tm.build_model(torch.bfloat16, DEV)
+    dimmer.install(model)
+    question = tm.question_ids().to(DEV)[None]
+    with torch.inference_mode():
+        # two pages hold 128 tokens; a question of 8 and three of four answered tokens are stored
+        for tokens, room, fits in ((117, 11, True), (118, 10, False), (121, 7, False)):
+            cache, _ = dimmer.prefill_with_scores(model, tm.context_ids().to(DEV)[:, :tokens])
+            keys, values = [l.keys for l in cache.layers], [l.values for l in cache.layers]
+            context = Q4Context(keys, values, model, dtype=torch.bfloat16, room=room)
+            args = (model, _Tokens(), context, context.exact_cache, question, tokens, 4)
+            if fits:
+                assert len(greedy_answer(*args)[0].split()) == 4
+                context.check_status()
+            else:
+                with pytest.raises(_lib.DimmerKVError, match="9112"):
+                    greedy_answer(*args)
+        values[1][0, 3, 17, 5] = float("inf")
+        context = Q4Context(keys, values, model, dtype=torch.bfloat16)
+        with pytest.raises(_lib.DimmerKVError, match="8113"):
+            greedy_answer(model, _Tokens(), context, context.exact_cache, question, tokens)
+    assert dimmer.STATE.compressed is None
