@@ -219,11 +219,15 @@ class Q4Batch:
 
     def attend(self, module, query, key, value, attention_mask, scaling):
         """Same contract as an HF attention function: (output, None). The pass's first layer plans its tokens. A
-        mask may only repeat the causal order of the new tokens; another one is refused through the status word."""
+        mask [rows or 1, any heads, q_len, q_len or more] may only repeat the causal order: of its columns the last q_len
+        are the new tokens, those before them held ones, which every new token sees. Another one is refused through the
+        status word."""
         q_len = query.shape[2]
         if key.shape[2] != q_len:
             raise ValueError(f"{key.shape[2]} keys for {q_len} queries: pass the batch's own cache (Q4Batch.cache) to "
                              "the model")
+        if attention_mask is not None and (attention_mask.dim() != 4 or attention_mask.shape[3] < q_len):
+            raise ValueError(f"a mask {tuple(attention_mask.shape)} is not [rows, heads, {q_len}, {q_len} or more]")
         if module.layer_idx == 0:
             counts, self._counts = self._counts, None
             self.plan(counts, q_len)
@@ -233,13 +237,15 @@ class Q4Batch:
         return self.attend_layer(module.layer_idx, query, key, value, scaling, out_dtype=out_dtype), None
 
     def _check_mask(self, mask: torch.Tensor, counts, q_len: int) -> None:
-        visible = mask[:, 0, :, -q_len:] if mask.dtype == torch.bool else mask[:, 0, :, -q_len:] == 0
+        visible = mask if mask.dtype == torch.bool else mask == 0
+        held = visible.shape[3] - q_len
         order = torch.ones(q_len, q_len, dtype=torch.bool, device=self.device).tril()
-        wrong = visible != order
+        wrong, hidden = visible[..., held:] != order, ~visible[..., :held]
         if counts is not None:
             real = torch.arange(q_len, device=self.device) < counts[:, None]
-            wrong = wrong & real[:, :, None] & real[:, None, :]
-        self.status.masked_fill_(wrong.any() & (self.status == 0), MASK_ERROR)
+            wrong = wrong & real[:, None, :, None] & real[:, None, None, :]
+            hidden = hidden & real[:, None, :, None]
+        self.status.masked_fill_((wrong.any() | hidden.any()) & (self.status == 0), MASK_ERROR)
 
     # ------------------------------------------------------------------ status
     @property

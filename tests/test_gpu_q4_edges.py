@@ -115,3 +115,46 @@ def test_an_answer_over_a_context_without_room_is_no_answer():
         with pytest.raises(_lib.DimmerKVError, match="8113"):
             greedy_answer(model, _Tokens(), context, context.exact_cache, question, tokens)
     assert dimmer.STATE.compressed is None
+
+
+class _Layer:
+    layer_idx = 0
+
+
+def test_masks_that_hide_what_the_attention_sees_are_told():
+    """A mask of more columns than new tokens has to show every older one, for each of its heads; of rows that bring
+    fewer tokens only the real ones count."""
+    batch = Q4Batch(2, layers=1, kv_heads=2, q_heads=4, head_dim=64, max_tokens=200)
+    k, v, q = (_rows(2, h, 3, 64, torch.bfloat16, 5 + h) for h in (2, 2, 4))
+    order = torch.ones(3, 3, dtype=torch.bool, device=DEV).tril()
+    low = torch.finfo(torch.bfloat16).min
+
+    def told(mask, counts=None):
+        batch.begin(counts)
+        batch.attend(_Layer, q, k, v, mask, 0.125)
+        code = int(batch.status)
+        batch.reset_status()
+        return code
+
+    def wide(old, heads=1, rows=2):
+        return torch.cat([torch.ones(rows, heads, 3, old, dtype=torch.bool, device=DEV),
+                          order.expand(rows, heads, 3, 3)], -1)
+
+    additive = lambda m: torch.zeros(m.shape, dtype=torch.bfloat16, device=DEV).masked_fill_(~m, low)
+    for old, heads, rows in ((0, 1, 2), (3, 1, 2), (6, 4, 1), (9, 4, 2)):
+        m = wide(old, heads, rows)
+        assert told(m) == 0 and told(additive(m)) == 0
+    hidden = wide(12)
+    hidden[1, 0, 2, 4] = False                       # an older token
+    assert told(hidden) == 115 and told(additive(hidden)) == 115
+    assert told(hidden, [3, 2]) == 0                 # its row is padding
+    assert told(hidden, [3, 3]) == 115
+    head = wide(15, heads=4)
+    head[0, 3, 1, 0] = False                         # of the last head alone
+    assert told(head) == 115
+    head = wide(0, heads=4)
+    head[0, 1, 0, 2] = True                          # shows a later token, in one head
+    assert told(head) == 115
+    for bad in (wide(0)[:, 0], wide(0)[..., :2]):
+        with pytest.raises(ValueError):
+            batch.attend(_Layer, q, k, v, bad, 0.125)
