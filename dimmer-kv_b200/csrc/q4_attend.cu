@@ -884,10 +884,12 @@ int64_t dkv_q4_attend_floats(const dkv_q4_attend_args* a) {
 
 int dkv_q4_attend(const dkv_q4_attend_args* a, void* stream) {
   if (a == nullptr || a->cells == nullptr || a->blocks == nullptr || a->lengths == nullptr || a->starts == nullptr ||
-      a->query == nullptr || a->out == nullptr || a->status == nullptr)
+      a->status == nullptr)
     return DKV_ERR_ARGS;
   const int rc = dkv::check_sizes(a);
   if (rc != DKV_OK) return rc;
+  if (a->n_seq == 0 || a->q_len == 0) return DKV_OK;  // tensors without an element have no address
+  if (a->query == nullptr || a->out == nullptr) return DKV_ERR_ARGS;
   if ((a->key == nullptr) != (a->value == nullptr) || (a->key != nullptr && a->slots == nullptr)) return DKV_ERR_ARGS;
   if (reinterpret_cast<uintptr_t>(a->cells) % 16 || reinterpret_cast<uintptr_t>(a->query) % 16 ||
       reinterpret_cast<uintptr_t>(a->key) % 16 || reinterpret_cast<uintptr_t>(a->value) % 16 ||
@@ -895,7 +897,6 @@ int dkv_q4_attend(const dkv_q4_attend_args* a, void* stream) {
     return DKV_ERR_ARGS;
   for (int k = 0; k < 3; ++k)
     if (a->q_stride[k] % 8 || (a->key != nullptr && (a->k_stride[k] % 8 || a->v_stride[k] % 8))) return DKV_ERR_ARGS;
-  if (a->n_seq == 0 || a->q_len == 0) return DKV_OK;
   if (a->workspace == nullptr || a->workspace_floats < dkv_q4_attend_floats(a)) return DKV_ERR_SCRATCH;
   const bool prefill = dkv::q4::prefill_takes(*a);
   const int nt = dkv::tiles_of(*a);

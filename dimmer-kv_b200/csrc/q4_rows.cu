@@ -140,11 +140,13 @@ __global__ void __launch_bounds__(kRowThreads) q4_read_kernel(const __grid_const
 }
 
 int check_rows(const dkv_q4_rows_args* a) {
-  if (a == nullptr || a->cells == nullptr || a->slots == nullptr || a->key == nullptr || a->value == nullptr ||
-      a->status == nullptr || a->n_pages < 1 || a->n_kv_heads < 1 || a->n_seq < 0 || a->q_len < 0)
+  if (a == nullptr || a->cells == nullptr || a->status == nullptr || a->n_pages < 1 || a->n_kv_heads < 1 ||
+      a->n_seq < 0 || a->q_len < 0)
     return DKV_ERR_ARGS;
   if (a->head_dim != 64 && a->head_dim != 128) return DKV_ERR_CONFIG;
   if (static_cast<int64_t>(a->n_pages) * q4::kPage > INT32_MAX) return DKV_ERR_CONFIG;
+  if (a->n_seq == 0 || a->q_len == 0) return DKV_OK;  // tensors without an element have no address
+  if (a->slots == nullptr || a->key == nullptr || a->value == nullptr) return DKV_ERR_ARGS;
   if (reinterpret_cast<uintptr_t>(a->cells) % 16 || reinterpret_cast<uintptr_t>(a->key) % 16 ||
       reinterpret_cast<uintptr_t>(a->value) % 16)
     return DKV_ERR_ARGS;

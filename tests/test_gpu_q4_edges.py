@@ -158,3 +158,26 @@ def test_masks_that_hide_what_the_attention_sees_are_told():
     for bad in (wide(0)[:, 0], wide(0)[..., :2]):
         with pytest.raises(ValueError):
             batch.attend(_Layer, q, k, v, bad, 0.125)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_calls_without_a_token(dtype):
+    batch = Q4Batch(2, layers=1, kv_heads=2, q_heads=4, head_dim=64, max_tokens=64, dtype=dtype)
+    batch.plan([3, 5], 5)
+    k, v = _rows(2, 2, 5, 64, dtype, 1), _rows(2, 2, 5, 64, dtype, 2)
+    batch.append(0, k, v)
+    first = batch._slots
+    want = batch.read(0)
+    none = torch.zeros(2, 2, 0, 64, dtype=dtype, device=DEV)
+    for counts in (None, [0, 0]):
+        assert batch.plan(counts, 0).shape == (2, 0)
+        batch.append(0, none, none)
+        assert [x.shape for x in batch.read(0)] == [none.shape] * 2
+        query = torch.zeros(2, 4, 0, 64, dtype=dtype, device=DEV)
+        for key in (none, None):
+            assert batch.attend_layer(0, query, key, key, 0.125).shape == (2, 0, 4, 64)
+    assert batch.lengths.tolist() == [3, 5]
+    assert all(torch.equal(a, b) for a, b in zip(batch.read(0, first), want))
+    keys, values = restore([none[:1]] * 2, [none[:1]] * 2)
+    assert [x.shape for x in keys + values] == [(1, 2, 0, 64)] * 4
+    batch.check_status()

@@ -160,3 +160,22 @@ def test_scales_have_no_sign():
     assert bool((low.float()[:, 0] >= x.float().amax(-1)).any())
     assert not scale.signbit().any() and not codes[:2].any()
     assert torch.equal(dequantise4(codes, scale, low).double(), cells64(x)[0])
+
+
+@needs_lib
+def test_entry_points_take_calls_without_a_token():
+    """Tensors without an element have no address: such calls do nothing, and their sizes are checked all the same."""
+    lib = _lib.lib()
+    p = 1 << 20  # never followed
+    rows = dict(cells=p, n_pages=4, n_kv_heads=2, head_dim=64, n_seq=1, q_len=0, status=p)
+    att = dict(cells=p, n_pages=4, n_kv_heads=2, n_q_heads=4, head_dim=64, blocks=p, max_blocks=1, lengths=p, starts=p, n_seq=1,
+               q_len=0, len_bound=64, scaling=1.0, status=p)
+    table = dict(blocks=p, max_blocks=2, lengths=p, starts=p, n_seq=1, counts=p, q_len=0, status=p)
+    for bad, rc in ((dict(), 0), (dict(n_seq=0, q_len=3), 0), (dict(head_dim=96), 2), (dict(n_kv_heads=0), 1),
+                    (dict(q_len=1), 1), (dict(cells=None), 1)):
+        for fn in (lib.dkv_q4_append, lib.dkv_q4_read):
+            assert fn(_lib.Q4RowsArgs(**{**rows, **bad}), None) == rc, bad
+        a = _lib.Q4AttendArgs(**{**att, **bad})
+        assert lib.dkv_q4_attend(a, None) == rc, bad
+    assert lib.dkv_q4_attend_floats(_lib.Q4AttendArgs(**att)) == 0
+    assert lib.dkv_page_slots(_lib.PageArgs(**table), None) == 0
