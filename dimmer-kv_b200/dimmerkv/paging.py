@@ -51,7 +51,7 @@ class PageTable:
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device) if status is None else status
         self.poll_wait_s = 60.0
         self._poller = None
-        self.bound = 0  # no length is above this (known on the host)
+        self.bound = 0  # no length is above this (known on the host), whatever replays of captured plans reach
         self._even: dict[int, torch.Tensor] = {}
         self._args = _lib.PageArgs(self.blocks.data_ptr(), self.max_blocks, self.lengths.data_ptr(),
                                    self.starts.data_ptr(), self.free.data_ptr(), self.n_free.data_ptr(), n_pages, n_seq,
@@ -96,7 +96,8 @@ class PageTable:
         counts = self.even(q_len) if counts is None else self._counts(counts)
         slots = torch.empty(self.n_seq, q_len, dtype=torch.int32, device=self.device)
         self._run("dkv_page_plan", counts, q_len, slots)
-        self.bound = min(self.max_tokens, self.bound + q_len)
+        # replays of a captured plan lengthen the conversations without passing here
+        self.bound = self.max_tokens if torch.cuda.is_current_stream_capturing() else min(self.max_tokens, self.bound + q_len)
         return slots
 
     def trim(self, keep) -> None:

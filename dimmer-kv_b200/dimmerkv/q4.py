@@ -205,7 +205,10 @@ class Q4Batch:
         a = _lib.Q4AttendArgs.from_buffer_copy(made)
         out = torch.empty((self.n_seq, q_len, self.q_heads, self.head_dim), dtype=out_dtype, device=self.device)
         workspace = torch.empty(a.workspace_floats, dtype=torch.float32, device=self.device)
-        a.cells, a.len_bound, a.scaling = self._layer(layer), self.table.bound, scaling
+        # a captured call serves whatever lengths the tables have when it is replayed: one that was split for the 64 tokens at
+        # its capture took 49 us over 16384 tokens (24 / 8 heads of 128) where 16 are enough
+        bound = self.table.max_tokens if torch.cuda.is_current_stream_capturing() else self.table.bound
+        a.cells, a.len_bound, a.scaling = self._layer(layer), bound, scaling
         a.query, a.out, a.workspace = query.data_ptr(), out.data_ptr(), workspace.data_ptr()
         if key is not None:
             a.key, a.value, a.slots = key.data_ptr(), value.data_ptr(), self._slots.data_ptr()

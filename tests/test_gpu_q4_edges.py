@@ -181,3 +181,33 @@ def test_calls_without_a_token(dtype):
     keys, values = restore([none[:1]] * 2, [none[:1]] * 2)
     assert [x.shape for x in keys + values] == [(1, 2, 0, 64)] * 4
     batch.check_status()
+
+
+def test_captured_steps_grow_over_the_whole_gpu():
+    """A step captured on an empty batch and replayed until it is long: the work is split as for the lengths that replays
+    reach, by the replays and by eager calls behind them, so that the results are an eager batch's."""
+    dim, kv, hq, n = 64, 2, 8, 512
+    batches = [Q4Batch(1, layers=1, kv_heads=kv, q_heads=hq, head_dim=dim, max_tokens=16000) for _ in range(2)]
+    k, v = _rows(1, kv, n, dim, torch.bfloat16, 3, "key"), _rows(1, kv, n, dim, torch.bfloat16, 4)
+    one = [_rows(1, h, 1, dim, torch.bfloat16, 5 + i) for i, h in enumerate((hq, kv, kv))]
+    captured, eager = batches
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured.plan(None, n)
+        captured.append(0, k, v)
+        captured.plan()
+        out = captured.attend_layer(0, *one, 0.125)
+    for _ in range(20):
+        graph.replay()
+        eager.plan(None, n)
+        eager.append(0, k, v)
+        eager.plan()
+        want = eager.attend_layer(0, *one, 0.125)
+        assert torch.equal(out, want)
+    assert captured.lengths.tolist() == eager.lengths.tolist() == [20 * (n + 1)]
+    for batch in batches:
+        batch.plan()
+    assert torch.equal(captured.attend_layer(0, *one, 0.125), eager.attend_layer(0, *one, 0.125))
+    assert captured.table.bound >= int(captured.lengths)
+    captured.check_status()
