@@ -441,7 +441,8 @@ __device__ __forceinline__ void attend(const uint8_t* page, int tile, int base, 
 }
 
 // The new tokens of a page (tokens first .. last of the conversation), quantised by the warp into the page's copy in
-// shared memory and into the cache: whatever the copy caught of them is overwritten.
+// shared memory and into the cache: whatever the copy caught of them is overwritten. Tokens without a slot (of a plan that
+// failed) stay out, as in dkv_q4_append: their places are those of an earlier plan's.
 template <int D, bool F16>
 __device__ __noinline__ void store_new(const dkv_q4_attend_args& a, int seq, int head, int start, int first, int last,
                                        uint8_t* copy, uint8_t* cell) {
@@ -450,16 +451,19 @@ __device__ __noinline__ void store_new(const dkv_q4_attend_args& a, int seq, int
   const int j = lane % kLanes, is_value = (lane / kLanes) & 1, sub = lane / (2 * kLanes);
   const int64_t* sd = is_value ? a.v_stride : a.k_stride;
   const uint16_t* src = static_cast<const uint16_t*>(is_value ? a.value : a.key) + seq * sd[0] + head * sd[1] + j * 16;
+  const int32_t* slots = a.slots + static_cast<int64_t>(seq) * a.q_len - start;
   for (int tok = first; tok < last; tok += kPer) {
     const int mine = tok + sub;
+    int slot = -1;
     uint4 raw[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-    if (mine < last) {
+    if (mine < last) {  // under way together
+      slot = slots[mine];
       const uint4* from = reinterpret_cast<const uint4*>(src + (mine - start) * sd[2]);
       raw[0] = from[0], raw[1] = from[1];
     }
     const q4::CellPart<2> c = q4::quantise<F16>(raw);
-    if (!c.fits) record_error(a.status, kSiteQ4Rows + kErrCellRange);
-    if (mine < last) {
+    if (slot >= 0) {
+      if (!c.fits) record_error(a.status, kSiteQ4Rows + kErrCellRange);
       const int r = mine % q4::kPage;
       if (is_value) {
         q4::store_value<D>(copy, r, j, c);

@@ -211,3 +211,25 @@ def test_captured_steps_grow_over_the_whole_gpu():
     assert torch.equal(captured.attend_layer(0, *one, 0.125), eager.attend_layer(0, *one, 0.125))
     assert captured.table.bound >= int(captured.lengths)
     captured.check_status()
+
+
+@pytest.mark.parametrize("q_len", [1, 4, 40])
+def test_a_plan_that_failed_stores_nothing(q_len):
+    """Attention with the slots of a failed plan, once the status word is cleared: the cells stay as they were, in the
+    form that stores the tokens itself as in the other."""
+    batch = Q4Batch(1, layers=1, kv_heads=2, q_heads=4, head_dim=64, max_tokens=128)
+    k, v, q = (_rows(1, h, q_len, 64, torch.bfloat16, i) for i, h in ((1, 2), (2, 2), (3, 4)))
+    held = 128 - q_len
+    batch.plan([held], held)
+    batch.append(0, *(_rows(1, 2, held, 64, torch.bfloat16, i) for i in (5, 6)))
+    batch.plan(None, q_len)
+    batch.attend_layer(0, q, k, v, 0.125)
+    slots = batch.table.slots(128)
+    want = batch.read(0, slots)
+    assert bool((batch.plan(None, q_len) == -1).all())
+    with pytest.raises(_lib.DimmerKVError, match="9112"):
+        batch.check_status()
+    batch.reset_status()
+    batch.attend_layer(0, q, 2 * k, 2 * v, 0.125)
+    assert all(torch.equal(a, b) for a, b in zip(batch.read(0, slots), want))
+    batch.check_status()
