@@ -28,10 +28,6 @@ enum DeviceError : int {
   kErrWaitAccumFree = 106, // MMA waiting for the epilogue to drain TMEM
   kErrWaitDrain = 107,     // exit path waiting for outstanding async work
   kErrBadDescriptor = 110, // a tile / group descriptor failed its bounds check
-  kErrNoPages = 111,       // fewer free pages than the plan needs
-  kErrCounts = 112,        // a token count or a length out of its range
-  kErrCellRange = 113,     // a key or value that no 4-bit cell holds (not finite, or beyond 2^15)
-  kErrHistory = 114,       // no room for a token in a history
 };
 // The kernel that recorded an error, added to the code (the host names it): status = site + error.
 constexpr int kSiteKeyPair = 1000;     // key_scores_pair_kernel (CTA pairs)
@@ -40,9 +36,6 @@ constexpr int kSiteValue = 3000;       // value_weights_kernel / vprobs_kernel (
 constexpr int kSiteValueDense = 4000;  // value_dense_kernel (coefficients decoded once per step)
 constexpr int kSiteUnpack = 5000;      // unpack_kernel
 constexpr int kSiteKeyDense = 6000;    // key_scores_dense_kernel (coefficients decoded once per step)
-constexpr int kSiteQ4Attend = 7000;    // q4_decode_kernel, q4_prefill_kernel
-constexpr int kSiteQ4Rows = 8000;      // q4_append_kernel, q4_read_kernel
-constexpr int kSitePages = 9000;       // page_plan_kernel, page_trim_kernel, page_slots_kernel
 
 // Bound on one wait. Healthy waits in these kernels last microseconds; a wait gives up after 2 s of
 // %globaltimer time. The time is summed over polls in steps clamped to 100 ms (a step backwards counts as

@@ -17,6 +17,7 @@
 #include "../../include/dimmer_kv.h"
 #include "dkv_launch.h"
 #include "dkv_ptx.cuh"
+#include "dkv_serving.h"
 
 namespace dkv {
 namespace {

@@ -114,3 +114,9 @@ def test_synthetic_ladder_feeds_the_drop_in_codec(tmp_path):
     assert key == 2 * width["key"] * heads * dim + 2 * middle * c.num_attention_heads * dim
     assert step == layers * (key + 2 * c.num_attention_heads * width["value"] + 2 * c.num_attention_heads * 256 * dim)
     assert code_bytes == (out.used_bytes - (tokens - middle) * 2 * codec.exact_bytes) * layers
+
+
+def test_the_profile_of_the_key_kernel_is_of_these_sources():
+    """The bench line's traffic comes from a capture of the kernel that this tree builds."""
+    line = bench.roofline(10**12, [1.0])
+    assert line["traffic"] is not None and line["traffic"] > 0
