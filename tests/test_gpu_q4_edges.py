@@ -233,3 +233,69 @@ def test_a_plan_that_failed_stores_nothing(q_len):
     batch.attend_layer(0, q, 2 * k, 2 * v, 0.125)
     assert all(torch.equal(a, b) for a, b in zip(batch.read(0, slots), want))
     batch.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,q_len", [(64, 3), (128, 40), (64, 90), (128, 150)])
+def test_attention_of_other_strides_signs_and_rows(dim, q_len, dtype):
+    """Both forms over tensors at odd offsets and strides, under a negative scaling, and with a row that is not finite."""
+    held, counts = [200, 0, 65], [q_len, q_len - 1, 1]
+    batch, query, k, v, keys, values = _filled(3, 8, 2, dim, dtype, held, counts, q_len, seed=41)
+    want = batch.attend_layer(0, query, k, v, 0.1)
+    _check(want, query, keys, values, held, counts, 0.1)
+    flat = torch.zeros(query.numel() + 3, dtype=dtype, device=DEV)
+    odd = flat[3:].view(3, q_len, 8, dim).transpose(1, 2)
+    odd.copy_(query)
+    wide = torch.zeros(3, 2, q_len, dim + 4, dtype=dtype, device=DEV)
+    wide[..., :dim] = k
+    backwards = v.flip(3).contiguous().flip(3)
+    assert torch.equal(batch.attend_layer(0, odd, wide[..., :dim], backwards, 0.1), want)
+    heads_last = query.permute(3, 0, 1, 2).contiguous().permute(1, 2, 3, 0)  # no dense last dimension
+    assert torch.equal(batch.attend_layer(0, heads_last, None, None, 0.1), want)
+    # a scaling below zero is the same as negated queries
+    negative = batch.attend_layer(0, query, None, None, -0.1)
+    _check(negative, -query, keys, values, held, counts, 0.1)
+    # one row that is not finite: the others as they were
+    for bad in (float("nan"), float("inf")):
+        spoilt = query.clone()
+        spoilt[0, 5, 1, 7] = bad
+        out = batch.attend_layer(0, spoilt, None, None, 0.1)
+        assert bad == bad or bool(out[0, 1, 5].isnan().all())
+        out[0, 1, 5] = want[0, 1, 5]
+        assert torch.equal(out, want)
+    batch.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_the_batch_driver_picks_the_formulas_tokens(dtype):
+    """greedy_decode_batch under penalties: every token is the best of the rules' formulas on the logits of its step,
+    made by the same model over a second batch with the same rows."""
+    model = tm.build_model(dtype, DEV)
+    dimmer.install(model)
+    rows, steps = 3, 7
+    with torch.inference_mode():
+        start, pos = torch.tensor([[4], [5], [6]]), torch.full((rows, 1), 40)
+        rules = LogitRules(rows, 1024, capacity=64, repetition=1.5, frequency=0.25, presence=0.125)
+        prompts = tm.context_ids().to(DEV)[0, :rows * 40].view(rows, 40)
+        rules.load(prompts)
+        batch = _prefilled(model, rows)
+        out, _ = greedy_decode_batch(model, batch, batch.cache, start, pos, steps, rules=rules)
+        again = _prefilled(model, rows)
+        dimmer.STATE.compressed = again
+        try:
+            ids = start.to(DEV)
+            for i in range(steps):
+                x = model(input_ids=ids, past_key_values=again.cache, position_ids=pos.to(DEV) + i, use_cache=True).logits
+                x = x[:, -1].float()
+                made = torch.zeros(rows, 1024, device=DEV)
+                if i:
+                    made.scatter_add_(1, out[:, :i].to(DEV), torch.ones(rows, i, device=DEV))
+                seen = made.scatter(1, prompts, 1.0) > 0
+                x = torch.where(seen, torch.where(x > 0, x / torch.full_like(x, 1.5), x * 1.5), x)
+                x = torch.where(made > 0, x - 0.25 * made - 0.125, x)
+                assert torch.equal(_first_best(x).cpu(), out[:, i])
+                ids = out[:, i:i + 1].to(DEV)
+        finally:
+            dimmer.STATE.compressed = None
+    assert rules.lengths.tolist() == [40 + steps] * rows
+    assert torch.equal(rules.history[:, 40:40 + steps].cpu().long(), out)
