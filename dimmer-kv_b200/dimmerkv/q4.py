@@ -120,12 +120,15 @@ class Q4Batch:
             raise ValueError(f"layer {layer} of {self.layers}")
         return self._cells_ptr + layer * self._layer_bytes
 
-    def _tensor(self, name: str, x: torch.Tensor, heads: int, rows: int):
-        """x [n_seq, heads, rows, head_dim] as the kernels take it, and its strides."""
+    def _check(self, name: str, x: torch.Tensor, heads: int, rows: int) -> None:
         if x.shape != (self.n_seq, heads, rows, self.head_dim):
             raise ValueError(f"{name} {tuple(x.shape)} is not [{self.n_seq}, {heads}, {rows}, {self.head_dim}]")
         if x.device != self.device:
             raise ValueError(f"{name} is on {x.device}, the cache on {self.device}")
+
+    def _tensor(self, name: str, x: torch.Tensor, heads: int, rows: int):
+        """x [n_seq, heads, rows, head_dim] as the kernels take it, and its strides."""
+        self._check(name, x, heads, rows)
         if x.dtype is not self.dtype:
             x = x.to(self.dtype)
         strides = x.stride()
@@ -229,9 +232,17 @@ class Q4Batch:
         if key.shape[2] != q_len:
             raise ValueError(f"{key.shape[2]} keys for {q_len} queries: pass the batch's own cache (Q4Batch.cache) to "
                              "the model")
-        if attention_mask is not None and (attention_mask.dim() != 4 or attention_mask.shape[3] < q_len):
-            raise ValueError(f"a mask {tuple(attention_mask.shape)} is not [rows, heads, {q_len}, {q_len} or more]")
+        if attention_mask is not None:
+            form = tuple(attention_mask.shape)
+            if len(form) != 4 or form[0] not in (1, self.n_seq) or form[2] != q_len or form[3] < q_len:
+                raise ValueError(f"a mask {form} is not [1 or {self.n_seq}, heads, {q_len}, {q_len} or more]")
+            if attention_mask.device != self.device:
+                raise ValueError(f"the mask is on {attention_mask.device}, the cache on {self.device}")
         if module.layer_idx == 0:
+            # what attend_layer would refuse is refused before the tokens have their places
+            self._check("query", query, self.q_heads, q_len)
+            self._check("key", key, self.kv_heads, q_len)
+            self._check("value", value, self.kv_heads, q_len)
             counts, self._counts = self._counts, None
             self.plan(counts, q_len)
             if attention_mask is not None:

@@ -299,3 +299,23 @@ def test_the_batch_driver_picks_the_formulas_tokens(dtype):
             dimmer.STATE.compressed = None
     assert rules.lengths.tolist() == [40 + steps] * rows
     assert torch.equal(rules.history[:, 40:40 + steps].cpu().long(), out)
+
+
+def test_a_pass_that_is_refused_plans_nothing():
+    """The hook looks at a pass's tensors before it makes room for their tokens."""
+    batch = Q4Batch(2, layers=1, kv_heads=2, q_heads=4, head_dim=64, max_tokens=64)
+    q, k = _rows(2, 4, 3, 64, torch.bfloat16, 1), _rows(2, 2, 3, 64, torch.bfloat16, 2)
+    batch.begin([3, 1])
+    for query, key, value in ((q[:1], k[:1], k[:1]), (q, k[:, :1], k[:, :1]), (q[:, :2], k, k), (q, k, k[..., :32]), (q, k.cpu(), k),
+                              (q, k, k[:, :, :2])):
+        with pytest.raises(ValueError):
+            batch.attend(_Layer, query, key, value, None, 0.125)
+        assert batch.lengths.tolist() == [0, 0]
+    order = torch.ones(2, 1, 3, 3, dtype=torch.bool, device=DEV).tril()
+    for mask in (order[:, :, :2], order[..., :2], order[0], order.cpu(), order.repeat(2, 1, 1, 1)[:3]):
+        with pytest.raises(ValueError):
+            batch.attend(_Layer, q, k, k, mask, 0.125)
+        assert batch.lengths.tolist() == [0, 0]
+    out, _ = batch.attend(_Layer, q, k, k, order, 0.125)
+    assert batch.lengths.tolist() == [3, 1] and not out[1, 1:].any()  # the counts of begin still held
+    batch.check_status()
