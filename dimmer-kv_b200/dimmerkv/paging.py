@@ -26,7 +26,7 @@ class PageTable:
 
     ``blocks`` int32 [n_seq, max_blocks] the pages in token order (-1: none), ``lengths`` int32 [n_seq] the tokens,
     ``starts`` int32 [n_seq] the tokens before the newest plan. ``free`` (optional, int32 [n]) gives the free
-    pages, the last one taken first; default: all, page 0 first."""
+    pages, each once, the last one taken first; default: all, page 0 first."""
 
     def __init__(self, n_seq: int, n_pages: int, max_tokens: int, device="cuda", free: torch.Tensor | None = None,
                  status: torch.Tensor | None = None):
@@ -38,6 +38,10 @@ class PageTable:
             raise ValueError("slots are 32-bit: at most 2^31 - 1 tokens in the pool and per conversation")
         if free is not None and (free.dtype != torch.int32 or free.dim() != 1 or free.numel() > n_pages):
             raise ValueError("free must be an int32 vector of at most n_pages pages")
+        if free is not None and free.numel():
+            pages = free.cpu().unique()
+            if pages.numel() != free.numel() or int(pages[0]) < 0 or int(pages[-1]) >= n_pages:
+                raise ValueError(f"free must list pages of 0 .. {n_pages - 1}, each once")
         self.device = _lib.cuda_device(device)
         self.n_seq, self.n_pages, self.max_tokens = n_seq, n_pages, max_tokens
         self.max_blocks = pages_of(max_tokens)

@@ -179,3 +179,13 @@ def test_entry_points_take_calls_without_a_token():
         assert lib.dkv_q4_attend(a, None) == rc, bad
     assert lib.dkv_q4_attend_floats(_lib.Q4AttendArgs(**att)) == 0
     assert lib.dkv_page_slots(_lib.PageArgs(**table), None) == 0
+
+
+def test_tables_refuse_free_lists_that_share_pages():
+    """A page that is listed twice would serve two conversations, one that the pool does not have none."""
+    for free in ([3, 3], [0, 8], [-1, 2], list(range(7)) + [0]):
+        with pytest.raises(ValueError, match="free"):
+            PageTable(2, 8, 100, free=torch.tensor(free, dtype=torch.int32), device="cpu")
+    for free in ([], [7, 0], list(range(8))):
+        with pytest.raises(ValueError, match="CUDA device"):  # (only the device is wrong)
+            PageTable(2, 8, 100, free=torch.tensor(free, dtype=torch.int32), device="cpu")
