@@ -22,7 +22,8 @@ from . import _lib
 from .paging import PAGE, PageTable, pages_of
 
 GROUP = 64
-MASK_ERROR = 115
+CELL_MAX = 32768.0  # largest magnitude that a cell holds
+CELL_ERROR, MASK_ERROR = 8113, 115
 
 
 def cell_bytes(head_dim: int) -> int:
@@ -316,7 +317,8 @@ class Q4Context:
 
 def restore(keys: list[torch.Tensor], values: list[torch.Tensor]):
     """Per-layer [1, kv_heads, tokens, head_dim] -> the same through 4 bits (the cache that ``Methods.apply("q4")``
-    rebuilds). CUDA tensors go through the cells; others through ``quantise4``."""
+    rebuilds). 16-bit CUDA tensors go through the cells; others through ``quantise4``. A key or value that is not
+    finite or beyond 2^15 raises ``DimmerKVError``."""
     if keys[0].is_cuda and keys[0].dtype in (torch.bfloat16, torch.float16):
         _, heads, tokens, dim = keys[0].shape
         batch = Q4Batch(1, layers=1, kv_heads=heads, q_heads=heads, head_dim=dim, max_tokens=max(1, tokens),
@@ -328,5 +330,9 @@ def restore(keys: list[torch.Tensor], values: list[torch.Tensor]):
             out.append(batch.read(0))
         batch.check_status()
         return [k for k, _ in out], [v for _, v in out]
-    through = lambda x: dequantise4(*quantise4(x)).to(x.dtype)
+    def through(x):
+        if x.numel() and not bool((x.abs() <= CELL_MAX).all()):  # (false for a NaN)
+            raise _lib.DimmerKVError(_lib.describe_device_error(CELL_ERROR))
+        return dequantise4(*quantise4(x)).to(x.dtype)
+
     return [through(k) for k in keys], [through(v) for v in values]

@@ -189,3 +189,22 @@ def test_tables_refuse_free_lists_that_share_pages():
     for free in ([], [7, 0], list(range(8))):
         with pytest.raises(ValueError, match="CUDA device"):  # (only the device is wrong)
             PageTable(2, 8, 100, free=torch.tensor(free, dtype=torch.int32), device="cpu")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf"), 40000.0, -32800.0])
+def test_values_without_a_cell_are_refused_on_the_host(bad, dtype):
+    """As on the GPU: a group that 4 bits cannot hold is no cache of zeros, infinities or NaN."""
+    keys = [torch.ones(1, 2, 3, 64, dtype=dtype) for _ in range(2)]
+    values = [k.clone() for k in keys]
+    values[1][0, 1, 2, 63] = -32768.0 if dtype != torch.float32 else 32768.0  # the largest that a cell holds
+    q4.restore(keys, values)
+    values[1][0, 1, 2, 63] = bad
+    if abs(float(values[1].amin())) == 32768.0:  # bfloat16 has steps of 256 there: -32800 is -32768 to it
+        assert dtype == torch.bfloat16 and bad == -32800.0
+        return
+    with pytest.raises(_lib.DimmerKVError, match="4-bit cell"):
+        q4.restore(keys, values)
+    with pytest.raises(_lib.DimmerKVError, match="4-bit cell"):
+        Methods("m", "none", "none", "cpu").apply("q4", values, keys, {})
+    q4.restore([k[:, :, :0] for k in keys], [v[:, :, :0] for v in values])
