@@ -39,8 +39,8 @@ class PageTable:
         if free is not None and (free.dtype != torch.int32 or free.dim() != 1 or free.numel() > n_pages):
             raise ValueError("free must be an int32 vector of at most n_pages pages")
         if free is not None and free.numel():
-            pages = free.cpu().unique()
-            if pages.numel() != free.numel() or int(pages[0]) < 0 or int(pages[-1]) >= n_pages:
+            pages = free.cpu()
+            if int(pages.min()) < 0 or int(pages.max()) >= n_pages or int(pages.bincount().max()) > 1:
                 raise ValueError(f"free must list pages of 0 .. {n_pages - 1}, each once")
         self.device = _lib.cuda_device(device)
         self.n_seq, self.n_pages, self.max_tokens = n_seq, n_pages, max_tokens
