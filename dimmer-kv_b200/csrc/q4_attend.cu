@@ -8,9 +8,14 @@
 // both products run over the codes themselves, which float16 holds exactly, the low terms in float32. The query enters
 // as float16 times a power of two of its row (exact but for what is below 2^-38 of the row's largest), so a score is
 // good to float32. p * scale enters as float16 of 2^7 * exp(score - m) * scale / 2^k, with m within 2^8 of the running
-// maximum and 2^k above the scales so far: a token down to 2^-21 of the largest keeps 11 bits, so that sums over a
-// long context of small probabilities do not vanish. That is one rounding of 2^-11 at most of each term; for float16
-// outputs, whose own step is as small, the factor enters as two float16 numbers (the rounded one and what it lacks).
+// maximum and 2^k one to four times the largest scale of the head so far, of either group: one rounding of 2^-11 at
+// most where p * scale is above 2^-19 of the largest, so that sums over a long context of small probabilities do not
+// vanish; below that float16 has fewer bits, and a term is off by up to 2^-26 of that largest scale (a step's half,
+// 2^-25, times a code of 15). So a group whose scales are a 2^12th of its neighbour's, or of an earlier token's, keeps
+// its bits for probabilities down to 2^-7, and no fewer than 7 of them down to 2^-11. For float16 outputs, whose own step
+// is as small as the rounding, the factor enters as two float16 numbers (the rounded one and what it lacks). Four
+// conversations of 4K to 16K tokens: bfloat16 outputs are off by 1.75e-3 of their size, 1.68e-3 in float32 arithmetic
+// and rounded once, float16 ones by 2.1e-4, as there.
 //
 // q4_decode_kernel: few query rows per KV head (one token, or a short draft). Bound by the cells' bytes, and close to it
 // by unpacking them (the integer pipe runs at half rate). The pages of all (conversation, KV head, row chunk) units
@@ -63,7 +68,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   return r;
 }
 
-// The pages of all units are dealt to the workers (warps) in the order (conversation, KV head, row chunk, page).
 __device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
 
 // How a warp holds its query rows: NT tiles of 8 columns, two columns per lane; or, NT = 0, up to 4 rows, each on the

@@ -23,13 +23,16 @@
 //
 // Keys and values are rounded to float16 (2^-11 at most of each), probabilities likewise. For float16 caches, whose
 // outputs show that, what the rounding of keys lacks forms a second tile, and what that of probabilities lacks a second
-// operand beside the first (each 32 columns of scores become 16 of either), that go through second products.
+// operand beside the first (each 32 columns of scores become 16 of either), that go through second products. The values
+// stay one float16 number: a key's rounding moves its token's weight in every dimension alike, those of the values are of
+// either sign and independent, and their sum shows less (the chunk below is off by 2.8e-4 of its values, 2.1e-4 in float32
+// arithmetic and rounded once), for a third product of the tensor core's bound that is already doubled.
 //
 // The steps of all (conversation, KV head, 256-row block) units form one line that is cut evenly over one CTA per
 // SM; blocks that several CTAs share leave partial results in the workspace, which q4_prefill_combine_kernel joins.
 //
-// 24 / 8 heads of 128: 4 x 512 tokens over 2K to 8K, float16, 204 us with the store and the joins, 64 tokens over 32K,
-// bfloat16, 60 us.
+// 24 / 8 heads of 128: 4 x 512 tokens over 2K to 8K, float16, 203 us with the store and the joins, 64 tokens over 32K,
+// bfloat16, 61 us.
 #include "q4_attend.cuh"
 
 namespace dkv {
@@ -243,6 +246,7 @@ __device__ __forceinline__ uint32_t lack2(uint64_t x, __half2 h) {
   const uint64_t d = fma_f32x2(wide2(h), f32x2_pack(0xbf800000u, 0xbf800000u), x);
   return pack_half2(__uint_as_float(static_cast<uint32_t>(d)), __uint_as_float(static_cast<uint32_t>(d >> 32)));
 }
+// By the exponent's bits: a nibble n in the low bits of the float16 0x6400 makes 1024 + n, four bits higher 1024 + 16 n.
 // Eight codes (nibbles of w) to eight float16 values scale * c + low in the order 0 4 1 5 2 6 3 7, each rounded once; with
 // LOW also what the rounding lacks.
 template <bool LOW>

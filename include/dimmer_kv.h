@@ -445,8 +445,11 @@ int dkv_q4_read(const dkv_q4_rows_args* args, void* stream);
 /* Causal attention of the newest tokens' queries over the 4-bit cells: query row i of conversation s sees the
  * tokens 0 .. starts[s] + i. Rows behind the last new token (i >= lengths[s] - starts[s]) come back as
  * zeros. With `key` and `value` (as in dkv_q4_append, slots of the newest plan) the new tokens are stored as well,
- * without a launch of its own where the query rows are few. Scores, softmax statistics and sums are float32;
- * probabilities enter the value product as float16 against the values rounded to float16. */
+ * without a launch of its own where the query rows are few; a token whose slot is -1 is not stored. Softmax statistics
+ * and sums are float32. Up to 64 query rows per KV head the scores are float32 sums over the exact codes, and the
+ * value product runs over the codes against probability * scale in float16 (for fp16 caches as two float16 numbers).
+ * With more rows the products run over keys, values and probabilities rounded to float16 (for fp16 caches keys and
+ * probabilities as two float16 numbers each, values as one). */
 typedef struct dkv_q4_attend_args {
   uint8_t* cells;                /* the layer's cells */
   int32_t n_pages, n_kv_heads, n_q_heads, head_dim;
@@ -456,7 +459,8 @@ typedef struct dkv_q4_attend_args {
   const int32_t* lengths;
   const int32_t* starts;
   int32_t n_seq, q_len;
-  int32_t len_bound;             /* no length is above this (it only chooses how the work is split) */
+  int32_t len_bound;             /* no length is above this when the call runs, in replays of a captured one too (it
+                                    only chooses how the work is split) */
   const void* query;             /* [n_seq][n_q_heads][q_len][head_dim] at q_stride */
   int64_t q_stride[3];           /* conversation, head, token (elements; multiples of 8, 16-byte aligned) */
   const void* key;               /* the new tokens, [n_seq][n_kv_heads][q_len][head_dim]; NULL: they are stored */
